@@ -178,6 +178,79 @@ int limn_b200_sdpa_bwd_kv_strided(const void* q, const void* k, const void* v, c
                                   int dtype, int batch, int heads, int t_q, int t_k, int hd, int hd_v,
                                   int causal, double scale, void* stream);
 
+/* ---- a paged key and value cache: append with rotary positions, attention over the pages, a shared prefix ----
+ * The step of a server that generates for many sequences at once. Keys and values lie in pages of page_size tokens; a
+ * sequence has a row of page numbers, its page table, and slot j of the sequence is slot j % page_size of page
+ * table[j / page_size]. The step's tokens are packed: sequence b has tokens q_start[b] to q_start[b + 1], and they are the
+ * last ones of its kv_lens[b] keys: token i of n is at slot kv_lens[b] - n + i. Table, offsets and lengths are read on the device
+ * by each call, so a captured call follows what they hold when it is replayed. No counterpart in the reference,
+ * which has no cache (its decode shape is t_q < t_k of dense tensors, tests/test_attention.py:385-396).
+ *   f16/bf16, hd and hd_v multiples of 8 up to 128, heads a multiple of kv_heads (query head h reads key head
+ *   h / (heads / kv_heads)) and at most 128 to a key head, page_size a multiple of 8; strides in elements, multiples of 8, columns
+ *   contiguous, bases 16-byte aligned. Anything else is refused and nothing is launched.
+ * What only the device knows is checked there. A sequence whose offsets or length are impossible (q_start falling, beyond
+ * `tokens` or more than max_t_q apart; kv_lens negative or beyond max_pages * page_size) is left out: nothing of it is appended
+ * and no row of its result is written (where q_start falls, other sequences may be left out too). A page number outside [0, pages) is never followed: a new token that belongs there is
+ * not appended, and a query row that sees a key there gets NaN (O and L). Either is noted in *errors (LIMN_B200_PAGED_BAD_*
+ * bits are or-ed in; the caller clears the word). Tokens from q_start[batch] on, empty slots of pages, and pages that no table
+ * names are neither read for a result nor written. */
+#define LIMN_B200_PAGED_BAD_PAGE 1u
+#define LIMN_B200_PAGED_BAD_SEQUENCE 2u
+typedef struct limn_b200_paged {
+  void* k_cache;              /* element (page, head, slot, column): base + page * k_strides[0] + head * k_strides[1] + slot * k_strides[2] + column */
+  void* v_cache;
+  const int* page_table;      /* (batch, max_pages), dense */
+  const int* q_start;         /* (batch + 1) */
+  const int* kv_lens;         /* (batch): keys in the sequence's pages, the step's tokens among them */
+  unsigned int* errors;       /* device word, or NULL */
+  long long k_strides[3];     /* page, head, slot */
+  long long v_strides[3];
+  int dtype;                  /* LIMN_B200_F16 or LIMN_B200_BF16 */
+  int batch, heads, kv_heads, hd, hd_v;
+  int page_size, pages, max_pages;
+  int tokens;                 /* rows that q, k, v and the results have */
+  int max_t_q;                /* a sequence brings at most this many tokens */
+  int first_position;         /* position (for the rotation) of a sequence's slot 0: the length of a prefix that lies elsewhere */
+} limn_b200_paged;
+
+/* Which columns turn together: j and j + rotated / 2, or 2 j and 2 j + 1. */
+enum limn_b200_pairing {
+  LIMN_B200_HALVES = 0,
+  LIMN_B200_NEIGHBOURS = 1
+};
+
+/* Put the step's keys and values into their slots, turned to their positions, and turn the queries beside them.
+ *   q (tokens, heads, hd) -> q_out, or both NULL; k (tokens, kv_heads, hd), v (tokens, kv_heads, hd_v) into the cache.
+ *   strides: (token, head) pairs of q, q_out, k, v (4 pairs; those of absent operands are not read). q_out may be q.
+ *   The first `rotated` columns of a row (a multiple of 8, 0 to hd) turn: pair j of a token at position p = first_position + slot
+ *   by the angle p * frequencies[j], (x, y) -> (x cos - y sin, x sin + y cos); frequencies is a device array of rotated / 2
+ *   doubles (NULL where rotated is 0). The angle is reduced in float64, the turn is float32, rounded once.
+ *   Two new tokens of the batch must not share a slot. */
+int limn_b200_kv_append(const limn_b200_paged* step, const void* q, const void* k, const void* v, void* q_out,
+                        const long long* strides, const double* frequencies, int rotated, int pairing, void* stream);
+
+/* Attention of the step's tokens over their sequences' pages (what limn_b200_kv_append has put there included).
+ *   q (tokens, heads, hd), out (tokens, heads, hd_v), lse (tokens, heads) float32, dense; strides: (token, head) pairs of q, out.
+ *   causal: token i sees the keys up to its own; otherwise all of its sequence's. A row that sees no key gets NaN and
+ *   lse = -inf. Keys and values that a row does not see but another row of its sequence in this step does count as 0 * v in its sum, as
+ *   everywhere in 16 bits here: an infinity among them gives NaN. Empty slots may hold anything.
+ *   workspace: device memory of limn_b200_sdpa_paged_workspace bytes, 16-byte aligned, contents of no concern before
+ *   and after the call; calls that can overlap on the GPU need one each. */
+int limn_b200_sdpa_paged(const limn_b200_paged* step, const void* q, void* out, float* lse, const long long* strides,
+                         int causal, double scale, void* workspace, unsigned long long workspace_bytes, void* stream);
+
+/* The same for a batch whose sequences all continue one prefix: every row sees the prefix_len keys of the pages prefix_table
+ * names (device array, ceil(prefix_len / page_size) entries) and behind them its sequence's own as above. The prefix is
+ * read once for the whole batch. Keys in a sequence's own pages are counted from the prefix's end: kv_lens, q_start and page_table do not
+ * include it, first_position does. */
+int limn_b200_sdpa_paged_prefix(const limn_b200_paged* step, const void* q, void* out, float* lse, const long long* strides,
+                                const int* prefix_table, int prefix_len, int causal, double scale,
+                                void* workspace, unsigned long long workspace_bytes, void* stream);
+
+/* Bytes of workspace a call for this step needs on the current device, whatever the device arrays hold; prefix_len 0 for
+ * limn_b200_sdpa_paged. Pointers in *step are not looked at. */
+int limn_b200_sdpa_paged_workspace(const limn_b200_paged* step, int prefix_len, unsigned long long* bytes);
+
 /* Which path the dispatcher picks for a problem (a limn_b200_path value), or -1 with an
  * error message if the arguments are invalid. Launches nothing. */
 int limn_b200_sdpa_path(int dtype, long long bh, int t_q, int t_k, int hd, int hd_v,

@@ -25,6 +25,19 @@ _LAYOUT_SHAPE = (c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, 
 LAYOUT_CODES = {"bhtd": 0, "bthd": 1}
 # strides, dtype, batch, heads, t_q, t_k, hd, hd_v, causal, scale, stream
 _STRIDED_SHAPE = (POINTER(c_longlong), c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_double, _P)
+
+
+class Paged(ctypes.Structure):
+    """struct limn_b200_paged of the header."""
+
+    _fields_ = [("k_cache", _P), ("v_cache", _P), ("page_table", _P), ("q_start", _P), ("kv_lens", _P), ("errors", _P),
+                ("k_strides", c_longlong * 3), ("v_strides", c_longlong * 3),
+                *((name, c_int) for name in ("dtype", "batch", "heads", "kv_heads", "hd", "hd_v", "page_size", "pages", "max_pages",
+                                             "tokens", "max_t_q", "first_position"))]
+
+
+PAIRING_CODES = {"halves": 0, "neighbours": 1}
+_STEP, _STRIDES = POINTER(Paged), POINTER(c_longlong)
 SIGNATURES = {
     "limn_b200_sdpa_fwd": (c_int, (_P, _P, _P, _P, _P, _P) + _SHAPE),
     "limn_b200_sdpa_bwd_q": (c_int, (_P, _P, _P, _P, _P, _P, _P, _P) + _SHAPE),
@@ -40,6 +53,10 @@ SIGNATURES = {
     "limn_b200_sdpa_bwd_q_fused_strided": (c_int, (_P, _P, _P, _P, _P, _P, _P, _P, _P) + _STRIDED_SHAPE),
     "limn_b200_sdpa_bwd_kv_strided": (c_int, (_P, _P, _P, _P, _P, _P, _P, _P, _P) + _STRIDED_SHAPE),
     "limn_b200_sdpa_delta_layout": (c_int, (_P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P)),
+    "limn_b200_kv_append": (c_int, (_STEP, _P, _P, _P, _P, _STRIDES, _P, c_int, c_int, _P)),
+    "limn_b200_sdpa_paged": (c_int, (_STEP, _P, _P, _P, _STRIDES, c_int, c_double, _P, c_ulonglong, _P)),
+    "limn_b200_sdpa_paged_prefix": (c_int, (_STEP, _P, _P, _P, _STRIDES, _P, c_int, c_int, c_double, _P, c_ulonglong, _P)),
+    "limn_b200_sdpa_paged_workspace": (c_int, (_STEP, c_int, POINTER(c_ulonglong))),
     "limn_b200_sdpa_path": (c_int, (c_int, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_double)),
     "limn_b200_last_launch_count": (c_int, ()),
     "limn_b200_last_error": (c_char_p, ()),

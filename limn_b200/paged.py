@@ -1,0 +1,110 @@
+"""A paged key and value cache: new tokens into it, attention over it, attention behind a prefix that a batch shares.
+
+    cache = PagedCache(k_pages, v_pages, dtype="bfloat16", pages=4096, page_size=16, kv_heads=8, hd=128)
+    step = PagedBatch(cache, heads=32, batch=64, tokens=64, max_t_q=1, max_pages=512,
+                      page_table=table, q_start=offsets, kv_lens=lengths)
+    step.append(k, v, q=q, q_out=q, frequencies=freqs, rotated=128)
+    step.attention(q, out, lse)
+
+The binding of limn_b200_kv_append, limn_b200_sdpa_paged and limn_b200_sdpa_paged_prefix (include/limn_b200.h, which says
+what each does with which extents). Every operand is device memory of the current device: an address, or an object
+that carries one as `.ptr` (limn's buffers, limn_b200.runtime.DeviceBuffer) or `data_ptr()`. Offsets, lengths and tables are
+int32 and are read on the device by each call, so one PagedBatch serves step after step, and its captured calls follow what
+the arrays hold when they are replayed. Calls launch on `stream` (None: the legacy default stream), do not synchronise and
+allocate nothing; a PagedBatch allocates its workspace when it is made, unless it is given one. Calls of one PagedBatch
+that can overlap on the GPU would share that workspace: give each stream a PagedBatch of its own.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+from typing import Any
+
+from limn_b200._lib import DTYPE_CODES, PAIRING_CODES, Paged, check, lib
+from limn_b200.registry import _note_launch
+from limn_b200.runtime import DeviceBuffer
+
+
+def _address(operand: Any) -> int | None:
+    if operand is None or isinstance(operand, int):
+        return operand
+    ptr = getattr(operand, "ptr", None)
+    return operand.data_ptr() if ptr is None else ptr
+
+
+@functools.lru_cache(maxsize=256)
+def _packed(strides: tuple[int, ...]):
+    return (ctypes.c_longlong * len(strides))(*strides)
+
+
+class PagedCache:
+    """The pages of one layer's keys and values. Strides are (page, head, slot) in elements; without them the pages are
+    dense, (pages, page_size, kv_heads, width)."""
+
+    def __init__(self, k: Any, v: Any, *, dtype: str, pages: int, page_size: int, kv_heads: int, hd: int, hd_v: int | None = None,
+                 k_strides=None, v_strides=None):
+        if dtype not in DTYPE_CODES:
+            raise NotImplementedError(f"limn_b200: a paged cache has no kernel for dtype {dtype}")
+        self.k, self.v = k, v
+        self.dtype = DTYPE_CODES[dtype]
+        self.pages, self.page_size, self.kv_heads = pages, page_size, kv_heads
+        self.hd, self.hd_v = hd, hd if hd_v is None else hd_v
+        self.k_strides = tuple(k_strides or (page_size * kv_heads * self.hd, self.hd, kv_heads * self.hd))
+        self.v_strides = tuple(v_strides or (page_size * kv_heads * self.hd_v, self.hd_v, kv_heads * self.hd_v))
+
+
+class PagedBatch:
+    """A batch of sequences over a cache. `errors` is a device word that collects LIMN_B200_PAGED_BAD_* bits (the caller zeroes
+    and reads it); `max_prefix` the longest shared prefix attention_with_prefix will be asked for. `workspace` is device
+    memory of `workspace_bytes`; without one the batch allocates its own."""
+
+    def __init__(self, cache: PagedCache, *, heads: int, batch: int, tokens: int, max_t_q: int, page_table: Any, max_pages: int,
+                 q_start: Any, kv_lens: Any, first_position: int = 0, errors: Any = None, max_prefix: int = 1, workspace: Any = None):
+        # the objects stay referenced as long as the step may read their memory
+        self._held = (cache, page_table, q_start, kv_lens, errors)
+        self._step = Paged(_address(cache.k), _address(cache.v), _address(page_table), _address(q_start), _address(kv_lens), _address(errors),
+                           (ctypes.c_longlong * 3)(*cache.k_strides), (ctypes.c_longlong * 3)(*cache.v_strides), cache.dtype, batch, heads,
+                           cache.kv_heads, cache.hd, cache.hd_v, cache.page_size, cache.pages, max_pages, tokens, max_t_q, first_position)
+        self._by_ref = ctypes.byref(self._step)
+        self.heads, self.kv_heads, self.hd, self.hd_v = heads, cache.kv_heads, cache.hd, cache.hd_v
+        need = ctypes.c_ulonglong()
+        check(lib().limn_b200_sdpa_paged_workspace(self._by_ref, max_prefix, ctypes.byref(need)), "sizing the workspace of a paged batch")
+        self.workspace_bytes = need.value
+        if workspace is None and need.value:
+            workspace = DeviceBuffer(need.value)
+        self._workspace = workspace
+        self._workspace_at = _address(workspace)
+
+    def append(self, k: Any, v: Any, *, q: Any = None, q_out: Any = None, k_strides=None, v_strides=None, q_strides=None, q_out_strides=None,
+               frequencies: Any = None, rotated: int = 0, pairing: str = "halves", stream: Any = None) -> None:
+        """Keys and values of the step's tokens into their slots, turned to their positions; q turned into q_out beside them.
+        Strides are (token, head) in elements; without them an operand is dense, (tokens, heads, width)."""
+        if pairing not in PAIRING_CODES:
+            raise ValueError(f"limn_b200: kv_append knows the pairings {sorted(PAIRING_CODES)}, not {pairing!r}")
+        hd, hd_v = self.hd, self.hd_v
+        strides = _packed((*(q_strides or (self.heads * hd, hd)), *(q_out_strides or (self.heads * hd, hd)),
+                           *(k_strides or (self.kv_heads * hd, hd)), *(v_strides or (self.kv_heads * hd_v, hd_v))))
+        check(lib().limn_b200_kv_append(self._by_ref, _address(q), _address(k), _address(v), _address(q_out), strides, _address(frequencies),
+                                        rotated, PAIRING_CODES[pairing], getattr(stream, "handle", stream)), "launching kv_append")
+
+    def attention(self, q: Any, out: Any, lse: Any, *, q_strides=None, out_strides=None, causal: bool = True, scale: float | None = None,
+                  stream: Any = None) -> None:
+        """out = softmax(q k^T scale) v over each sequence's pages, lse its row statistic (tokens, heads) in float32. `scale`
+        is hd ** -0.5 unless it is given."""
+        check(lib().limn_b200_sdpa_paged(self._by_ref, _address(q), _address(out), _address(lse), self._strides(q_strides, out_strides), int(causal),
+                                         self.hd**-0.5 if scale is None else scale, self._workspace_at, self.workspace_bytes,
+                                         getattr(stream, "handle", stream)), "launching sdpa_paged")
+        _note_launch()
+
+    def attention_with_prefix(self, q: Any, out: Any, lse: Any, *, prefix_table: Any, prefix_len: int, q_strides=None, out_strides=None,
+                              causal: bool = True, scale: float | None = None, stream: Any = None) -> None:
+        """The same with prefix_len keys of the pages prefix_table names in front of every sequence's own."""
+        check(lib().limn_b200_sdpa_paged_prefix(self._by_ref, _address(q), _address(out), _address(lse), self._strides(q_strides, out_strides),
+                                                _address(prefix_table), prefix_len, int(causal), self.hd**-0.5 if scale is None else scale,
+                                                self._workspace_at, self.workspace_bytes, getattr(stream, "handle", stream)),
+              "launching sdpa_paged_prefix")
+        _note_launch()
+
+    def _strides(self, q_strides, out_strides):
+        return _packed((*(q_strides or (self.heads * self.hd, self.hd)), *(out_strides or (self.heads * self.hd_v, self.hd_v))))
