@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
         if (e.keys < e.n) {  // more tokens than keys: there is no slot for the first of them
           if (lane == 0 && prm.errors != nullptr) atomicOr(prm.errors, LIMN_B200_PAGED_BAD_SEQUENCE);
         } else {
-          page = page_at(prm.table + static_cast<long long>(low) * prm.max_pages, slot / prm.page_size, prm.pages, prm.errors);
+          page = checked_page(prm.table[static_cast<long long>(low) * prm.max_pages + slot / prm.page_size], prm.pages, prm.errors);
         }
       }
     }

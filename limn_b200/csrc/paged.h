@@ -1,5 +1,5 @@
 // What the kernels over a paged key and value cache share: the step as they take it, how a sequence's extents are read and checked
-// on the device, and how a page is found.
+// on the device, how a page is found, how work is cut into equal shares, and where rows and parts of rows go.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -15,6 +15,34 @@ struct Pages {
   long long page = 0, head = 0, slot = 0;
 };
 
+// One worker's share of the work may begin and end inside a problem. What it has of a problem that others share is a part: the sums
+// O (unnormalised) and the statistics m (the score the weights are measured against, raw units) and l of its rows. A worker has
+// room for two parts, 2 w: of a problem that began with a worker before, 2 w + 1: of one that begins here and goes on. The worker where
+// a problem begins says in heads[w] which rows the parts are of and how many workers follow; 0 followers: nothing to join.
+struct Head {
+  int followers;
+  int first, n;   // the sequence's first token, and tokens
+  int kv_head;
+  int row0;       // the tile's first row, rows being (token, head of the group)
+};
+struct Parts {
+  float* o = nullptr;      // (2 workers, rows, width)
+  float2* ml = nullptr;    // (2 workers, rows)
+  Head* heads = nullptr;   // (workers)
+  int workers = 0, rows = 0, width = 0;
+  __host__ __device__ static size_t o_bytes(int workers, int rows, int width) { return static_cast<size_t>(2) * workers * rows * width * 4; }
+  __host__ __device__ static size_t ml_bytes(int workers, int rows) { return static_cast<size_t>(2) * workers * rows * 8; }
+  __host__ __device__ static size_t head_bytes(int workers) { return (static_cast<size_t>(workers) * sizeof(Head) + 255) / 256 * 256; }
+  __host__ static size_t bytes(int workers, int rows, int width) { return o_bytes(workers, rows, width) + ml_bytes(workers, rows) + head_bytes(workers); }
+};
+
+// Sums and statistics of every (token, head) row over some of its keys, in memory: what a pass over a shared prefix leaves and the
+// pass over the sequences' own keys joins to its own.
+struct RowSums {
+  float* o = nullptr;    // (tokens * heads, width), unnormalised
+  float2* ml = nullptr;  // (tokens * heads)
+};
+
 // A pass of queries over paged keys.
 struct Pass {
   const unsigned char* q = nullptr;
@@ -23,16 +51,18 @@ struct Pass {
   long long q_token = 0, q_head = 0, o_token = 0, o_head = 0;  // bytes
   Pages k, v;
   const int* table = nullptr;    // (batch, max_pages)
-  const int* q_start = nullptr;  // (batch + 1)
-  const int* kv_lens = nullptr;  // (batch)
+  const int* q_start = nullptr;  // (batch + 1); null: one sequence of all tokens
+  const int* kv_lens = nullptr;  // (batch); null with q_start: `keys` of them
   unsigned* errors = nullptr;
-  const int* prefix_table = nullptr;
-  int prefix_len = 0;
+  int keys = 0;
   int batch = 0, heads = 0, kv_heads = 0, group = 1;  // group: query heads to a key head
   int pieces = 0, pieces_v = 0;                       // groups of 8 columns of a row of Q and K, of V and O
   int page_size = 0, pages = 0, max_pages = 0, tokens = 0, max_t_q = 0;
   int causal = 0;
   float scale = 0.f;
+  Parts parts;
+  RowSums leave;  // where rows go instead of `out`, or null
+  RowSums join;   // what rows are joined with on their way out, or null
 };
 
 // A sequence's extents: `first` token of `n`, `keys` in its pages. One that cannot be has n = 0 and is noted.
@@ -46,6 +76,10 @@ __device__ __forceinline__ Extent extent_of(const int* q_start, const int* kv_le
     return Extent{0, 0, 0};
   }
   return Extent{static_cast<int>(first), static_cast<int>(end - first), static_cast<int>(keys)};
+}
+__device__ __forceinline__ Extent extent_of(const Pass& p, int b) {
+  if (p.q_start == nullptr) return Extent{0, p.tokens, p.keys};
+  return extent_of(p.q_start, p.kv_lens, b, p.tokens, p.max_t_q, p.max_pages, p.page_size, p.errors);
 }
 
 // The sequence whose tokens `token` is among: how many sequences end at or before it (batch: none of them goes on past it). A warp's
@@ -68,12 +102,23 @@ __device__ __forceinline__ int sequence_of(const int* q_start, int batch, int to
   return low;
 }
 
-// The page that `table` has at `at`, or -1 where it is none.
-__device__ __forceinline__ int page_at(const int* table, int at, int pages, unsigned* errors) {
-  const int page = table[at];
+// `page` as the table has it, or -1 where it is none.
+__device__ __forceinline__ int checked_page(int page, int pages, unsigned* errors) {
   if (page >= 0 && page < pages) return page;
   if (errors != nullptr) atomicOr(errors, LIMN_B200_PAGED_BAD_PAGE);
   return -1;
+}
+
+// Where row r of a sequence's (token, head of the group) rows has its result and its statistics.
+struct RowPlace {
+  long long row;      // token * heads + head
+  unsigned char* out;
+};
+__device__ __forceinline__ RowPlace row_place(const Pass& p, int first, int kv_head, int r) {
+  const int i = r / p.group, g = r - i * p.group;
+  const long long token = first + i;
+  const int head = kv_head * p.group + g;
+  return RowPlace{token * p.heads + head, p.out + token * p.o_token + head * p.o_head};
 }
 
 }  // namespace paged
@@ -81,5 +126,11 @@ __device__ __forceinline__ int page_at(const int* table, int at, int pages, unsi
 // Checks of a step that every entry point makes, of its extents and strides and of its pointers; `name` is the op's.
 int check_paged(const char* name, const limn_b200_paged* step);
 int check_paged_pointers(const char* name, const limn_b200_paged* step);
+
+// The kernels that make a pass (each puts a second one behind itself that joins the parts): few rows to a key head, and any number.
+constexpr int kPagedFewRows = 16;  // max_t_q * group up to here
+size_t paged_few_workspace(int rows, int width, int sms);
+int paged_few_launch(const paged::Pass& pass, bool fp16, int rows, void* workspace, cudaStream_t stream);
+int paged_join_launch(const paged::Pass& pass, bool fp16, cudaStream_t stream);
 
 }  // namespace limn_b200

@@ -18,9 +18,9 @@ __global__ void __launch_bounds__(128) sdpa_paged_row_kernel(const Pass prm) {
   const long long row = blockIdx.x * 4LL + (threadIdx.x >> 5);
   if (row >= static_cast<long long>(prm.tokens) * prm.heads) return;
   const int token = static_cast<int>(row / prm.heads), head = static_cast<int>(row - static_cast<long long>(token) * prm.heads), kv_head = head / prm.group;
-  const int b = sequence_of(prm.q_start, prm.batch, token, lane);
+  const int b = prm.q_start == nullptr ? 0 : sequence_of(prm.q_start, prm.batch, token, lane);
   if (b >= prm.batch) return;
-  const Extent e = extent_of(prm.q_start, prm.kv_lens, b, prm.tokens, prm.max_t_q, prm.max_pages, prm.page_size, prm.errors);
+  const Extent e = extent_of(prm, b);
   if (token < e.first || token - e.first >= e.n) return;
   const int own = prm.causal ? max(0, e.keys - e.n + (token - e.first) + 1) : e.keys;
   auto load4 = [&](const unsigned char* at, int pieces, float (&x)[4]) {
@@ -36,41 +36,74 @@ __global__ void __launch_bounds__(128) sdpa_paged_row_kernel(const Pass prm) {
   };
   float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
   load4(prm.q + token * prm.q_token + head * prm.q_head, prm.pieces, q);
-  auto walk = [&](const int* table, int keys) {
-    for (int j = 0; j < keys; ++j) {
-      const int page = page_at(table, j / prm.page_size, prm.pages, prm.errors), slot = j % prm.page_size;
-      float s = NAN, v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (page >= 0) {
-        float k[4];
-        load4(prm.k.base + page * prm.k.page + kv_head * prm.k.head + slot * prm.k.slot, prm.pieces, k);
-        load4(prm.v.base + page * prm.v.page + kv_head * prm.v.head + slot * prm.v.slot, prm.pieces_v, v);
-        s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+  const int* table = prm.table + static_cast<long long>(b) * prm.max_pages;
+  for (int j = 0; j < own; ++j) {
+    const int page = checked_page(table[j / prm.page_size], prm.pages, prm.errors), slot = j % prm.page_size;
+    float s = NAN, v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (page >= 0) {
+      float k[4];
+      load4(prm.k.base + page * prm.k.page + kv_head * prm.k.head + slot * prm.k.slot, prm.pieces, k);
+      load4(prm.v.base + page * prm.v.page + kv_head * prm.v.head + slot * prm.v.slot, prm.pieces_v, v);
+      s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
 #pragma unroll
-        for (int step = 16; step > 0; step >>= 1) s += __shfl_xor_sync(0xffffffffu, s, step);
-        s *= prm.scale;
-      }
-      const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, alpha = expf(m - base), p = expf(s - base);
-      m = top, l = l * alpha + p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * alpha + p * v[i];
+      for (int step = 16; step > 0; step >>= 1) s += __shfl_xor_sync(0xffffffffu, s, step);
     }
-  };
-  walk(prm.prefix_table, prm.prefix_len);
-  walk(prm.table + static_cast<long long>(b) * prm.max_pages, own);
+    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, alpha = expf((m - base) * prm.scale), p = expf((s - base) * prm.scale);
+    m = top, l = l * alpha + p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * alpha + p * v[i];
+  }
+  const int width = prm.pieces <= 8 && prm.pieces_v <= 8 ? 64 : 128;
+  if (prm.leave.o != nullptr) {
+    if (4 * lane < width) *reinterpret_cast<float4*>(prm.leave.o + row * width + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (lane == 0) prm.leave.ml[row] = make_float2(m, l);
+    return;
+  }
+  if (prm.join.o != nullptr) {
+    const float2 ml = prm.join.ml[row];
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (4 * lane < width) o = *reinterpret_cast<const float4*>(prm.join.o + row * width + 4 * lane);
+    const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top, keep = expf((m - base) * prm.scale), add = expf((ml.x - base) * prm.scale);
+    m = top, l = l * keep + ml.y * add;
+    acc[0] = acc[0] * keep + o.x * add, acc[1] = acc[1] * keep + o.y * add, acc[2] = acc[2] * keep + o.z * add, acc[3] = acc[3] * keep + o.w * add;
+  }
   if (lane < 2 * prm.pieces_v) {
     const float a = acc[0] / l, c = acc[1] / l, d = acc[2] / l, f = acc[3] / l;
     *reinterpret_cast<uint2*>(prm.out + token * prm.o_token + head * prm.o_head + 8 * lane) =
         kFp16 ? make_uint2(ptx::pack_f16(a, c), ptx::pack_f16(d, f)) : make_uint2(ptx::pack_bf16(a, c), ptx::pack_bf16(d, f));
   }
-  if (lane == 0) prm.lse[row] = m + logf(l);
+  if (lane == 0) prm.lse[row] = m * prm.scale + logf(l);
 }
 
-int launch_rows(const Pass& prm, int dtype, cudaStream_t stream) {
+int launch_rows(const Pass& prm, bool fp16, cudaStream_t stream) {
   const long long blocks = (static_cast<long long>(prm.tokens) * prm.heads + 3) / 4;
   if (blocks > 0x7fffffffLL) return fail(LIMN_B200_UNSUPPORTED, "sdpa_paged: %d tokens of %d heads need more blocks than one grid holds", prm.tokens, prm.heads);
-  auto kernel = dtype == LIMN_B200_F16 ? sdpa_paged_row_kernel<true> : sdpa_paged_row_kernel<false>;
+  auto kernel = fp16 ? sdpa_paged_row_kernel<true> : sdpa_paged_row_kernel<false>;
   LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, stream, prm), "launching the paged sdpa kernel");
   note_launches(1);
+  return LIMN_B200_OK;
+}
+
+// Which kernel a pass of at most `rows` rows to a (sequence, key head) takes, and the workspace it has to itself.
+size_t pass_workspace(long long rows, int width, int sms) { return rows <= kPagedFewRows ? paged_few_workspace(static_cast<int>(rows), width, sms) : 0; }
+int launch_pass(const Pass& pass, bool fp16, long long rows, void* workspace, cudaStream_t stream) {
+  return rows <= kPagedFewRows ? paged_few_launch(pass, fp16, static_cast<int>(rows), workspace, stream) : launch_rows(pass, fp16, stream);
+}
+
+// The workspace of a call: the parts of whichever pass has more, and behind them the rows' sums over the prefix.
+struct Workspace {
+  size_t parts, sums, stats;
+  size_t bytes() const { return parts + sums + stats; }
+};
+int workspace_of(const limn_b200_paged* step, int prefix_len, Workspace* w) {
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const int width = step->hd <= 64 && step->hd_v <= 64 ? 64 : 128;
+  const long long group = step->heads / step->kv_heads;
+  const size_t own = pass_workspace(step->max_t_q * group, width, sms), front = prefix_len > 0 ? pass_workspace(step->tokens * group, width, sms) : 0;
+  w->parts = ((own > front ? own : front) + 255) / 256 * 256;
+  const size_t rows = static_cast<size_t>(step->tokens) * step->heads;
+  w->sums = prefix_len > 0 ? rows * width * 4 : 0, w->stats = prefix_len > 0 ? rows * 8 : 0;
   return LIMN_B200_OK;
 }
 
@@ -86,22 +119,34 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   for (int i = 0; i < 4; ++i)
     if (strides[i] < 0 || (strides[i] & 7)) return fail(LIMN_B200_BAD_ARGUMENT, "%s: strides must be non-negative multiples of 8 elements, got %lld", name, strides[i]);
   if (!(scale > 0.0) || scale > 1e30) return fail(LIMN_B200_UNSUPPORTED, "%s: the scale must be positive and finite", name);
-  unsigned long long need = 0;
-  if (int rc = limn_b200_sdpa_paged_workspace(step, prefix_len, &need)) return rc;
-  if (need > 0 && (!workspace || workspace_bytes < need)) return fail(LIMN_B200_BAD_ARGUMENT, "%s: the workspace has %llu bytes, %llu are needed", name, workspace_bytes, need);
   if (step->tokens == 0 || step->batch == 0) return LIMN_B200_OK;
+  Workspace w;
+  if (int rc = workspace_of(step, prefix_len, &w)) return rc;
+  if (w.bytes() > 0 && (!workspace || workspace_bytes < w.bytes()))
+    return fail(LIMN_B200_BAD_ARGUMENT, "%s: the workspace has %llu bytes, %llu are needed", name, workspace_bytes, static_cast<unsigned long long>(w.bytes()));
   Pass prm;
   prm.q = static_cast<const unsigned char*>(q), prm.out = static_cast<unsigned char*>(out), prm.lse = lse;
   prm.q_token = 2 * strides[0], prm.q_head = 2 * strides[1], prm.o_token = 2 * strides[2], prm.o_head = 2 * strides[3];
   prm.k = {static_cast<unsigned char*>(step->k_cache), 2 * step->k_strides[0], 2 * step->k_strides[1], 2 * step->k_strides[2]};
   prm.v = {static_cast<unsigned char*>(step->v_cache), 2 * step->v_strides[0], 2 * step->v_strides[1], 2 * step->v_strides[2]};
   prm.table = step->page_table, prm.q_start = step->q_start, prm.kv_lens = step->kv_lens, prm.errors = step->errors;
-  prm.prefix_table = prefix_table, prm.prefix_len = prefix_len;
   prm.batch = step->batch, prm.heads = step->heads, prm.kv_heads = step->kv_heads, prm.group = step->heads / step->kv_heads;
   prm.pieces = step->hd / 8, prm.pieces_v = step->hd_v / 8;
   prm.page_size = step->page_size, prm.pages = step->pages, prm.max_pages = step->max_pages, prm.tokens = step->tokens, prm.max_t_q = step->max_t_q;
   prm.causal = causal != 0, prm.scale = static_cast<float>(scale);
-  return launch_rows(prm, step->dtype, static_cast<cudaStream_t>(stream));
+  const bool fp16 = step->dtype == LIMN_B200_F16;
+  const cudaStream_t on = static_cast<cudaStream_t>(stream);
+  if (prefix_len > 0) {
+    // every row over the prefix, as one sequence of all tokens that sees all of it; tokens that belong to no sequence get sums
+    // too, which nothing reads
+    Pass front = prm;
+    front.table = prefix_table, front.q_start = nullptr, front.kv_lens = nullptr, front.keys = prefix_len, front.batch = 1, front.causal = 0;
+    front.leave.o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + w.parts);
+    front.leave.ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + w.parts + w.sums);
+    if (int rc = launch_pass(front, fp16, static_cast<long long>(step->tokens) * prm.group, workspace, on)) return rc;
+    prm.join = front.leave;
+  }
+  return launch_pass(prm, fp16, static_cast<long long>(step->max_t_q) * prm.group, workspace, on);
 }
 
 }  // namespace
@@ -144,7 +189,9 @@ int limn_b200_sdpa_paged_workspace(const limn_b200_paged* step, int prefix_len, 
   if (int rc = check_paged("sdpa_paged_workspace", step)) return rc;
   if (!bytes) return fail(LIMN_B200_BAD_ARGUMENT, "sdpa_paged_workspace: null result pointer");
   if (prefix_len < 0) return fail(LIMN_B200_BAD_ARGUMENT, "sdpa_paged_workspace: the prefix has %d keys", prefix_len);
-  *bytes = 0;
+  Workspace w;
+  if (int rc = workspace_of(step, prefix_len, &w)) return rc;
+  *bytes = w.bytes();
   return LIMN_B200_OK;
 }
 

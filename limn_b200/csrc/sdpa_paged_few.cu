@@ -1,0 +1,522 @@
+// Attention over paged keys for few query rows to a key head (a new token, or a few, times the query heads that share the key head: up
+// to 16): generation from a cache. K and V are read once, and that is the time it takes; the arithmetic has to stay out of the way.
+//
+// Work is cut into equal shares, whatever the sequences' lengths: the unit is 16 keys of one (sequence, key head), every warp of the
+// grid takes the same number of consecutive units, and what it has of a problem that its neighbours share goes into its parts
+// (paged.h), joined by a kernel behind this one. A warp works alone: it copies its units' rows into its own ring in shared memory with
+// 16-byte asynchronous copies, so that bytes are in flight all the time and nothing waits for other warps.
+//
+// Per unit, with mma.sync m16n8k16 and the keys as M so that 8 query rows are enough for a tile:
+//   S^T (16 keys x rows) = K Q^T            A = K by ldmatrix, B = Q, in registers
+//   P^T = exp2(S^T - m) as 16-bit           the accumulator's layout turned into B's by movmatrix
+//   O^T (columns x rows) += V^T P^T         A = V by ldmatrix.trans
+// Tensor-memory MMAs have nothing to add here: their 128 rows would hold 1 to 16, and the tensor pipe is idle most of the time.
+// m moves only when a row's maximum has outgrown it by 8 in log2 units (weights then reach 2^8, which 16 bits hold), as in
+// the tensor-core forward; l is summed from the weights before they are rounded.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged.h"
+#include "sm100_ptx.cuh"
+
+namespace limn_b200 {
+namespace {
+
+using namespace paged;
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kUnit = 16;  // keys
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+template <bool kFp16>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (kFp16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes global -> shared; `there` false: zeros, and `from` is not read
+__device__ __forceinline__ void copy16(uint32_t to, const unsigned char* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int D>
+struct Ring {
+  static constexpr int kSide = kUnit * D * 2;  // K or V of a unit
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kWarpBytes = kStages * 2 * kSide;
+  static constexpr int kBytes = kWarps * kWarpBytes;  // 192 KB
+};
+
+// Where a warp is in the work: unit `unit` of `units` of problem (b, kv_head).
+struct Cursor {
+  int b, kv_head, unit, units;
+  Extent e;
+};
+__device__ __forceinline__ int units_of(const Extent& e) { return e.n == 0 ? 0 : max(1, (e.keys + kUnit - 1) / kUnit); }
+__device__ __forceinline__ void next_problem(const Pass& prm, Cursor& c) {
+  c.unit = 0;
+  if (++c.kv_head < prm.kv_heads) return;
+  c.kv_head = 0, c.units = 0;
+  while (c.units == 0 && ++c.b < prm.batch) c.e = extent_of(prm, c.b), c.units = units_of(c.e);
+}
+
+template <int D, bool kFp16, int NT>
+__global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass prm, const int least) {
+  using R = Ring<D>;
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ long long share_end[kThreads];  // units of the sequences up to and with a thread's, per key head
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float sl2 = prm.scale * kLog2e;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+
+  // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
+  const int run = (prm.batch + kThreads - 1) / kThreads;
+  {
+    long long mine = 0;
+    for (int i = 0; i < run; ++i) {
+      const int b = threadIdx.x * run + i;
+      if (b < prm.batch) mine += units_of(extent_of(prm, b));
+    }
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += other;
+    }
+    __shared__ long long warp_sum[kWarps];
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += warp_sum[w];
+    share_end[threadIdx.x] = upto;
+    __syncthreads();
+  }
+  const int worker = blockIdx.x * kWarps + warp;
+  const long long total = share_end[kThreads - 1] * prm.kv_heads;
+  long long share = (total + prm.parts.workers - 1) / prm.parts.workers;
+  if (share < least) share = least;
+  const long long from = worker * share, to = min(total, from + share);
+  if (lane == 0) prm.parts.heads[worker].followers = 0;
+  if (from >= to) return;
+
+  Cursor at;
+  {
+    // the run of sequences that `from` falls into: how many threads' sums end at or before it
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) before += __popc(__ballot_sync(0xffffffffu, share_end[i * 32 + lane] * prm.kv_heads <= from));
+    long long rest = from - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
+    at.b = before * run - 1;
+    do {
+      ++at.b;
+      at.e = extent_of(prm, at.b);
+      at.units = units_of(at.e);
+      if (rest < static_cast<long long>(at.units) * prm.kv_heads) break;
+      rest -= static_cast<long long>(at.units) * prm.kv_heads;
+    } while (at.b + 1 < prm.batch);
+    at.kv_head = static_cast<int>(rest / at.units);
+    at.unit = static_cast<int>(rest - static_cast<long long>(at.kv_head) * at.units);
+  }
+  const int steps = static_cast<int>(to - from);
+
+  // ---- copies: run ahead of the arithmetic with a cursor of their own ----
+  Cursor ahead = at;
+  int loaded = 0;
+  const uint32_t mine = ptx::smem_addr(ring) + warp * R::kWarpBytes;
+  constexpr int kLanes = D / 8;         // lanes to a row of 16-byte pieces
+  constexpr int kRows = 32 / kLanes;    // rows a copy of the warp takes
+  const int piece = lane % kLanes, row_in = lane / kLanes;
+  // A lane keeps the page of one of 32 groups of 8 keys (no page ends inside one), 16 units, and the table's entry for the 16 units behind.
+  int block = -1, page = -1, entry_next = -1;
+  unsigned none = 0;  // two bits for each place of the ring: which 8 of its unit's keys have a page that is none
+  auto entry_of = [&](const Cursor& c, int blk) {
+    const int key = (blk * 32 + lane) * 8;
+    return key < c.e.keys ? prm.table[static_cast<long long>(c.b) * prm.max_pages + key / prm.page_size] : 0;
+  };
+  auto issue = [&]() {
+    if (loaded < steps) {
+      if (ahead.unit == ahead.units) next_problem(prm, ahead), block = -1;
+      const int blk = ahead.unit / 16;
+      if (blk != block) {
+        const int raw = block >= 0 && blk == block + 1 ? entry_next : entry_of(ahead, blk);
+        block = blk;
+        entry_next = entry_of(ahead, blk + 1);
+        page = (blk * 32 + lane) * 8 < ahead.e.keys ? checked_page(raw, prm.pages, prm.errors) : -1;
+      }
+      const int place_at = loaded % R::kStages;
+      const uint32_t k_to = mine + place_at * 2 * R::kSide, v_to = k_to + R::kSide;
+      none &= ~(3u << (2 * place_at));
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int key0 = ahead.unit * kUnit + half * 8;
+        const int p = __shfl_sync(0xffffffffu, page, (key0 / 8) & 31);
+        const int slot = key0 % prm.page_size;
+        const long long in_page = max(p, 0);
+        if (p < 0 && key0 < ahead.e.keys) none |= 1u << (2 * place_at + half);
+        const unsigned char* k_from = prm.k.base + in_page * prm.k.page + ahead.kv_head * prm.k.head + slot * prm.k.slot + 16 * (piece < prm.pieces ? piece : 0);
+        const unsigned char* v_from = prm.v.base + in_page * prm.v.page + ahead.kv_head * prm.v.head + slot * prm.v.slot + 16 * (piece < prm.pieces_v ? piece : 0);
+#pragma unroll
+        for (int i = 0; i < 8 / kRows; ++i) {
+          const int r = i * kRows + row_in;  // of the 8
+          const bool there = p >= 0 && key0 + r < ahead.e.keys;
+          const uint32_t place = (half * 8 + r) * (D * 2) + ((piece ^ r) << 4);
+          copy16(k_to + place, k_from + r * prm.k.slot, there && piece < prm.pieces);
+          copy16(v_to + place, v_from + r * prm.v.slot, there && piece < prm.pieces_v);
+        }
+      }
+      ++ahead.unit, ++loaded;
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < R::kStages - 1; ++s) issue();
+
+  // ---- arithmetic ----
+  const int kq = lane >> 2, cq = lane & 3;  // in a fragment: row (key or column of O), and pair of query rows
+  uint32_t q[NT][D / 16][2];
+  float o[NT][D / 16][4];
+  float m[NT][2], l[NT][2];
+  int limit[NT][2], least_limit = 0;
+  bool begun = at.unit == 0;
+  auto begin = [&] {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + kq;
+      const int i = r / prm.group, g = r - i * prm.group;
+      const unsigned char* row = prm.q + (static_cast<long long>(at.e.first) + i) * prm.q_token + (at.kv_head * prm.group + g) * prm.q_head;
+      const bool there = i < at.e.n;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          q[nt][kk][j] = there && kk * 2 + j < prm.pieces ? *reinterpret_cast<const uint32_t*>(row + (kk * 16 + j * 8 + cq * 2) * 2) : 0u;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int token = (nt * 8 + cq * 2 + c) / prm.group;
+        limit[nt][c] = prm.causal ? min(at.e.keys, at.e.keys - at.e.n + token + 1) : at.e.keys;
+        m[nt][c] = -INFINITY, l[nt][c] = 0.f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[nt][mt][c] = 0.f;
+    }
+    least_limit = prm.causal ? at.e.keys - at.e.n + 1 : at.e.keys;
+  };
+  begin();
+  for (int step = 0; step < steps; ++step) {
+    copies_wait<R::kStages - 2>();
+    __syncwarp();
+    issue();
+    const int place_at = step % R::kStages;
+    const uint32_t k_at = mine + place_at * 2 * R::kSide, v_at = k_at + R::kSide;
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[nt][c] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      // A: 16 keys x 16 columns; lanes 0-15 name the keys' first 8 columns' pieces, 16-31 the second's
+      uint32_t a[4];
+      const int r = lane & 15, pc = kk * 2 + (lane >> 4);
+      ldmatrix4(a, k_at + r * (D * 2) + ((pc ^ (r & 7)) << 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma<kFp16>(s[nt], a, q[nt][kk][0], q[nt][kk][1]);
+    }
+    const int key = at.unit * kUnit + kq;
+    if ((none >> (2 * place_at)) & 3u) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if ((none >> (2 * place_at + (c >> 1))) & 1u) s[nt][c] = NAN;
+    }
+    if (at.unit * kUnit + kUnit > least_limit) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (key + (c >> 1) * 8 >= limit[nt][c & 1]) s[nt][c] = -INFINITY;
+    }
+    uint32_t p[NT][2];
+    bool moved = false;
+    float alpha[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        alpha[nt][c] = 1.f;
+        if ((top - m[nt][c]) * sl2 > kSlack) {  // (true at the first score above -inf, where m is -inf)
+          alpha[nt][c] = ptx::exp2_approx((m[nt][c] - top) * sl2);
+          m[nt][c] = top, moved = true;
+        }
+        const float shift = m[nt][c] == -INFINITY ? 0.f : -m[nt][c] * sl2;
+        s[nt][c] = ptx::exp2_approx(fmaf(s[nt][c], sl2, shift));
+        s[nt][c + 2] = ptx::exp2_approx(fmaf(s[nt][c + 2], sl2, shift));
+        l[nt][c] = fmaf(l[nt][c], alpha[nt][c], s[nt][c] + s[nt][c + 2]);
+      }
+      p[nt][0] = transposed(kFp16 ? ptx::pack_f16(s[nt][0], s[nt][1]) : ptx::pack_bf16(s[nt][0], s[nt][1]));
+      p[nt][1] = transposed(kFp16 ? ptx::pack_f16(s[nt][2], s[nt][3]) : ptx::pack_bf16(s[nt][2], s[nt][3]));
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[nt][mt][c] *= alpha[nt][c & 1];
+    }
+#pragma unroll
+    for (int mt = 0; mt < D / 16; ++mt) {
+      // A: 16 columns x 16 keys out of rows of keys: (keys 0-7, columns 0-7), (keys 0-7, columns 8-15), (keys 8-15, ...)
+      uint32_t a[4];
+      const int r = (lane & 7) + ((lane >> 4) << 3), pc = mt * 2 + ((lane >> 3) & 1);
+      ldmatrix4_trans(a, v_at + r * (D * 2) + ((pc ^ (r & 7)) << 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma<kFp16>(o[nt][mt], a, p[nt][0], p[nt][1]);
+    }
+    ++at.unit;
+    const bool ends = at.unit == at.units;
+    if (!ends && step + 1 < steps) continue;
+
+    // ---- the problem, or this warp's part of it, is done ----
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
+    const bool whole = begun && ends;
+    const int part = 2 * worker + (begun ? 1 : 0);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = nt * 8 + cq * 2 + c;
+        if (r >= at.e.n * prm.group) continue;
+        if (!whole || prm.leave.o != nullptr) {
+          float* to_o = prm.parts.o + (static_cast<long long>(part) * (NT * 8) + r) * D;
+          float2* to_ml = prm.parts.ml + static_cast<long long>(part) * (NT * 8) + r;
+          if (whole) {
+            const long long row = row_place(prm, at.e.first, at.kv_head, r).row;
+            to_o = prm.leave.o + row * D, to_ml = prm.leave.ml + row;
+          }
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt) to_o[mt * 16 + kq] = o[nt][mt][c], to_o[mt * 16 + 8 + kq] = o[nt][mt][c + 2];
+          if (kq == 0) *to_ml = make_float2(m[nt][c], l[nt][c]);
+          continue;
+        }
+        const RowPlace place = row_place(prm, at.e.first, at.kv_head, r);
+        float keep = 1.f, add = 0.f, top = m[nt][c], sum = l[nt][c];
+        const float* more = nullptr;
+        if (prm.join.o != nullptr) {
+          const float2 ml = prm.join.ml[place.row];
+          more = prm.join.o + place.row * D;
+          top = fmaxf(top, ml.x);
+          const float base = top == -INFINITY ? 0.f : top;
+          keep = exp2f((m[nt][c] - base) * sl2), add = exp2f((ml.x - base) * sl2);
+          sum = sum * keep + ml.y * add;
+        }
+        const float inv = 1.f / sum;  // (no key: 0 * inf = NaN)
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (mt * 2 + half >= prm.pieces_v) continue;
+            const int column = mt * 16 + half * 8 + kq;
+            float value = o[nt][mt][c + 2 * half];
+            if (more != nullptr) value = value * keep + more[column] * add;
+            value *= inv;
+            if (kFp16) *reinterpret_cast<__half*>(place.out + 2 * column) = __float2half_rn(value);
+            else *reinterpret_cast<__nv_bfloat16*>(place.out + 2 * column) = __float2bfloat16_rn(value);
+          }
+        if (kq == 0) prm.lse[place.row] = top * prm.scale + logf(sum);
+      }
+    if (begun && !ends && lane == 0) {
+      const long long behind = at.units - at.unit;  // units of the problem that the next workers have
+      prm.parts.heads[worker] = Head{static_cast<int>((behind + share - 1) / share), at.e.first, at.e.n, at.kv_head, 0};
+    }
+    if (step + 1 < steps) {
+      next_problem(prm, at);
+      begun = true;
+      begin();
+    }
+  }
+}
+
+// ---- joining the parts ----
+constexpr int kJoinWarps = 16;
+
+// A row of one problem: kSplit warps share its parts, a lane has 4 columns (the last warps of a row with fewer than 128 columns idle).
+template <int D, bool kFp16, int kSplit>
+__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const Pass prm) {
+  constexpr int kRows = kJoinWarps / kSplit;
+  constexpr int kLanes = D / 4;            // lanes to a row
+  constexpr int kAtOnce = 32 / kLanes;     // parts a warp takes side by side
+  __shared__ float4 sums[kJoinWarps][32];
+  __shared__ float2 stats[kJoinWarps];
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * kRows + warp / kSplit, split = warp % kSplit;
+  const int column = (lane % kLanes) * 4, side = lane / kLanes;
+  const float sl2 = prm.scale * kLog2e;
+  for (int w = blockIdx.x; w < prm.parts.workers; w += gridDim.x) {
+    const Head head = prm.parts.heads[w];
+    if (head.followers == 0) continue;  // (the same in the whole block)
+    const bool there = r < prm.parts.rows && head.row0 + r < head.n * prm.group;
+    // part 0 is the head's, part i the i-th follower's
+    auto part = [&](int i) { return static_cast<long long>(i == 0 ? 2 * w + 1 : 2 * (w + i)) * prm.parts.rows + r; };
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (there) {
+      constexpr int kUnroll = 4;
+      for (int i0 = split * kAtOnce + side; i0 <= head.followers; i0 += kUnroll * kSplit * kAtOnce) {
+        float2 ml[kUnroll];
+        float4 o[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int i = i0 + u * kSplit * kAtOnce;
+          ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i <= head.followers) ml[u] = prm.parts.ml[part(i)], o[u] = *reinterpret_cast<const float4*>(prm.parts.o + part(i) * D + column);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const float top = fmaxf(m, ml[u].x), base = top == -INFINITY ? 0.f : top;
+          const float keep = exp2f((m - base) * sl2), add = exp2f((ml[u].x - base) * sl2);
+          m = top, l = l * keep + ml[u].y * add;
+          acc.x = acc.x * keep + o[u].x * add, acc.y = acc.y * keep + o[u].y * add, acc.z = acc.z * keep + o[u].z * add, acc.w = acc.w * keep + o[u].w * add;
+        }
+      }
+    }
+    auto fold = [&](float m_b, float l_b, const float4& o_b) {
+      const float top = fmaxf(m, m_b), base = top == -INFINITY ? 0.f : top;
+      const float keep = exp2f((m - base) * sl2), add = exp2f((m_b - base) * sl2);
+      m = top, l = l * keep + l_b * add;
+      acc.x = acc.x * keep + o_b.x * add, acc.y = acc.y * keep + o_b.y * add, acc.z = acc.z * keep + o_b.z * add, acc.w = acc.w * keep + o_b.w * add;
+    };
+#pragma unroll
+    for (int d = kLanes; d < 32; d <<= 1) {
+      const float4 other = make_float4(__shfl_down_sync(0xffffffffu, acc.x, d), __shfl_down_sync(0xffffffffu, acc.y, d), __shfl_down_sync(0xffffffffu, acc.z, d),
+                                       __shfl_down_sync(0xffffffffu, acc.w, d));
+      const float m_b = __shfl_down_sync(0xffffffffu, m, d), l_b = __shfl_down_sync(0xffffffffu, l, d);
+      fold(m_b, l_b, other);
+    }
+    if (kSplit > 1) {
+      __syncthreads();  // (what the last problem left has been read)
+      if (split > 0) {
+        sums[warp][lane] = acc;
+        if (lane == 0) stats[warp] = make_float2(m, l);
+      }
+      __syncthreads();
+      if (split > 0) continue;
+#pragma unroll 1
+      for (int i = 1; i < kSplit; ++i) fold(stats[warp + i].x, stats[warp + i].y, sums[warp + i][lane]);
+    }
+    if (!there || side > 0) continue;
+    const RowPlace place = row_place(prm, head.first, head.kv_head, head.row0 + r);
+    if (prm.leave.o != nullptr) {
+      *reinterpret_cast<float4*>(prm.leave.o + place.row * D + column) = acc;
+      if (lane == 0) prm.leave.ml[place.row] = make_float2(m, l);
+      continue;
+    }
+    if (prm.join.o != nullptr) {
+      const float2 ml = prm.join.ml[place.row];
+      fold(ml.x, ml.y, *reinterpret_cast<const float4*>(prm.join.o + place.row * D + column));
+    }
+    const float inv = 1.f / l;
+    if (column < prm.pieces_v * 8)
+      *reinterpret_cast<uint2*>(place.out + 2 * column) = kFp16 ? make_uint2(ptx::pack_f16(acc.x * inv, acc.y * inv), ptx::pack_f16(acc.z * inv, acc.w * inv))
+                                                                : make_uint2(ptx::pack_bf16(acc.x * inv, acc.y * inv), ptx::pack_bf16(acc.z * inv, acc.w * inv));
+    if (lane == 0) prm.lse[place.row] = m * prm.scale + logf(l);
+  }
+}
+
+template <int D, bool kFp16, int NT>
+int launch_few(const Pass& pass, cudaStream_t stream) {
+  auto kernel = sdpa_paged_few_kernel<D, kFp16, NT>;
+  static bool sized[64] = {};
+  int device = 0;
+  LIMN_CUDA(cudaGetDevice(&device), "asking for the current device");
+  if (device >= 0 && device < 64 && !sized[device]) {
+    LIMN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<D>::kBytes), "sizing shared memory for the paged sdpa kernel");
+    sized[device] = true;
+  }
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers / kWarps)), dim3(kThreads), Ring<D>::kBytes, stream, pass, 1), "launching the paged sdpa kernel");
+  note_launches(1);
+  return LIMN_B200_OK;
+}
+
+}  // namespace
+
+size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(sms * kWarps, rows <= 8 ? 8 : 16, width <= 64 ? 64 : 128); }
+
+// Lays the parts out in `memory`, which has the bytes for them.
+static void place_parts(Parts& parts, void* memory, int workers, int rows, int width) {
+  unsigned char* at = static_cast<unsigned char*>(memory);
+  parts.workers = workers, parts.rows = rows, parts.width = width;
+  parts.o = reinterpret_cast<float*>(at), at += Parts::o_bytes(workers, rows, width);
+  parts.ml = reinterpret_cast<float2*>(at), at += Parts::ml_bytes(workers, rows);
+  parts.heads = reinterpret_cast<Head*>(at);
+}
+
+int paged_few_launch(const Pass& given, bool fp16, int rows, void* workspace, cudaStream_t stream) {
+  Pass pass = given;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
+  place_parts(pass.parts, workspace, sms * kWarps, rows <= 8 ? 8 : 16, width);
+  int rc;
+  if (width == 64) {
+    if (rows <= 8) rc = fp16 ? launch_few<64, true, 1>(pass, stream) : launch_few<64, false, 1>(pass, stream);
+    else rc = fp16 ? launch_few<64, true, 2>(pass, stream) : launch_few<64, false, 2>(pass, stream);
+  } else {
+    if (rows <= 8) rc = fp16 ? launch_few<128, true, 1>(pass, stream) : launch_few<128, false, 1>(pass, stream);
+    else rc = fp16 ? launch_few<128, true, 2>(pass, stream) : launch_few<128, false, 2>(pass, stream);
+  }
+  if (rc) return rc;
+  return paged_join_launch(pass, fp16, stream);
+}
+
+namespace {
+template <int D, bool kFp16, int kSplit>
+int launch_join(const Pass& pass, unsigned across, cudaStream_t stream) {
+  const unsigned rows = (pass.parts.rows * kSplit + kJoinWarps - 1) / kJoinWarps;
+  LIMN_CUDA(launch_overlapped(sdpa_paged_join_kernel<D, kFp16, kSplit>, dim3(across, rows), dim3(kJoinWarps * 32), 0, stream, pass), "launching the kernel that joins parts");
+  note_launches(1);
+  return LIMN_B200_OK;
+}
+}  // namespace
+
+int paged_join_launch(const Pass& pass, bool fp16, cudaStream_t stream) {
+  const unsigned across = static_cast<unsigned>(pass.parts.workers < 148 ? pass.parts.workers : 148);
+  if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 16>(pass, across, stream) : launch_join<64, false, 16>(pass, across, stream);
+  return fp16 ? launch_join<128, true, 16>(pass, across, stream) : launch_join<128, false, 16>(pass, across, stream);
+}
+
+}  // namespace limn_b200
