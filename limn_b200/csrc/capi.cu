@@ -116,8 +116,9 @@ Strides strides_of(int layout, int heads, int rows, int width) {
   return Strides{static_cast<long long>(heads) * rows * width, static_cast<long long>(rows) * width, width};
 }
 
-int make_tile_map(CUtensorMap* map, const void* base, bool fp16, int batch, int heads, int rows, int width, int box_rows,
-                  const Strides& strides) {
+namespace {
+// Looks the driver's tensor-map encoder up, once.
+int find_encoder() {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult found;
@@ -127,6 +128,49 @@ int make_tile_map(CUtensorMap* map, const void* base, bool fp16, int batch, int 
   });
   if (g_encode_tiled == nullptr)
     return fail(LIMN_B200_CUDA_ERROR, "cuda: the driver does not export cuTensorMapEncodeTiled");
+  return LIMN_B200_OK;
+}
+}  // namespace
+
+int make_box_map(const char* name, CUtensorMap* map, const void* base, bool fp16, const BoxShape& shape) {
+  if (int rc = find_encoder()) return rc;
+  // kept for the same reason as in make_tile_map
+  struct Entry {
+    const void* base;
+    int fp16;
+    BoxShape shape;
+    CUtensorMap map;
+  };
+  constexpr int kEntries = 16;
+  thread_local Entry cache[kEntries];
+  thread_local int used = 0, next_slot = 0;
+  for (int i = 0; i < used; ++i) {
+    const Entry& e = cache[i];
+    bool same = e.base == base && e.fp16 == (fp16 ? 1 : 0);
+    for (int d = 0; d < 4; ++d) same = same && e.shape.dims[d] == shape.dims[d] && e.shape.box[d] == shape.box[d] && (d == 3 || e.shape.strides[d] == shape.strides[d]);
+    if (same) {
+      *map = e.map;
+      return LIMN_B200_OK;
+    }
+  }
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4];
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  for (int d = 0; d < 4; ++d) dims[d] = shape.dims[d], box[d] = shape.box[d];
+  for (int d = 0; d < 3; ++d) strides[d] = static_cast<cuuint64_t>(shape.strides[d]);
+  const CUresult res = g_encode_tiled(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, elem,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) return fail(LIMN_B200_CUDA_ERROR, "cuda: %s: encoding a tensor map failed with CUresult %d", name, (int)res);
+  Entry& slot = cache[next_slot];
+  slot.base = base, slot.fp16 = fp16 ? 1 : 0, slot.shape = shape, slot.map = *map;
+  next_slot = (next_slot + 1) % kEntries;
+  if (used < kEntries) ++used;
+  return LIMN_B200_OK;
+}
+
+int make_tile_map(CUtensorMap* map, const void* base, bool fp16, int batch, int heads, int rows, int width, int box_rows,
+                  const Strides& strides) {
+  if (int rc = find_encoder()) return rc;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0)
     return fail(LIMN_B200_BAD_ARGUMENT, "sdpa: tensor base %p is not 16-byte aligned", base);
   if ((strides.batch | strides.head | strides.row) & 7)

@@ -23,17 +23,26 @@ struct Head {
   int followers;
   int first, n;   // the sequence's first token, and tokens
   int kv_head;
-  int row0;       // the tile's first row, rows being (token, head of the group)
+  int row0;       // the first row, rows being (token, head of the group)
+  int tile_rows;  // rows of a tile: row r of a part is row row0 + r / 128 * tile_rows + r % 128, if r % 128 < tile_rows
 };
 struct Parts {
   float* o = nullptr;      // (2 workers, rows, width)
   float2* ml = nullptr;    // (2 workers, rows)
   Head* heads = nullptr;   // (workers)
   int workers = 0, rows = 0, width = 0;
-  __host__ __device__ static size_t o_bytes(int workers, int rows, int width) { return static_cast<size_t>(2) * workers * rows * width * 4; }
-  __host__ __device__ static size_t ml_bytes(int workers, int rows) { return static_cast<size_t>(2) * workers * rows * 8; }
-  __host__ __device__ static size_t head_bytes(int workers) { return (static_cast<size_t>(workers) * sizeof(Head) + 255) / 256 * 256; }
-  __host__ static size_t bytes(int workers, int rows, int width) { return o_bytes(workers, rows, width) + ml_bytes(workers, rows) + head_bytes(workers); }
+  static size_t o_bytes(int workers, int rows, int width) { return static_cast<size_t>(2) * workers * rows * width * 4; }
+  static size_t ml_bytes(int workers, int rows) { return static_cast<size_t>(2) * workers * rows * 8; }
+  static size_t head_bytes(int workers) { return (static_cast<size_t>(workers) * sizeof(Head) + 255) / 256 * 256; }
+  static size_t bytes(int workers, int rows, int width) { return o_bytes(workers, rows, width) + ml_bytes(workers, rows) + head_bytes(workers); }
+  // Lays the parts out in `memory`, which has the bytes for them.
+  void place(void* memory, int workers_, int rows_, int width_) {
+    unsigned char* at = static_cast<unsigned char*>(memory);
+    workers = workers_, rows = rows_, width = width_;
+    o = reinterpret_cast<float*>(at), at += o_bytes(workers, rows, width);
+    ml = reinterpret_cast<float2*>(at), at += ml_bytes(workers, rows);
+    heads = reinterpret_cast<Head*>(at);
+  }
 };
 
 // Sums and statistics of every (token, head) row over some of its keys, in memory: what a pass over a shared prefix leaves and the
@@ -129,8 +138,11 @@ int check_paged_pointers(const char* name, const limn_b200_paged* step);
 
 // The kernels that make a pass (each puts a second one behind itself that joins the parts): few rows to a key head, and any number.
 constexpr int kPagedFewRows = 16;  // max_t_q * group up to here
+size_t paged_many_workspace(int width, int sms);
+int paged_many_launch(const paged::Pass& pass, bool fp16, void* workspace, cudaStream_t stream);
 size_t paged_few_workspace(int rows, int width, int sms);
 int paged_few_launch(const paged::Pass& pass, bool fp16, int rows, void* workspace, cudaStream_t stream);
-int paged_join_launch(const paged::Pass& pass, bool fp16, cudaStream_t stream);
+// `many`: parts of many rows and few workers each (a warp takes a row), else of few rows and many workers (a block takes a row)
+int paged_join_launch(const paged::Pass& pass, bool fp16, bool many, cudaStream_t stream);
 
 }  // namespace limn_b200

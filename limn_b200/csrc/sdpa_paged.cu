@@ -10,84 +10,12 @@ namespace {
 
 using namespace paged;
 
-// One warp to a (token, head) row: four columns to a lane, keys one after the other.
-template <bool kFp16>
-__global__ void __launch_bounds__(128) sdpa_paged_row_kernel(const Pass prm) {
-  ptx::grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const long long row = blockIdx.x * 4LL + (threadIdx.x >> 5);
-  if (row >= static_cast<long long>(prm.tokens) * prm.heads) return;
-  const int token = static_cast<int>(row / prm.heads), head = static_cast<int>(row - static_cast<long long>(token) * prm.heads), kv_head = head / prm.group;
-  const int b = prm.q_start == nullptr ? 0 : sequence_of(prm.q_start, prm.batch, token, lane);
-  if (b >= prm.batch) return;
-  const Extent e = extent_of(prm, b);
-  if (token < e.first || token - e.first >= e.n) return;
-  const int own = prm.causal ? max(0, e.keys - e.n + (token - e.first) + 1) : e.keys;
-  auto load4 = [&](const unsigned char* at, int pieces, float (&x)[4]) {
-    x[0] = x[1] = x[2] = x[3] = 0.f;
-    if (lane >= 2 * pieces) return;
-    const uint2 w = *reinterpret_cast<const uint2*>(at + 8 * lane);
-    if (kFp16) {
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), c = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-      x[0] = a.x, x[1] = a.y, x[2] = c.x, x[3] = c.y;
-    } else {
-      x[0] = __uint_as_float(w.x << 16), x[1] = __uint_as_float(w.x & 0xffff0000u), x[2] = __uint_as_float(w.y << 16), x[3] = __uint_as_float(w.y & 0xffff0000u);
-    }
-  };
-  float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  load4(prm.q + token * prm.q_token + head * prm.q_head, prm.pieces, q);
-  const int* table = prm.table + static_cast<long long>(b) * prm.max_pages;
-  for (int j = 0; j < own; ++j) {
-    const int page = checked_page(table[j / prm.page_size], prm.pages, prm.errors), slot = j % prm.page_size;
-    float s = NAN, v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (page >= 0) {
-      float k[4];
-      load4(prm.k.base + page * prm.k.page + kv_head * prm.k.head + slot * prm.k.slot, prm.pieces, k);
-      load4(prm.v.base + page * prm.v.page + kv_head * prm.v.head + slot * prm.v.slot, prm.pieces_v, v);
-      s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-      for (int step = 16; step > 0; step >>= 1) s += __shfl_xor_sync(0xffffffffu, s, step);
-    }
-    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, alpha = expf((m - base) * prm.scale), p = expf((s - base) * prm.scale);
-    m = top, l = l * alpha + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * alpha + p * v[i];
-  }
-  const int width = prm.pieces <= 8 && prm.pieces_v <= 8 ? 64 : 128;
-  if (prm.leave.o != nullptr) {
-    if (4 * lane < width) *reinterpret_cast<float4*>(prm.leave.o + row * width + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    if (lane == 0) prm.leave.ml[row] = make_float2(m, l);
-    return;
-  }
-  if (prm.join.o != nullptr) {
-    const float2 ml = prm.join.ml[row];
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (4 * lane < width) o = *reinterpret_cast<const float4*>(prm.join.o + row * width + 4 * lane);
-    const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top, keep = expf((m - base) * prm.scale), add = expf((ml.x - base) * prm.scale);
-    m = top, l = l * keep + ml.y * add;
-    acc[0] = acc[0] * keep + o.x * add, acc[1] = acc[1] * keep + o.y * add, acc[2] = acc[2] * keep + o.z * add, acc[3] = acc[3] * keep + o.w * add;
-  }
-  if (lane < 2 * prm.pieces_v) {
-    const float a = acc[0] / l, c = acc[1] / l, d = acc[2] / l, f = acc[3] / l;
-    *reinterpret_cast<uint2*>(prm.out + token * prm.o_token + head * prm.o_head + 8 * lane) =
-        kFp16 ? make_uint2(ptx::pack_f16(a, c), ptx::pack_f16(d, f)) : make_uint2(ptx::pack_bf16(a, c), ptx::pack_bf16(d, f));
-  }
-  if (lane == 0) prm.lse[row] = m * prm.scale + logf(l);
-}
-
-int launch_rows(const Pass& prm, bool fp16, cudaStream_t stream) {
-  const long long blocks = (static_cast<long long>(prm.tokens) * prm.heads + 3) / 4;
-  if (blocks > 0x7fffffffLL) return fail(LIMN_B200_UNSUPPORTED, "sdpa_paged: %d tokens of %d heads need more blocks than one grid holds", prm.tokens, prm.heads);
-  auto kernel = fp16 ? sdpa_paged_row_kernel<true> : sdpa_paged_row_kernel<false>;
-  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, stream, prm), "launching the paged sdpa kernel");
-  note_launches(1);
-  return LIMN_B200_OK;
-}
-
 // Which kernel a pass of at most `rows` rows to a (sequence, key head) takes, and the workspace it has to itself.
-size_t pass_workspace(long long rows, int width, int sms) { return rows <= kPagedFewRows ? paged_few_workspace(static_cast<int>(rows), width, sms) : 0; }
+size_t pass_workspace(long long rows, int width, int sms) {
+  return rows <= kPagedFewRows ? paged_few_workspace(static_cast<int>(rows), width, sms) : paged_many_workspace(width, sms);
+}
 int launch_pass(const Pass& pass, bool fp16, long long rows, void* workspace, cudaStream_t stream) {
-  return rows <= kPagedFewRows ? paged_few_launch(pass, fp16, static_cast<int>(rows), workspace, stream) : launch_rows(pass, fp16, stream);
+  return rows <= kPagedFewRows ? paged_few_launch(pass, fp16, static_cast<int>(rows), workspace, stream) : paged_many_launch(pass, fp16, workspace, stream);
 }
 
 // The workspace of a call: the parts of whichever pass has more, and behind them the rows' sums over the prefix.

@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       }
     if (begun && !ends && lane == 0) {
       const long long behind = at.units - at.unit;  // units of the problem that the next workers have
-      prm.parts.heads[worker] = Head{static_cast<int>((behind + share - 1) / share), at.e.first, at.e.n, at.kv_head, 0};
+      prm.parts.heads[worker] = Head{static_cast<int>((behind + share - 1) / share), at.e.first, at.e.n, at.kv_head, 0, kPagedFewRows};
     }
     if (step + 1 < steps) {
       next_problem(prm, at);
@@ -389,7 +389,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
   for (int w = blockIdx.x; w < prm.parts.workers; w += gridDim.x) {
     const Head head = prm.parts.heads[w];
     if (head.followers == 0) continue;  // (the same in the whole block)
-    const bool there = r < prm.parts.rows && head.row0 + r < head.n * prm.group;
+    const int row = head.row0 + r / 128 * head.tile_rows + r % 128;
+    const bool there = r % 128 < head.tile_rows && row < head.n * prm.group;
     // part 0 is the head's, part i the i-th follower's
     auto part = [&](int i) { return static_cast<long long>(i == 0 ? 2 * w + 1 : 2 * (w + i)) * prm.parts.rows + r; };
     float m = -INFINITY, l = 0.f;
@@ -403,7 +404,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
         for (int u = 0; u < kUnroll; ++u) {
           const int i = i0 + u * kSplit * kAtOnce;
           ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (i <= head.followers) ml[u] = prm.parts.ml[part(i)], o[u] = *reinterpret_cast<const float4*>(prm.parts.o + part(i) * D + column);
+          if (i > head.followers) continue;
+          ml[u] = prm.parts.ml[part(i)];
+          // (a part that has seen no key has no sums)
+          if (!(ml[u].x == -INFINITY && ml[u].y == 0.f)) o[u] = *reinterpret_cast<const float4*>(prm.parts.o + part(i) * D + column);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
       for (int i = 1; i < kSplit; ++i) fold(stats[warp + i].x, stats[warp + i].y, sums[warp + i][lane]);
     }
     if (!there || side > 0) continue;
-    const RowPlace place = row_place(prm, head.first, head.kv_head, head.row0 + r);
+    const RowPlace place = row_place(prm, head.first, head.kv_head, row);
     if (prm.leave.o != nullptr) {
       *reinterpret_cast<float4*>(prm.leave.o + place.row * D + column) = acc;
       if (lane == 0) prm.leave.ml[place.row] = make_float2(m, l);
@@ -476,21 +480,12 @@ int launch_few(const Pass& pass, cudaStream_t stream) {
 
 size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(sms * kWarps, rows <= 8 ? 8 : 16, width <= 64 ? 64 : 128); }
 
-// Lays the parts out in `memory`, which has the bytes for them.
-static void place_parts(Parts& parts, void* memory, int workers, int rows, int width) {
-  unsigned char* at = static_cast<unsigned char*>(memory);
-  parts.workers = workers, parts.rows = rows, parts.width = width;
-  parts.o = reinterpret_cast<float*>(at), at += Parts::o_bytes(workers, rows, width);
-  parts.ml = reinterpret_cast<float2*>(at), at += Parts::ml_bytes(workers, rows);
-  parts.heads = reinterpret_cast<Head*>(at);
-}
-
 int paged_few_launch(const Pass& given, bool fp16, int rows, void* workspace, cudaStream_t stream) {
   Pass pass = given;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
-  place_parts(pass.parts, workspace, sms * kWarps, rows <= 8 ? 8 : 16, width);
+  pass.parts.place(workspace, sms * kWarps, rows <= 8 ? 8 : 16, width);
   int rc;
   if (width == 64) {
     if (rows <= 8) rc = fp16 ? launch_few<64, true, 1>(pass, stream) : launch_few<64, false, 1>(pass, stream);
@@ -500,7 +495,7 @@ int paged_few_launch(const Pass& given, bool fp16, int rows, void* workspace, cu
     else rc = fp16 ? launch_few<128, true, 2>(pass, stream) : launch_few<128, false, 2>(pass, stream);
   }
   if (rc) return rc;
-  return paged_join_launch(pass, fp16, stream);
+  return paged_join_launch(pass, fp16, false, stream);
 }
 
 namespace {
@@ -513,8 +508,12 @@ int launch_join(const Pass& pass, unsigned across, cudaStream_t stream) {
 }
 }  // namespace
 
-int paged_join_launch(const Pass& pass, bool fp16, cudaStream_t stream) {
+int paged_join_launch(const Pass& pass, bool fp16, bool many, cudaStream_t stream) {
   const unsigned across = static_cast<unsigned>(pass.parts.workers < 148 ? pass.parts.workers : 148);
+  if (many) {
+    if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 1>(pass, across, stream) : launch_join<64, false, 1>(pass, across, stream);
+    return fp16 ? launch_join<128, true, 1>(pass, across, stream) : launch_join<128, false, 1>(pass, across, stream);
+  }
   if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 16>(pass, across, stream) : launch_join<64, false, 16>(pass, across, stream);
   return fp16 ? launch_join<128, true, 16>(pass, across, stream) : launch_join<128, false, 16>(pass, across, stream);
 }

@@ -1,0 +1,760 @@
+// Attention over paged keys for any number of query rows to a key head, on the tensor cores: prompts and pieces of prompts behind what
+// is cached, batches in which some sequences bring one token and others thousands, and all rows of a batch over the prefix they share.
+//
+// The rows of a sequence and key head are its (token, head of the group) pairs, token by token, so that grouped heads share a tile and
+// with it the keys they read. A tile is as many whole tokens as 128 rows hold (one box of a tensor map: group heads x tokens), an item
+// is two consecutive tiles and the key tiles of 128 they see, fetched page by page:
+//   S_t = Q_t K_j^T          tcgen05.mma, both operands K-major in shared memory, S_t in tensor memory
+//   P_t = exp2(S_t - m_t)    128 softmax threads per tile, one row each; P_t overwrites S_t as 16-bit
+//   O_t += P_t V_j           tcgen05.mma, A = P_t from tensor memory, B = V_j (MN-major) from shared memory
+// An item with one tile has it in both places, the even key tiles to the first and the odd ones to the second, and the epilogue puts the
+// two together.
+//
+// Lengths are known on the device only, and they differ. So the work is cut there, into equal shares of (item, key) cost, one share to a
+// CTA and one CTA to an SM: a share is the rest of an item, whole items, and the beginning of one. Whole items go to the result; what a
+// CTA has of an item that others share goes into its parts (paged.h), which a kernel behind this one joins. The cost of an item is the number of keys its last
+// token sees, half of it where one tile has both places; its sum over a sequence has a closed form, and so has the share a CTA begins
+// with: nothing is planned on the host or by a kernel in front.
+//
+// Keys past a sequence's end are zeros (a page coordinate outside the cache makes TMA fill them), except those of its last page, which
+// hold whatever lies there: their scores are replaced, and their rows of V are zeroed before the product that reads them, since
+// 0 * NaN would reach every row.
+//
+// Warp roles (10 warps): 0-3 softmax and epilogue of tile 0, 4-7 of tile 1, 8 TMA producer, 9 MMA issuer and tensor-memory owner.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged.h"
+#include "sm100_ptx.cuh"
+#include "tensor_map.h"
+
+namespace limn_b200 {
+namespace {
+
+using namespace ptx;
+using namespace paged;
+
+constexpr int kTile = 128;     // rows of a tile, keys of a key tile
+constexpr int kThreads = 320;
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleSlack = 8.f;
+constexpr int kLeast = 256;    // cost of the smallest share: a CTA's part of an item costs it a load of Q and a store of sums besides
+
+template <int D>
+struct Layout {
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kAtomBytes = kTile * 128;  // one 64-element-wide column block of a tile
+  static constexpr int kStages = 2;
+  static constexpr int kQOff = 0;
+  static constexpr int kKOff = kQOff + 2 * kTileBytes;
+  static constexpr int kVOff = kKOff + kStages * kTileBytes;
+  static constexpr int kBarOff = kVOff + kStages * kTileBytes;
+  static constexpr int kBytes = kBarOff + 512 + 1024;
+  static constexpr int kSCol = 0;    // S_t at kSCol + 128 t (P_t overlays its first 64)
+  static constexpr int kOCol = 256;  // O_t at kOCol + D t
+};
+struct Bars {
+  static constexpr int kS = 2;                   // stages
+  static constexpr int q_full = 0;               // + t
+  static constexpr int k_full = 2;               // + stage
+  static constexpr int k_empty = k_full + kS;
+  static constexpr int v_full = k_empty + kS;
+  static constexpr int v_empty = v_full + kS;
+  static constexpr int s_full = v_empty + kS;    // + t
+  static constexpr int p_full = s_full + 2;      // + t
+  static constexpr int o_full = p_full + 2;      // + t
+  static constexpr int p_half = o_full + 2;      // + t: the first 64 keys' worth of P_t is in place (and O_t rescaled)
+  static constexpr int q_empty = p_half + 2;     // + t: the last S_t of the segment has been computed
+  static constexpr int o_free = q_empty + 2;     // + t: the epilogue has read O_t
+  static constexpr int work_full = o_free + 2;   // + slot
+  static constexpr int work_empty = work_full + 2;
+  static constexpr int merge_full = work_empty + 2;  // tile 1's part of every row is complete (both places one tile)
+  static constexpr int count = merge_full + 1;
+};
+
+// What a CTA does of one item, as the producer hands it to the others.
+struct Segment {
+  int valid;
+  int b, first, n, keys, kv_head;
+  int row0;        // first row of tile 0
+  int first_tile;  // first key tile
+  int loads;       // key tiles it streams
+  int count[2];    // of them, those that the tile in each place goes through
+  int both;        // one tile in both places
+  int begun;       // it begins with the item's first key tile
+  int whole;       // and ends with its last
+};
+
+// ---- the cost of items, in keys. A sequence has `pairs` items per key head, pair j of tokens [j span, (j + 1) span) ----
+struct Costs {
+  int pairs, span, half, seen_first;  // span: tokens of a pair; half: of a tile; seen_first: keys that are there before the first token
+  int keys, n, causal;
+  __device__ __forceinline__ Costs(const Extent& e, int tokens_of_tile, int causal_)
+      : pairs((e.n + 2 * tokens_of_tile - 1) / (2 * tokens_of_tile)), span(2 * tokens_of_tile), half(tokens_of_tile), seen_first(e.keys - e.n), keys(e.keys), n(e.n), causal(causal_) {}
+  // keys that the first `tokens` tokens see at most; one, masked, where that is none
+  __device__ __forceinline__ int seen(int tokens) const { return max(1, causal ? seen_first + min(tokens, n) : keys); }
+  __device__ __forceinline__ bool single(int j) const { return n - j * span <= half; }
+  __device__ __forceinline__ int of(int j) const { return single(j) ? (seen((j + 1) * span) + 1) / 2 : seen((j + 1) * span); }
+  // sum over the pairs in front of j (all of them two whole tiles)
+  __device__ __forceinline__ long long before(long long j) const {
+    if (!causal) return j * max(1, keys);
+    const long long none = seen_first >= 0 ? 0 : min(j, static_cast<long long>(-seen_first / span));  // pairs whose last token sees nothing: 1 each
+    return none + (j - none) * seen_first + span * (j * (j + 1) / 2 - none * (none + 1) / 2);
+  }
+  __device__ __forceinline__ long long all() const { return pairs == 0 ? 0 : before(pairs - 1) + of(pairs - 1); }
+  // steps of key tiles (pairs of key tiles for a single tile) of pair j
+  __device__ __forceinline__ int steps(int j) const {
+    const int tiles = (seen((j + 1) * span) + kTile - 1) / kTile;
+    return single(j) ? (tiles + 1) / 2 : tiles;
+  }
+  // the step nearest to `cost` into pair j
+  __device__ __forceinline__ int step_at(int j, long long cost) const { return static_cast<int>(min(static_cast<long long>(steps(j)), (cost + kTile / 2) / kTile)); }
+};
+
+struct Place {
+  int b, kv_head, j, step;
+  Extent e;
+  long long into;  // cost from the item's beginning
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+template <int D, bool kFp16>
+__global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __grid_constant__ Maps maps, const Pass prm, const int tile_tokens, const int chunk, unsigned* status) {
+  using L = Layout<D>;
+  using B = Bars;
+  extern __shared__ unsigned char smem_unaligned[];
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t abort_flag;
+  __shared__ Segment ring[2];
+  __shared__ float merge_m[kTile], merge_l[kTile];
+  __shared__ long long share_end[kThreads];
+  __shared__ long long warp_sum[kThreads / 32];
+
+  const uint32_t base = (smem_addr(smem_unaligned) + 1023u) & ~1023u;
+  const uint32_t bars = base + L::kBarOff;
+  auto bar = [&](int i) { return bars + 8u * i; };
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31;
+  const int tile_rows = tile_tokens * prm.group;
+
+  if (threadIdx.x == kProducerWarp * 32) {
+    for (int i = 0; i < B::count; ++i) {
+      unsigned arrivals = 1u;
+      if ((i >= B::p_full && i < B::p_full + 2) || (i >= B::p_half && i < B::p_half + 2) || (i >= B::o_free && i < B::o_free + 2) || i == B::merge_full)
+        arrivals = 128u;                                               // every thread of a softmax group
+      if (i >= B::work_empty && i < B::work_empty + 2) arrivals = 9u;  // the MMA warp and the eight softmax warps
+      mbar_init(bar(i), arrivals);
+    }
+    mbar_init_fence();
+    tma_prefetch_descriptor(&maps.q);
+    tma_prefetch_descriptor(&maps.k);
+    tma_prefetch_descriptor(&maps.v);
+  }
+  // up to here nothing has touched global memory
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (threadIdx.x == 0) {
+    abort_flag = *reinterpret_cast<volatile unsigned*>(status) != kStatusOk;  // an earlier kernel gave up: this one stands down
+    prm.parts.heads[blockIdx.x].followers = 0;                                // (also then: nothing is joined)
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_addr(&tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
+  const int run = (prm.batch + kThreads - 1) / kThreads;
+  {
+    long long mine = 0;
+    for (int i = 0; i < run; ++i) {
+      const int b = threadIdx.x * run + i;
+      if (b < prm.batch) mine += Costs(extent_of(prm, b), tile_tokens, prm.causal).all();
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, mine, d);
+      if (lane >= d) mine += other;
+    }
+    if (lane == 31) warp_sum[warp] = mine;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) mine += warp_sum[w];
+    share_end[threadIdx.x] = mine;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  bool ok = !abort_flag;
+
+  auto wait = [&](int i, uint32_t parity, unsigned tag) { return __all_sync(0xffffffffu, mbar_wait(bar(i), parity, status, tag)); };
+  auto next_segment = [&](unsigned n_item, Segment& s) {
+    const unsigned slot = n_item & 1u;
+    if (!wait(B::work_full + slot, (n_item >> 1) & 1u, 0x0400u | slot)) return false;
+    const volatile int* from = reinterpret_cast<const volatile int*>(&ring[slot]);
+    int* to = reinterpret_cast<int*>(&s);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(Segment) / sizeof(int)); ++i) to[i] = from[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(B::work_empty + slot));
+    return true;
+  };
+
+  if (warp == kProducerWarp) {
+    // ================= the share, and TMA =================
+    const long long total = share_end[kThreads - 1] * prm.kv_heads;
+    const long long share = max(static_cast<long long>(kLeast), (total + gridDim.x - 1) / gridDim.x);
+    auto place_of = [&](long long x) {
+      Place p;
+      int before = 0;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) before += __popc(__ballot_sync(0xffffffffu, share_end[i * 32 + lane] * prm.kv_heads <= x));
+      long long rest = x - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
+      p.b = before * run - 1;
+      long long all;
+      do {
+        ++p.b;
+        p.e = extent_of(prm, p.b);
+        all = Costs(p.e, tile_tokens, prm.causal).all();
+        if (rest < all * prm.kv_heads) break;
+        rest -= all * prm.kv_heads;
+      } while (p.b + 1 < prm.batch);
+      const Costs costs(p.e, tile_tokens, prm.causal);
+      p.kv_head = static_cast<int>(rest / all);
+      rest -= p.kv_head * all;
+      int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
+      while (low < high) {
+        const int mid = (low + high + 1) / 2;
+        if (costs.before(mid) <= rest) low = mid;
+        else high = mid - 1;
+      }
+      p.j = low;
+      p.into = rest - costs.before(low);
+      p.step = costs.step_at(low, p.into);
+      return p;
+    };
+    const long long from = blockIdx.x * share;
+    const bool any = ok && from < total;
+    const long long to = from + share;
+    Place at = {}, end = {};
+    end.b = prm.batch;
+    if (any) at = place_of(from);
+    if (any && to < total) end = place_of(to);
+    unsigned n_item = 0, q_uses[2] = {0u, 0u}, step = 0;
+    bool more = any;
+    // a lane fetches one box of a key tile: `chunk` keys of one page, 64 columns
+    const int chunks = kTile / chunk;
+    const int my_chunk = lane % chunks, my_atom = lane / chunks;
+    while (more && ok) {
+      const Costs costs(at.e, tile_tokens, prm.causal);
+      const bool last = at.b == end.b && at.kv_head == end.kv_head && at.j == end.j;
+      const int steps = costs.steps(at.j), until = last ? end.step : steps;
+      if (until > at.step) {
+        Segment s;
+        const bool single = costs.single(at.j);
+        const int tiles = (costs.seen((at.j + 1) * costs.span) + kTile - 1) / kTile;  // key tiles of the item
+        s.valid = 1, s.b = at.b, s.first = at.e.first, s.n = at.e.n, s.keys = at.e.keys, s.kv_head = at.kv_head;
+        s.row0 = at.j * 2 * tile_rows;
+        s.begun = at.step == 0, s.whole = at.step == 0 && until == steps;
+        if (single) {
+          s.first_tile = 2 * at.step;
+          s.loads = min(2 * until, tiles) - s.first_tile;
+          s.both = s.loads > 1;
+          s.count[1] = s.loads / 2, s.count[0] = s.loads - s.count[1];
+        } else {
+          s.first_tile = at.step;
+          const int tiles_0 = (costs.seen(at.j * costs.span + costs.half) + kTile - 1) / kTile;
+          s.count[0] = max(0, min(until, tiles_0) - at.step);
+          s.count[1] = until - at.step;
+          s.loads = s.count[1], s.both = 0;
+        }
+        const unsigned slot = n_item & 1u;
+        ok = wait(B::work_empty + slot, ((n_item >> 1) & 1u) ^ 1u, 0x0120u | slot);
+        if (!ok) break;
+        if (lane == 0) {
+          ring[slot] = s;
+          mbar_arrive(bar(B::work_full + slot));
+          if (s.begun && !s.whole) {
+            // workers c behind this one whose share begins inside the item, before the middle of its last step
+            const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), steps * static_cast<long long>(kTile) - kTile / 2);
+            prm.parts.heads[blockIdx.x] = Head{static_cast<int>((begins + limit - 1) / share - blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
+          }
+        }
+        __syncwarp();
+        ++n_item;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (s.count[t] == 0) continue;
+          ok = wait(B::q_empty + t, (q_uses[t] & 1u) ^ 1u, 0x0130u | t);
+          if (!ok) break;
+          ++q_uses[t];
+          if (lane == 0) {
+            mbar_expect_tx(bar(B::q_full + t), static_cast<uint32_t>(tile_rows) * D * 2);
+            const int token = s.first + (2 * at.j + (s.both ? 0 : t)) * tile_tokens;
+#pragma unroll
+            for (int a = 0; a < D / 64; ++a) tma_load_4d(base + L::kQOff + t * L::kTileBytes + a * L::kAtomBytes, &maps.q, bar(B::q_full + t), a * 64, s.kv_head * prm.group, token, 0);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        const int* table = prm.table + static_cast<long long>(s.b) * prm.max_pages;
+        // the page of this lane's box of key tile `tile`; -1, whose boxes TMA fills with zeros, past the end and where it is none
+        auto entry = [&](int tile) {
+          const int key = tile * kTile + my_chunk * chunk;
+          return key < s.keys ? table[key / prm.page_size] : -1;
+        };
+        int page_next = entry(s.first_tile);
+        for (int j = 0; j < s.loads && ok; ++j, ++step) {
+          const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
+          int page = page_next;
+          if (key < s.keys) page = checked_page(page, prm.pages, prm.errors);
+          if (j + 1 < s.loads) page_next = entry(tile + 1);
+          const int in_page = key % prm.page_size;
+          const int stage = step % B::kS;
+          const uint32_t wrap = (step / B::kS) & 1;
+          ok = wait(B::k_empty + stage, wrap ^ 1u, 0x0100u | stage);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(bar(B::k_full + stage), L::kTileBytes);
+          __syncwarp();
+          const uint32_t box = stage * L::kTileBytes + my_atom * L::kAtomBytes + my_chunk * chunk * 128;
+          if (my_atom < D / 64) tma_load_4d(base + L::kKOff + box, &maps.k, bar(B::k_full + stage), my_atom * 64, in_page, s.kv_head, page);
+          __syncwarp();
+          ok = wait(B::v_empty + stage, wrap ^ 1u, 0x0110u | stage);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(bar(B::v_full + stage), L::kTileBytes);
+          __syncwarp();
+          if (my_atom < D / 64) tma_load_4d(base + L::kVOff + box, &maps.v, bar(B::v_full + stage), my_atom * 64, in_page, s.kv_head, page);
+          __syncwarp();
+        }
+      }
+      // the next item
+      if (last) break;
+      at.step = 0;
+      if (++at.j < costs.pairs) continue;
+      at.j = 0;
+      if (++at.kv_head < prm.kv_heads) continue;
+      at.kv_head = 0;
+      do {
+        if (++at.b >= prm.batch) {
+          more = false;
+          break;
+        }
+        at.e = extent_of(prm, at.b);
+      } while (at.e.n == 0);
+    }
+    const unsigned slot = n_item & 1u;
+    if (ok) ok = wait(B::work_empty + slot, ((n_item >> 1) & 1u) ^ 1u, 0x0121u | slot);
+    if (ok && lane == 0) {
+      ring[slot].valid = 0;
+      mbar_arrive(bar(B::work_full + slot));
+    }
+  } else if (warp == kMmaWarp) {
+    // ================= MMA issuer =================
+    constexpr uint32_t idesc_s = mma_idesc(kTile, kTile, kFp16, false, false);
+    constexpr uint32_t idesc_pv = mma_idesc(kTile, D, kFp16, false, true);
+    auto issue_s = [&](int t, int stage) {
+      const uint32_t q_lo = desc_lo(base + L::kQOff + t * L::kTileBytes, 0);
+      const uint32_t k_lo = desc_lo(base + L::kKOff + stage * L::kTileBytes, 0);
+      const uint32_t c = tmem + L::kSCol + t * 128;
+      mma_ss_lo<false>(c, q_lo, k_lo, idesc_s);
+#pragma unroll
+      for (int kk = 1; kk < D / 16; ++kk) {
+        const uint32_t off = (kk / 4) * (L::kAtomBytes >> 4) + (kk % 4) * 2;  // in 16-byte units
+        mma_ss_lo<true>(c, q_lo + off, k_lo + off, idesc_s);
+      }
+    };
+    auto issue_pv = [&](int t, int stage, int part, bool first) {
+      const uint32_t v_lo = desc_lo(base + L::kVOff + stage * L::kTileBytes, L::kAtomBytes);
+      const uint32_t c = tmem + L::kOCol + t * D;
+      const uint32_t a = tmem + L::kSCol + t * 128;
+#pragma unroll
+      for (int kk = 4 * part; kk < 4 * part + 4; ++kk) mma_ts_lo(c, a + kk * 8, v_lo + kk * (16 * 128 / 16), idesc_pv, (kk > 0 || !first) ? 1u : 0u);
+    };
+    // rows [from, to) of the V tile in `stage` become zeros: slots of a sequence's last page that it has not filled
+    auto clear_rows = [&](int stage, int from, int to) {
+      for (int i = from * (D / 8) + lane; i < to * (D / 8); i += 32) {
+        const int row = i / (D / 8), piece = i % (D / 8);
+        st_shared_v4(base + L::kVOff + stage * L::kTileBytes + (piece / 8) * L::kAtomBytes + row * 128 + (piece % 8) * 16, 0u, 0u, 0u, 0u);
+      }
+      fence_async_shared();
+      __syncwarp();
+    };
+    unsigned q_uses[2] = {0u, 0u};  // segments finished in which the tile in place t had key tiles
+    unsigned tiles[2] = {0u, 0u};   // key tiles it has been through, over all segments
+    unsigned step = 0;
+    for (unsigned n_item = 0; ok; ++n_item) {
+      Segment s;
+      ok = next_segment(n_item, s);
+      if (!ok || !s.valid) break;
+      const bool both = s.both != 0;
+      auto at = [&](int t, int j) { return step + (both ? 2 * j + t : j); };
+      unsigned cleared = 0;  // + 1 of the load whose rows past the sequence's end have been cleared
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (s.count[t] > 0 && ok) ok = wait(B::q_full + t, q_uses[t] & 1u, 0x0200u | t);
+      if (!ok) break;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (s.count[t] > 0 && ok) {
+          const unsigned first = at(t, 0);
+          const int stage = first % B::kS;
+          ok = wait(B::k_full + stage, (first / B::kS) & 1, 0x0210u);
+          if (!ok) break;
+          tc_fence_after_sync();
+          // (the S_t region is free: MMAs run in issue order, and the last one issued for this tile consumed the P_t there)
+          if (elect_one()) {
+            issue_s(t, stage);
+            mma_commit(bar(B::s_full + t));
+            if (s.count[t] == 1) mma_commit(bar(B::q_empty + t));
+            if (both) mma_commit(bar(B::k_empty + stage));
+          }
+          __syncwarp();
+        }
+      if (!ok) break;
+      if (!both && elect_one()) mma_commit(bar(B::k_empty + step % B::kS));
+      __syncwarp();
+      const int rounds = max(s.count[0], s.count[1]);
+      for (int j = 0; j < rounds && ok; ++j) {
+        bool issued_next = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || j >= s.count[t]) continue;
+          const unsigned here = at(t, j), then = at(t, j + 1);
+          const int stage = here % B::kS, next = then % B::kS;
+          ok = wait(B::v_full + stage, (here / B::kS) & 1, 0x0220u | stage);
+          if (!ok) break;
+          const int left = s.keys - (s.first_tile + static_cast<int>(here - step)) * kTile;  // keys of the tile that there are, if fewer than all
+          if (left > 0 && left < kTile && left % chunk != 0 && cleared != here + 1) {
+            clear_rows(stage, left, (left + chunk - 1) / chunk * chunk);
+            cleared = here + 1;
+          }
+          const uint32_t phase = tiles[t] & 1u;
+          ok = wait(B::p_half + t, phase, 0x0260u | t);
+          if (!ok) break;
+          // the segment's first product overwrites O_t: the epilogue before must have read it
+          if (j == 0) ok = wait(B::o_free + t, (q_uses[t] & 1u) ^ 1u, 0x0270u | t);
+          if (!ok) break;
+          tc_fence_after_sync();
+          if (elect_one()) issue_pv(t, stage, 0, j == 0);
+          __syncwarp();
+          ok = wait(B::p_full + t, phase, 0x0230u | t);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const bool last = j + 1 >= s.count[t];
+          if (elect_one()) {
+            issue_pv(t, stage, 1, j == 0);
+            if (last) mma_commit(bar(B::o_full + t));
+            if (both) mma_commit(bar(B::v_empty + stage));
+          }
+          __syncwarp();
+          ++tiles[t];
+          if (!last) {
+            // the scores can only follow the product that consumed the P_t lying over them
+            ok = wait(B::k_full + next, (then / B::kS) & 1, 0x0240u | next);
+            if (!ok) break;
+            tc_fence_after_sync();
+            if (elect_one()) {
+              issue_s(t, next);
+              mma_commit(bar(B::s_full + t));
+              if (j + 2 == s.count[t]) mma_commit(bar(B::q_empty + t));
+              if (both) mma_commit(bar(B::k_empty + next));
+            }
+            __syncwarp();
+            issued_next = true;
+          }
+        }
+        if (!ok) break;
+        if (!both && elect_one()) {
+          mma_commit(bar(B::v_empty + (step + j) % B::kS));
+          if (issued_next) mma_commit(bar(B::k_empty + (step + j + 1) % B::kS));
+        }
+        __syncwarp();
+      }
+      step += s.loads;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (s.count[t] > 0) ++q_uses[t];
+    }
+  } else {
+    // ================= softmax + epilogue, one thread per row =================
+    const int t = warp >> 2;
+    const int row_in_tile = threadIdx.x & 127;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + L::kSCol + t * 128;
+    const uint32_t t_o = tmem + lane_base + L::kOCol + t * D;
+    const float sl2 = prm.scale * kLog2e;
+    const uint64_t sl2_2 = f2_pack(sl2, sl2);
+    const int chunk_log = 31 - __clz(chunk), chunks = kTile >> chunk_log;
+    unsigned tiles = 0;   // key tiles this group has been through, over all segments
+    unsigned o_uses = 0;  // segments it has finished with key tiles
+    unsigned merges = 0;
+    for (unsigned n_item = 0; ok; ++n_item) {
+      Segment s;
+      ok = next_segment(n_item, s);
+      if (!ok || !s.valid) break;
+      const bool both = s.both != 0;
+      const int n = s.count[t];
+      const int top_row = s.row0 + (both ? 0 : t) * tile_rows;       // the tile's first row
+      const int row = top_row + row_in_tile;
+      const bool there = row_in_tile < tile_rows && row < s.n * prm.group;
+      const long long part = (2LL * blockIdx.x + (s.begun ? 1 : 0)) * (2 * kTile) + t * kTile + row_in_tile;
+      if (n == 0) {
+        // nothing of this share for the tile's rows (its keys end before): a part without keys, if they have one
+        if (!s.whole && there) prm.parts.ml[part] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
+      const int seen_first = s.keys - s.n;
+      const int sees = prm.causal ? min(s.keys, seen_first + row / prm.group + 1) : s.keys;                // keys [0, sees)
+      const int sees_least = prm.causal ? min(s.keys, seen_first + top_row / prm.group + 1) : s.keys;      // the tile's first token
+      const int* table = prm.table + static_cast<long long>(s.b) * prm.max_pages;
+      auto key0 = [&](int j) { return (s.first_tile + (both ? 2 * j + t : j)) * kTile; };
+      // pages are looked at once more here, a key tile ahead: scores against one that is none are NaN
+      auto entry = [&](int j) {
+        const int key = key0(j) + lane * chunk;
+        return lane < chunks && key < s.keys ? table[key / prm.page_size] : 0;
+      };
+      int entry_next = entry(0);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++tiles) {
+        const unsigned none = __ballot_sync(0xffffffffu, entry_next < 0 || entry_next >= prm.pages);
+        if (j + 1 < n) entry_next = entry(j + 1);
+        ok = wait(B::s_full + t, tiles & 1u, 0x0300u | t);
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t x[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x[c]);
+        tmem_ld_wait();
+        const int kv0 = key0(j);
+        if (none != 0u) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if ((none >> ((c * 32 + i) >> chunk_log)) & 1u) x[c][i] = 0x7fffffffu;  // NaN
+        }
+        if (kv0 + kTile > sees_least) {
+          const int limit = sees - kv0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= limit) x[c][i] = 0xff800000u;  // -inf
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        const bool moves = (mx - m) * sl2 > kRescaleSlack;  // true at the first score above -inf, where m is -inf
+        float alpha = 1.f;
+        if (moves) {
+          alpha = exp2_approx((m - mx) * sl2);
+          m = mx;
+        }
+        const float shift = m == -INFINITY ? 0.f : -m * sl2;
+        const uint64_t shift2 = f2_pack(shift, shift);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1) {
+            // O_t was last written by the product of tile j - 1, which s_full also covers
+            if (j > 0 && __any_sync(0xffffffffu, moves)) {
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(t_o + 32 * c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st32(t_o + 32 * c, o);
+              }
+            }
+          }
+          uint32_t packed[32];
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const int c = 2 * h + cc;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const uint64_t x2 = f2_fma(f2_pack_bits(x[c][i], x[c][i + 1]), sl2_2, shift2);
+              float p0, p1;
+              if (D == 64 && ((i >> 1) & 7) < 2) {  // (as in the dense forward: some of the exponentials on the FMA pipe)
+                exp2_poly2<5>(x2, p0, p1);
+              } else {
+                f2_unpack(x2, p0, p1);
+                p0 = exp2_approx(p0);
+                p1 = exp2_approx(p1);
+              }
+              sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(p0, p1));
+              packed[cc * 16 + (i >> 1)] = kFp16 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+            }
+            if (h == 1 && cc == 0) {
+              // the first half's store was issued a chunk of exponentials ago; hand it over
+              tmem_st_wait();
+              tc_fence_before_sync();
+              mbar_arrive(bar(B::p_half + t));
+            }
+          }
+          tmem_st32(t_s + 32 * h, packed);
+        }
+        float sum_a, sum_b, sum_c, sum_d;
+        f2_unpack(sum2[0], sum_a, sum_b);
+        f2_unpack(sum2[1], sum_c, sum_d);
+        l = l * alpha + ((sum_a + sum_b) + (sum_c + sum_d));
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(bar(B::p_full + t));
+      }
+      if (!ok) break;
+      ok = wait(B::o_full + t, o_uses & 1u, 0x0310u | t);
+      if (!ok) break;
+      tc_fence_after_sync();
+      ++o_uses;
+      float keep = 1.f, from_1 = 0.f;  // what this place's sums and the other one's count (one tile in both)
+      if (both) {
+        if (t == 1) {
+          merge_m[row_in_tile] = m, merge_l[row_in_tile] = l;
+          tc_fence_before_sync();
+          mbar_arrive(bar(B::merge_full));
+          continue;
+        }
+        ok = wait(B::merge_full, merges & 1u, 0x0340u);
+        if (!ok) break;
+        ++merges;
+        tc_fence_after_sync();
+        const float m_1 = *const_cast<volatile float*>(&merge_m[row_in_tile]), l_1 = *const_cast<volatile float*>(&merge_l[row_in_tile]);
+        const float top = fmaxf(m, m_1), zero = top == -INFINITY ? 0.f : top;
+        keep = exp2f((m - zero) * sl2), from_1 = exp2f((m_1 - zero) * sl2);
+        l = l * keep + l_1 * from_1;
+        m = top;
+      }
+      auto take = [&](int col, uint32_t (&o)[32]) {
+        tmem_ld32(t_o + col, o);
+        if (both) {
+          uint32_t o_1[32];
+          tmem_ld32(t_o + D + col, o_1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep + __uint_as_float(o_1[i]) * from_1);
+        } else {
+          tmem_ld_wait();
+        }
+      };
+      const RowPlace place = row_place(prm, s.first, s.kv_head, there ? row : 0);
+      if (s.whole && prm.leave.o == nullptr) {
+        float add = 0.f, mine = 1.f;
+        const float* more = nullptr;
+        if (prm.join.o != nullptr && there) {
+          const float2 ml = prm.join.ml[place.row];
+          more = prm.join.o + place.row * D;
+          const float top = fmaxf(m, ml.x), zero = top == -INFINITY ? 0.f : top;
+          mine = exp2f((m - zero) * sl2), add = exp2f((ml.x - zero) * sl2);
+          l = l * mine + ml.y * add;
+          m = top;
+        }
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          take(32 * c, o);
+          if (more != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(more + 32 * c + i);
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * mine + f.x * add), o[i + 1] = __float_as_uint(__uint_as_float(o[i + 1]) * mine + f.y * add);
+              o[i + 2] = __float_as_uint(__uint_as_float(o[i + 2]) * mine + f.z * add), o[i + 3] = __float_as_uint(__uint_as_float(o[i + 3]) * mine + f.w * add);
+            }
+          }
+          if (there) store_row32<kFp16>(place.out + 64 * c, o, inv, prm.pieces_v * 8 - 32 * c);
+        }
+        if (there) prm.lse[place.row] = m * prm.scale + logf(l);
+      } else {
+        float* to = s.whole ? prm.leave.o + place.row * D : prm.parts.o + part * D;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          take(32 * c, o);
+          if (there) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+        if (there) *(s.whole ? prm.leave.ml + place.row : prm.parts.ml + part) = make_float2(m, l);
+      }
+      // O_t is in registers or stored: the next segment's first product may overwrite it
+      tc_fence_before_sync();
+      mbar_arrive(bar(B::o_free + t));
+      if (both) mbar_arrive(bar(B::o_free + 1));
+    }
+  }
+
+  // ---- teardown ----
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    if (abort_flag || *reinterpret_cast<volatile unsigned*>(status) != kStatusOk) {
+      // a wait gave up somewhere: give copies and MMAs still in flight time to land before the memory they target is released
+      for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    }
+    tc_fence_after_sync();
+    tmem_free(tmem, kTmemCols);
+  }
+}
+
+template <int D, bool kFp16>
+int launch_many(const Pass& pass, unsigned* status, cudaStream_t stream) {
+  using L = Layout<D>;
+  int chunk = pass.page_size;  // the largest run of keys that neither a page nor a key tile cuts: the common divisor of both, a power of two
+  for (int rest = kTile % chunk; rest != 0;) {
+    const int r = chunk % rest;
+    chunk = rest, rest = r;
+  }
+  const int tile_tokens = kTile / pass.group;
+  Maps maps;
+  const auto u = [](long long x) { return static_cast<unsigned long long>(x); };
+  BoxShape q = {{u(pass.pieces) * 8, u(pass.heads), u(pass.tokens), 1}, {pass.q_head, pass.q_token, pass.q_token * pass.tokens}, {64, static_cast<unsigned>(pass.group), static_cast<unsigned>(tile_tokens), 1}};
+  BoxShape k = {{u(pass.pieces) * 8, u(pass.page_size), u(pass.kv_heads), u(pass.pages)}, {pass.k.slot, pass.k.head, pass.k.page}, {64, static_cast<unsigned>(chunk), 1, 1}};
+  BoxShape v = {{u(pass.pieces_v) * 8, u(pass.page_size), u(pass.kv_heads), u(pass.pages)}, {pass.v.slot, pass.v.head, pass.v.page}, {64, static_cast<unsigned>(chunk), 1, 1}};
+  if (int rc = make_box_map("sdpa_paged", &maps.q, pass.q, kFp16, q)) return rc;
+  if (int rc = make_box_map("sdpa_paged", &maps.k, pass.k.base, kFp16, k)) return rc;
+  if (int rc = make_box_map("sdpa_paged", &maps.v, pass.v.base, kFp16, v)) return rc;
+  auto kernel = sdpa_paged_many_kernel<D, kFp16>;
+  static bool sized[64] = {};
+  int device = 0;
+  LIMN_CUDA(cudaGetDevice(&device), "asking for the current device");
+  if (device >= 0 && device < 64 && !sized[device]) {
+    LIMN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "sizing shared memory for the paged sdpa kernel");
+    sized[device] = true;
+  }
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers)), dim3(kThreads), L::kBytes, stream, maps, pass, tile_tokens, chunk, status),
+            "launching the paged sdpa kernel");
+  note_launches(1);
+  return LIMN_B200_OK;
+}
+
+}  // namespace
+
+size_t paged_many_workspace(int width, int sms) { return Parts::bytes(sms, 2 * kTile, width); }
+
+int paged_many_launch(const Pass& given, bool fp16, void* workspace, cudaStream_t stream) {
+  Pass pass = given;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  unsigned* status = nullptr;
+  if (int rc = status_word(&status)) return rc;
+  const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
+  pass.parts.place(workspace, sms, 2 * kTile, width);
+  int rc;
+  if (width == 64) rc = fp16 ? launch_many<64, true>(pass, status, stream) : launch_many<64, false>(pass, status, stream);
+  else rc = fp16 ? launch_many<128, true>(pass, status, stream) : launch_many<128, false>(pass, status, stream);
+  if (rc) return rc;
+  return paged_join_launch(pass, fp16, true, stream);
+}
+
+}  // namespace limn_b200
