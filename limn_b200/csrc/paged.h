@@ -36,12 +36,11 @@ struct Parts {
   static size_t head_bytes(int workers) { return (static_cast<size_t>(workers) * sizeof(Head) + 255) / 256 * 256; }
   static size_t bytes(int workers, int rows, int width) { return o_bytes(workers, rows, width) + ml_bytes(workers, rows) + head_bytes(workers); }
   // Lays the parts out in `memory`, which has the bytes for them.
-  void place(void* memory, int workers_, int rows_, int width_) {
-    unsigned char* at = static_cast<unsigned char*>(memory);
+  void place(unsigned char* memory, int workers_, int rows_, int width_) {
     workers = workers_, rows = rows_, width = width_;
-    o = reinterpret_cast<float*>(at), at += o_bytes(workers, rows, width);
-    ml = reinterpret_cast<float2*>(at), at += ml_bytes(workers, rows);
-    heads = reinterpret_cast<Head*>(at);
+    o = reinterpret_cast<float*>(memory), memory += o_bytes(workers, rows, width);
+    ml = reinterpret_cast<float2*>(memory), memory += ml_bytes(workers, rows);
+    heads = reinterpret_cast<Head*>(memory);
   }
 };
 
@@ -71,7 +70,7 @@ struct Pass {
   float scale = 0.f;
   Parts parts;
   RowSums leave;  // where rows go instead of `out`, or null
-  RowSums join;   // what rows are joined with on their way out, or null
+  RowSums join;   // what rows are joined with on their way out, or null. The kernel that leaves these sums may still run when the pass begins
 };
 
 // A sequence's extents: `first` token of `n`, `keys` in its pages. One that cannot be has n = 0 and is noted.
@@ -130,6 +129,20 @@ __device__ __forceinline__ RowPlace row_place(const Pass& p, int first, int kv_h
   return RowPlace{token * p.heads + head, p.out + token * p.o_token + head * p.o_head};
 }
 
+// Two sides of a row put together: statistics (m, l) and (m_b, l_b) become those of both, `keep` and `add` what the sums of either count.
+// (A side that has seen no key has m = -inf, l = 0 and counts 0; a NaN in l stays one.)
+__device__ __forceinline__ void merge_stats(float& m, float& l, float m_b, float l_b, float sl2, float& keep, float& add) {
+  const float top = fmaxf(m, m_b), base = top == -INFINITY ? 0.f : top;
+  keep = exp2f((m - base) * sl2), add = exp2f((m_b - base) * sl2);
+  m = top, l = l * keep + l_b * add;
+}
+
+// A quotient of numbers that are not negative, by the short division where both allow it (the long one takes some 100 instructions).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
 }  // namespace paged
 
 // Checks of a step that every entry point makes, of its extents and strides and of its pointers; `name` is the op's.
@@ -138,11 +151,11 @@ int check_paged_pointers(const char* name, const limn_b200_paged* step);
 
 // The kernels that make a pass (each puts a second one behind itself that joins the parts): few rows to a key head, and any number.
 constexpr int kPagedFewRows = 16;  // max_t_q * group up to here
-size_t paged_many_workspace(int width, int sms);
-int paged_many_launch(const paged::Pass& pass, bool fp16, void* workspace, cudaStream_t stream);
 size_t paged_few_workspace(int rows, int width, int sms);
-int paged_few_launch(const paged::Pass& pass, bool fp16, int rows, void* workspace, cudaStream_t stream);
-// `many`: parts of many rows and few workers each (a warp takes a row), else of few rows and many workers (a block takes a row)
-int paged_join_launch(const paged::Pass& pass, bool fp16, bool many, cudaStream_t stream);
+int paged_few_launch(const paged::Pass& pass, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream);
+size_t paged_many_workspace(int width, int sms);
+int paged_many_launch(const paged::Pass& pass, bool fp16, unsigned char* workspace, cudaStream_t stream);
+// A row's parts to a warp, or to the eight warps of a block.
+int paged_join_launch(const paged::Pass& pass, bool fp16, bool warp_a_row, cudaStream_t stream);
 
 }  // namespace limn_b200

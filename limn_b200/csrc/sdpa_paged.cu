@@ -14,23 +14,24 @@ using namespace paged;
 size_t pass_workspace(long long rows, int width, int sms) {
   return rows <= kPagedFewRows ? paged_few_workspace(static_cast<int>(rows), width, sms) : paged_many_workspace(width, sms);
 }
-int launch_pass(const Pass& pass, bool fp16, long long rows, void* workspace, cudaStream_t stream) {
+int launch_pass(const Pass& pass, bool fp16, long long rows, unsigned char* workspace, cudaStream_t stream) {
   return rows <= kPagedFewRows ? paged_few_launch(pass, fp16, static_cast<int>(rows), workspace, stream) : paged_many_launch(pass, fp16, workspace, stream);
 }
 
-// The workspace of a call: the parts of whichever pass has more, and behind them the rows' sums over the prefix.
+// The workspace of a call: the parts of the pass over the own keys, those of the pass over the prefix (the kernel that joins them may still run when the
+// other pass begins), and the rows' sums over the prefix.
 struct Workspace {
-  size_t parts, sums, stats;
-  size_t bytes() const { return parts + sums + stats; }
+  size_t own, front, sums, stats;
+  size_t bytes() const { return own + front + sums + stats; }
 };
 int workspace_of(const limn_b200_paged* step, int prefix_len, Workspace* w) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int width = step->hd <= 64 && step->hd_v <= 64 ? 64 : 128;
   const long long group = step->heads / step->kv_heads;
-  const size_t own = pass_workspace(step->max_t_q * group, width, sms), front = prefix_len > 0 ? pass_workspace(step->tokens * group, width, sms) : 0;
-  w->parts = ((own > front ? own : front) + 255) / 256 * 256;
   const size_t rows = static_cast<size_t>(step->tokens) * step->heads;
+  w->own = pass_workspace(step->max_t_q * group, width, sms);
+  w->front = prefix_len > 0 ? pass_workspace(step->tokens * group, width, sms) : 0;
   w->sums = prefix_len > 0 ? rows * width * 4 : 0, w->stats = prefix_len > 0 ? rows * 8 : 0;
   return LIMN_B200_OK;
 }
@@ -64,17 +65,18 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   prm.causal = causal != 0, prm.scale = static_cast<float>(scale);
   const bool fp16 = step->dtype == LIMN_B200_F16;
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
+  unsigned char* memory = static_cast<unsigned char*>(workspace);
   if (prefix_len > 0) {
     // every row over the prefix, as one sequence of all tokens that sees all of it; tokens that belong to no sequence get sums
     // too, which nothing reads
     Pass front = prm;
     front.table = prefix_table, front.q_start = nullptr, front.kv_lens = nullptr, front.keys = prefix_len, front.batch = 1, front.causal = 0;
-    front.leave.o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + w.parts);
-    front.leave.ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + w.parts + w.sums);
-    if (int rc = launch_pass(front, fp16, static_cast<long long>(step->tokens) * prm.group, workspace, on)) return rc;
+    front.leave.o = reinterpret_cast<float*>(memory + w.own + w.front);
+    front.leave.ml = reinterpret_cast<float2*>(memory + w.own + w.front + w.sums);
+    if (int rc = launch_pass(front, fp16, static_cast<long long>(step->tokens) * prm.group, memory + w.own, on)) return rc;
     prm.join = front.leave;
   }
-  return launch_pass(prm, fp16, static_cast<long long>(step->max_t_q) * prm.group, workspace, on);
+  return launch_pass(prm, fp16, static_cast<long long>(step->max_t_q) * prm.group, memory, on);
 }
 
 }  // namespace

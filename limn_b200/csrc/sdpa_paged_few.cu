@@ -2,9 +2,10 @@
 // to 16): generation from a cache. K and V are read once, and that is the time it takes; the arithmetic has to stay out of the way.
 //
 // Work is cut into equal shares, whatever the sequences' lengths: the unit is 16 keys of one (sequence, key head), every warp of the
-// grid takes the same number of consecutive units, and what it has of a problem that its neighbours share goes into its parts
-// (paged.h), joined by a kernel behind this one. A warp works alone: it copies its units' rows into its own ring in shared memory with
-// 16-byte asynchronous copies, so that bytes are in flight all the time and nothing waits for other warps.
+// grid takes the same number of consecutive units. A warp works alone: it copies its units' rows into its own ring in shared memory with
+// 16-byte asynchronous copies, so that bytes are in flight all the time and nothing waits for other warps. What it has of a problem that
+// its neighbours share it leaves in memory; at the end the block puts its warps' parts together, and a problem that reaches into other
+// blocks is joined by a kernel behind this one (paged.h).
 //
 // Per unit, with mma.sync m16n8k16 and the keys as M so that 8 query rows are enough for a tile:
 //   S^T (16 keys x rows) = K Q^T            A = K by ldmatrix, B = Q, in registers
@@ -27,6 +28,7 @@ using namespace paged;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;  // keys
+constexpr int kBegin = 3;  // units that a problem costs besides its keys: its queries, its page table, its way out
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;
 
@@ -68,27 +70,62 @@ struct Ring {
   static constexpr int kBytes = kWarps * kWarpBytes;  // 192 KB
 };
 
-// Where a warp is in the work: unit `unit` of `units` of problem (b, kv_head).
+// Where a warp is in the work: unit `unit` of `units` of problem (b, kv_head), `cost` into its share. What a problem costs besides its keys
+// lies in front of its first unit, which belongs to whoever has that place.
 struct Cursor {
-  int b, kv_head, unit, units;
+  int b, kv_head, unit, units, cost;
   Extent e;
 };
 __device__ __forceinline__ int units_of(const Extent& e) { return e.n == 0 ? 0 : max(1, (e.keys + kUnit - 1) / kUnit); }
+__device__ __forceinline__ int cost_of(const Extent& e) { return e.n == 0 ? 0 : kBegin + units_of(e); }
 __device__ __forceinline__ void next_problem(const Pass& prm, Cursor& c) {
-  c.unit = 0;
+  c.unit = 0, c.cost += kBegin;
   if (++c.kv_head < prm.kv_heads) return;
   c.kv_head = 0, c.units = 0;
   while (c.units == 0 && ++c.b < prm.batch) c.e = extent_of(prm, c.b), c.units = units_of(c.e);
 }
 
+// A row on its way out: four columns of its sums, to where the pass wants them.
+template <int D, bool kFp16>
+__device__ __forceinline__ void finish4(const Pass& prm, const RowPlace& place, int column, float4 acc, float m, float l, float sl2) {
+  if (prm.leave.o != nullptr) {
+    *reinterpret_cast<float4*>(prm.leave.o + place.row * D + column) = acc;
+    if (column == 0) prm.leave.ml[place.row] = make_float2(m, l);
+    return;
+  }
+  if (prm.join.o != nullptr) {
+    const float2 ml = prm.join.ml[place.row];
+    const float4 o = *reinterpret_cast<const float4*>(prm.join.o + place.row * D + column);
+    float keep, add;
+    merge_stats(m, l, ml.x, ml.y, sl2, keep, add);
+    acc = make_float4(acc.x * keep + o.x * add, acc.y * keep + o.y * add, acc.z * keep + o.z * add, acc.w * keep + o.w * add);
+  }
+  const float inv = 1.f / l;  // (no key: 0 * inf = NaN)
+  if (column < prm.pieces_v * 8)
+    *reinterpret_cast<uint2*>(place.out + 2 * column) = kFp16 ? make_uint2(ptx::pack_f16(acc.x * inv, acc.y * inv), ptx::pack_f16(acc.z * inv, acc.w * inv))
+                                                              : make_uint2(ptx::pack_bf16(acc.x * inv, acc.y * inv), ptx::pack_bf16(acc.z * inv, acc.w * inv));
+  if (column == 0) prm.lse[place.row] = m * prm.scale + logf(l);
+}
+
+// What a warp has of problems that its neighbours share, for the block to put together.
+struct Shared {
+  int enters, through;      // part 2 w is there; and its problem goes on behind this warp
+  int begins;               // part 2 w + 1 is there: a problem begins here and goes on
+  int first[2], n[2], kv_head[2];  // of either
+  long long end;            // the unit behind the beginning problem's last
+};
+
 template <int D, bool kFp16, int NT>
-__global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass prm, const int least) {
+__global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass prm, const Parts by_warp) {
   using R = Ring<D>;
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ long long share_end[kThreads];  // units of the sequences up to and with a thread's, per key head
+  __shared__ long long share_end[kThreads];  // cost of the sequences up to and with a thread's, per key head
+  __shared__ Shared shared[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float sl2 = prm.scale * kLog2e;
-  ptx::grid_dependency_wait();
+  // (behind a pass over a prefix all but its last kernel are done when this one begins, and only the rows' way out needs that one)
+  const bool late = prm.join.o != nullptr;
+  if (!late) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
   // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
@@ -97,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     long long mine = 0;
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
-      if (b < prm.batch) mine += units_of(extent_of(prm, b));
+      if (b < prm.batch) mine += cost_of(extent_of(prm, b));
     }
     long long upto = mine;
 #pragma unroll
@@ -114,31 +151,32 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   }
   const int worker = blockIdx.x * kWarps + warp;
   const long long total = share_end[kThreads - 1] * prm.kv_heads;
-  long long share = (total + prm.parts.workers - 1) / prm.parts.workers;
-  if (share < least) share = least;
-  const long long from = worker * share, to = min(total, from + share);
-  if (lane == 0) prm.parts.heads[worker].followers = 0;
-  if (from >= to) return;
+  const long long share = quotient(total + by_warp.workers - 1, by_warp.workers);
+  const long long from = min(total, worker * share), to = min(total, from + share);
+  const int span = static_cast<int>(to - from);
+  if (lane == 0) shared[warp].enters = shared[warp].begins = 0;
+  if (threadIdx.x == 0) prm.parts.heads[blockIdx.x].followers = 0;
 
-  Cursor at;
-  {
+  Cursor at = {};
+  if (span > 0) {
     // the run of sequences that `from` falls into: how many threads' sums end at or before it
     int before = 0;
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) before += __popc(__ballot_sync(0xffffffffu, share_end[i * 32 + lane] * prm.kv_heads <= from));
     long long rest = from - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
     at.b = before * run - 1;
+    int cost;
     do {
       ++at.b;
       at.e = extent_of(prm, at.b);
-      at.units = units_of(at.e);
-      if (rest < static_cast<long long>(at.units) * prm.kv_heads) break;
-      rest -= static_cast<long long>(at.units) * prm.kv_heads;
+      at.units = units_of(at.e), cost = cost_of(at.e);
+      if (rest < static_cast<long long>(cost) * prm.kv_heads) break;
+      rest -= static_cast<long long>(cost) * prm.kv_heads;
     } while (at.b + 1 < prm.batch);
-    at.kv_head = static_cast<int>(rest / at.units);
-    at.unit = static_cast<int>(rest - static_cast<long long>(at.kv_head) * at.units);
+    at.kv_head = static_cast<int>(quotient(rest, cost));
+    const int into = static_cast<int>(rest - static_cast<long long>(at.kv_head) * cost);
+    at.unit = max(0, into - kBegin), at.cost = max(0, kBegin - into);
   }
-  const int steps = static_cast<int>(to - from);
 
   // ---- copies: run ahead of the arithmetic with a cursor of their own ----
   Cursor ahead = at;
@@ -155,8 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     return key < c.e.keys ? prm.table[static_cast<long long>(c.b) * prm.max_pages + key / prm.page_size] : 0;
   };
   auto issue = [&]() {
-    if (loaded < steps) {
-      if (ahead.unit == ahead.units) next_problem(prm, ahead), block = -1;
+    if (ahead.cost < span) {
       const int blk = ahead.unit / 16;
       if (blk != block) {
         const int raw = block >= 0 && blk == block + 1 ? entry_next : entry_of(ahead, blk);
@@ -185,7 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
           copy16(v_to + place, v_from + r * prm.v.slot, there && piece < prm.pieces_v);
         }
       }
-      ++ahead.unit, ++loaded;
+      ++loaded, ++ahead.cost;
+      if (++ahead.unit == ahead.units && ahead.cost + kBegin < span) next_problem(prm, ahead), block = -1;
     }
     copies_commit();
   };
@@ -224,8 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     }
     least_limit = prm.causal ? at.e.keys - at.e.n + 1 : at.e.keys;
   };
-  begin();
-  for (int step = 0; step < steps; ++step) {
+  if (at.cost < span) begin();
+  bool waited = !late;
+  for (int step = 0; at.cost < span; ++step) {
     copies_wait<R::kStages - 2>();
     __syncwarp();
     issue();
@@ -246,19 +285,21 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       for (int nt = 0; nt < NT; ++nt) mma<kFp16>(s[nt], a, q[nt][kk][0], q[nt][kk][1]);
     }
     const int key = at.unit * kUnit + kq;
-    if ((none >> (2 * place_at)) & 3u) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if ((none >> (2 * place_at + (c >> 1))) & 1u) s[nt][c] = NAN;
-    }
     if (at.unit * kUnit + kUnit > least_limit) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           if (key + (c >> 1) * 8 >= limit[nt][c & 1]) s[nt][c] = -INFINITY;
+    }
+    const unsigned none_here = (none >> (2 * place_at)) & 3u;
+    if (none_here != 0u) {  // a row that sees a key of a page that is none: l is NaN from here on
+      const int seen_from = at.unit * kUnit + (none_here & 1u ? 0 : 8);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (seen_from < limit[nt][c]) l[nt][c] = NAN;
     }
     uint32_t p[NT][2];
     bool moved = false;
@@ -300,9 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) mma<kFp16>(o[nt][mt], a, p[nt][0], p[nt][1]);
     }
-    ++at.unit;
+    ++at.unit, ++at.cost;
     const bool ends = at.unit == at.units;
-    if (!ends && step + 1 < steps) continue;
+    if (!ends && at.cost < span) continue;
 
     // ---- the problem, or this warp's part of it, is done ----
 #pragma unroll
@@ -312,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
     const bool whole = begun && ends;
-    const int part = 2 * worker + (begun ? 1 : 0);
+    if (!waited && whole) ptx::grid_dependency_wait(), waited = true;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -320,8 +361,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
         const int r = nt * 8 + cq * 2 + c;
         if (r >= at.e.n * prm.group) continue;
         if (!whole || prm.leave.o != nullptr) {
-          float* to_o = prm.parts.o + (static_cast<long long>(part) * (NT * 8) + r) * D;
-          float2* to_ml = prm.parts.ml + static_cast<long long>(part) * (NT * 8) + r;
+          const long long part = (2LL * worker + (begun ? 1 : 0)) * (NT * 8) + r;
+          float* to_o = by_warp.o + part * D;
+          float2* to_ml = by_warp.ml + part;
           if (whole) {
             const long long row = row_place(prm, at.e.first, at.kv_head, r).row;
             to_o = prm.leave.o + row * D, to_ml = prm.leave.ml + row;
@@ -333,14 +375,15 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
         }
         const RowPlace place = row_place(prm, at.e.first, at.kv_head, r);
         float keep = 1.f, add = 0.f, top = m[nt][c], sum = l[nt][c];
-        const float* more = nullptr;
+        float more[D / 16][2];
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) more[mt][0] = more[mt][1] = 0.f;
         if (prm.join.o != nullptr) {
+          const float* from_o = prm.join.o + place.row * D + kq;
           const float2 ml = prm.join.ml[place.row];
-          more = prm.join.o + place.row * D;
-          top = fmaxf(top, ml.x);
-          const float base = top == -INFINITY ? 0.f : top;
-          keep = exp2f((m[nt][c] - base) * sl2), add = exp2f((ml.x - base) * sl2);
-          sum = sum * keep + ml.y * add;
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt) more[mt][0] = from_o[mt * 16], more[mt][1] = from_o[mt * 16 + 8];
+          merge_stats(top, sum, ml.x, ml.y, sl2, keep, add);
         }
         const float inv = 1.f / sum;  // (no key: 0 * inf = NaN)
 #pragma unroll
@@ -349,120 +392,143 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
           for (int half = 0; half < 2; ++half) {
             if (mt * 2 + half >= prm.pieces_v) continue;
             const int column = mt * 16 + half * 8 + kq;
-            float value = o[nt][mt][c + 2 * half];
-            if (more != nullptr) value = value * keep + more[column] * add;
-            value *= inv;
+            const float value = (o[nt][mt][c + 2 * half] * keep + more[mt][half] * add) * inv;
             if (kFp16) *reinterpret_cast<__half*>(place.out + 2 * column) = __float2half_rn(value);
             else *reinterpret_cast<__nv_bfloat16*>(place.out + 2 * column) = __float2bfloat16_rn(value);
           }
         if (kq == 0) prm.lse[place.row] = top * prm.scale + logf(sum);
       }
-    if (begun && !ends && lane == 0) {
-      const long long behind = at.units - at.unit;  // units of the problem that the next workers have
-      prm.parts.heads[worker] = Head{static_cast<int>((behind + share - 1) / share), at.e.first, at.e.n, at.kv_head, 0, kPagedFewRows};
+    if (!whole && lane == 0) {
+      Shared& mine_shared = shared[warp];
+      const int which = begun ? 1 : 0;
+      mine_shared.first[which] = at.e.first, mine_shared.n[which] = at.e.n, mine_shared.kv_head[which] = at.kv_head;
+      if (begun) mine_shared.begins = 1, mine_shared.end = to + at.units - at.unit;
+      else mine_shared.enters = 1, mine_shared.through = !ends;
     }
-    if (step + 1 < steps) {
-      next_problem(prm, at);
-      begun = true;
-      begin();
+    if (!ends || at.cost + kBegin >= span) break;
+    next_problem(prm, at);
+    begun = true;
+    begin();
+  }
+  if (!waited) ptx::grid_dependency_wait();
+
+  // ---- the block's parts: chain 0 enters from the block before, chain 1 + w begins with warp w ----
+  __syncthreads();
+  int turn = 0;
+  for (int chain = 0; chain <= kWarps; ++chain) {
+    if (!(chain == 0 ? shared[0].enters : shared[chain - 1].begins)) continue;
+    int members = 0;  // warps chain, chain + 1, ... that it enters
+    bool open = true;
+    while (open && chain + members < kWarps) open = shared[chain + members].through != 0, ++members;
+    const Shared& at_head = shared[chain == 0 ? 0 : chain - 1];
+    const int which = chain == 0 ? 0 : 1;
+    const int rows = at_head.n[which] * prm.group;
+    const int warp0 = blockIdx.x * kWarps + chain;  // the first worker it enters
+    if (chain > 0 && open && threadIdx.x == 0) {
+      const int last = static_cast<int>(quotient(quotient(at_head.end - 1, share), kWarps));  // the block that has the problem's last unit
+      prm.parts.heads[blockIdx.x] = Head{last - static_cast<int>(blockIdx.x), at_head.first[which], at_head.n[which], at_head.kv_head[which], 0, kPagedFewRows};
+    }
+    for (int r = 0; r < rows; ++r) {
+      if (turn++ % kWarps != warp) continue;
+      constexpr int kLanesO = D / 4;
+      const int column = (lane % kLanesO) * 4;
+      float2 ml[kWarps];
+      float4 sums[kWarps];
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {  // the beginning's own part first (chain > 0), then those it enters
+        const int member = i - which;
+        const long long part = (member < 0 ? 2LL * (warp0 - 1) + 1 : 2LL * (warp0 + member)) * (NT * 8) + r;
+        ml[i] = make_float2(-INFINITY, 0.f), sums[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (member < members) ml[i] = by_warp.ml[part], sums[i] = *reinterpret_cast<const float4*>(by_warp.o + part * D + column);
+      }
+      float m = ml[0].x, l = ml[0].y;
+      float4 acc = sums[0];
+#pragma unroll
+      for (int i = 1; i < kWarps; ++i) {
+        float keep, add;
+        merge_stats(m, l, ml[i].x, ml[i].y, sl2, keep, add);
+        acc = make_float4(acc.x * keep + sums[i].x * add, acc.y * keep + sums[i].y * add, acc.z * keep + sums[i].z * add, acc.w * keep + sums[i].w * add);
+      }
+      if (lane >= kLanesO) continue;
+      if (chain > 0 && !open) {
+        finish4<D, kFp16>(prm, row_place(prm, at_head.first[which], at_head.kv_head[which], r), column, acc, m, l, sl2);
+      } else {
+        const long long part = (2LL * blockIdx.x + which) * (NT * 8) + r;
+        *reinterpret_cast<float4*>(prm.parts.o + part * D + column) = acc;
+        if (column == 0) prm.parts.ml[part] = make_float2(m, l);
+      }
     }
   }
 }
 
 // ---- joining the parts ----
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = 8;
 
-// A row of one problem: kSplit warps share its parts, a lane has 4 columns (the last warps of a row with fewer than 128 columns idle).
+// A row of one problem: kSplit warps share its parts, a lane has 4 columns.
 template <int D, bool kFp16, int kSplit>
 __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const Pass prm) {
   constexpr int kRows = kJoinWarps / kSplit;
-  constexpr int kLanes = D / 4;            // lanes to a row
-  constexpr int kAtOnce = 32 / kLanes;     // parts a warp takes side by side
+  constexpr int kLanesO = D / 4;           // lanes to a row
+  constexpr int kAtOnce = 32 / kLanesO;    // parts a warp takes side by side
+  constexpr int kUnroll = 4;
   __shared__ float4 sums[kJoinWarps][32];
   __shared__ float2 stats[kJoinWarps];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
+  const Head head = prm.parts.heads[blockIdx.x];
+  if (head.followers == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.y * kRows + warp / kSplit, split = warp % kSplit;
-  const int column = (lane % kLanes) * 4, side = lane / kLanes;
+  const int column = (lane % kLanesO) * 4, side = lane / kLanesO;
   const float sl2 = prm.scale * kLog2e;
-  for (int w = blockIdx.x; w < prm.parts.workers; w += gridDim.x) {
-    const Head head = prm.parts.heads[w];
-    if (head.followers == 0) continue;  // (the same in the whole block)
-    const int row = head.row0 + r / 128 * head.tile_rows + r % 128;
-    const bool there = r % 128 < head.tile_rows && row < head.n * prm.group;
-    // part 0 is the head's, part i the i-th follower's
-    auto part = [&](int i) { return static_cast<long long>(i == 0 ? 2 * w + 1 : 2 * (w + i)) * prm.parts.rows + r; };
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (there) {
-      constexpr int kUnroll = 4;
-      for (int i0 = split * kAtOnce + side; i0 <= head.followers; i0 += kUnroll * kSplit * kAtOnce) {
-        float2 ml[kUnroll];
-        float4 o[kUnroll];
+  const int row = head.row0 + r / 128 * head.tile_rows + r % 128;
+  if (r % 128 >= head.tile_rows || row >= head.n * prm.group) return;  // (in the whole block, or without a barrier behind it)
+  // part 0 is the head's, part i the i-th follower's
+  auto part = [&](int i) { return (i == 0 ? 2LL * blockIdx.x + 1 : 2LL * (blockIdx.x + i)) * prm.parts.rows + r; };
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto fold = [&](float m_b, float l_b, const float4& o_b) {
+    float keep, add;
+    merge_stats(m, l, m_b, l_b, sl2, keep, add);
+    acc = make_float4(acc.x * keep + o_b.x * add, acc.y * keep + o_b.y * add, acc.z * keep + o_b.z * add, acc.w * keep + o_b.w * add);
+  };
+  for (int i0 = split * kAtOnce + side; i0 <= head.followers; i0 += kUnroll * kSplit * kAtOnce) {
+    float2 ml[kUnroll];
+    float4 o[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int i = i0 + u * kSplit * kAtOnce;
-          ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (i > head.followers) continue;
-          ml[u] = prm.parts.ml[part(i)];
-          // (a part that has seen no key has no sums)
-          if (!(ml[u].x == -INFINITY && ml[u].y == 0.f)) o[u] = *reinterpret_cast<const float4*>(prm.parts.o + part(i) * D + column);
-        }
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * kSplit * kAtOnce;
+      ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i <= head.followers) ml[u] = prm.parts.ml[part(i)], o[u] = *reinterpret_cast<const float4*>(prm.parts.o + part(i) * D + column);
+    }
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const float top = fmaxf(m, ml[u].x), base = top == -INFINITY ? 0.f : top;
-          const float keep = exp2f((m - base) * sl2), add = exp2f((ml[u].x - base) * sl2);
-          m = top, l = l * keep + ml[u].y * add;
-          acc.x = acc.x * keep + o[u].x * add, acc.y = acc.y * keep + o[u].y * add, acc.z = acc.z * keep + o[u].z * add, acc.w = acc.w * keep + o[u].w * add;
-        }
-      }
+    for (int u = 0; u < kUnroll; ++u) {
+      // (a part that has seen no key has no sums: what lies there is not looked at)
+      if (ml[u].x == -INFINITY && ml[u].y == 0.f) continue;
+      fold(ml[u].x, ml[u].y, o[u]);
     }
-    auto fold = [&](float m_b, float l_b, const float4& o_b) {
-      const float top = fmaxf(m, m_b), base = top == -INFINITY ? 0.f : top;
-      const float keep = exp2f((m - base) * sl2), add = exp2f((m_b - base) * sl2);
-      m = top, l = l * keep + l_b * add;
-      acc.x = acc.x * keep + o_b.x * add, acc.y = acc.y * keep + o_b.y * add, acc.z = acc.z * keep + o_b.z * add, acc.w = acc.w * keep + o_b.w * add;
-    };
-#pragma unroll
-    for (int d = kLanes; d < 32; d <<= 1) {
-      const float4 other = make_float4(__shfl_down_sync(0xffffffffu, acc.x, d), __shfl_down_sync(0xffffffffu, acc.y, d), __shfl_down_sync(0xffffffffu, acc.z, d),
-                                       __shfl_down_sync(0xffffffffu, acc.w, d));
-      const float m_b = __shfl_down_sync(0xffffffffu, m, d), l_b = __shfl_down_sync(0xffffffffu, l, d);
-      fold(m_b, l_b, other);
-    }
-    if (kSplit > 1) {
-      __syncthreads();  // (what the last problem left has been read)
-      if (split > 0) {
-        sums[warp][lane] = acc;
-        if (lane == 0) stats[warp] = make_float2(m, l);
-      }
-      __syncthreads();
-      if (split > 0) continue;
-#pragma unroll 1
-      for (int i = 1; i < kSplit; ++i) fold(stats[warp + i].x, stats[warp + i].y, sums[warp + i][lane]);
-    }
-    if (!there || side > 0) continue;
-    const RowPlace place = row_place(prm, head.first, head.kv_head, row);
-    if (prm.leave.o != nullptr) {
-      *reinterpret_cast<float4*>(prm.leave.o + place.row * D + column) = acc;
-      if (lane == 0) prm.leave.ml[place.row] = make_float2(m, l);
-      continue;
-    }
-    if (prm.join.o != nullptr) {
-      const float2 ml = prm.join.ml[place.row];
-      fold(ml.x, ml.y, *reinterpret_cast<const float4*>(prm.join.o + place.row * D + column));
-    }
-    const float inv = 1.f / l;
-    if (column < prm.pieces_v * 8)
-      *reinterpret_cast<uint2*>(place.out + 2 * column) = kFp16 ? make_uint2(ptx::pack_f16(acc.x * inv, acc.y * inv), ptx::pack_f16(acc.z * inv, acc.w * inv))
-                                                                : make_uint2(ptx::pack_bf16(acc.x * inv, acc.y * inv), ptx::pack_bf16(acc.z * inv, acc.w * inv));
-    if (lane == 0) prm.lse[place.row] = m * prm.scale + logf(l);
   }
+  __syncwarp();
+#pragma unroll
+  for (int d = kLanesO; d < 32; d <<= 1) {
+    const float4 other = make_float4(__shfl_down_sync(0xffffffffu, acc.x, d), __shfl_down_sync(0xffffffffu, acc.y, d), __shfl_down_sync(0xffffffffu, acc.z, d),
+                                     __shfl_down_sync(0xffffffffu, acc.w, d));
+    const float m_b = __shfl_down_sync(0xffffffffu, m, d), l_b = __shfl_down_sync(0xffffffffu, l, d);
+    fold(m_b, l_b, other);
+  }
+  if (kSplit > 1) {
+    sums[warp][lane] = acc;
+    if (lane == 0) stats[warp] = make_float2(m, l);
+    __syncthreads();
+    if (split > 0) return;
+#pragma unroll
+    for (int i = 1; i < kSplit; ++i) fold(stats[warp + i].x, stats[warp + i].y, sums[warp + i][lane]);
+  }
+  if (side == 0) finish4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row), column, acc, m, l, sl2);
 }
 
 template <int D, bool kFp16, int NT>
-int launch_few(const Pass& pass, cudaStream_t stream) {
+int launch_few(const Pass& pass, const Parts& by_warp, cudaStream_t stream) {
   auto kernel = sdpa_paged_few_kernel<D, kFp16, NT>;
   static bool sized[64] = {};
   int device = 0;
@@ -471,51 +537,53 @@ int launch_few(const Pass& pass, cudaStream_t stream) {
     LIMN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<D>::kBytes), "sizing shared memory for the paged sdpa kernel");
     sized[device] = true;
   }
-  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers / kWarps)), dim3(kThreads), Ring<D>::kBytes, stream, pass, 1), "launching the paged sdpa kernel");
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers)), dim3(kThreads), Ring<D>::kBytes, stream, pass, by_warp), "launching the paged sdpa kernel");
   note_launches(1);
   return LIMN_B200_OK;
 }
 
+template <int D, bool kFp16, int kSplit>
+int launch_join(const Pass& pass, cudaStream_t stream) {
+  const unsigned rows = static_cast<unsigned>((pass.parts.rows * kSplit + kJoinWarps - 1) / kJoinWarps);
+  LIMN_CUDA(launch_overlapped(sdpa_paged_join_kernel<D, kFp16, kSplit>, dim3(static_cast<unsigned>(pass.parts.workers), rows), dim3(kJoinWarps * 32), 0, stream, pass),
+            "launching the kernel that joins parts");
+  note_launches(1);
+  return LIMN_B200_OK;
+}
+
+int few_tile(int rows) { return rows <= 8 ? 8 : kPagedFewRows; }
+
 }  // namespace
 
-size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(sms * kWarps, rows <= 8 ? 8 : 16, width <= 64 ? 64 : 128); }
+size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(sms, few_tile(rows), width) + Parts::bytes(sms * kWarps, few_tile(rows), width); }
 
-int paged_few_launch(const Pass& given, bool fp16, int rows, void* workspace, cudaStream_t stream) {
+int paged_few_launch(const Pass& given, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream) {
   Pass pass = given;
+  Parts by_warp;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
-  pass.parts.place(workspace, sms * kWarps, rows <= 8 ? 8 : 16, width);
+  pass.parts.place(workspace, sms, few_tile(rows), width);
+  by_warp.place(workspace + Parts::bytes(sms, few_tile(rows), width), sms * kWarps, few_tile(rows), width);
   int rc;
   if (width == 64) {
-    if (rows <= 8) rc = fp16 ? launch_few<64, true, 1>(pass, stream) : launch_few<64, false, 1>(pass, stream);
-    else rc = fp16 ? launch_few<64, true, 2>(pass, stream) : launch_few<64, false, 2>(pass, stream);
+    if (rows <= 8) rc = fp16 ? launch_few<64, true, 1>(pass, by_warp, stream) : launch_few<64, false, 1>(pass, by_warp, stream);
+    else rc = fp16 ? launch_few<64, true, 2>(pass, by_warp, stream) : launch_few<64, false, 2>(pass, by_warp, stream);
   } else {
-    if (rows <= 8) rc = fp16 ? launch_few<128, true, 1>(pass, stream) : launch_few<128, false, 1>(pass, stream);
-    else rc = fp16 ? launch_few<128, true, 2>(pass, stream) : launch_few<128, false, 2>(pass, stream);
+    if (rows <= 8) rc = fp16 ? launch_few<128, true, 1>(pass, by_warp, stream) : launch_few<128, false, 1>(pass, by_warp, stream);
+    else rc = fp16 ? launch_few<128, true, 2>(pass, by_warp, stream) : launch_few<128, false, 2>(pass, by_warp, stream);
   }
   if (rc) return rc;
   return paged_join_launch(pass, fp16, false, stream);
 }
 
-namespace {
-template <int D, bool kFp16, int kSplit>
-int launch_join(const Pass& pass, unsigned across, cudaStream_t stream) {
-  const unsigned rows = (pass.parts.rows * kSplit + kJoinWarps - 1) / kJoinWarps;
-  LIMN_CUDA(launch_overlapped(sdpa_paged_join_kernel<D, kFp16, kSplit>, dim3(across, rows), dim3(kJoinWarps * 32), 0, stream, pass), "launching the kernel that joins parts");
-  note_launches(1);
-  return LIMN_B200_OK;
-}
-}  // namespace
-
-int paged_join_launch(const Pass& pass, bool fp16, bool many, cudaStream_t stream) {
-  const unsigned across = static_cast<unsigned>(pass.parts.workers < 148 ? pass.parts.workers : 148);
-  if (many) {
-    if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 1>(pass, across, stream) : launch_join<64, false, 1>(pass, across, stream);
-    return fp16 ? launch_join<128, true, 1>(pass, across, stream) : launch_join<128, false, 1>(pass, across, stream);
+int paged_join_launch(const Pass& pass, bool fp16, bool warp_a_row, cudaStream_t stream) {
+  if (warp_a_row) {
+    if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 1>(pass, stream) : launch_join<64, false, 1>(pass, stream);
+    return fp16 ? launch_join<128, true, 1>(pass, stream) : launch_join<128, false, 1>(pass, stream);
   }
-  if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 16>(pass, across, stream) : launch_join<64, false, 16>(pass, across, stream);
-  return fp16 ? launch_join<128, true, 16>(pass, across, stream) : launch_join<128, false, 16>(pass, across, stream);
+  if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 8>(pass, stream) : launch_join<64, false, 8>(pass, stream);
+  return fp16 ? launch_join<128, true, 8>(pass, stream) : launch_join<128, false, 8>(pass, stream);
 }
 
 }  // namespace limn_b200

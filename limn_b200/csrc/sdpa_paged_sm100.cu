@@ -13,12 +13,12 @@
 // Lengths are known on the device only, and they differ. So the work is cut there, into equal shares of (item, key) cost, one share to a
 // CTA and one CTA to an SM: a share is the rest of an item, whole items, and the beginning of one. Whole items go to the result; what a
 // CTA has of an item that others share goes into its parts (paged.h), which a kernel behind this one joins. The cost of an item is the number of keys its last
-// token sees, half of it where one tile has both places; its sum over a sequence has a closed form, and so has the share a CTA begins
+// token sees, half of it where one tile has both places, and a constant; its sum over a sequence has a closed form, and so has the share a CTA begins
 // with: nothing is planned on the host or by a kernel in front.
 //
-// Keys past a sequence's end are zeros (a page coordinate outside the cache makes TMA fill them), except those of its last page, which
-// hold whatever lies there: their scores are replaced, and their rows of V are zeroed before the product that reads them, since
-// 0 * NaN would reach every row.
+// Past a sequence's end a tile holds what its last page has there, or what the stage held before: the scores are replaced, and the rows of V
+// are zeroed before the product that reads them, since 0 * NaN would reach every row. (Boxes outside the cache, which TMA fills with zeros,
+// would do too: pages that are none are fetched so.)
 //
 // Warp roles (10 warps): 0-3 softmax and epilogue of tile 0, 4-7 of tile 1, 8 TMA producer, 9 MMA issuer and tensor-memory owner.
 #include <cuda_bf16.h>
@@ -41,7 +41,8 @@ constexpr int kMmaWarp = 9;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
-constexpr int kLeast = 256;    // cost of the smallest share: a CTA's part of an item costs it a load of Q and a store of sums besides
+constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
+constexpr int kLeast = 512;    // cost of the smallest share
 
 template <int D>
 struct Layout {
@@ -88,7 +89,7 @@ struct Segment {
   int whole;       // and ends with its last
 };
 
-// ---- the cost of items, in keys. A sequence has `pairs` items per key head, pair j of tokens [j span, (j + 1) span) ----
+// ---- the cost of items, in keys (int holds an item's: 2^31 keys would be 2^35 bytes of a head). A sequence has `pairs` items per key head, pair j of tokens [j span, (j + 1) span) ----
 struct Costs {
   int pairs, span, half, seen_first;  // span: tokens of a pair; half: of a tile; seen_first: keys that are there before the first token
   int keys, n, causal;
@@ -97,12 +98,12 @@ struct Costs {
   // keys that the first `tokens` tokens see at most; one, masked, where that is none
   __device__ __forceinline__ int seen(int tokens) const { return max(1, causal ? seen_first + min(tokens, n) : keys); }
   __device__ __forceinline__ bool single(int j) const { return n - j * span <= half; }
-  __device__ __forceinline__ int of(int j) const { return single(j) ? (seen((j + 1) * span) + 1) / 2 : seen((j + 1) * span); }
+  __device__ __forceinline__ int of(int j) const { return kItem + (single(j) ? (seen((j + 1) * span) + 1) / 2 : seen((j + 1) * span)); }
   // sum over the pairs in front of j (all of them two whole tiles)
   __device__ __forceinline__ long long before(long long j) const {
-    if (!causal) return j * max(1, keys);
+    if (!causal) return j * (kItem + max(1, keys));
     const long long none = seen_first >= 0 ? 0 : min(j, static_cast<long long>(-seen_first / span));  // pairs whose last token sees nothing: 1 each
-    return none + (j - none) * seen_first + span * (j * (j + 1) / 2 - none * (none + 1) / 2);
+    return j * kItem + none + (j - none) * seen_first + span * (j * (j + 1) / 2 - none * (none + 1) / 2);
   }
   __device__ __forceinline__ long long all() const { return pairs == 0 ? 0 : before(pairs - 1) + of(pairs - 1); }
   // steps of key tiles (pairs of key tiles for a single tile) of pair j
@@ -110,8 +111,10 @@ struct Costs {
     const int tiles = (seen((j + 1) * span) + kTile - 1) / kTile;
     return single(j) ? (tiles + 1) / 2 : tiles;
   }
-  // the step nearest to `cost` into pair j
-  __device__ __forceinline__ int step_at(int j, long long cost) const { return static_cast<int>(min(static_cast<long long>(steps(j)), (cost + kTile / 2) / kTile)); }
+  // the step nearest to `cost` into pair j; what lies in front of the keys counts as the first one's beginning
+  __device__ __forceinline__ int step_at(int j, long long cost) const {
+    return static_cast<int>(min(static_cast<long long>(steps(j)), max(0LL, cost - kItem + kTile / 2) / kTile));
+  }
 };
 
 struct Place {
@@ -157,7 +160,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     tma_prefetch_descriptor(&maps.v);
   }
   // up to here nothing has touched global memory
-  grid_dependency_wait();
+  // (behind a pass over a prefix all but its last kernel are done when this one begins, and only the rows' way out needs that one)
+  const bool late = prm.join.o != nullptr;
+  if (!late) grid_dependency_wait();
   grid_launch_dependents();
   if (threadIdx.x == 0) {
     abort_flag = *reinterpret_cast<volatile unsigned*>(status) != kStatusOk;  // an earlier kernel gave up: this one stands down
@@ -207,15 +212,22 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   if (warp == kProducerWarp) {
     // ================= the share, and TMA =================
     const long long total = share_end[kThreads - 1] * prm.kv_heads;
-    const long long share = max(static_cast<long long>(kLeast), (total + gridDim.x - 1) / gridDim.x);
-    auto place_of = [&](long long x) {
-      Place p;
-      int before = 0;
+    const long long share = max(static_cast<long long>(kLeast), quotient(total + gridDim.x - 1, gridDim.x));
+    const long long from = blockIdx.x * share, to = from + share;
+    const bool any = ok && from < total;
+    // where the share begins and ends, in the warp's halves
+    Place p = {};
+    if (any) {
+      const long long x = lane < 16 ? from : min(to, total - 1);
+      int before_from = 0, before_to = 0;
 #pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) before += __popc(__ballot_sync(0xffffffffu, share_end[i * 32 + lane] * prm.kv_heads <= x));
-      long long rest = x - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
+      for (int i = 0; i < kThreads / 32; ++i) {
+        const long long end = share_end[i * 32 + lane] * prm.kv_heads;
+        before_from += __popc(__ballot_sync(0xffffffffu, end <= from)), before_to += __popc(__ballot_sync(0xffffffffu, end <= min(to, total - 1)));
+      }
+      const int before = lane < 16 ? before_from : before_to;
+      long long rest = x - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads), all;
       p.b = before * run - 1;
-      long long all;
       do {
         ++p.b;
         p.e = extent_of(prm, p.b);
@@ -224,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         rest -= all * prm.kv_heads;
       } while (p.b + 1 < prm.batch);
       const Costs costs(p.e, tile_tokens, prm.causal);
-      p.kv_head = static_cast<int>(rest / all);
+      p.kv_head = static_cast<int>(quotient(rest, all));
       rest -= p.kv_head * all;
       int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
       while (low < high) {
@@ -235,15 +247,18 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       p.j = low;
       p.into = rest - costs.before(low);
       p.step = costs.step_at(low, p.into);
-      return p;
+      __syncwarp();
+    }
+    auto of_half = [&](int from_lane) {
+      Place q;
+      int* words = reinterpret_cast<int*>(&q);
+      const int* mine = reinterpret_cast<const int*>(&p);
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(Place) / sizeof(int)); ++i) words[i] = __shfl_sync(0xffffffffu, mine[i], from_lane);
+      return q;
     };
-    const long long from = blockIdx.x * share;
-    const bool any = ok && from < total;
-    const long long to = from + share;
-    Place at = {}, end = {};
-    end.b = prm.batch;
-    if (any) at = place_of(from);
-    if (any && to < total) end = place_of(to);
+    Place at = of_half(0), end = of_half(16);
+    if (to >= total) end.b = prm.batch, end.kv_head = end.j = 0;  // nothing ends it
     unsigned n_item = 0, q_uses[2] = {0u, 0u}, step = 0;
     bool more = any;
     // a lane fetches one box of a key tile: `chunk` keys of one page, 64 columns
@@ -280,8 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           mbar_arrive(bar(B::work_full + slot));
           if (s.begun && !s.whole) {
             // workers c behind this one whose share begins inside the item, before the middle of its last step
-            const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), steps * static_cast<long long>(kTile) - kTile / 2);
-            prm.parts.heads[blockIdx.x] = Head{static_cast<int>((begins + limit - 1) / share - blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
+            const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(kTile) - kTile / 2);
+            prm.parts.heads[blockIdx.x] = Head{static_cast<int>(quotient(begins + limit - 1, share)) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
           }
         }
         __syncwarp();
@@ -302,32 +317,34 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         }
         if (!ok) break;
         const int* table = prm.table + static_cast<long long>(s.b) * prm.max_pages;
-        // the page of this lane's box of key tile `tile`; -1, whose boxes TMA fills with zeros, past the end and where it is none
+        // the page of this lane's box of key tile `tile`; one that is none is a coordinate outside the cache, whose box TMA fills with zeros
         auto entry = [&](int tile) {
           const int key = tile * kTile + my_chunk * chunk;
-          return key < s.keys ? table[key / prm.page_size] : -1;
+          return key < s.keys ? table[key / prm.page_size] : 0;
         };
         int page_next = entry(s.first_tile);
         for (int j = 0; j < s.loads && ok; ++j, ++step) {
           const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
-          int page = page_next;
-          if (key < s.keys) page = checked_page(page, prm.pages, prm.errors);
+          const bool fetch = key < s.keys && my_atom < D / 64;
+          const int page = fetch ? checked_page(page_next, prm.pages, prm.errors) : 0;
+          const int boxes = min(chunks, max(0, (s.keys - tile * kTile + chunk - 1) / chunk));  // those that have keys
+          const uint32_t bytes = static_cast<uint32_t>(boxes * chunk) * (D * 2);
           if (j + 1 < s.loads) page_next = entry(tile + 1);
           const int in_page = key % prm.page_size;
           const int stage = step % B::kS;
           const uint32_t wrap = (step / B::kS) & 1;
           ok = wait(B::k_empty + stage, wrap ^ 1u, 0x0100u | stage);
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(bar(B::k_full + stage), L::kTileBytes);
+          if (lane == 0) mbar_expect_tx(bar(B::k_full + stage), bytes);
           __syncwarp();
           const uint32_t box = stage * L::kTileBytes + my_atom * L::kAtomBytes + my_chunk * chunk * 128;
-          if (my_atom < D / 64) tma_load_4d(base + L::kKOff + box, &maps.k, bar(B::k_full + stage), my_atom * 64, in_page, s.kv_head, page);
+          if (fetch) tma_load_4d(base + L::kKOff + box, &maps.k, bar(B::k_full + stage), my_atom * 64, in_page, s.kv_head, page);
           __syncwarp();
           ok = wait(B::v_empty + stage, wrap ^ 1u, 0x0110u | stage);
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(bar(B::v_full + stage), L::kTileBytes);
+          if (lane == 0) mbar_expect_tx(bar(B::v_full + stage), bytes);
           __syncwarp();
-          if (my_atom < D / 64) tma_load_4d(base + L::kVOff + box, &maps.v, bar(B::v_full + stage), my_atom * 64, in_page, s.kv_head, page);
+          if (fetch) tma_load_4d(base + L::kVOff + box, &maps.v, bar(B::v_full + stage), my_atom * 64, in_page, s.kv_head, page);
           __syncwarp();
         }
       }
@@ -374,9 +391,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
 #pragma unroll
       for (int kk = 4 * part; kk < 4 * part + 4; ++kk) mma_ts_lo(c, a + kk * 8, v_lo + kk * (16 * 128 / 16), idesc_pv, (kk > 0 || !first) ? 1u : 0u);
     };
-    // rows [from, to) of the V tile in `stage` become zeros: slots of a sequence's last page that it has not filled
-    auto clear_rows = [&](int stage, int from, int to) {
-      for (int i = from * (D / 8) + lane; i < to * (D / 8); i += 32) {
+    // rows from `from` on of the V tile in `stage` become zeros: slots of a sequence's last page that it has not filled, and what was there before
+    auto clear_rows = [&](int stage, int from) {
+      for (int i = from * (D / 8) + lane; i < kTile * (D / 8); i += 32) {
         const int row = i / (D / 8), piece = i % (D / 8);
         st_shared_v4(base + L::kVOff + stage * L::kTileBytes + (piece / 8) * L::kAtomBytes + row * 128 + (piece % 8) * 16, 0u, 0u, 0u, 0u);
       }
@@ -427,9 +444,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           const int stage = here % B::kS, next = then % B::kS;
           ok = wait(B::v_full + stage, (here / B::kS) & 1, 0x0220u | stage);
           if (!ok) break;
-          const int left = s.keys - (s.first_tile + static_cast<int>(here - step)) * kTile;  // keys of the tile that there are, if fewer than all
-          if (left > 0 && left < kTile && left % chunk != 0 && cleared != here + 1) {
-            clear_rows(stage, left, (left + chunk - 1) / chunk * chunk);
+          const int left = s.keys - (s.first_tile + static_cast<int>(here - step)) * kTile;  // keys of the tile that there are
+          if (left < kTile && cleared != here + 1) {
+            clear_rows(stage, max(0, left));
             cleared = here + 1;
           }
           const uint32_t phase = tiles[t] & 1u;
@@ -488,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     const uint32_t t_o = tmem + lane_base + L::kOCol + t * D;
     const float sl2 = prm.scale * kLog2e;
     const uint64_t sl2_2 = f2_pack(sl2, sl2);
-    const int chunk_log = 31 - __clz(chunk), chunks = kTile >> chunk_log;
+    const int chunks = kTile / chunk;
     unsigned tiles = 0;   // key tiles this group has been through, over all segments
     unsigned o_uses = 0;  // segments it has finished with key tiles
     unsigned merges = 0;
@@ -512,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       const int sees_least = prm.causal ? min(s.keys, seen_first + top_row / prm.group + 1) : s.keys;      // the tile's first token
       const int* table = prm.table + static_cast<long long>(s.b) * prm.max_pages;
       auto key0 = [&](int j) { return (s.first_tile + (both ? 2 * j + t : j)) * kTile; };
-      // pages are looked at once more here, a key tile ahead: scores against one that is none are NaN
+      // pages are looked at once more here, a key tile ahead
       auto entry = [&](int j) {
         const int key = key0(j) + lane * chunk;
         return lane < chunks && key < s.keys ? table[key / prm.page_size] : 0;
@@ -530,13 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x[c]);
         tmem_ld_wait();
         const int kv0 = key0(j);
-        if (none != 0u) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if ((none >> ((c * 32 + i) >> chunk_log)) & 1u) x[c][i] = 0x7fffffffu;  // NaN
-        }
+        // a row that sees a key of a page that is none: l, and with it all of the row, is NaN from here on
+        if (none != 0u && (__ffs(none) - 1) * chunk < sees - kv0) l = NAN;
         if (kv0 + kTile > sees_least) {
           const int limit = sees - kv0;
 #pragma unroll
@@ -629,10 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         ++merges;
         tc_fence_after_sync();
         const float m_1 = *const_cast<volatile float*>(&merge_m[row_in_tile]), l_1 = *const_cast<volatile float*>(&merge_l[row_in_tile]);
-        const float top = fmaxf(m, m_1), zero = top == -INFINITY ? 0.f : top;
-        keep = exp2f((m - zero) * sl2), from_1 = exp2f((m_1 - zero) * sl2);
-        l = l * keep + l_1 * from_1;
-        m = top;
+        merge_stats(m, l, m_1, l_1, sl2, keep, from_1);
       }
       auto take = [&](int col, uint32_t (&o)[32]) {
         tmem_ld32(t_o + col, o);
@@ -650,13 +659,11 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       if (s.whole && prm.leave.o == nullptr) {
         float add = 0.f, mine = 1.f;
         const float* more = nullptr;
-        if (prm.join.o != nullptr && there) {
+        if (late) grid_dependency_wait();
+        if (late && there) {
           const float2 ml = prm.join.ml[place.row];
           more = prm.join.o + place.row * D;
-          const float top = fmaxf(m, ml.x), zero = top == -INFINITY ? 0.f : top;
-          mine = exp2f((m - zero) * sl2), add = exp2f((ml.x - zero) * sl2);
-          l = l * mine + ml.y * add;
-          m = top;
+          merge_stats(m, l, ml.x, ml.y, sl2, mine, add);
         }
         const float inv = 1.f / l;
 #pragma unroll
@@ -675,14 +682,28 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         }
         if (there) prm.lse[place.row] = m * prm.scale + logf(l);
       } else {
-        float* to = s.whole ? prm.leave.o + place.row * D : prm.parts.o + part * D;
+        // to the parts, whose rows follow one another, neighbouring rows' pieces are exchanged first, so that an instruction writes 64
+        // bytes of each row it touches; rows that there are not go along. To the rows' sums every thread writes its own row
+        float* to = s.whole ? prm.leave.o + place.row * D : prm.parts.o + (part - lane + (lane & ~3)) * D + 4 * (lane & 3);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           take(32 * c, o);
-          if (there) {
+          if (s.whole) {
+            if (there) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint32_t w[4][4];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i / 4][i % 4] = o[16 * half + i];
+              swap_rows_for_pieces<4>(w);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(to + i * D + 32 * c + 16 * half) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+            }
           }
         }
         if (there) *(s.whole ? prm.leave.ml + place.row : prm.parts.ml + part) = make_float2(m, l);
@@ -695,6 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   }
 
   // ---- teardown ----
+  if (late) grid_dependency_wait();  // (whoever waits for this kernel has waited for the one before it)
   tc_fence_before_sync();
   __syncthreads();
   if (warp == kMmaWarp) {
@@ -742,7 +764,7 @@ int launch_many(const Pass& pass, unsigned* status, cudaStream_t stream) {
 
 size_t paged_many_workspace(int width, int sms) { return Parts::bytes(sms, 2 * kTile, width); }
 
-int paged_many_launch(const Pass& given, bool fp16, void* workspace, cudaStream_t stream) {
+int paged_many_launch(const Pass& given, bool fp16, unsigned char* workspace, cudaStream_t stream) {
   Pass pass = given;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
