@@ -34,6 +34,7 @@ struct AppendParams {
   int batch, heads, kv_heads;  // heads: 0 without queries
   int width, width_v;          // columns
   int page_size, pages, max_pages, tokens, max_t_q, first_position;
+  Div by_page;
   int rotated;                 // columns
 };
 
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
         if (e.keys < e.n) {  // more tokens than keys: there is no slot for the first of them
           if (lane == 0 && prm.errors != nullptr) atomicOr(prm.errors, LIMN_B200_PAGED_BAD_SEQUENCE);
         } else {
-          page = checked_page(prm.table[static_cast<long long>(low) * prm.max_pages + slot / prm.page_size], prm.pages, prm.errors);
+          page = checked_page(prm.table[static_cast<long long>(low) * prm.max_pages + prm.by_page.of(slot)], prm.pages, prm.errors);
         }
       }
     }
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
     turns[threadIdx.x] = make_float2(c, s);
   }
   __syncthreads();
-  const int in_page = slot % prm.page_size;
+  const int in_page = prm.by_page.rest(slot);
   const long long at = token;
   turn_rows<kFp16, E, kNeighbours>(prm.k + at * prm.k_token, prm.k_head, prm.k_pages.base + page * prm.k_pages.page + in_page * prm.k_pages.slot, prm.k_pages.head,
                                    prm.kv_heads, prm.width, prm.rotated, turns);
@@ -204,6 +205,6 @@ extern "C" int limn_b200_kv_append(const limn_b200_paged* step, const void* q, c
   prm.batch = step->batch, prm.kv_heads = step->kv_heads, prm.width = step->hd, prm.width_v = step->hd_v;
   prm.page_size = step->page_size, prm.pages = step->pages, prm.max_pages = step->max_pages;
   prm.tokens = step->tokens, prm.max_t_q = step->max_t_q, prm.first_position = step->first_position;
-  prm.rotated = rotated;
+  prm.rotated = rotated, prm.by_page = Div(step->page_size);
   return step->dtype == LIMN_B200_F16 ? launch_append<true>(prm, pairing, static_cast<cudaStream_t>(stream)) : launch_append<false>(prm, pairing, static_cast<cudaStream_t>(stream));
 }

@@ -51,6 +51,20 @@ struct RowSums {
   float2* ml = nullptr;  // (tokens * heads)
 };
 
+// Quotients by a number that a launch knows: a product and a shift (exact for numerators from 0 to 2^31 - 1: the factor is 2^(31 + s) / d rounded
+// up, with 2^s >= d, so its excess times the numerator stays below 2^(31 + s) / d).
+struct Div {
+  unsigned d = 1, factor = 1u << 31, shift = 31;
+  Div() = default;
+  explicit Div(int by) : d(static_cast<unsigned>(by)) {
+    unsigned s = 0;
+    while ((1ull << s) < d) ++s;
+    shift = 31 + s, factor = static_cast<unsigned>(((1ull << shift) + d - 1) / d);
+  }
+  __host__ __device__ __forceinline__ int of(int n) const { return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(n)) * factor) >> shift); }
+  __host__ __device__ __forceinline__ int rest(int n) const { return n - of(n) * static_cast<int>(d); }
+};
+
 // A pass of queries over paged keys.
 struct Pass {
   const unsigned char* q = nullptr;
@@ -64,6 +78,7 @@ struct Pass {
   unsigned* errors = nullptr;
   int keys = 0;
   int batch = 0, heads = 0, kv_heads = 0, group = 1;  // group: query heads to a key head
+  Div by_group, by_page;                              // quotients by it and by page_size
   int pieces = 0, pieces_v = 0;                       // groups of 8 columns of a row of Q and K, of V and O
   int page_size = 0, pages = 0, max_pages = 0, tokens = 0, max_t_q = 0;
   int causal = 0;
@@ -123,7 +138,7 @@ struct RowPlace {
   unsigned char* out;
 };
 __device__ __forceinline__ RowPlace row_place(const Pass& p, int first, int kv_head, int r) {
-  const int i = r / p.group, g = r - i * p.group;
+  const int i = p.by_group.of(r), g = r - i * p.group;
   const long long token = first + i;
   const int head = kv_head * p.group + g;
   return RowPlace{token * p.heads + head, p.out + token * p.o_token + head * p.o_head};

@@ -62,6 +62,7 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   prm.batch = step->batch, prm.heads = step->heads, prm.kv_heads = step->kv_heads, prm.group = step->heads / step->kv_heads;
   prm.pieces = step->hd / 8, prm.pieces_v = step->hd_v / 8;
   prm.page_size = step->page_size, prm.pages = step->pages, prm.max_pages = step->max_pages, prm.tokens = step->tokens, prm.max_t_q = step->max_t_q;
+  prm.by_group = Div(prm.group), prm.by_page = Div(prm.page_size);
   prm.causal = causal != 0, prm.scale = static_cast<float>(scale);
   const bool fp16 = step->dtype == LIMN_B200_F16;
   const cudaStream_t on = static_cast<cudaStream_t>(stream);

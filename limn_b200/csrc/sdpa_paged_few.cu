@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   unsigned none = 0;  // two bits for each place of the ring: which 8 of its unit's keys have a page that is none
   auto entry_of = [&](const Cursor& c, int blk) {
     const int key = (blk * 32 + lane) * 8;
-    return key < c.e.keys ? prm.table[static_cast<long long>(c.b) * prm.max_pages + key / prm.page_size] : 0;
+    return key < c.e.keys ? prm.table[static_cast<long long>(c.b) * prm.max_pages + prm.by_page.of(key)] : 0;
   };
   auto issue = [&]() {
     if (ahead.cost < span) {
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       for (int half = 0; half < 2; ++half) {
         const int key0 = ahead.unit * kUnit + half * 8;
         const int p = __shfl_sync(0xffffffffu, page, (key0 / 8) & 31);
-        const int slot = key0 % prm.page_size;
+        const int slot = prm.by_page.rest(key0);
         const long long in_page = max(p, 0);
         if (p < 0 && key0 < ahead.e.keys) none |= 1u << (2 * place_at + half);
         const unsigned char* k_from = prm.k.base + in_page * prm.k.page + ahead.kv_head * prm.k.head + slot * prm.k.slot + 16 * (piece < prm.pieces ? piece : 0);
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 8 + kq;
-      const int i = r / prm.group, g = r - i * prm.group;
+      const int i = prm.by_group.of(r), g = r - i * prm.group;
       const unsigned char* row = prm.q + (static_cast<long long>(at.e.first) + i) * prm.q_token + (at.kv_head * prm.group + g) * prm.q_head;
       const bool there = i < at.e.n;
 #pragma unroll
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
           q[nt][kk][j] = there && kk * 2 + j < prm.pieces ? *reinterpret_cast<const uint32_t*>(row + (kk * 16 + j * 8 + cq * 2) * 2) : 0u;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int token = (nt * 8 + cq * 2 + c) / prm.group;
+        const int token = prm.by_group.of(nt * 8 + cq * 2 + c);
         limit[nt][c] = prm.causal ? min(at.e.keys, at.e.keys - at.e.n + token + 1) : at.e.keys;
         m[nt][c] = -INFINITY, l[nt][c] = 0.f;
       }

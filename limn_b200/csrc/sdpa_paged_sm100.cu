@@ -42,7 +42,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
 constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
-constexpr int kLeast = 512;    // cost of the smallest share
+constexpr int kLeast = kItem + kTile;  // cost of the smallest share: not less than the smallest item's
 
 template <int D>
 struct Layout {
@@ -89,12 +89,15 @@ struct Segment {
   int whole;       // and ends with its last
 };
 
+__device__ __forceinline__ int tiles_of(int keys) { return (keys + kTile - 1) >> 7; }
+
 // ---- the cost of items, in keys (int holds an item's: 2^31 keys would be 2^35 bytes of a head). A sequence has `pairs` items per key head, pair j of tokens [j span, (j + 1) span) ----
 struct Costs {
   int pairs, span, half, seen_first;  // span: tokens of a pair; half: of a tile; seen_first: keys that are there before the first token
   int keys, n, causal;
-  __device__ __forceinline__ Costs(const Extent& e, int tokens_of_tile, int causal_)
-      : pairs((e.n + 2 * tokens_of_tile - 1) / (2 * tokens_of_tile)), span(2 * tokens_of_tile), half(tokens_of_tile), seen_first(e.keys - e.n), keys(e.keys), n(e.n), causal(causal_) {}
+  Div by_span;
+  __device__ __forceinline__ Costs(const Extent& e, const Div& by_span_, int causal_)
+      : pairs(by_span_.of(e.n + static_cast<int>(by_span_.d) - 1)), span(by_span_.d), half(by_span_.d / 2), seen_first(e.keys - e.n), keys(e.keys), n(e.n), causal(causal_), by_span(by_span_) {}
   // keys that the first `tokens` tokens see at most; one, masked, where that is none
   __device__ __forceinline__ int seen(int tokens) const { return max(1, causal ? seen_first + min(tokens, n) : keys); }
   __device__ __forceinline__ bool single(int j) const { return n - j * span <= half; }
@@ -102,18 +105,18 @@ struct Costs {
   // sum over the pairs in front of j (all of them two whole tiles)
   __device__ __forceinline__ long long before(long long j) const {
     if (!causal) return j * (kItem + max(1, keys));
-    const long long none = seen_first >= 0 ? 0 : min(j, static_cast<long long>(-seen_first / span));  // pairs whose last token sees nothing: 1 each
+    const long long none = seen_first >= 0 ? 0 : min(j, static_cast<long long>(by_span.of(-seen_first)));  // pairs whose last token sees nothing: 1 each
     return j * kItem + none + (j - none) * seen_first + span * (j * (j + 1) / 2 - none * (none + 1) / 2);
   }
   __device__ __forceinline__ long long all() const { return pairs == 0 ? 0 : before(pairs - 1) + of(pairs - 1); }
   // steps of key tiles (pairs of key tiles for a single tile) of pair j
   __device__ __forceinline__ int steps(int j) const {
-    const int tiles = (seen((j + 1) * span) + kTile - 1) / kTile;
-    return single(j) ? (tiles + 1) / 2 : tiles;
+    const int tiles = tiles_of(seen((j + 1) * span));
+    return single(j) ? (tiles + 1) >> 1 : tiles;
   }
   // the step nearest to `cost` into pair j; what lies in front of the keys counts as the first one's beginning
   __device__ __forceinline__ int step_at(int j, long long cost) const {
-    return static_cast<int>(min(static_cast<long long>(steps(j)), max(0LL, cost - kItem + kTile / 2) / kTile));
+    return static_cast<int>(min(static_cast<long long>(steps(j)), max(0LL, cost - kItem + kTile / 2) >> 7));
   }
 };
 
@@ -128,7 +131,7 @@ struct Maps {
 };
 
 template <int D, bool kFp16>
-__global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __grid_constant__ Maps maps, const Pass prm, const int tile_tokens, const int chunk, unsigned* status) {
+__global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __grid_constant__ Maps maps, const Pass prm, const Div by_span, const int chunk_log, unsigned* status) {
   using L = Layout<D>;
   using B = Bars;
   extern __shared__ unsigned char smem_unaligned[];
@@ -144,7 +147,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   auto bar = [&](int i) { return bars + 8u * i; };
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
-  const int tile_rows = tile_tokens * prm.group;
+  const int tile_tokens = by_span.d / 2, tile_rows = tile_tokens * prm.group;  // an item's two tiles have by_span.d tokens
+  const int chunk = 1 << chunk_log;
 
   if (threadIdx.x == kProducerWarp * 32) {
     for (int i = 0; i < B::count; ++i) {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     long long mine = 0;
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
-      if (b < prm.batch) mine += Costs(extent_of(prm, b), tile_tokens, prm.causal).all();
+      if (b < prm.batch) mine += Costs(extent_of(prm, b), by_span, prm.causal).all();
     }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -231,11 +235,11 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       do {
         ++p.b;
         p.e = extent_of(prm, p.b);
-        all = Costs(p.e, tile_tokens, prm.causal).all();
+        all = Costs(p.e, by_span, prm.causal).all();
         if (rest < all * prm.kv_heads) break;
         rest -= all * prm.kv_heads;
       } while (p.b + 1 < prm.batch);
-      const Costs costs(p.e, tile_tokens, prm.causal);
+      const Costs costs(p.e, by_span, prm.causal);
       p.kv_head = static_cast<int>(quotient(rest, all));
       rest -= p.kv_head * all;
       int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
@@ -262,16 +266,16 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     unsigned n_item = 0, q_uses[2] = {0u, 0u}, step = 0;
     bool more = any;
     // a lane fetches one box of a key tile: `chunk` keys of one page, 64 columns
-    const int chunks = kTile / chunk;
-    const int my_chunk = lane % chunks, my_atom = lane / chunks;
+    const int chunks = kTile >> chunk_log;
+    const int my_chunk = lane & (chunks - 1), my_atom = (lane << chunk_log) / kTile;
     while (more && ok) {
-      const Costs costs(at.e, tile_tokens, prm.causal);
+      const Costs costs(at.e, by_span, prm.causal);
       const bool last = at.b == end.b && at.kv_head == end.kv_head && at.j == end.j;
       const int steps = costs.steps(at.j), until = last ? end.step : steps;
       if (until > at.step) {
         Segment s;
         const bool single = costs.single(at.j);
-        const int tiles = (costs.seen((at.j + 1) * costs.span) + kTile - 1) / kTile;  // key tiles of the item
+        const int tiles = tiles_of(costs.seen((at.j + 1) * costs.span));  // key tiles of the item
         s.valid = 1, s.b = at.b, s.first = at.e.first, s.n = at.e.n, s.keys = at.e.keys, s.kv_head = at.kv_head;
         s.row0 = at.j * 2 * tile_rows;
         s.begun = at.step == 0, s.whole = at.step == 0 && until == steps;
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           s.count[1] = s.loads / 2, s.count[0] = s.loads - s.count[1];
         } else {
           s.first_tile = at.step;
-          const int tiles_0 = (costs.seen(at.j * costs.span + costs.half) + kTile - 1) / kTile;
+          const int tiles_0 = tiles_of(costs.seen(at.j * costs.span + costs.half));
           s.count[0] = max(0, min(until, tiles_0) - at.step);
           s.count[1] = until - at.step;
           s.loads = s.count[1], s.both = 0;
@@ -320,17 +324,17 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         // the page of this lane's box of key tile `tile`; one that is none is a coordinate outside the cache, whose box TMA fills with zeros
         auto entry = [&](int tile) {
           const int key = tile * kTile + my_chunk * chunk;
-          return key < s.keys ? table[key / prm.page_size] : 0;
+          return key < s.keys ? table[prm.by_page.of(key)] : 0;
         };
         int page_next = entry(s.first_tile);
         for (int j = 0; j < s.loads && ok; ++j, ++step) {
           const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
           const bool fetch = key < s.keys && my_atom < D / 64;
           const int page = fetch ? checked_page(page_next, prm.pages, prm.errors) : 0;
-          const int boxes = min(chunks, max(0, (s.keys - tile * kTile + chunk - 1) / chunk));  // those that have keys
+          const int boxes = min(chunks, max(0, (s.keys - tile * kTile + chunk - 1) >> chunk_log));  // those that have keys
           const uint32_t bytes = static_cast<uint32_t>(boxes * chunk) * (D * 2);
           if (j + 1 < s.loads) page_next = entry(tile + 1);
-          const int in_page = key % prm.page_size;
+          const int in_page = prm.by_page.rest(key);
           const int stage = step % B::kS;
           const uint32_t wrap = (step / B::kS) & 1;
           ok = wait(B::k_empty + stage, wrap ^ 1u, 0x0100u | stage);
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     const uint32_t t_o = tmem + lane_base + L::kOCol + t * D;
     const float sl2 = prm.scale * kLog2e;
     const uint64_t sl2_2 = f2_pack(sl2, sl2);
-    const int chunks = kTile / chunk;
+    const int chunks = kTile >> chunk_log;
     unsigned tiles = 0;   // key tiles this group has been through, over all segments
     unsigned o_uses = 0;  // segments it has finished with key tiles
     unsigned merges = 0;
@@ -525,14 +529,14 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         continue;
       }
       const int seen_first = s.keys - s.n;
-      const int sees = prm.causal ? min(s.keys, seen_first + row / prm.group + 1) : s.keys;                // keys [0, sees)
-      const int sees_least = prm.causal ? min(s.keys, seen_first + top_row / prm.group + 1) : s.keys;      // the tile's first token
+      const int sees = prm.causal ? min(s.keys, seen_first + prm.by_group.of(row) + 1) : s.keys;                // keys [0, sees)
+      const int sees_least = prm.causal ? min(s.keys, seen_first + prm.by_group.of(top_row) + 1) : s.keys;      // the tile's first token
       const int* table = prm.table + static_cast<long long>(s.b) * prm.max_pages;
       auto key0 = [&](int j) { return (s.first_tile + (both ? 2 * j + t : j)) * kTile; };
       // pages are looked at once more here, a key tile ahead
       auto entry = [&](int j) {
         const int key = key0(j) + lane * chunk;
-        return lane < chunks && key < s.keys ? table[key / prm.page_size] : 0;
+        return lane < chunks && key < s.keys ? table[prm.by_page.of(key)] : 0;
       };
       int entry_next = entry(0);
       float m = -INFINITY, l = 0.f;
@@ -666,6 +670,14 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           merge_stats(m, l, ml.x, ml.y, sl2, mine, add);
         }
         const float inv = 1.f / l;
+        // neighbouring rows' pieces are exchanged before they are stored, so that an instruction writes 64 bytes of each row it touches
+        unsigned char* to_row[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned long long mine_at = there ? reinterpret_cast<unsigned long long>(place.out) : 0ull;
+          const unsigned long long at = __shfl_sync(0xffffffffu, mine_at, (lane & ~3) + i);
+          to_row[i] = at == 0ull ? nullptr : reinterpret_cast<unsigned char*>(at) + 16 * (lane & 3);
+        }
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -678,7 +690,16 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
               o[i + 2] = __float_as_uint(__uint_as_float(o[i + 2]) * mine + f.z * add), o[i + 3] = __float_as_uint(__uint_as_float(o[i + 3]) * mine + f.w * add);
             }
           }
-          if (there) store_row32<kFp16>(place.out + 64 * c, o, inv, prm.pieces_v * 8 - 32 * c);
+          uint32_t w[4][4];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
+            w[i / 4][i % 4] = kFp16 ? pack_f16(a, b) : pack_bf16(a, b);
+          }
+          swap_rows_for_pieces<4>(w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (to_row[i] != nullptr && 4 * c + (lane & 3) < prm.pieces_v) *reinterpret_cast<uint4*>(to_row[i] + 64 * c) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
         }
         if (there) prm.lse[place.row] = m * prm.scale + logf(l);
       } else {
@@ -737,6 +758,8 @@ int launch_many(const Pass& pass, unsigned* status, cudaStream_t stream) {
     const int r = chunk % rest;
     chunk = rest, rest = r;
   }
+  int chunk_log = 3;
+  while (1 << chunk_log < chunk) ++chunk_log;
   const int tile_tokens = kTile / pass.group;
   Maps maps;
   const auto u = [](long long x) { return static_cast<unsigned long long>(x); };
@@ -754,7 +777,7 @@ int launch_many(const Pass& pass, unsigned* status, cudaStream_t stream) {
     LIMN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes), "sizing shared memory for the paged sdpa kernel");
     sized[device] = true;
   }
-  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers)), dim3(kThreads), L::kBytes, stream, maps, pass, tile_tokens, chunk, status),
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers)), dim3(kThreads), L::kBytes, stream, maps, pass, Div(2 * tile_tokens), chunk_log, status),
             "launching the paged sdpa kernel");
   note_launches(1);
   return LIMN_B200_OK;
