@@ -227,9 +227,6 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     }
     copies_commit();
   };
-#pragma unroll
-  for (int s = 0; s < R::kStages - 1; ++s) issue();
-
   // ---- arithmetic ----
   const int kq = lane >> 2, cq = lane & 3;  // in a fragment: row (key or column of O), and pair of query rows
   uint32_t q[NT][D / 16][2];
@@ -263,6 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     least_limit = prm.causal ? at.e.keys - at.e.n + 1 : at.e.keys;
   };
   if (at.cost < span) begin();
+#pragma unroll
+  for (int s = 0; s < R::kStages - 1; ++s) issue();
   bool waited = !late;
   for (int step = 0; at.cost < span; ++step) {
     copies_wait<R::kStages - 2>();

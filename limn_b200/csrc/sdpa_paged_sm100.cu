@@ -42,7 +42,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
 constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
-constexpr int kLeast = kItem + kTile;  // cost of the smallest share: not less than the smallest item's
+constexpr int kLeast = kItem;  // cost of the smallest share: about that of the smallest item
 
 template <int D>
 struct Layout {
@@ -172,10 +172,6 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     abort_flag = *reinterpret_cast<volatile unsigned*>(status) != kStatusOk;  // an earlier kernel gave up: this one stands down
     prm.parts.heads[blockIdx.x].followers = 0;                                // (also then: nothing is joined)
   }
-  if (warp == kMmaWarp) {
-    tmem_alloc(smem_addr(&tmem_slot), kTmemCols);
-    tmem_relinquish();
-  }
   // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
   const int run = (prm.batch + kThreads - 1) / kThreads;
   {
@@ -194,11 +190,20 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     for (int w = 0; w < warp; ++w) mine += warp_sum[w];
     share_end[threadIdx.x] = mine;
   }
-  tc_fence_before_sync();
   __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   bool ok = !abort_flag;
+  // tensor memory is allocated beside the producer's first loads
+  uint32_t tmem = 0;
+  if (warp != kProducerWarp) {
+    if (warp == kMmaWarp) {
+      tmem_alloc(smem_addr(&tmem_slot), kTmemCols);
+      tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    named_barrier_sync(kSetUp, kThreads - 32);
+    tc_fence_after_sync();
+    tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  }
 
   auto wait = [&](int i, uint32_t parity, unsigned tag) { return __all_sync(0xffffffffu, mbar_wait(bar(i), parity, status, tag)); };
   auto next_segment = [&](unsigned n_item, Segment& s) {
@@ -297,11 +302,6 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         if (lane == 0) {
           ring[slot] = s;
           mbar_arrive(bar(B::work_full + slot));
-          if (s.begun && !s.whole) {
-            // workers c behind this one whose share begins inside the item, before the middle of its last step
-            const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(kTile) - kTile / 2);
-            prm.parts.heads[blockIdx.x] = Head{static_cast<int>(quotient(begins + limit - 1, share)) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
-          }
         }
         __syncwarp();
         ++n_item;
@@ -326,14 +326,14 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           const int key = tile * kTile + my_chunk * chunk;
           return key < s.keys ? table[prm.by_page.of(key)] : 0;
         };
-        int page_next = entry(s.first_tile);
+        int page_next[2] = {entry(s.first_tile), entry(s.first_tile + 1)};  // two tiles ahead
         for (int j = 0; j < s.loads && ok; ++j, ++step) {
           const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
           const bool fetch = key < s.keys && my_atom < D / 64;
-          const int page = fetch ? checked_page(page_next, prm.pages, prm.errors) : 0;
+          const int page = fetch ? checked_page(page_next[0], prm.pages, prm.errors) : 0;
           const int boxes = min(chunks, max(0, (s.keys - tile * kTile + chunk - 1) >> chunk_log));  // those that have keys
           const uint32_t bytes = static_cast<uint32_t>(boxes * chunk) * (D * 2);
-          if (j + 1 < s.loads) page_next = entry(tile + 1);
+          page_next[0] = page_next[1], page_next[1] = entry(tile + 2);
           const int in_page = prm.by_page.rest(key);
           const int stage = step % B::kS;
           const uint32_t wrap = (step / B::kS) & 1;
@@ -350,6 +350,11 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           __syncwarp();
           if (fetch) tma_load_4d(base + L::kVOff + box, &maps.v, bar(B::v_full + stage), my_atom * 64, in_page, s.kv_head, page);
           __syncwarp();
+        }
+        if (s.begun && !s.whole && lane == 0) {
+          // workers behind this one whose share begins inside the item, before the middle of its last step
+          const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(kTile) - kTile / 2);
+          prm.parts.heads[blockIdx.x] = Head{static_cast<int>(quotient(begins + limit - 1, share)) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
         }
       }
       // the next item

@@ -18,24 +18,25 @@ that can overlap on the GPU would share that workspace: give each stream a Paged
 from __future__ import annotations
 
 import ctypes
-import functools
+from collections.abc import Callable
+from operator import attrgetter, methodcaller
 from typing import Any
 
 from limn_b200._lib import DTYPE_CODES, PAIRING_CODES, Paged, check, lib
 from limn_b200.registry import _note_launch
-from limn_b200.runtime import DeviceBuffer
+from limn_b200.runtime import DeviceBuffer, Stream
+
+
+# How an operand's address is read, by its type (asking an object for an attribute it lacks takes longer than all the rest of a call).
+_ADDRESS_OF: dict[type, Callable[[Any], int | None]] = {type(None): lambda x: None, int: lambda x: x}
 
 
 def _address(operand: Any) -> int | None:
-    if operand is None or isinstance(operand, int):
-        return operand
-    ptr = getattr(operand, "ptr", None)
-    return operand.data_ptr() if ptr is None else ptr
-
-
-@functools.lru_cache(maxsize=256)
-def _packed(strides: tuple[int, ...]):
-    return (ctypes.c_longlong * len(strides))(*strides)
+    kind = type(operand)
+    read = _ADDRESS_OF.get(kind)
+    if read is None:
+        read = _ADDRESS_OF[kind] = attrgetter("ptr") if hasattr(operand, "ptr") else methodcaller("data_ptr")
+    return read(operand)
 
 
 class PagedCache:
@@ -67,7 +68,13 @@ class PagedBatch:
                            (ctypes.c_longlong * 3)(*cache.k_strides), (ctypes.c_longlong * 3)(*cache.v_strides), cache.dtype, batch, heads,
                            cache.kv_heads, cache.hd, cache.hd_v, cache.page_size, cache.pages, max_pages, tokens, max_t_q, first_position)
         self._by_ref = ctypes.byref(self._step)
-        self.heads, self.kv_heads, self.hd, self.hd_v = heads, cache.kv_heads, cache.hd, cache.hd_v
+        self._head_dim = cache.hd
+        # (token, head) strides of dense operands: q, q_out, k, v and out
+        self._dense = {"q": (heads * cache.hd, cache.hd), "k": (cache.kv_heads * cache.hd, cache.hd),
+                       "v": (cache.kv_heads * cache.hd_v, cache.hd_v), "out": (heads * cache.hd_v, cache.hd_v)}
+        self._packed: dict[tuple, Any] = {}
+        loaded = lib()
+        self._append, self._attend, self._attend_prefix = loaded.limn_b200_kv_append, loaded.limn_b200_sdpa_paged, loaded.limn_b200_sdpa_paged_prefix
         need = ctypes.c_ulonglong()
         check(lib().limn_b200_sdpa_paged_workspace(self._by_ref, max_prefix, ctypes.byref(need)), "sizing the workspace of a paged batch")
         self.workspace_bytes = need.value
@@ -79,32 +86,50 @@ class PagedBatch:
     def append(self, k: Any, v: Any, *, q: Any = None, q_out: Any = None, k_strides=None, v_strides=None, q_strides=None, q_out_strides=None,
                frequencies: Any = None, rotated: int = 0, pairing: str = "halves", stream: Any = None) -> None:
         """Keys and values of the step's tokens into their slots, turned to their positions; q turned into q_out beside them.
-        Strides are (token, head) in elements; without them an operand is dense, (tokens, heads, width)."""
+        Strides are (token, head) tuples in
+        elements; without them an operand is dense, (tokens, heads, width)."""
         if pairing not in PAIRING_CODES:
             raise ValueError(f"limn_b200: kv_append knows the pairings {sorted(PAIRING_CODES)}, not {pairing!r}")
-        hd, hd_v = self.hd, self.hd_v
-        strides = _packed((*(q_strides or (self.heads * hd, hd)), *(q_out_strides or (self.heads * hd, hd)),
-                           *(k_strides or (self.kv_heads * hd, hd)), *(v_strides or (self.kv_heads * hd_v, hd_v))))
-        check(lib().limn_b200_kv_append(self._by_ref, _address(q), _address(k), _address(v), _address(q_out), strides, _address(frequencies),
-                                        rotated, PAIRING_CODES[pairing], getattr(stream, "handle", stream)), "launching kv_append")
+        strides = self._packed.get((q_strides, q_out_strides, k_strides, v_strides))
+        if strides is None:
+            strides = self._pack((q_strides, q_out_strides, k_strides, v_strides), ("q", "q", "k", "v"))
+        code = self._append(self._by_ref, _address(q), _address(k), _address(v), _address(q_out), strides, _address(frequencies), rotated,
+                            PAIRING_CODES[pairing], stream.handle if isinstance(stream, Stream) else stream)
+        if code:
+            check(code, "launching kv_append")
 
     def attention(self, q: Any, out: Any, lse: Any, *, q_strides=None, out_strides=None, causal: bool = True, scale: float | None = None,
                   stream: Any = None) -> None:
         """out = softmax(q k^T scale) v over each sequence's pages, lse its row statistic (tokens, heads) in float32. `scale`
         is hd ** -0.5 unless it is given."""
-        check(lib().limn_b200_sdpa_paged(self._by_ref, _address(q), _address(out), _address(lse), self._strides(q_strides, out_strides), int(causal),
-                                         self.hd**-0.5 if scale is None else scale, self._workspace_at, self.workspace_bytes,
-                                         getattr(stream, "handle", stream)), "launching sdpa_paged")
+        strides = self._packed.get((q_strides, out_strides))
+        if strides is None:
+            strides = self._pack((q_strides, out_strides), ("q", "out"))
+        code = self._attend(self._by_ref, _address(q), _address(out), _address(lse), strides, causal, self._head_dim**-0.5 if scale is None else scale,
+                            self._workspace_at, self.workspace_bytes, stream.handle if isinstance(stream, Stream) else stream)
+        if code:
+            check(code, "launching sdpa_paged")
         _note_launch()
 
     def attention_with_prefix(self, q: Any, out: Any, lse: Any, *, prefix_table: Any, prefix_len: int, q_strides=None, out_strides=None,
                               causal: bool = True, scale: float | None = None, stream: Any = None) -> None:
         """The same with prefix_len keys of the pages prefix_table names in front of every sequence's own."""
-        check(lib().limn_b200_sdpa_paged_prefix(self._by_ref, _address(q), _address(out), _address(lse), self._strides(q_strides, out_strides),
-                                                _address(prefix_table), prefix_len, int(causal), self.hd**-0.5 if scale is None else scale,
-                                                self._workspace_at, self.workspace_bytes, getattr(stream, "handle", stream)),
-              "launching sdpa_paged_prefix")
+        strides = self._packed.get((q_strides, out_strides))
+        if strides is None:
+            strides = self._pack((q_strides, out_strides), ("q", "out"))
+        code = self._attend_prefix(self._by_ref, _address(q), _address(out), _address(lse), strides, _address(prefix_table), prefix_len, causal,
+                                   self._head_dim**-0.5 if scale is None else scale, self._workspace_at, self.workspace_bytes,
+                                   stream.handle if isinstance(stream, Stream) else stream)
+        if code:
+            check(code, "launching sdpa_paged_prefix")
         _note_launch()
 
-    def _strides(self, q_strides, out_strides):
-        return _packed((*(q_strides or (self.heads * self.hd, self.hd)), *(out_strides or (self.heads * self.hd_v, self.hd_v))))
+    def _pack(self, given: tuple, names: tuple[str, ...]):
+        """The strides of a call as the library takes them; kept, since a batch's calls are alike step after step."""
+        flat = [int(x) for strides, name in zip(given, names, strict=True) for x in (self._dense[name] if strides is None else strides)]
+        if len(flat) != 2 * len(names):
+            raise ValueError(f"limn_b200: strides are (token, head) pairs, got {given}")
+        if len(self._packed) >= 64:
+            self._packed.clear()
+        packed = self._packed[given] = (ctypes.c_longlong * len(flat))(*flat)
+        return packed
