@@ -1,9 +1,9 @@
 // New keys and values into their pages, turned to their positions on the way, and the queries turned beside them.
 //
-// A token's row of H + Hk + Hk heads is read once and written once; that traffic is the floor. A CTA has one token: one warp finds
-// the token's sequence (its offset among q_start, 32 probes at a time), its slot and its page; the first threads make the
-// token's cosines and sines, which all of its heads share, and leave them in shared memory; then every thread keeps to one column unit
-// and walks the heads. A unit is what turns together: 16 bytes of a row and the 16 bytes half the rotated width further on (halves),
+// A token's H + Hk + Hk rows are read once and written once; that traffic is the floor. One to eight warps have a token, each on its own:
+// it finds the token's sequence (its offset among q_start, 32 probes at a time), its slot and its page, makes the token's cosines and
+// sines, two to a lane, which all of its heads share, and then every lane keeps to one column unit and walks the heads, four rows in
+// flight. A unit is what turns together: 16 bytes of a row and the 16 bytes half the rotated width further on (halves),
 // or 16 bytes that hold their own pairs (neighbours), 8 bytes where a half is no multiple of 16 bytes.
 //
 // The angle p * f is taken as a number of turns in float64 and only its fraction goes to float32: at position 10^6 a float32
@@ -19,7 +19,8 @@ namespace {
 
 using namespace paged;
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
 constexpr int kMaxPairs = 64;
 constexpr double kTurn = 6.283185307179586476925286766559;
 
@@ -34,7 +35,8 @@ struct AppendParams {
   int batch, heads, kv_heads;  // heads: 0 without queries
   int width, width_v;          // columns
   int page_size, pages, max_pages, tokens, max_t_q, first_position;
-  Div by_page;
+  Div by_page, by_units, by_units_v;  // units of a row of q and k, of v
+  int warps_log;                      // 2^this warps to a token
   int rotated;                 // columns
 };
 
@@ -69,103 +71,117 @@ __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
   return kFp16 ? ptx::pack_f16(lo, hi) : ptx::pack_bf16(lo, hi);
 }
 
-// Units of a row: the turning ones first, then the others.
+// A lane's unit of rows row0, row0 + step, ...: the turning units of a row come first, then the others.
 template <bool kFp16, int E, bool kNeighbours>
-__device__ __forceinline__ void turn_rows(const unsigned char* from, long long from_head, unsigned char* to, long long to_head, int rows, int width,
+__device__ __forceinline__ void turn_rows(const unsigned char* from, long long from_head, unsigned char* to, long long to_head, int row0, int step, int rows, int unit, int turning,
                                           int rotated, const float2* turns) {
-  const int turning = kNeighbours ? rotated / E : rotated / 2 / E;
-  const int units = turning + (width - rotated) / E;
-  const int step = kThreads / units;  // (width <= 128 and E >= 4: at most 32 units)
-  const int row0 = threadIdx.x / units, unit = threadIdx.x - row0 * units;
-  if (row0 >= step) return;
+  constexpr int kAtOnce = 4;
   const int column = unit < turning ? unit * E : rotated + (unit - turning) * E;
-  from += 2 * column, to += 2 * column;
-  if (unit >= turning) {
-#pragma unroll 2
-    for (int r = row0; r < rows; r += step) store_unit<E>(to + r * to_head, load_unit<E>(from + r * from_head));
-    return;
-  }
-  if constexpr (kNeighbours) {
-    float2 t[E / 2];
+  from += row0 * from_head + 2 * column, to += row0 * to_head + 2 * column;
+  from_head *= step, to_head *= step;
+  const int many = row0 < rows ? (rows - row0 + step - 1) / step : 0;
+  const bool turns_here = unit < turning;
+  const int half = kNeighbours || !turns_here ? 0 : rotated;  // bytes from a column to its partner: rotated / 2 elements
+  float2 t[kNeighbours ? E / 2 : E];
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) t[i] = turns[unit * (E / 2) + i];
-#pragma unroll 2
-    for (int r = row0; r < rows; r += step) {
-      Unit<E> u = load_unit<E>(from + r * from_head);
+  for (int i = 0; i < (kNeighbours ? E / 2 : E); ++i) t[i] = turns_here ? turns[unit * (kNeighbours ? E / 2 : E) + i] : make_float2(1.f, 0.f);
+  for (int done = 0; done < many; done += kAtOnce) {
+    Unit<E> a[kAtOnce], b[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const float2 x = widen<kFp16>(u.w[i]);
-        u.w[i] = narrow<kFp16>(x.x * t[i].x - x.y * t[i].y, x.x * t[i].y + x.y * t[i].x);
-      }
-      store_unit<E>(to + r * to_head, u);
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (done + u >= many) break;
+      a[u] = load_unit<E>(from + u * from_head);
+      if (!kNeighbours && turns_here) b[u] = load_unit<E>(from + u * from_head + half);
     }
-  } else {
-    float2 t[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) t[i] = turns[unit * E + i];
-    const int half = rotated;  // bytes from a column to its partner: rotated / 2 elements
-#pragma unroll 2
-    for (int r = row0; r < rows; r += step) {
-      Unit<E> a = load_unit<E>(from + r * from_head), b = load_unit<E>(from + r * from_head + half);
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (done + u >= many) break;
+      if (turns_here) {
 #pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const float2 x = widen<kFp16>(a.w[i]), y = widen<kFp16>(b.w[i]);
-        a.w[i] = narrow<kFp16>(x.x * t[2 * i].x - y.x * t[2 * i].y, x.y * t[2 * i + 1].x - y.y * t[2 * i + 1].y);
-        b.w[i] = narrow<kFp16>(x.x * t[2 * i].y + y.x * t[2 * i].x, x.y * t[2 * i + 1].y + y.y * t[2 * i + 1].x);
+        for (int i = 0; i < E / 2; ++i) {
+          const float2 x = widen<kFp16>(a[u].w[i]);
+          if constexpr (kNeighbours) {
+            a[u].w[i] = narrow<kFp16>(x.x * t[i].x - x.y * t[i].y, x.x * t[i].y + x.y * t[i].x);
+          } else {
+            const float2 y = widen<kFp16>(b[u].w[i]);
+            a[u].w[i] = narrow<kFp16>(x.x * t[2 * i].x - y.x * t[2 * i].y, x.y * t[2 * i + 1].x - y.y * t[2 * i + 1].y);
+            b[u].w[i] = narrow<kFp16>(x.x * t[2 * i].y + y.x * t[2 * i].x, x.y * t[2 * i + 1].y + y.y * t[2 * i + 1].x);
+          }
+        }
+        if (!kNeighbours) store_unit<E>(to + u * to_head + half, b[u]);
       }
-      store_unit<E>(to + r * to_head, a);
-      store_unit<E>(to + r * to_head + half, b);
+      store_unit<E>(to + u * to_head, a[u]);
     }
+    from += kAtOnce * from_head, to += kAtOnce * to_head;
   }
 }
 
 template <bool kFp16, int E, bool kNeighbours>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams prm) {
-  __shared__ float2 turns[kMaxPairs];
-  __shared__ int found_page, found_slot;
-  const int token = blockIdx.x, lane = threadIdx.x & 31;
+  __shared__ float2 turns_of[kWarps][kMaxPairs];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long id = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const int token = static_cast<int>(id >> prm.warps_log), share = static_cast<int>(id & ((1 << prm.warps_log) - 1)), shares = 1 << prm.warps_log;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  if (threadIdx.x < 32) {
-    const int low = sequence_of(prm.q_start, prm.batch, token, lane);
-    int page = -1, slot = 0;
-    if (low < prm.batch) {
-      const Extent e = extent_of(prm.q_start, prm.kv_lens, low, prm.tokens, prm.max_t_q, prm.max_pages, prm.page_size, prm.errors);
-      if (token >= e.first && token - e.first < e.n) {  // (not so where the offsets are out of order)
-        slot = e.keys - e.n + (token - e.first);
-        if (e.keys < e.n) {  // more tokens than keys: there is no slot for the first of them
-          if (lane == 0 && prm.errors != nullptr) atomicOr(prm.errors, LIMN_B200_PAGED_BAD_SEQUENCE);
-        } else {
-          page = checked_page(prm.table[static_cast<long long>(low) * prm.max_pages + prm.by_page.of(slot)], prm.pages, prm.errors);
-        }
-      }
-    }
-    if (lane == 0) found_page = page, found_slot = slot;
+  if (token >= prm.tokens) return;
+  double frequency[2];  // (asked for before what the sequence's place hangs on)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) frequency[i] = i * 32 + lane < prm.rotated / 2 ? prm.frequencies[i * 32 + lane] * (1.0 / kTurn) : 0.0;
+  const int b = sequence_of(prm.q_start, prm.batch, token, lane);
+  if (b >= prm.batch) return;
+  const Extent e = extent_of(prm.q_start, prm.kv_lens, b, prm.tokens, prm.max_t_q, prm.max_pages, prm.page_size, prm.errors);
+  if (token < e.first || token - e.first >= e.n) return;  // (so where the offsets are out of order)
+  if (e.keys < e.n) {  // more tokens than keys: there is no slot for the first of them
+    if (lane == 0 && prm.errors != nullptr) atomicOr(prm.errors, LIMN_B200_PAGED_BAD_SEQUENCE);
+    return;
   }
-  __syncthreads();
-  const int page = found_page, slot = found_slot;
+  const int slot = e.keys - e.n + (token - e.first), at_page = prm.by_page.of(slot);
+  const int page = checked_page(prm.table[static_cast<long long>(b) * prm.max_pages + at_page], prm.pages, prm.errors);
   if (page < 0) return;
-  if (threadIdx.x < prm.rotated / 2) {
-    const double round = (static_cast<double>(prm.first_position) + slot) * (prm.frequencies[threadIdx.x] * (1.0 / kTurn));
+  float2* turns = turns_of[warp];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int pair = i * 32 + lane;
+    if (pair >= prm.rotated / 2) break;
+    const double round = (static_cast<double>(prm.first_position) + slot) * frequency[i];
     float s, c;
     sincospif(2.f * static_cast<float>(round - rint(round)), &s, &c);
-    turns[threadIdx.x] = make_float2(c, s);
+    turns[pair] = make_float2(c, s);
   }
-  __syncthreads();
-  const int in_page = prm.by_page.rest(slot);
-  const long long at = token;
-  turn_rows<kFp16, E, kNeighbours>(prm.k + at * prm.k_token, prm.k_head, prm.k_pages.base + page * prm.k_pages.page + in_page * prm.k_pages.slot, prm.k_pages.head,
-                                   prm.kv_heads, prm.width, prm.rotated, turns);
-  turn_rows<kFp16, 8, true>(prm.v + at * prm.v_token, prm.v_head, prm.v_pages.base + page * prm.v_pages.page + in_page * prm.v_pages.slot, prm.v_pages.head,
-                            prm.kv_heads, prm.width_v, 0, turns);
-  if (prm.heads > 0)
-    turn_rows<kFp16, E, kNeighbours>(prm.q + at * prm.q_token, prm.q_head, prm.q_out + at * prm.o_token, prm.o_head, prm.heads, prm.width, prm.rotated, turns);
+  __syncwarp();
+  const long long in_page = slot - at_page * prm.page_size, at = token;
+  {
+    const int units = prm.by_units.d, rows_at_once = 32 / units, row0 = prm.by_units.of(lane), unit = lane - row0 * units;
+    const int turning = kNeighbours ? prm.rotated / E : prm.rotated / 2 / E;
+    if (row0 < rows_at_once) {
+      const int first = share * rows_at_once + row0, step = shares * rows_at_once;
+      if (prm.heads > 0)
+        turn_rows<kFp16, E, kNeighbours>(prm.q + at * prm.q_token, prm.q_head, prm.q_out + at * prm.o_token, prm.o_head, first, step, prm.heads, unit, turning, prm.rotated, turns);
+      turn_rows<kFp16, E, kNeighbours>(prm.k + at * prm.k_token, prm.k_head, prm.k_pages.base + page * prm.k_pages.page + in_page * prm.k_pages.slot, prm.k_pages.head, first, step,
+                                       prm.kv_heads, unit, turning, prm.rotated, turns);
+    }
+  }
+  {
+    const int units = prm.by_units_v.d, rows_at_once = 32 / units, row0 = prm.by_units_v.of(lane), unit = lane - row0 * units;
+    if (row0 < rows_at_once)
+      turn_rows<kFp16, 8, true>(prm.v + at * prm.v_token, prm.v_head, prm.v_pages.base + page * prm.v_pages.page + in_page * prm.v_pages.slot, prm.v_pages.head,
+                                share * rows_at_once + row0, shares * rows_at_once, prm.kv_heads, unit, 0, 0, turns);
+  }
 }
 
 template <bool kFp16>
-int launch_append(const AppendParams& prm, int pairing, cudaStream_t stream) {
-  auto kernel = pairing == LIMN_B200_NEIGHBOURS ? kv_append_kernel<kFp16, 8, true> : (prm.rotated % 16 == 0 ? kv_append_kernel<kFp16, 8, false> : kv_append_kernel<kFp16, 4, false>);
-  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(prm.tokens)), dim3(kThreads), 0, stream, prm), "launching the append kernel");
+int launch_append(AppendParams& prm, int pairing, cudaStream_t stream) {
+  const bool neighbours = pairing == LIMN_B200_NEIGHBOURS;
+  const int unit = neighbours || prm.rotated % 16 == 0 ? 8 : 4;
+  prm.by_units = Div(neighbours ? prm.width / 8 : (prm.width - prm.rotated / 2) / unit), prm.by_units_v = Div(prm.width_v / 8);
+  auto kernel = neighbours ? kv_append_kernel<kFp16, 8, true> : (unit == 8 ? kv_append_kernel<kFp16, 8, false> : kv_append_kernel<kFp16, 4, false>);
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  prm.warps_log = 3;
+  while (prm.warps_log > 0 && (static_cast<long long>(prm.tokens) << prm.warps_log) > 32LL * sms) --prm.warps_log;
+  const long long blocks = ((static_cast<long long>(prm.tokens) << prm.warps_log) + kWarps - 1) / kWarps;
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, prm), "launching the append kernel");
   note_launches(1);
   return LIMN_B200_OK;
 }
