@@ -44,10 +44,16 @@ constexpr float kRescaleSlack = 8.f;
 constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
 constexpr int kLeast = kItem;  // cost of the smallest share: about that of the smallest item
 
-template <int D>
+// kPacked: how a tile of K or V lies in shared memory at head dim 128. Column block after column block (64 columns of all 128 rows each), a box
+// of TMA fetches 64 columns of a run of keys; packed, the two column blocks of 8 rows lie side by side, and a box fetches all columns of the
+// run. A box costs the producer about 100 clocks to issue, whatever it holds, and a key tile of pages of 16 is 32 boxes or 16.
+template <int D, bool kPacked>
 struct Layout {
   static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kAtomBytes = kTile * 128;  // one 64-element-wide column block of a tile
+  static constexpr int kAtomBytes = kTile * 128;                     // Q: from one column block to the next
+  static constexpr int kKVAtom = kPacked ? 1024 : kAtomBytes;        // K and V: from one column block to the next
+  static constexpr int kKVGroup = kPacked ? 1024 * (D / 64) : 1024;  // and from 8 rows to the next 8
+  static_assert(!kPacked || D == 128);
   static constexpr int kStages = 2;
   static constexpr int kQOff = 0;
   static constexpr int kKOff = kQOff + 2 * kTileBytes;
@@ -128,11 +134,13 @@ struct Place {
 
 struct Maps {
   CUtensorMap q, k, v;
+  // packed maps have the key head in the dimension of column blocks (heads side by side: k_side) or in that of pages
+  int k_side, v_side;
 };
 
-template <int D, bool kFp16>
+template <int D, bool kFp16, bool kPacked>
 __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __grid_constant__ Maps maps, const Pass prm, const Div by_span, const int chunk_log, unsigned* status) {
-  using L = Layout<D>;
+  using L = Layout<D, kPacked>;
   using B = Bars;
   extern __shared__ unsigned char smem_unaligned[];
   __shared__ uint32_t tmem_slot;
@@ -273,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     // a lane fetches one box of a key tile: `chunk` keys of one page, 64 columns
     const int chunks = kTile >> chunk_log;
     const int my_chunk = lane & (chunks - 1), my_atom = (lane << chunk_log) / kTile;
+    constexpr int kBoxAtoms = kPacked ? 1 : D / 64;  // boxes to a chunk
     while (more && ok) {
       const Costs costs(at.e, by_span, prm.causal);
       const bool last = at.b == end.b && at.kv_head == end.kv_head && at.j == end.j;
@@ -315,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
             mbar_expect_tx(bar(B::q_full + t), static_cast<uint32_t>(tile_rows) * D * 2);
             const int token = s.first + (2 * at.j + (s.both ? 0 : t)) * tile_tokens;
 #pragma unroll
-            for (int a = 0; a < D / 64; ++a) tma_load_4d(base + L::kQOff + t * L::kTileBytes + a * L::kAtomBytes, &maps.q, bar(B::q_full + t), a * 64, s.kv_head * prm.group, token, 0);
+            for (int a = 0; a < D / 64; ++a) tma_load_5d(base + L::kQOff + t * L::kTileBytes + a * L::kAtomBytes, &maps.q, bar(B::q_full + t), a * 64, s.kv_head * prm.group, token, 0, 0);
           }
           __syncwarp();
         }
@@ -329,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         int page_next[2] = {entry(s.first_tile), entry(s.first_tile + 1)};  // two tiles ahead
         for (int j = 0; j < s.loads && ok; ++j, ++step) {
           const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
-          const bool fetch = key < s.keys && my_atom < D / 64;
+          const bool fetch = key < s.keys && my_atom < kBoxAtoms;
           const int page = fetch ? checked_page(page_next[0], prm.pages, prm.errors) : 0;
           const int boxes = min(chunks, max(0, (s.keys - tile * kTile + chunk - 1) >> chunk_log));  // those that have keys
           const uint32_t bytes = static_cast<uint32_t>(boxes * chunk) * (D * 2);
@@ -341,14 +350,18 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(bar(B::k_full + stage), bytes);
           __syncwarp();
-          const uint32_t box = stage * L::kTileBytes + my_atom * L::kAtomBytes + my_chunk * chunk * 128;
-          if (fetch) tma_load_4d(base + L::kKOff + box, &maps.k, bar(B::k_full + stage), my_atom * 64, in_page, s.kv_head, page);
+          const uint32_t box = stage * L::kTileBytes + my_atom * L::kAtomBytes + my_chunk * (chunk / 8) * L::kKVGroup;
+          auto load = [&](uint32_t to, const CUtensorMap& map, int side, uint32_t full) {
+            if constexpr (kPacked) tma_load_5d(to, &map, full, 0, 0, side ? s.kv_head * (D / 64) : 0, in_page >> 3, side ? page : page * prm.kv_heads + s.kv_head);
+            else tma_load_5d(to, &map, full, my_atom * 64, in_page, s.kv_head, page, 0);
+          };
+          if (fetch) load(base + L::kKOff + box, maps.k, maps.k_side, bar(B::k_full + stage));
           __syncwarp();
           ok = wait(B::v_empty + stage, wrap ^ 1u, 0x0110u | stage);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(bar(B::v_full + stage), bytes);
           __syncwarp();
-          if (fetch) tma_load_4d(base + L::kVOff + box, &maps.v, bar(B::v_full + stage), my_atom * 64, in_page, s.kv_head, page);
+          if (fetch) load(base + L::kVOff + box, maps.v, maps.v_side, bar(B::v_full + stage));
           __syncwarp();
         }
         if (s.begun && !s.whole && lane == 0) {
@@ -386,25 +399,24 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       const uint32_t q_lo = desc_lo(base + L::kQOff + t * L::kTileBytes, 0);
       const uint32_t k_lo = desc_lo(base + L::kKOff + stage * L::kTileBytes, 0);
       const uint32_t c = tmem + L::kSCol + t * 128;
-      mma_ss_lo<false>(c, q_lo, k_lo, idesc_s);
+      mma_ss_lo<false, desc_hi(L::kKVGroup)>(c, q_lo, k_lo, idesc_s);
 #pragma unroll
-      for (int kk = 1; kk < D / 16; ++kk) {
-        const uint32_t off = (kk / 4) * (L::kAtomBytes >> 4) + (kk % 4) * 2;  // in 16-byte units
-        mma_ss_lo<true>(c, q_lo + off, k_lo + off, idesc_s);
+      for (int kk = 1; kk < D / 16; ++kk) {  // (offsets in 16-byte units)
+        mma_ss_lo<true, desc_hi(L::kKVGroup)>(c, q_lo + (kk / 4) * (L::kAtomBytes >> 4) + (kk % 4) * 2, k_lo + (kk / 4) * (L::kKVAtom >> 4) + (kk % 4) * 2, idesc_s);
       }
     };
     auto issue_pv = [&](int t, int stage, int part, bool first) {
-      const uint32_t v_lo = desc_lo(base + L::kVOff + stage * L::kTileBytes, L::kAtomBytes);
+      const uint32_t v_lo = desc_lo(base + L::kVOff + stage * L::kTileBytes, L::kKVAtom);
       const uint32_t c = tmem + L::kOCol + t * D;
       const uint32_t a = tmem + L::kSCol + t * 128;
 #pragma unroll
-      for (int kk = 4 * part; kk < 4 * part + 4; ++kk) mma_ts_lo(c, a + kk * 8, v_lo + kk * (16 * 128 / 16), idesc_pv, (kk > 0 || !first) ? 1u : 0u);
+      for (int kk = 4 * part; kk < 4 * part + 4; ++kk) mma_ts_lo<desc_hi(L::kKVGroup)>(c, a + kk * 8, v_lo + kk * (2 * L::kKVGroup >> 4), idesc_pv, (kk > 0 || !first) ? 1u : 0u);
     };
     // rows from `from` on of the V tile in `stage` become zeros: slots of a sequence's last page that it has not filled, and what was there before
     auto clear_rows = [&](int stage, int from) {
       for (int i = from * (D / 8) + lane; i < kTile * (D / 8); i += 32) {
         const int row = i / (D / 8), piece = i % (D / 8);
-        st_shared_v4(base + L::kVOff + stage * L::kTileBytes + (piece / 8) * L::kAtomBytes + row * 128 + (piece % 8) * 16, 0u, 0u, 0u, 0u);
+        st_shared_v4(base + L::kVOff + stage * L::kTileBytes + (row / 8) * L::kKVGroup + (piece / 8) * L::kKVAtom + (row % 8) * 128 + (piece % 8) * 16, 0u, 0u, 0u, 0u);
       }
       fence_async_shared();
       __syncwarp();
@@ -755,9 +767,26 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   }
 }
 
-template <int D, bool kFp16>
+unsigned long long u(long long x) { return static_cast<unsigned long long>(x); }
+
+// Boxes of `chunk` keys of one page and key head: 64 columns each.
+BoxShape pages_map(const Pass& p, const Pages& side, int pieces, int chunk) {
+  return BoxShape{{u(pieces) * 8, u(p.page_size), u(p.kv_heads), u(p.pages), 1}, {side.slot, side.head, side.page, side.page}, {64, static_cast<unsigned>(chunk), 1, 1, 1}};
+}
+// Or all 128 columns, the two column blocks of 8 keys side by side. Five dimensions hold (column, key of 8, column block, 8 keys, page) and leave
+// none for the head, so it has to continue the column blocks (heads side by side in a token) or the pages (heads of a page one after the other).
+bool packs(const Pass& p, const Pages& side, int pieces) { return pieces == 16 && (p.kv_heads == 1 || side.head == 256 || side.page == p.kv_heads * side.head); }
+BoxShape packed_map(const Pass& p, const Pages& side, int chunk, int* heads_side_by_side) {
+  const bool beside = p.kv_heads == 1 || side.head == 256;
+  *heads_side_by_side = beside;
+  return BoxShape{{64, 8, beside ? 2 * u(p.kv_heads) : 2, u(p.page_size) / 8, beside ? u(p.pages) : u(p.pages) * u(p.kv_heads)},
+                  {side.slot, 128, 8 * side.slot, beside ? side.page : side.head},
+                  {64, 8, 2, static_cast<unsigned>(chunk) / 8, 1}};
+}
+
+template <int D, bool kFp16, bool kPacked>
 int launch_many(const Pass& pass, unsigned* status, cudaStream_t stream) {
-  using L = Layout<D>;
+  using L = Layout<D, kPacked>;
   int chunk = pass.page_size;  // the largest run of keys that neither a page nor a key tile cuts: the common divisor of both, a power of two
   for (int rest = kTile % chunk; rest != 0;) {
     const int r = chunk % rest;
@@ -766,15 +795,14 @@ int launch_many(const Pass& pass, unsigned* status, cudaStream_t stream) {
   int chunk_log = 3;
   while (1 << chunk_log < chunk) ++chunk_log;
   const int tile_tokens = kTile / pass.group;
-  Maps maps;
-  const auto u = [](long long x) { return static_cast<unsigned long long>(x); };
-  BoxShape q = {{u(pass.pieces) * 8, u(pass.heads), u(pass.tokens), 1}, {pass.q_head, pass.q_token, pass.q_token * pass.tokens}, {64, static_cast<unsigned>(pass.group), static_cast<unsigned>(tile_tokens), 1}};
-  BoxShape k = {{u(pass.pieces) * 8, u(pass.page_size), u(pass.kv_heads), u(pass.pages)}, {pass.k.slot, pass.k.head, pass.k.page}, {64, static_cast<unsigned>(chunk), 1, 1}};
-  BoxShape v = {{u(pass.pieces_v) * 8, u(pass.page_size), u(pass.kv_heads), u(pass.pages)}, {pass.v.slot, pass.v.head, pass.v.page}, {64, static_cast<unsigned>(chunk), 1, 1}};
+  Maps maps = {};
+  const BoxShape q = {{u(pass.pieces) * 8, u(pass.heads), u(pass.tokens), 1, 1},
+                      {pass.q_head, pass.q_token, pass.q_token, pass.q_token},
+                      {64, static_cast<unsigned>(pass.group), static_cast<unsigned>(tile_tokens), 1, 1}};
   if (int rc = make_box_map("sdpa_paged", &maps.q, pass.q, kFp16, q)) return rc;
-  if (int rc = make_box_map("sdpa_paged", &maps.k, pass.k.base, kFp16, k)) return rc;
-  if (int rc = make_box_map("sdpa_paged", &maps.v, pass.v.base, kFp16, v)) return rc;
-  auto kernel = sdpa_paged_many_kernel<D, kFp16>;
+  if (int rc = make_box_map("sdpa_paged", &maps.k, pass.k.base, kFp16, kPacked ? packed_map(pass, pass.k, chunk, &maps.k_side) : pages_map(pass, pass.k, pass.pieces, chunk))) return rc;
+  if (int rc = make_box_map("sdpa_paged", &maps.v, pass.v.base, kFp16, kPacked ? packed_map(pass, pass.v, chunk, &maps.v_side) : pages_map(pass, pass.v, pass.pieces_v, chunk))) return rc;
+  auto kernel = sdpa_paged_many_kernel<D, kFp16, kPacked>;
   static bool sized[64] = {};
   int device = 0;
   LIMN_CUDA(cudaGetDevice(&device), "asking for the current device");
@@ -786,6 +814,11 @@ int launch_many(const Pass& pass, unsigned* status, cudaStream_t stream) {
             "launching the paged sdpa kernel");
   note_launches(1);
   return LIMN_B200_OK;
+}
+
+template <int D, bool kPacked>
+int launch_many_d(const Pass& pass, bool fp16, unsigned* status, cudaStream_t stream) {
+  return fp16 ? launch_many<D, true, kPacked>(pass, status, stream) : launch_many<D, false, kPacked>(pass, status, stream);
 }
 
 }  // namespace
@@ -801,8 +834,9 @@ int paged_many_launch(const Pass& given, bool fp16, unsigned char* workspace, cu
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
   pass.parts.place(workspace, sms, 2 * kTile, width);
   int rc;
-  if (width == 64) rc = fp16 ? launch_many<64, true>(pass, status, stream) : launch_many<64, false>(pass, status, stream);
-  else rc = fp16 ? launch_many<128, true>(pass, status, stream) : launch_many<128, false>(pass, status, stream);
+  if (width == 64) rc = launch_many_d<64, false>(pass, fp16, status, stream);
+  else if (packs(pass, pass.k, pass.pieces) && packs(pass, pass.v, pass.pieces_v)) rc = launch_many_d<128, true>(pass, fp16, status, stream);
+  else rc = launch_many_d<128, false>(pass, fp16, status, stream);
   if (rc) return rc;
   return paged_join_launch(pass, fp16, true, stream);
 }

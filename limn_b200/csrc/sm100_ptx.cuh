@@ -132,6 +132,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
 // ---- tensor memory ----
 // Allocate `cols` columns (power of two, 32..512); the base address lands in *slot (shared).
 // Executed by one whole warp; the same warp frees it.
@@ -230,20 +237,23 @@ constexpr uint32_t kDescHiSw128 = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading_bytes) {
   return ((addr & 0x3ffffu) >> 4) | (((leading_bytes >> 4) & 0x3fffu) << 16);
 }
-template <bool kAccumulate>
+// The same with `bytes` between the groups of 8 rows.
+constexpr uint32_t desc_hi(uint32_t bytes) { return (bytes >> 4) | (1u << 14) | (2u << 29); }
+template <bool kAccumulate, uint32_t kBHi = kDescHiSw128>
 __device__ __forceinline__ void mma_ss_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
       ".reg .b64 da, db;\n\t"
       "mov.b64 da, {%1, %4};\n\t"
-      "mov.b64 db, {%2, %4};\n\t"
+      "mov.b64 db, {%2, %6};\n\t"
       "setp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t"
       "}\n" ::"r"(d_tmem),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHiSw128), "n"(kAccumulate ? 1 : 0)
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHiSw128), "n"(kAccumulate ? 1 : 0), "r"(kBHi)
       : "memory");
 }
+template <uint32_t kBHi = kDescHiSw128>
 __device__ __forceinline__ void mma_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
                                           uint32_t accumulate) {
   asm volatile(
@@ -254,7 +264,7 @@ __device__ __forceinline__ void mma_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint
       "setp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t"
       "}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(kDescHiSw128), "r"(accumulate)
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(kBHi), "r"(accumulate)
       : "memory");
 }
 

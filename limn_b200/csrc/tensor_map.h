@@ -15,12 +15,12 @@ namespace limn_b200 {
 int make_tile_map(CUtensorMap* map, const void* base, bool fp16, int batch, int heads, int rows, int width, int box_rows,
                   const Strides& strides);
 
-// A 4-D map of 2-byte elements with any extents and boxes: dims and box innermost first, strides in bytes of dims 1 to 3 (multiples of 16). The
+// A 5-D map of 2-byte elements with any extents and boxes: dims and box innermost first, strides in bytes of dims 1 to 4 (multiples of 16). The
 // box's first extent is 64 elements; the same swizzle, and zeros outside. Errors name `name`.
 struct BoxShape {
-  unsigned long long dims[4];
-  long long strides[3];
-  unsigned box[4];
+  unsigned long long dims[5];
+  long long strides[4];
+  unsigned box[5];
 };
 int make_box_map(const char* name, CUtensorMap* map, const void* base, bool fp16, const BoxShape& shape);
 
