@@ -9,6 +9,8 @@
 namespace limn_b200 {
 namespace paged {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 // One side (K or V) of the cache: element (page, head, slot, 0) at base + page * page_stride + ..., in bytes.
 struct Pages {
   unsigned char* base = nullptr;
@@ -44,11 +46,20 @@ struct Parts {
   }
 };
 
-// Sums and statistics of every (token, head) row over some of its keys, in memory: what a pass over a shared prefix leaves and the
-// pass over the sequences' own keys joins to its own.
+// Sums and statistics of every (token, head) row over some of its keys, in memory: what the pass over a shared prefix leaves and what the
+// pass over the sequences' own keys does, for a last kernel to put together. Where a row's problem was shared by workers its sums are
+// parts, and the statistics say so: kInParts in place of l, the worker where the problem begins as the bits of m, and in `part_row` the row there.
+constexpr float kInParts = -1.f;  // (l is a sum of exponentials: never negative)
 struct RowSums {
-  float* o = nullptr;    // (tokens * heads, width), unnormalised
-  float2* ml = nullptr;  // (tokens * heads)
+  float* o = nullptr;       // (tokens * heads, width), unnormalised
+  float2* ml = nullptr;     // (tokens * heads)
+  int* part_row = nullptr;  // (tokens * heads)
+  static size_t bytes(size_t rows, int width) { return rows * (static_cast<size_t>(width) * 4 + 8) + (rows * 4 + 255) / 256 * 256; }
+  void place(unsigned char* memory, size_t rows, int width) {
+    o = reinterpret_cast<float*>(memory), memory += rows * width * 4;
+    ml = reinterpret_cast<float2*>(memory), memory += rows * 8;
+    part_row = reinterpret_cast<int*>(memory);
+  }
 };
 
 // Quotients by a number that a launch knows: a product and a shift (exact for numerators from 0 to 2^31 - 1: the factor is 2^(31 + s) / d rounded
@@ -85,7 +96,9 @@ struct Pass {
   float scale = 0.f;
   Parts parts;
   RowSums leave;  // where rows go instead of `out`, or null
-  RowSums join;   // what rows are joined with on their way out, or null. The kernel that leaves these sums may still run when the pass begins
+  // The kernel in front of this one in the stream is of the same call and concerns it not: what this pass reads was there before that one began. So it
+  // need not be waited for until the end.
+  int beside = 0;
 };
 
 // A sequence's extents: `first` token of `n`, `keys` in its pages. One that cannot be has n = 0 and is noted.
@@ -164,13 +177,15 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 int check_paged(const char* name, const limn_b200_paged* step);
 int check_paged_pointers(const char* name, const limn_b200_paged* step);
 
-// The kernels that make a pass (each puts a second one behind itself that joins the parts): few rows to a key head, and any number.
+// The kernels that make a pass, for few rows to a key head and for any number. Each lays its parts out in `workspace` and says so in pass.parts.
 constexpr int kPagedFewRows = 16;  // max_t_q * group up to here
 size_t paged_few_workspace(int rows, int width, int sms);
-int paged_few_launch(const paged::Pass& pass, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream);
+int paged_few_launch(paged::Pass& pass, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream);
 size_t paged_many_workspace(int width, int sms);
-int paged_many_launch(const paged::Pass& pass, bool fp16, unsigned char* workspace, cudaStream_t stream);
-// A row's parts to a warp, or to the eight warps of a block.
+int paged_many_launch(paged::Pass& pass, bool fp16, unsigned char* workspace, cudaStream_t stream);
+// Behind a pass: rows whose problems were shared, out of their parts (a row to a warp, or to the eight warps of a block).
 int paged_join_launch(const paged::Pass& pass, bool fp16, bool warp_a_row, cudaStream_t stream);
+// Behind two passes that leave their rows' sums: the rows of both together.
+int paged_finish_launch(const paged::Pass& front, const paged::Pass& own, bool fp16, cudaStream_t stream);
 
 }  // namespace limn_b200

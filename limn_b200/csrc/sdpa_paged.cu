@@ -14,15 +14,15 @@ using namespace paged;
 size_t pass_workspace(long long rows, int width, int sms) {
   return rows <= kPagedFewRows ? paged_few_workspace(static_cast<int>(rows), width, sms) : paged_many_workspace(width, sms);
 }
-int launch_pass(const Pass& pass, bool fp16, long long rows, unsigned char* workspace, cudaStream_t stream) {
+int launch_pass(Pass& pass, bool fp16, long long rows, unsigned char* workspace, cudaStream_t stream) {
   return rows <= kPagedFewRows ? paged_few_launch(pass, fp16, static_cast<int>(rows), workspace, stream) : paged_many_launch(pass, fp16, workspace, stream);
 }
 
-// The workspace of a call: the parts of the pass over the own keys, those of the pass over the prefix (the kernel that joins them may still run when the
-// other pass begins), and the rows' sums over the prefix.
+// The workspace of a call: the parts of the pass over the own keys; behind a prefix also those of the pass over it, and the rows' sums
+// over either.
 struct Workspace {
-  size_t own, front, sums, stats;
-  size_t bytes() const { return own + front + sums + stats; }
+  size_t own, front, sums;  // sums: of one pass
+  size_t bytes() const { return own + front + 2 * sums; }
 };
 int workspace_of(const limn_b200_paged* step, int prefix_len, Workspace* w) {
   int sms = 0;
@@ -32,7 +32,7 @@ int workspace_of(const limn_b200_paged* step, int prefix_len, Workspace* w) {
   const size_t rows = static_cast<size_t>(step->tokens) * step->heads;
   w->own = pass_workspace(step->max_t_q * group, width, sms);
   w->front = prefix_len > 0 ? pass_workspace(step->tokens * group, width, sms) : 0;
-  w->sums = prefix_len > 0 ? rows * width * 4 : 0, w->stats = prefix_len > 0 ? rows * 8 : 0;
+  w->sums = prefix_len > 0 ? (RowSums::bytes(rows, width) + 255) / 256 * 256 : 0;
   return LIMN_B200_OK;
 }
 
@@ -67,17 +67,22 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   const bool fp16 = step->dtype == LIMN_B200_F16;
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   unsigned char* memory = static_cast<unsigned char*>(workspace);
-  if (prefix_len > 0) {
-    // every row over the prefix, as one sequence of all tokens that sees all of it; tokens that belong to no sequence get sums
-    // too, which nothing reads
-    Pass front = prm;
-    front.table = prefix_table, front.q_start = nullptr, front.kv_lens = nullptr, front.keys = prefix_len, front.batch = 1, front.causal = 0;
-    front.leave.o = reinterpret_cast<float*>(memory + w.own + w.front);
-    front.leave.ml = reinterpret_cast<float2*>(memory + w.own + w.front + w.sums);
-    if (int rc = launch_pass(front, fp16, static_cast<long long>(step->tokens) * prm.group, memory + w.own, on)) return rc;
-    prm.join = front.leave;
+  const long long rows = static_cast<long long>(step->max_t_q) * prm.group;
+  if (prefix_len == 0) {
+    if (int rc = launch_pass(prm, fp16, rows, memory, on)) return rc;
+    return paged_join_launch(prm, fp16, rows > kPagedFewRows, on);
   }
-  return launch_pass(prm, fp16, static_cast<long long>(step->max_t_q) * prm.group, memory, on);
+  // every row over the prefix, as one sequence of all tokens that sees all of it (tokens that belong to no sequence too: nothing asks for those); every row
+  // over its own keys, on the multiprocessors as they become free; and the two together
+  const int width = prm.pieces <= 8 && prm.pieces_v <= 8 ? 64 : 128;
+  const size_t all_rows = static_cast<size_t>(step->tokens) * step->heads;
+  Pass front = prm;
+  front.table = prefix_table, front.q_start = nullptr, front.kv_lens = nullptr, front.keys = prefix_len, front.batch = 1, front.causal = 0;
+  front.leave.place(memory + w.own + w.front, all_rows, width), prm.leave.place(memory + w.own + w.front + w.sums, all_rows, width);
+  prm.beside = 1;
+  if (int rc = launch_pass(front, fp16, static_cast<long long>(step->tokens) * prm.group, memory + w.own, on)) return rc;
+  if (int rc = launch_pass(prm, fp16, rows, memory, on)) return rc;
+  return paged_finish_launch(front, prm, fp16, on);
 }
 
 }  // namespace

@@ -17,7 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "paged.h"
+#include "paged_rows.cuh"
 #include "sm100_ptx.cuh"
 
 namespace limn_b200 {
@@ -29,7 +29,6 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;  // keys
 constexpr int kBegin = 3;  // units that a problem costs besides its keys: its queries, its page table, its way out
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -85,28 +84,6 @@ __device__ __forceinline__ void next_problem(const Pass& prm, Cursor& c) {
   while (c.units == 0 && ++c.b < prm.batch) c.e = extent_of(prm, c.b), c.units = units_of(c.e);
 }
 
-// A row on its way out: four columns of its sums, to where the pass wants them.
-template <int D, bool kFp16>
-__device__ __forceinline__ void finish4(const Pass& prm, const RowPlace& place, int column, float4 acc, float m, float l, float sl2) {
-  if (prm.leave.o != nullptr) {
-    *reinterpret_cast<float4*>(prm.leave.o + place.row * D + column) = acc;
-    if (column == 0) prm.leave.ml[place.row] = make_float2(m, l);
-    return;
-  }
-  if (prm.join.o != nullptr) {
-    const float2 ml = prm.join.ml[place.row];
-    const float4 o = *reinterpret_cast<const float4*>(prm.join.o + place.row * D + column);
-    float keep, add;
-    merge_stats(m, l, ml.x, ml.y, sl2, keep, add);
-    acc = make_float4(acc.x * keep + o.x * add, acc.y * keep + o.y * add, acc.z * keep + o.z * add, acc.w * keep + o.w * add);
-  }
-  const float inv = 1.f / l;  // (no key: 0 * inf = NaN)
-  if (column < prm.pieces_v * 8)
-    *reinterpret_cast<uint2*>(place.out + 2 * column) = kFp16 ? make_uint2(ptx::pack_f16(acc.x * inv, acc.y * inv), ptx::pack_f16(acc.z * inv, acc.w * inv))
-                                                              : make_uint2(ptx::pack_bf16(acc.x * inv, acc.y * inv), ptx::pack_bf16(acc.z * inv, acc.w * inv));
-  if (column == 0) prm.lse[place.row] = m * prm.scale + logf(l);
-}
-
 // What a warp has of problems that its neighbours share, for the block to put together.
 struct Shared {
   int enters, through;      // part 2 w is there; and its problem goes on behind this warp
@@ -123,9 +100,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   __shared__ Shared shared[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float sl2 = prm.scale * kLog2e;
-  // (behind a pass over a prefix all but its last kernel are done when this one begins, and only the rows' way out needs that one)
-  const bool late = prm.join.o != nullptr;
-  if (!late) ptx::grid_dependency_wait();
+  if (!prm.beside) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
   // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
@@ -259,14 +234,17 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     }
     least_limit = prm.causal ? at.e.keys - at.e.n + 1 : at.e.keys;
   };
-  if (at.cost < span) begin();
-#pragma unroll
-  for (int s = 0; s < R::kStages - 1; ++s) issue();
-  bool waited = !late;
-  for (int step = 0; at.cost < span; ++step) {
-    copies_wait<R::kStages - 2>();
-    __syncwarp();
+  bool fresh = true;  //  a problem, or the share, begins
+  // (the first turns only issue copies; one loop for all, since code that a launch runs once is fetched once, at some 50 clocks a line)
+#pragma unroll 1
+  for (int step = 1 - R::kStages; at.cost < span; ++step) {
+    if (fresh) begin(), fresh = false;
+    if (step >= 0) {
+      copies_wait<R::kStages - 2>();
+      __syncwarp();
+    }
     issue();
+    if (step < 0) continue;
     const int place_at = step % R::kStages;
     const uint32_t k_at = mine + place_at * 2 * R::kSide, v_at = k_at + R::kSide;
     float s[NT][4];
@@ -352,51 +330,41 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
     const bool whole = begun && ends;
-    if (!waited && whole) ptx::grid_dependency_wait(), waited = true;
+    const long long part = (2LL * worker + (begun ? 1 : 0)) * (NT * 8);
+    const int rows = at.e.n * prm.group;
+    if (!whole || prm.leave.o != nullptr) {
+      // sums and statistics as they are: to the warp's part, or where the pass leaves them
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = nt * 8 + cq * 2 + c;
-        if (r >= at.e.n * prm.group) continue;
-        if (!whole || prm.leave.o != nullptr) {
-          const long long part = (2LL * worker + (begun ? 1 : 0)) * (NT * 8) + r;
-          float* to_o = by_warp.o + part * D;
-          float2* to_ml = by_warp.ml + part;
-          if (whole) {
-            const long long row = row_place(prm, at.e.first, at.kv_head, r).row;
-            to_o = prm.leave.o + row * D, to_ml = prm.leave.ml + row;
-          }
+        for (int c = 0; c < 2; ++c) {
+          const int r = nt * 8 + cq * 2 + c;
+          if (r >= rows) continue;
+          const long long row = whole ? row_place(prm, at.e.first, at.kv_head, r).row : part + r;
+          float* to_o = (whole ? prm.leave.o : by_warp.o) + row * D + kq;
 #pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt) to_o[mt * 16 + kq] = o[nt][mt][c], to_o[mt * 16 + 8 + kq] = o[nt][mt][c + 2];
-          if (kq == 0) *to_ml = make_float2(m[nt][c], l[nt][c]);
-          continue;
+          for (int mt = 0; mt < D / 16; ++mt) to_o[mt * 16] = o[nt][mt][c], to_o[mt * 16 + 8] = o[nt][mt][c + 2];
+          if (kq == 0) (whole ? prm.leave.ml : by_warp.ml)[row] = make_float2(m[nt][c], l[nt][c]);
         }
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float inv[2] = {1.f / l[nt][0], 1.f / l[nt][1]};  // (no key: 0 * inf = NaN)
+        const int r = nt * 8 + kq;  // the row whose columns this lane has once they are turned round
         const RowPlace place = row_place(prm, at.e.first, at.kv_head, r);
-        float keep = 1.f, add = 0.f, top = m[nt][c], sum = l[nt][c];
-        float more[D / 16][2];
-#pragma unroll
-        for (int mt = 0; mt < D / 16; ++mt) more[mt][0] = more[mt][1] = 0.f;
-        if (prm.join.o != nullptr) {
-          const float* from_o = prm.join.o + place.row * D + kq;
-          const float2 ml = prm.join.ml[place.row];
-#pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt) more[mt][0] = from_o[mt * 16], more[mt][1] = from_o[mt * 16 + 8];
-          merge_stats(top, sum, ml.x, ml.y, sl2, keep, add);
-        }
-        const float inv = 1.f / sum;  // (no key: 0 * inf = NaN)
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if (mt * 2 + half >= prm.pieces_v) continue;
-            const int column = mt * 16 + half * 8 + kq;
-            const float value = (o[nt][mt][c + 2 * half] * keep + more[mt][half] * add) * inv;
-            if (kFp16) *reinterpret_cast<__half*>(place.out + 2 * column) = __float2half_rn(value);
-            else *reinterpret_cast<__nv_bfloat16*>(place.out + 2 * column) = __float2bfloat16_rn(value);
+            const float a = o[nt][mt][2 * half] * inv[0], b = o[nt][mt][2 * half + 1] * inv[1];
+            const uint32_t pair = transposed(kFp16 ? ptx::pack_f16(a, b) : ptx::pack_bf16(a, b));
+            if (r < rows && mt * 2 + half < prm.pieces_v) *reinterpret_cast<uint32_t*>(place.out + 2 * (mt * 16 + half * 8 + cq * 2)) = pair;
           }
-        if (kq == 0) prm.lse[place.row] = top * prm.scale + logf(sum);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (kq == 0 && nt * 8 + cq * 2 + c < rows) prm.lse[row_place(prm, at.e.first, at.kv_head, nt * 8 + cq * 2 + c).row] = m[nt][c] * prm.scale + logf(l[nt][c]);
       }
+    }
     if (!whole && lane == 0) {
       Shared& mine_shared = shared[warp];
       const int which = begun ? 1 : 0;
@@ -406,10 +374,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     }
     if (!ends || at.cost + kBegin >= span) break;
     next_problem(prm, at);
-    begun = true;
-    begin();
+    begun = fresh = true;
   }
-  if (!waited) ptx::grid_dependency_wait();
+  if (prm.beside) ptx::grid_dependency_wait();  // (whoever waits for this kernel has waited for the one before it)
 
   // ---- the block's parts: chain 0 enters from the block before, chain 1 + w begins with warp w ----
   __syncthreads();
@@ -450,80 +417,17 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       }
       if (lane >= kLanesO) continue;
       if (chain > 0 && !open) {
-        finish4<D, kFp16>(prm, row_place(prm, at_head.first[which], at_head.kv_head[which], r), column, acc, m, l, sl2);
+        finish4<D, kFp16>(prm, row_place(prm, at_head.first[which], at_head.kv_head[which], r), column, acc, m, l);
       } else {
         const long long part = (2LL * blockIdx.x + which) * (NT * 8) + r;
         *reinterpret_cast<float4*>(prm.parts.o + part * D + column) = acc;
-        if (column == 0) prm.parts.ml[part] = make_float2(m, l);
+        if (column == 0) {
+          prm.parts.ml[part] = make_float2(m, l);
+          if (chain > 0 && prm.leave.o != nullptr) leave_in_parts(prm, row_place(prm, at_head.first[which], at_head.kv_head[which], r).row, r);
+        }
       }
     }
   }
-}
-
-// ---- joining the parts ----
-constexpr int kJoinWarps = 8;
-
-// A row of one problem: kSplit warps share its parts, a lane has 4 columns.
-template <int D, bool kFp16, int kSplit>
-__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const Pass prm) {
-  constexpr int kRows = kJoinWarps / kSplit;
-  constexpr int kLanesO = D / 4;           // lanes to a row
-  constexpr int kAtOnce = 32 / kLanesO;    // parts a warp takes side by side
-  constexpr int kUnroll = 4;
-  __shared__ float4 sums[kJoinWarps][32];
-  __shared__ float2 stats[kJoinWarps];
-  ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
-  const Head head = prm.parts.heads[blockIdx.x];
-  if (head.followers == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.y * kRows + warp / kSplit, split = warp % kSplit;
-  const int column = (lane % kLanesO) * 4, side = lane / kLanesO;
-  const float sl2 = prm.scale * kLog2e;
-  const int row = head.row0 + r / 128 * head.tile_rows + r % 128;
-  if (r % 128 >= head.tile_rows || row >= head.n * prm.group) return;  // (in the whole block, or without a barrier behind it)
-  // part 0 is the head's, part i the i-th follower's
-  auto part = [&](int i) { return (i == 0 ? 2LL * blockIdx.x + 1 : 2LL * (blockIdx.x + i)) * prm.parts.rows + r; };
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto fold = [&](float m_b, float l_b, const float4& o_b) {
-    float keep, add;
-    merge_stats(m, l, m_b, l_b, sl2, keep, add);
-    acc = make_float4(acc.x * keep + o_b.x * add, acc.y * keep + o_b.y * add, acc.z * keep + o_b.z * add, acc.w * keep + o_b.w * add);
-  };
-  for (int i0 = split * kAtOnce + side; i0 <= head.followers; i0 += kUnroll * kSplit * kAtOnce) {
-    float2 ml[kUnroll];
-    float4 o[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = i0 + u * kSplit * kAtOnce;
-      ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i <= head.followers) ml[u] = prm.parts.ml[part(i)], o[u] = *reinterpret_cast<const float4*>(prm.parts.o + part(i) * D + column);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      // (a part that has seen no key has no sums: what lies there is not looked at)
-      if (ml[u].x == -INFINITY && ml[u].y == 0.f) continue;
-      fold(ml[u].x, ml[u].y, o[u]);
-    }
-  }
-  __syncwarp();
-#pragma unroll
-  for (int d = kLanesO; d < 32; d <<= 1) {
-    const float4 other = make_float4(__shfl_down_sync(0xffffffffu, acc.x, d), __shfl_down_sync(0xffffffffu, acc.y, d), __shfl_down_sync(0xffffffffu, acc.z, d),
-                                     __shfl_down_sync(0xffffffffu, acc.w, d));
-    const float m_b = __shfl_down_sync(0xffffffffu, m, d), l_b = __shfl_down_sync(0xffffffffu, l, d);
-    fold(m_b, l_b, other);
-  }
-  if (kSplit > 1) {
-    sums[warp][lane] = acc;
-    if (lane == 0) stats[warp] = make_float2(m, l);
-    __syncthreads();
-    if (split > 0) return;
-#pragma unroll
-    for (int i = 1; i < kSplit; ++i) fold(stats[warp + i].x, stats[warp + i].y, sums[warp + i][lane]);
-  }
-  if (side == 0) finish4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row), column, acc, m, l, sl2);
 }
 
 template <int D, bool kFp16, int NT>
@@ -541,48 +445,25 @@ int launch_few(const Pass& pass, const Parts& by_warp, cudaStream_t stream) {
   return LIMN_B200_OK;
 }
 
-template <int D, bool kFp16, int kSplit>
-int launch_join(const Pass& pass, cudaStream_t stream) {
-  const unsigned rows = static_cast<unsigned>((pass.parts.rows * kSplit + kJoinWarps - 1) / kJoinWarps);
-  LIMN_CUDA(launch_overlapped(sdpa_paged_join_kernel<D, kFp16, kSplit>, dim3(static_cast<unsigned>(pass.parts.workers), rows), dim3(kJoinWarps * 32), 0, stream, pass),
-            "launching the kernel that joins parts");
-  note_launches(1);
-  return LIMN_B200_OK;
-}
-
 int few_tile(int rows) { return rows <= 8 ? 8 : kPagedFewRows; }
 
 }  // namespace
 
 size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(sms, few_tile(rows), width) + Parts::bytes(sms * kWarps, few_tile(rows), width); }
 
-int paged_few_launch(const Pass& given, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream) {
-  Pass pass = given;
+int paged_few_launch(Pass& pass, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream) {
   Parts by_warp;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
   pass.parts.place(workspace, sms, few_tile(rows), width);
   by_warp.place(workspace + Parts::bytes(sms, few_tile(rows), width), sms * kWarps, few_tile(rows), width);
-  int rc;
   if (width == 64) {
-    if (rows <= 8) rc = fp16 ? launch_few<64, true, 1>(pass, by_warp, stream) : launch_few<64, false, 1>(pass, by_warp, stream);
-    else rc = fp16 ? launch_few<64, true, 2>(pass, by_warp, stream) : launch_few<64, false, 2>(pass, by_warp, stream);
-  } else {
-    if (rows <= 8) rc = fp16 ? launch_few<128, true, 1>(pass, by_warp, stream) : launch_few<128, false, 1>(pass, by_warp, stream);
-    else rc = fp16 ? launch_few<128, true, 2>(pass, by_warp, stream) : launch_few<128, false, 2>(pass, by_warp, stream);
+    if (rows <= 8) return fp16 ? launch_few<64, true, 1>(pass, by_warp, stream) : launch_few<64, false, 1>(pass, by_warp, stream);
+    return fp16 ? launch_few<64, true, 2>(pass, by_warp, stream) : launch_few<64, false, 2>(pass, by_warp, stream);
   }
-  if (rc) return rc;
-  return paged_join_launch(pass, fp16, false, stream);
-}
-
-int paged_join_launch(const Pass& pass, bool fp16, bool warp_a_row, cudaStream_t stream) {
-  if (warp_a_row) {
-    if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 1>(pass, stream) : launch_join<64, false, 1>(pass, stream);
-    return fp16 ? launch_join<128, true, 1>(pass, stream) : launch_join<128, false, 1>(pass, stream);
-  }
-  if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 8>(pass, stream) : launch_join<64, false, 8>(pass, stream);
-  return fp16 ? launch_join<128, true, 8>(pass, stream) : launch_join<128, false, 8>(pass, stream);
+  if (rows <= 8) return fp16 ? launch_few<128, true, 1>(pass, by_warp, stream) : launch_few<128, false, 1>(pass, by_warp, stream);
+  return fp16 ? launch_few<128, true, 2>(pass, by_warp, stream) : launch_few<128, false, 2>(pass, by_warp, stream);
 }
 
 }  // namespace limn_b200

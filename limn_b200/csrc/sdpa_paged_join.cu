@@ -1,0 +1,149 @@
+// What workers of a paged pass left of problems that they shared, put together; and the rows of two passes, over a prefix and over a
+// sequence's own keys. Sums of up to 148 parts, 512 bytes a row and part at most: bound by the latency of the loads, which are made four
+// at a time. The order is fixed, so two runs give the same bits.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged_rows.cuh"
+
+namespace limn_b200 {
+namespace {
+
+using namespace paged;
+
+constexpr int kJoinWarps = 8;
+constexpr int kUnroll = 4;
+
+// The parts of a problem that begins with worker `w`, `by` of them at a time beginning with part `from`: part 0 is the head's, part i the i-th follower's.
+template <int D>
+__device__ __forceinline__ void add_parts(Sums& sums, const Parts& parts, int w, int followers, int r, int column, int from, int by, float sl2) {
+  auto part = [&](int i) { return (i == 0 ? 2LL * w + 1 : 2LL * (w + i)) * parts.rows + r; };
+#pragma unroll 1
+  for (int i0 = from; i0 <= followers; i0 += kUnroll * by) {
+    float2 ml[kUnroll];
+    float4 o[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * by;
+      ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i <= followers) ml[u] = parts.ml[part(i)], o[u] = *reinterpret_cast<const float4*>(parts.o + part(i) * D + column);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) sums.add(ml[u].x, ml[u].y, o[u], sl2);
+  }
+}
+
+// The sides of a warp that has several parts at once, in lane order, into the first.
+template <int D>
+__device__ __forceinline__ void add_sides(Sums& sums, float sl2) {
+  __syncwarp();
+#pragma unroll
+  for (int d = D / 4; d < 32; d <<= 1) {
+    const float4 o = make_float4(__shfl_down_sync(0xffffffffu, sums.acc.x, d), __shfl_down_sync(0xffffffffu, sums.acc.y, d), __shfl_down_sync(0xffffffffu, sums.acc.z, d),
+                                 __shfl_down_sync(0xffffffffu, sums.acc.w, d));
+    const float m = __shfl_down_sync(0xffffffffu, sums.m, d), l = __shfl_down_sync(0xffffffffu, sums.l, d);
+    sums.add(m, l, o, sl2);
+  }
+}
+
+// A row of one problem: kSplit warps share its parts.
+template <int D, bool kFp16, int kSplit>
+__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const Pass prm) {
+  constexpr int kRows = kJoinWarps / kSplit;
+  constexpr int kLanes = D / 4;          // lanes to a row
+  constexpr int kAtOnce = 32 / kLanes;   // parts a warp takes side by side
+  __shared__ float4 all_sums[kJoinWarps][32];
+  __shared__ float2 all_stats[kJoinWarps];
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const Head head = prm.parts.heads[blockIdx.x];
+  if (head.followers == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * kRows + warp / kSplit, split = warp % kSplit;
+  const int column = (lane % kLanes) * 4, side = lane / kLanes;
+  const float sl2 = prm.scale * kLog2e;
+  const int row = head.row0 + r / 128 * head.tile_rows + r % 128;
+  if (r % 128 >= head.tile_rows || row >= head.n * prm.group) return;  // (in the whole block, or without a barrier behind it)
+  Sums sums;
+  add_parts<D>(sums, prm.parts, blockIdx.x, head.followers, r, column, split * kAtOnce + side, kSplit * kAtOnce, sl2);
+  add_sides<D>(sums, sl2);
+  if (kSplit > 1) {
+    all_sums[warp][lane] = sums.acc;
+    if (lane == 0) all_stats[warp] = make_float2(sums.m, sums.l);
+    __syncthreads();
+    if (split > 0) return;
+#pragma unroll 1
+    for (int i = 1; i < kSplit; ++i) sums.add(all_stats[warp + i].x, all_stats[warp + i].y, all_sums[warp + i][lane], sl2);
+  }
+  if (side == 0) store4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row), column, sums.acc, sums.m, sums.l);
+}
+
+// A warp to a (token, head) row: what both passes left of it, of a sequence that is one. Rows of tokens that belong to none are left alone.
+template <int D, bool kFp16>
+__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_finish_kernel(const Pass front, const Pass own) {
+  constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int token = blockIdx.x, head = blockIdx.y * kJoinWarps + warp;
+  if (head >= own.heads) return;
+  const int b = sequence_of(own.q_start, own.batch, token, lane);
+  if (b >= own.batch) return;
+  const Extent e = extent_of(own, b);
+  if (token < e.first || token - e.first >= e.n) return;  // (so where the offsets are out of order)
+  const int column = (lane % kLanes) * 4, side = lane / kLanes;
+  const float sl2 = own.scale * kLog2e;
+  const long long row = static_cast<long long>(token) * own.heads + head;
+  Sums sums;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const RowSums& left = pass == 0 ? front.leave : own.leave;
+    const Parts& parts = pass == 0 ? front.parts : own.parts;
+    const float2 ml = left.ml[row];
+    if (ml.y == kInParts) {
+      // (a pass that stood down, or gave up, may have left anything: no number from memory is followed out of the workspace)
+      const int w = __float_as_int(ml.x), r = left.part_row[row];
+      if (w < 0 || w >= parts.workers || r < 0 || r >= parts.rows) continue;
+      add_parts<D>(sums, parts, w, min(parts.heads[w].followers, parts.workers - 1 - w), r, column, side, kAtOnce, sl2);
+    } else if (side == 0) {
+      sums.add(ml.x, ml.y, *reinterpret_cast<const float4*>(left.o + row * D + column), sl2);
+    }
+  }
+  add_sides<D>(sums, sl2);
+  if (side == 0) store4<D, kFp16>(own, RowPlace{row, own.out + token * own.o_token + head * own.o_head}, column, sums.acc, sums.m, sums.l);
+}
+
+template <int D, bool kFp16, int kSplit>
+int launch_join(const Pass& pass, cudaStream_t stream) {
+  const unsigned rows = static_cast<unsigned>((pass.parts.rows * kSplit + kJoinWarps - 1) / kJoinWarps);
+  LIMN_CUDA(launch_overlapped(sdpa_paged_join_kernel<D, kFp16, kSplit>, dim3(static_cast<unsigned>(pass.parts.workers), rows), dim3(kJoinWarps * 32), 0, stream, pass),
+            "launching the kernel that joins parts");
+  note_launches(1);
+  return LIMN_B200_OK;
+}
+
+template <int D, bool kFp16>
+int launch_finish(const Pass& front, const Pass& own, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(own.tokens), static_cast<unsigned>((own.heads + kJoinWarps - 1) / kJoinWarps));
+  LIMN_CUDA(launch_overlapped(sdpa_paged_finish_kernel<D, kFp16>, grid, dim3(kJoinWarps * 32), 0, stream, front, own), "launching the kernel that joins a prefix");
+  note_launches(1);
+  return LIMN_B200_OK;
+}
+
+}  // namespace
+
+int paged_join_launch(const Pass& pass, bool fp16, bool warp_a_row, cudaStream_t stream) {
+  if (warp_a_row) {
+    if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 1>(pass, stream) : launch_join<64, false, 1>(pass, stream);
+    return fp16 ? launch_join<128, true, 1>(pass, stream) : launch_join<128, false, 1>(pass, stream);
+  }
+  if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 8>(pass, stream) : launch_join<64, false, 8>(pass, stream);
+  return fp16 ? launch_join<128, true, 8>(pass, stream) : launch_join<128, false, 8>(pass, stream);
+}
+
+int paged_finish_launch(const Pass& front, const Pass& own, bool fp16, cudaStream_t stream) {
+  if (own.parts.width == 64) return fp16 ? launch_finish<64, true>(front, own, stream) : launch_finish<64, false>(front, own, stream);
+  return fp16 ? launch_finish<128, true>(front, own, stream) : launch_finish<128, false>(front, own, stream);
+}
+
+}  // namespace limn_b200

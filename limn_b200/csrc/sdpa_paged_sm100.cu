@@ -24,8 +24,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "paged.h"
-#include "sm100_ptx.cuh"
+#include "paged_rows.cuh"
 #include "tensor_map.h"
 
 namespace limn_b200 {
@@ -39,7 +38,6 @@ constexpr int kThreads = 320;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr uint32_t kTmemCols = 512;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
 constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
 constexpr int kLeast = kItem;  // cost of the smallest share: about that of the smallest item
@@ -172,9 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     tma_prefetch_descriptor(&maps.v);
   }
   // up to here nothing has touched global memory
-  // (behind a pass over a prefix all but its last kernel are done when this one begins, and only the rows' way out needs that one)
-  const bool late = prm.join.o != nullptr;
-  if (!late) grid_dependency_wait();
+  if (!prm.beside) grid_dependency_wait();
   grid_launch_dependents();
   if (threadIdx.x == 0) {
     abort_flag = *reinterpret_cast<volatile unsigned*>(status) != kStatusOk;  // an earlier kernel gave up: this one stands down
@@ -184,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   const int run = (prm.batch + kThreads - 1) / kThreads;
   {
     long long mine = 0;
+#pragma unroll 1
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
       if (b < prm.batch) mine += Costs(extent_of(prm, b), by_span, prm.causal).all();
@@ -195,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     }
     if (lane == 31) warp_sum[warp] = mine;
     __syncthreads();
+#pragma unroll 1
     for (int w = 0; w < warp; ++w) mine += warp_sum[w];
     share_end[threadIdx.x] = mine;
   }
@@ -256,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       p.kv_head = static_cast<int>(quotient(rest, all));
       rest -= p.kv_head * all;
       int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
+#pragma unroll 1
       while (low < high) {
         const int mid = (low + high + 1) / 2;
         if (costs.before(mid) <= rest) low = mid;
@@ -336,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           return key < s.keys ? table[prm.by_page.of(key)] : 0;
         };
         int page_next[2] = {entry(s.first_tile), entry(s.first_tile + 1)};  // two tiles ahead
+#pragma unroll 1
         for (int j = 0; j < s.loads && ok; ++j, ++step) {
           const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
           const bool fetch = key < s.keys && my_atom < kBoxAtoms;
@@ -414,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     };
     // rows from `from` on of the V tile in `stage` become zeros: slots of a sequence's last page that it has not filled, and what was there before
     auto clear_rows = [&](int stage, int from) {
+#pragma unroll 1
       for (int i = from * (D / 8) + lane; i < kTile * (D / 8); i += 32) {
         const int row = i / (D / 8), piece = i % (D / 8);
         st_shared_v4(base + L::kVOff + stage * L::kTileBytes + (row / 8) * L::kKVGroup + (piece / 8) * L::kKVAtom + (row % 8) * 128 + (piece % 8) * 16, 0u, 0u, 0u, 0u);
@@ -456,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       if (!both && elect_one()) mma_commit(bar(B::k_empty + step % B::kS));
       __syncwarp();
       const int rounds = max(s.count[0], s.count[1]);
+#pragma unroll 1
       for (int j = 0; j < rounds && ok; ++j) {
         bool issued_next = false;
 #pragma unroll
@@ -543,6 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       if (n == 0) {
         // nothing of this share for the tile's rows (its keys end before): a part without keys, if they have one
         if (!s.whole && there) prm.parts.ml[part] = make_float2(-INFINITY, 0.f);
+        if (!s.whole && there && s.begun && prm.leave.o != nullptr) leave_in_parts(prm, row_place(prm, s.first, s.kv_head, row).row, t * kTile + row_in_tile);
         continue;
       }
       const int seen_first = s.keys - s.n;
@@ -557,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       };
       int entry_next = entry(0);
       float m = -INFINITY, l = 0.f;
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++tiles) {
         const unsigned none = __ballot_sync(0xffffffffu, entry_next < 0 || entry_next >= prm.pages);
         if (j + 1 < n) entry_next = entry(j + 1);
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           if (h == 1) {
             // O_t was last written by the product of tile j - 1, which s_full also covers
             if (j > 0 && __any_sync(0xffffffffu, moves)) {
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld32(t_o + 32 * c, o);
@@ -678,14 +682,6 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       };
       const RowPlace place = row_place(prm, s.first, s.kv_head, there ? row : 0);
       if (s.whole && prm.leave.o == nullptr) {
-        float add = 0.f, mine = 1.f;
-        const float* more = nullptr;
-        if (late) grid_dependency_wait();
-        if (late && there) {
-          const float2 ml = prm.join.ml[place.row];
-          more = prm.join.o + place.row * D;
-          merge_stats(m, l, ml.x, ml.y, sl2, mine, add);
-        }
         const float inv = 1.f / l;
         // neighbouring rows' pieces are exchanged before they are stored, so that an instruction writes 64 bytes of each row it touches
         unsigned char* to_row[4];
@@ -695,18 +691,10 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           const unsigned long long at = __shfl_sync(0xffffffffu, mine_at, (lane & ~3) + i);
           to_row[i] = at == 0ull ? nullptr : reinterpret_cast<unsigned char*>(at) + 16 * (lane & 3);
         }
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           take(32 * c, o);
-          if (more != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(more + 32 * c + i);
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * mine + f.x * add), o[i + 1] = __float_as_uint(__uint_as_float(o[i + 1]) * mine + f.y * add);
-              o[i + 2] = __float_as_uint(__uint_as_float(o[i + 2]) * mine + f.z * add), o[i + 3] = __float_as_uint(__uint_as_float(o[i + 3]) * mine + f.w * add);
-            }
-          }
           uint32_t w[4][4];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -723,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         // to the parts, whose rows follow one another, neighbouring rows' pieces are exchanged first, so that an instruction writes 64
         // bytes of each row it touches; rows that there are not go along. To the rows' sums every thread writes its own row
         float* to = s.whole ? prm.leave.o + place.row * D : prm.parts.o + (part - lane + (lane & ~3)) * D + 4 * (lane & 3);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           take(32 * c, o);
@@ -745,6 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           }
         }
         if (there) *(s.whole ? prm.leave.ml + place.row : prm.parts.ml + part) = make_float2(m, l);
+        if (there && !s.whole && s.begun && prm.leave.o != nullptr) leave_in_parts(prm, place.row, t * kTile + row_in_tile);
       }
       // O_t is in registers or stored: the next segment's first product may overwrite it
       tc_fence_before_sync();
@@ -754,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   }
 
   // ---- teardown ----
-  if (late) grid_dependency_wait();  // (whoever waits for this kernel has waited for the one before it)
+  if (prm.beside) grid_dependency_wait();  // (whoever waits for this kernel has waited for the one before it)
   tc_fence_before_sync();
   __syncthreads();
   if (warp == kMmaWarp) {
@@ -825,20 +814,16 @@ int launch_many_d(const Pass& pass, bool fp16, unsigned* status, cudaStream_t st
 
 size_t paged_many_workspace(int width, int sms) { return Parts::bytes(sms, 2 * kTile, width); }
 
-int paged_many_launch(const Pass& given, bool fp16, unsigned char* workspace, cudaStream_t stream) {
-  Pass pass = given;
+int paged_many_launch(Pass& pass, bool fp16, unsigned char* workspace, cudaStream_t stream) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   unsigned* status = nullptr;
   if (int rc = status_word(&status)) return rc;
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
   pass.parts.place(workspace, sms, 2 * kTile, width);
-  int rc;
-  if (width == 64) rc = launch_many_d<64, false>(pass, fp16, status, stream);
-  else if (packs(pass, pass.k, pass.pieces) && packs(pass, pass.v, pass.pieces_v)) rc = launch_many_d<128, true>(pass, fp16, status, stream);
-  else rc = launch_many_d<128, false>(pass, fp16, status, stream);
-  if (rc) return rc;
-  return paged_join_launch(pass, fp16, true, stream);
+  if (width == 64) return launch_many_d<64, false>(pass, fp16, status, stream);
+  if (packs(pass, pass.k, pass.pieces) && packs(pass, pass.v, pass.pieces_v)) return launch_many_d<128, true>(pass, fp16, status, stream);
+  return launch_many_d<128, false>(pass, fp16, status, stream);
 }
 
 }  // namespace limn_b200
