@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include "common.h"
+#include "sm100_ptx.cuh"
 
 namespace limn_b200 {
 namespace paged {
@@ -161,7 +162,7 @@ __device__ __forceinline__ RowPlace row_place(const Pass& p, int first, int kv_h
 // (A side that has seen no key has m = -inf, l = 0 and counts 0; a NaN in l stays one.)
 __device__ __forceinline__ void merge_stats(float& m, float& l, float m_b, float l_b, float sl2, float& keep, float& add) {
   const float top = fmaxf(m, m_b), base = top == -INFINITY ? 0.f : top;
-  keep = exp2f((m - base) * sl2), add = exp2f((m_b - base) * sl2);
+  keep = ptx::exp2_approx((m - base) * sl2), add = ptx::exp2_approx((m_b - base) * sl2);
   m = top, l = l * keep + l_b * add;
 }
 

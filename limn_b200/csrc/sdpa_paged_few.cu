@@ -28,7 +28,7 @@ using namespace paged;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;  // keys
-constexpr int kBegin = 3;  // units that a problem costs besides its keys: its queries, its page table, its way out
+constexpr int kBegin = 2;  // units that a problem costs besides its keys: its queries, its page table, its way out
 constexpr float kSlack = 8.f;
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -61,12 +61,20 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// D: columns the kernel computes with, of which a row has `pieces` groups of 8; the others are zeros in shared memory from the start. The 16-byte pieces
+// of a row are exchanged so that the eight rows of a matrix that ldmatrix reads fall on distinct banks and a copied row fills whole lines (rows of 96
+// columns as 64 and 32; rows 16 bytes further apart than they are long instead: 10 % slower).
 template <int D>
 struct Ring {
   static constexpr int kSide = kUnit * D * 2;  // K or V of a unit
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kStages = D == 128 ? 3 : (D == 96 ? 4 : 6);
   static constexpr int kWarpBytes = kStages * 2 * kSide;
   static constexpr int kBytes = kWarps * kWarpBytes;  // 192 KB
+  static constexpr int kWidth = D == 96 ? 128 : D;    // columns of a row's sums in memory
+  __device__ static __forceinline__ uint32_t place(int row, int piece) {
+    if (D != 96) return row * (D * 2) + ((piece ^ (row & 7)) << 4);
+    return piece < 8 ? row * 128 + ((piece ^ (row & 7)) << 4) : kUnit * 128 + row * 64 + (((piece - 8) ^ ((row >> 1) & 3)) << 4);
+  }
 };
 
 // Where a warp is in the work: unit `unit` of `units` of problem (b, kv_head), `cost` into its share. What a problem costs besides its keys
@@ -157,9 +165,25 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   Cursor ahead = at;
   int loaded = 0;
   const uint32_t mine = ptx::smem_addr(ring) + warp * R::kWarpBytes;
-  constexpr int kLanes = D / 8;         // lanes to a row of 16-byte pieces
-  constexpr int kRows = 32 / kLanes;    // rows a copy of the warp takes
-  const int piece = lane % kLanes, row_in = lane / kLanes;
+  // a lane's copies of the 8 rows of a half unit: where from (beyond the first row's first byte) and where to
+  constexpr int kPieces = D / 8, kCopies = kPieces / 4;
+  long long k_off[kCopies], v_off[kCopies];
+  uint32_t to_off[kCopies];
+  bool k_there[kCopies], v_there[kCopies];
+  int row_of[kCopies];
+#pragma unroll
+  for (int j = 0; j < kCopies; ++j) {
+    const int r = (j * 32 + lane) / kPieces, piece = (j * 32 + lane) % kPieces;
+    row_of[j] = r, to_off[j] = R::place(r, piece);
+    k_off[j] = r * prm.k.slot + piece * 16, v_off[j] = r * prm.v.slot + piece * 16;
+    k_there[j] = piece < prm.pieces, v_there[j] = piece < prm.pieces_v;
+  }
+  if (prm.pieces < kPieces || prm.pieces_v < kPieces) {
+    for (int i = lane; i < R::kStages * 2 * kUnit * kPieces; i += 32) {
+      const int side_row = i / kPieces, piece = i % kPieces;
+      if (piece >= ((side_row / kUnit) & 1 ? prm.pieces_v : prm.pieces)) ptx::st_shared_v4(mine + side_row / kUnit * R::kSide + R::place(side_row % kUnit, piece), 0u, 0u, 0u, 0u);
+    }
+  }
   // A lane keeps the page of one of 32 groups of 8 keys (no page ends inside one), 16 units, and the table's entry for the 16 units behind.
   int block = -1, page = -1, entry_next = -1;
   unsigned none = 0;  // two bits for each place of the ring: which 8 of its unit's keys have a page that is none
@@ -186,15 +210,15 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
         const int slot = prm.by_page.rest(key0);
         const long long in_page = max(p, 0);
         if (p < 0 && key0 < ahead.e.keys) none |= 1u << (2 * place_at + half);
-        const unsigned char* k_from = prm.k.base + in_page * prm.k.page + ahead.kv_head * prm.k.head + slot * prm.k.slot + 16 * (piece < prm.pieces ? piece : 0);
-        const unsigned char* v_from = prm.v.base + in_page * prm.v.page + ahead.kv_head * prm.v.head + slot * prm.v.slot + 16 * (piece < prm.pieces_v ? piece : 0);
+        const unsigned char* k_from = prm.k.base + in_page * prm.k.page + ahead.kv_head * prm.k.head + slot * prm.k.slot;
+        const unsigned char* v_from = prm.v.base + in_page * prm.v.page + ahead.kv_head * prm.v.head + slot * prm.v.slot;
+        const int rows_there = p >= 0 ? ahead.e.keys - key0 : 0;  // (the others are zeros, and what they would be is not read)
 #pragma unroll
-        for (int i = 0; i < 8 / kRows; ++i) {
-          const int r = i * kRows + row_in;  // of the 8
-          const bool there = p >= 0 && key0 + r < ahead.e.keys;
-          const uint32_t place = (half * 8 + r) * (D * 2) + ((piece ^ r) << 4);
-          copy16(k_to + place, k_from + r * prm.k.slot, there && piece < prm.pieces);
-          copy16(v_to + place, v_from + r * prm.v.slot, there && piece < prm.pieces_v);
+        for (int j = 0; j < kCopies; ++j) {
+          const bool there = row_of[j] < rows_there;
+          const uint32_t to = to_off[j] + half * 8 * (D != 96 ? D * 2 : (to_off[j] < kUnit * 128 ? 128 : 64));  // (the second 8 rows lie as the first)
+          if (k_there[j]) copy16(k_to + to, k_from + k_off[j], there);
+          if (v_there[j]) copy16(v_to + to, v_from + v_off[j], there);
         }
       }
       ++loaded, ++ahead.cost;
@@ -257,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       // A: 16 keys x 16 columns; lanes 0-15 name the keys' first 8 columns' pieces, 16-31 the second's
       uint32_t a[4];
       const int r = lane & 15, pc = kk * 2 + (lane >> 4);
-      ldmatrix4(a, k_at + r * (D * 2) + ((pc ^ (r & 7)) << 4));
+      ldmatrix4(a, k_at + R::place(r, pc));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) mma<kFp16>(s[nt], a, q[nt][kk][0], q[nt][kk][1]);
     }
@@ -314,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       // A: 16 columns x 16 keys out of rows of keys: (keys 0-7, columns 0-7), (keys 0-7, columns 8-15), (keys 8-15, ...)
       uint32_t a[4];
       const int r = (lane & 7) + ((lane >> 4) << 3), pc = mt * 2 + ((lane >> 3) & 1);
-      ldmatrix4_trans(a, v_at + r * (D * 2) + ((pc ^ (r & 7)) << 4));
+      ldmatrix4_trans(a, v_at + R::place(r, pc));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) mma<kFp16>(o[nt][mt], a, p[nt][0], p[nt][1]);
     }
@@ -341,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
           const int r = nt * 8 + cq * 2 + c;
           if (r >= rows) continue;
           const long long row = whole ? row_place(prm, at.e.first, at.kv_head, r).row : part + r;
-          float* to_o = (whole ? prm.leave.o : by_warp.o) + row * D + kq;
+          float* to_o = (whole ? prm.leave.o : by_warp.o) + row * R::kWidth + kq;
 #pragma unroll
           for (int mt = 0; mt < D / 16; ++mt) to_o[mt * 16] = o[nt][mt][c], to_o[mt * 16 + 8] = o[nt][mt][c + 2];
           if (kq == 0) (whole ? prm.leave.ml : by_warp.ml)[row] = make_float2(m[nt][c], l[nt][c]);
@@ -380,50 +404,51 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 
   // ---- the block's parts: chain 0 enters from the block before, chain 1 + w begins with warp w ----
   __syncthreads();
+  constexpr int kLanes = R::kWidth / 4, kAtOnce = 32 / kLanes;  // lanes to a row of sums, rows a warp has at once
   int turn = 0;
+#pragma unroll 1
   for (int chain = 0; chain <= kWarps; ++chain) {
-    if (!(chain == 0 ? shared[0].enters : shared[chain - 1].begins)) continue;
+    const Shared& at_head = shared[chain == 0 ? 0 : chain - 1];
+    if (!(chain == 0 ? at_head.enters : at_head.begins)) continue;
     int members = 0;  // warps chain, chain + 1, ... that it enters
     bool open = true;
     while (open && chain + members < kWarps) open = shared[chain + members].through != 0, ++members;
-    const Shared& at_head = shared[chain == 0 ? 0 : chain - 1];
     const int which = chain == 0 ? 0 : 1;
-    const int rows = at_head.n[which] * prm.group;
+    const int first = at_head.first[which], n = at_head.n[which], kv_head = at_head.kv_head[which], rows = n * prm.group;
     const int warp0 = blockIdx.x * kWarps + chain;  // the first worker it enters
     if (chain > 0 && open && threadIdx.x == 0) {
-      const int last = static_cast<int>(quotient(quotient(at_head.end - 1, share), kWarps));  // the block that has the problem's last unit
-      prm.parts.heads[blockIdx.x] = Head{last - static_cast<int>(blockIdx.x), at_head.first[which], at_head.n[which], at_head.kv_head[which], 0, kPagedFewRows};
+      const int last = static_cast<int>(quotient(at_head.end - 1, share)) / kWarps;  // the block that has the problem's last unit
+      prm.parts.heads[blockIdx.x] = Head{last - static_cast<int>(blockIdx.x), first, n, kv_head, 0, kPagedFewRows};
     }
-    for (int r = 0; r < rows; ++r) {
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
       if (turn++ % kWarps != warp) continue;
-      constexpr int kLanesO = D / 4;
-      const int column = (lane % kLanesO) * 4;
-      float2 ml[kWarps];
-      float4 sums[kWarps];
+      const int r = r0 + lane / kLanes, column = (lane % kLanes) * 4;
+      if (r >= rows) continue;
+      Sums sums;
+      // four parts at a time: the beginning's own first (chain > 0), then those of the warps it enters
+#pragma unroll 1
+      for (int i0 = -which; i0 < members; i0 += 4) {
+        float2 ml[4];
+        float4 o[4];
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) {  // the beginning's own part first (chain > 0), then those it enters
-        const int member = i - which;
-        const long long part = (member < 0 ? 2LL * (warp0 - 1) + 1 : 2LL * (warp0 + member)) * (NT * 8) + r;
-        ml[i] = make_float2(-INFINITY, 0.f), sums[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (member < members) ml[i] = by_warp.ml[part], sums[i] = *reinterpret_cast<const float4*>(by_warp.o + part * D + column);
-      }
-      float m = ml[0].x, l = ml[0].y;
-      float4 acc = sums[0];
+        for (int u = 0; u < 4; ++u) {
+          const int member = i0 + u;
+          const long long part = (member < 0 ? 2LL * (warp0 - 1) + 1 : 2LL * (warp0 + member)) * (NT * 8) + r;
+          ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (member < members) ml[u] = by_warp.ml[part], o[u] = *reinterpret_cast<const float4*>(by_warp.o + part * R::kWidth + column);
+        }
 #pragma unroll
-      for (int i = 1; i < kWarps; ++i) {
-        float keep, add;
-        merge_stats(m, l, ml[i].x, ml[i].y, sl2, keep, add);
-        acc = make_float4(acc.x * keep + sums[i].x * add, acc.y * keep + sums[i].y * add, acc.z * keep + sums[i].z * add, acc.w * keep + sums[i].w * add);
+        for (int u = 0; u < 4; ++u) sums.add(ml[u].x, ml[u].y, o[u], sl2);
       }
-      if (lane >= kLanesO) continue;
       if (chain > 0 && !open) {
-        finish4<D, kFp16>(prm, row_place(prm, at_head.first[which], at_head.kv_head[which], r), column, acc, m, l);
+        finish4<R::kWidth, kFp16>(prm, row_place(prm, first, kv_head, r), column, sums.acc, sums.m, sums.l);
       } else {
         const long long part = (2LL * blockIdx.x + which) * (NT * 8) + r;
-        *reinterpret_cast<float4*>(prm.parts.o + part * D + column) = acc;
+        *reinterpret_cast<float4*>(prm.parts.o + part * R::kWidth + column) = sums.acc;
         if (column == 0) {
-          prm.parts.ml[part] = make_float2(m, l);
-          if (chain > 0 && prm.leave.o != nullptr) leave_in_parts(prm, row_place(prm, at_head.first[which], at_head.kv_head[which], r).row, r);
+          prm.parts.ml[part] = make_float2(sums.m, sums.l);
+          if (chain > 0 && prm.leave.o != nullptr) leave_in_parts(prm, row_place(prm, first, kv_head, r).row, r);
         }
       }
     }
@@ -445,6 +470,12 @@ int launch_few(const Pass& pass, const Parts& by_warp, cudaStream_t stream) {
   return LIMN_B200_OK;
 }
 
+template <int D>
+int launch_few_d(const Pass& pass, const Parts& by_warp, bool fp16, int rows, cudaStream_t stream) {
+  if (rows <= 8) return fp16 ? launch_few<D, true, 1>(pass, by_warp, stream) : launch_few<D, false, 1>(pass, by_warp, stream);
+  return fp16 ? launch_few<D, true, 2>(pass, by_warp, stream) : launch_few<D, false, 2>(pass, by_warp, stream);
+}
+
 int few_tile(int rows) { return rows <= 8 ? 8 : kPagedFewRows; }
 
 }  // namespace
@@ -458,12 +489,9 @@ int paged_few_launch(Pass& pass, bool fp16, int rows, unsigned char* workspace, 
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
   pass.parts.place(workspace, sms, few_tile(rows), width);
   by_warp.place(workspace + Parts::bytes(sms, few_tile(rows), width), sms * kWarps, few_tile(rows), width);
-  if (width == 64) {
-    if (rows <= 8) return fp16 ? launch_few<64, true, 1>(pass, by_warp, stream) : launch_few<64, false, 1>(pass, by_warp, stream);
-    return fp16 ? launch_few<64, true, 2>(pass, by_warp, stream) : launch_few<64, false, 2>(pass, by_warp, stream);
-  }
-  if (rows <= 8) return fp16 ? launch_few<128, true, 1>(pass, by_warp, stream) : launch_few<128, false, 1>(pass, by_warp, stream);
-  return fp16 ? launch_few<128, true, 2>(pass, by_warp, stream) : launch_few<128, false, 2>(pass, by_warp, stream);
+  if (width == 64) return launch_few_d<64>(pass, by_warp, fp16, rows, stream);
+  if (pass.pieces <= 12 && pass.pieces_v <= 12) return launch_few_d<96>(pass, by_warp, fp16, rows, stream);
+  return launch_few_d<128>(pass, by_warp, fp16, rows, stream);
 }
 
 }  // namespace limn_b200

@@ -78,38 +78,48 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
   if (side == 0) store4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row), column, sums.acc, sums.m, sums.l);
 }
 
-// A warp to a (token, head) row: what both passes left of it, of a sequence that is one. Rows of tokens that belong to none are left alone.
-template <int D, bool kFp16>
+// A (token, head) row to kSplit warps: what both passes left of it, of a sequence that is one. Rows of tokens that belong to none are left alone.
+template <int D, bool kFp16, int kSplit>
 __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_finish_kernel(const Pass front, const Pass own) {
-  constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
+  constexpr int kRows = kJoinWarps / kSplit, kLanes = D / 4, kAtOnce = 32 / kLanes;
+  __shared__ float4 all_sums[kJoinWarps][32];
+  __shared__ float2 all_stats[kJoinWarps];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int token = blockIdx.x, head = blockIdx.y * kJoinWarps + warp;
-  if (head >= own.heads) return;
-  const int b = sequence_of(own.q_start, own.batch, token, lane);
-  if (b >= own.batch) return;
-  const Extent e = extent_of(own, b);
-  if (token < e.first || token - e.first >= e.n) return;  // (so where the offsets are out of order)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, split = warp % kSplit;
+  const int token = blockIdx.x, head = min(static_cast<int>(blockIdx.y) * kRows + warp / kSplit, own.heads - 1);  // (the last block's spare warps repeat a row)
   const int column = (lane % kLanes) * 4, side = lane / kLanes;
   const float sl2 = own.scale * kLog2e;
   const long long row = static_cast<long long>(token) * own.heads + head;
+  // (all asked for before whose token it is is known: the memory is there for every row)
+  const float2 front_ml = front.leave.ml[row], own_ml = own.leave.ml[row];
+  const float4 front_o = *reinterpret_cast<const float4*>(front.leave.o + row * D + column), own_o = *reinterpret_cast<const float4*>(own.leave.o + row * D + column);
+  const int b = sequence_of(own.q_start, own.batch, token, lane);
+  if (b >= own.batch) return;  // (as is all of the block)
+  const Extent e = extent_of(own, b);
+  if (token < e.first || token - e.first >= e.n) return;  // (so where the offsets are out of order)
   Sums sums;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    const RowSums& left = pass == 0 ? front.leave : own.leave;
-    const Parts& parts = pass == 0 ? front.parts : own.parts;
-    const float2 ml = left.ml[row];
+  auto add = [&](const Pass& pass, const float2& ml, const float4& o) {
     if (ml.y == kInParts) {
       // (a pass that stood down, or gave up, may have left anything: no number from memory is followed out of the workspace)
-      const int w = __float_as_int(ml.x), r = left.part_row[row];
-      if (w < 0 || w >= parts.workers || r < 0 || r >= parts.rows) continue;
-      add_parts<D>(sums, parts, w, min(parts.heads[w].followers, parts.workers - 1 - w), r, column, side, kAtOnce, sl2);
-    } else if (side == 0) {
-      sums.add(ml.x, ml.y, *reinterpret_cast<const float4*>(left.o + row * D + column), sl2);
+      const int w = __float_as_int(ml.x), r = pass.leave.part_row[row];
+      if (w < 0 || w >= pass.parts.workers || r < 0 || r >= pass.parts.rows) return;
+      add_parts<D>(sums, pass.parts, w, min(pass.parts.heads[w].followers, pass.parts.workers - 1 - w), r, column, split * kAtOnce + side, kSplit * kAtOnce, sl2);
+    } else if (side == 0 && split == 0) {
+      sums.add(ml.x, ml.y, o, sl2);
     }
-  }
+  };
+  add(front, front_ml, front_o);
+  add(own, own_ml, own_o);
   add_sides<D>(sums, sl2);
+  if (kSplit > 1) {
+    all_sums[warp][lane] = sums.acc;
+    if (lane == 0) all_stats[warp] = make_float2(sums.m, sums.l);
+    __syncthreads();
+    if (split > 0) return;
+#pragma unroll
+    for (int i = 1; i < kSplit; ++i) sums.add(all_stats[warp + i].x, all_stats[warp + i].y, all_sums[warp + i][lane], sl2);
+  }
   if (side == 0) store4<D, kFp16>(own, RowPlace{row, own.out + token * own.o_token + head * own.o_head}, column, sums.acc, sums.m, sums.l);
 }
 
@@ -122,12 +132,20 @@ int launch_join(const Pass& pass, cudaStream_t stream) {
   return LIMN_B200_OK;
 }
 
-template <int D, bool kFp16>
-int launch_finish(const Pass& front, const Pass& own, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(own.tokens), static_cast<unsigned>((own.heads + kJoinWarps - 1) / kJoinWarps));
-  LIMN_CUDA(launch_overlapped(sdpa_paged_finish_kernel<D, kFp16>, grid, dim3(kJoinWarps * 32), 0, stream, front, own), "launching the kernel that joins a prefix");
+template <int D, bool kFp16, int kSplit>
+int launch_finish_s(const Pass& front, const Pass& own, cudaStream_t stream) {
+  constexpr int kRows = kJoinWarps / kSplit;
+  const dim3 grid(static_cast<unsigned>(own.tokens), static_cast<unsigned>((own.heads + kRows - 1) / kRows));
+  LIMN_CUDA(launch_overlapped(sdpa_paged_finish_kernel<D, kFp16, kSplit>, grid, dim3(kJoinWarps * 32), 0, stream, front, own), "launching the kernel that joins a prefix");
   note_launches(1);
   return LIMN_B200_OK;
+}
+
+// Few rows have many parts each, and wait for them; many rows have few.
+template <int D, bool kFp16>
+int launch_finish(const Pass& front, const Pass& own, cudaStream_t stream) {
+  if (static_cast<long long>(own.tokens) * own.heads <= 4096) return launch_finish_s<D, kFp16, 4>(front, own, stream);
+  return launch_finish_s<D, kFp16, 1>(front, own, stream);
 }
 
 }  // namespace
