@@ -30,6 +30,7 @@ struct Head {
   int tile_rows;  // rows of a tile: row r of a part is row row0 + r / 128 * tile_rows + r % 128, if r % 128 < tile_rows
 };
 struct Parts {
+  double share = 0.0;      // 1 / workers
   float* o = nullptr;      // (2 workers, rows, width)
   float2* ml = nullptr;    // (2 workers, rows)
   Head* heads = nullptr;   // (workers)
@@ -38,9 +39,11 @@ struct Parts {
   static size_t ml_bytes(int workers, int rows) { return static_cast<size_t>(2) * workers * rows * 8; }
   static size_t head_bytes(int workers) { return (static_cast<size_t>(workers) * sizeof(Head) + 255) / 256 * 256; }
   static size_t bytes(int workers, int rows, int width) { return o_bytes(workers, rows, width) + ml_bytes(workers, rows) + head_bytes(workers); }
+  // A worker's share of `total`: shares of all workers cover it.
+  __device__ __forceinline__ long long share_of(long long total) const { return static_cast<long long>(static_cast<double>(total) * share) + 1; }
   // Lays the parts out in `memory`, which has the bytes for them.
   void place(unsigned char* memory, int workers_, int rows_, int width_) {
-    workers = workers_, rows = rows_, width = width_;
+    workers = workers_, rows = rows_, width = width_, share = 1.0 / workers_;
     o = reinterpret_cast<float*>(memory), memory += o_bytes(workers, rows, width);
     ml = reinterpret_cast<float2*>(memory), memory += ml_bytes(workers, rows);
     heads = reinterpret_cast<Head*>(memory);
@@ -166,10 +169,24 @@ __device__ __forceinline__ void merge_stats(float& m, float& l, float m_b, float
   m = top, l = l * keep + l_b * add;
 }
 
-// A quotient of numbers that are not negative, by the short division where both allow it (the long one takes some 100 instructions).
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
-  return a / b;
+// a / b of numbers below 2^52 whose quotient fits an int: by float64 and put right. (The compiler's 64-bit division is some 100 instructions.)
+__device__ __forceinline__ int small_quotient(long long a, long long b) {
+  long long q = static_cast<long long>(static_cast<double>(a) * (1.0 / static_cast<double>(b)));
+  while (q * b > a) --q;
+  while ((q + 1) * b <= a) ++q;
+  return static_cast<int>(q);
+}
+
+// The place in ends[0..n), which rises, of the first that times `by` is above x.
+__device__ __forceinline__ int first_above(const long long* ends, int n, int by, long long x) {
+  int low = 0, high = n;
+#pragma unroll 1
+  while (low < high) {
+    const int mid = (low + high) >> 1;
+    if (ends[mid] * by <= x) low = mid + 1;
+    else high = mid;
+  }
+  return low;
 }
 
 }  // namespace paged

@@ -28,7 +28,7 @@ using namespace paged;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;  // keys
-constexpr int kBegin = 2;  // units that a problem costs besides its keys: its queries, its page table, its way out
+constexpr int kBegin = 4;  // units that a problem costs besides its keys: its queries, its page table, its way out
 constexpr float kSlack = 8.f;
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -61,20 +61,17 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// D: columns the kernel computes with, of which a row has `pieces` groups of 8; the others are zeros in shared memory from the start. The 16-byte pieces
-// of a row are exchanged so that the eight rows of a matrix that ldmatrix reads fall on distinct banks and a copied row fills whole lines (rows of 96
-// columns as 64 and 32; rows 16 bytes further apart than they are long instead: 10 % slower).
+// D: columns the kernel computes with, of which a row has `pieces` groups of 8; the others are zeros in shared memory from the start (computing with 96
+// columns instead, for rows that have no more: 8 % slower at 80, the lanes' copies and rows of memory no longer matching). The 16-byte
+// pieces of a row are exchanged so that the eight rows of a matrix that ldmatrix reads fall on distinct banks and a copied row fills whole lines (rows
+// 16 bytes further apart than they are long instead: 10 % slower).
 template <int D>
 struct Ring {
   static constexpr int kSide = kUnit * D * 2;  // K or V of a unit
-  static constexpr int kStages = D == 128 ? 3 : (D == 96 ? 4 : 6);
+  static constexpr int kStages = D == 128 ? 3 : 6;
   static constexpr int kWarpBytes = kStages * 2 * kSide;
   static constexpr int kBytes = kWarps * kWarpBytes;  // 192 KB
-  static constexpr int kWidth = D == 96 ? 128 : D;    // columns of a row's sums in memory
-  __device__ static __forceinline__ uint32_t place(int row, int piece) {
-    if (D != 96) return row * (D * 2) + ((piece ^ (row & 7)) << 4);
-    return piece < 8 ? row * 128 + ((piece ^ (row & 7)) << 4) : kUnit * 128 + row * 64 + (((piece - 8) ^ ((row >> 1) & 3)) << 4);
-  }
+  __device__ static __forceinline__ uint32_t place(int row, int piece) { return row * (D * 2) + ((piece ^ (row & 7)) << 4); }
 };
 
 // Where a warp is in the work: unit `unit` of `units` of problem (b, kv_head), `cost` into its share. What a problem costs besides its keys
@@ -134,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   }
   const int worker = blockIdx.x * kWarps + warp;
   const long long total = share_end[kThreads - 1] * prm.kv_heads;
-  const long long share = quotient(total + by_warp.workers - 1, by_warp.workers);
+  const long long share = by_warp.share_of(total);
   const long long from = min(total, worker * share), to = min(total, from + share);
   const int span = static_cast<int>(to - from);
   if (lane == 0) shared[warp].enters = shared[warp].begins = 0;
@@ -142,10 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 
   Cursor at = {};
   if (span > 0) {
-    // the run of sequences that `from` falls into: how many threads' sums end at or before it
-    int before = 0;
-#pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) before += __popc(__ballot_sync(0xffffffffu, share_end[i * 32 + lane] * prm.kv_heads <= from));
+    const int before = first_above(share_end, kThreads, prm.kv_heads, from);  // the run of sequences that `from` falls into
     long long rest = from - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
     at.b = before * run - 1;
     int cost;
@@ -156,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       if (rest < static_cast<long long>(cost) * prm.kv_heads) break;
       rest -= static_cast<long long>(cost) * prm.kv_heads;
     } while (at.b + 1 < prm.batch);
-    at.kv_head = static_cast<int>(quotient(rest, cost));
+    at.kv_head = small_quotient(rest, cost);
     const int into = static_cast<int>(rest - static_cast<long long>(at.kv_head) * cost);
     at.unit = max(0, into - kBegin), at.cost = max(0, kBegin - into);
   }
@@ -216,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 #pragma unroll
         for (int j = 0; j < kCopies; ++j) {
           const bool there = row_of[j] < rows_there;
-          const uint32_t to = to_off[j] + half * 8 * (D != 96 ? D * 2 : (to_off[j] < kUnit * 128 ? 128 : 64));  // (the second 8 rows lie as the first)
+          const uint32_t to = to_off[j] + half * 8 * (D * 2);  // (the second 8 rows lie as the first)
           if (k_there[j]) copy16(k_to + to, k_from + k_off[j], there);
           if (v_there[j]) copy16(v_to + to, v_from + v_off[j], there);
         }
@@ -365,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
           const int r = nt * 8 + cq * 2 + c;
           if (r >= rows) continue;
           const long long row = whole ? row_place(prm, at.e.first, at.kv_head, r).row : part + r;
-          float* to_o = (whole ? prm.leave.o : by_warp.o) + row * R::kWidth + kq;
+          float* to_o = (whole ? prm.leave.o : by_warp.o) + row * D + kq;
 #pragma unroll
           for (int mt = 0; mt < D / 16; ++mt) to_o[mt * 16] = o[nt][mt][c], to_o[mt * 16 + 8] = o[nt][mt][c + 2];
           if (kq == 0) (whole ? prm.leave.ml : by_warp.ml)[row] = make_float2(m[nt][c], l[nt][c]);
@@ -404,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 
   // ---- the block's parts: chain 0 enters from the block before, chain 1 + w begins with warp w ----
   __syncthreads();
-  constexpr int kLanes = R::kWidth / 4, kAtOnce = 32 / kLanes;  // lanes to a row of sums, rows a warp has at once
+  constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;  // lanes to a row of sums, rows a warp has at once
   int turn = 0;
 #pragma unroll 1
   for (int chain = 0; chain <= kWarps; ++chain) {
@@ -417,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     const int first = at_head.first[which], n = at_head.n[which], kv_head = at_head.kv_head[which], rows = n * prm.group;
     const int warp0 = blockIdx.x * kWarps + chain;  // the first worker it enters
     if (chain > 0 && open && threadIdx.x == 0) {
-      const int last = static_cast<int>(quotient(at_head.end - 1, share)) / kWarps;  // the block that has the problem's last unit
+      const int last = small_quotient(at_head.end - 1, share) / kWarps;  // the block that has the problem's last unit
       prm.parts.heads[blockIdx.x] = Head{last - static_cast<int>(blockIdx.x), first, n, kv_head, 0, kPagedFewRows};
     }
 #pragma unroll 1
@@ -436,16 +430,16 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
           const int member = i0 + u;
           const long long part = (member < 0 ? 2LL * (warp0 - 1) + 1 : 2LL * (warp0 + member)) * (NT * 8) + r;
           ml[u] = make_float2(-INFINITY, 0.f), o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (member < members) ml[u] = by_warp.ml[part], o[u] = *reinterpret_cast<const float4*>(by_warp.o + part * R::kWidth + column);
+          if (member < members) ml[u] = by_warp.ml[part], o[u] = *reinterpret_cast<const float4*>(by_warp.o + part * D + column);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) sums.add(ml[u].x, ml[u].y, o[u], sl2);
       }
       if (chain > 0 && !open) {
-        finish4<R::kWidth, kFp16>(prm, row_place(prm, first, kv_head, r), column, sums.acc, sums.m, sums.l);
+        finish4<D, kFp16>(prm, row_place(prm, first, kv_head, r), column, sums.acc, sums.m, sums.l);
       } else {
         const long long part = (2LL * blockIdx.x + which) * (NT * 8) + r;
-        *reinterpret_cast<float4*>(prm.parts.o + part * R::kWidth + column) = sums.acc;
+        *reinterpret_cast<float4*>(prm.parts.o + part * D + column) = sums.acc;
         if (column == 0) {
           prm.parts.ml[part] = make_float2(sums.m, sums.l);
           if (chain > 0 && prm.leave.o != nullptr) leave_in_parts(prm, row_place(prm, first, kv_head, r).row, r);
@@ -490,7 +484,6 @@ int paged_few_launch(Pass& pass, bool fp16, int rows, unsigned char* workspace, 
   pass.parts.place(workspace, sms, few_tile(rows), width);
   by_warp.place(workspace + Parts::bytes(sms, few_tile(rows), width), sms * kWarps, few_tile(rows), width);
   if (width == 64) return launch_few_d<64>(pass, by_warp, fp16, rows, stream);
-  if (pass.pieces <= 12 && pass.pieces_v <= 12) return launch_few_d<96>(pass, by_warp, fp16, rows, stream);
   return launch_few_d<128>(pass, by_warp, fp16, rows, stream);
 }
 

@@ -227,20 +227,14 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   if (warp == kProducerWarp) {
     // ================= the share, and TMA =================
     const long long total = share_end[kThreads - 1] * prm.kv_heads;
-    const long long share = max(static_cast<long long>(kLeast), quotient(total + gridDim.x - 1, gridDim.x));
+    const long long share = max(static_cast<long long>(kLeast), prm.parts.share_of(total));
     const long long from = blockIdx.x * share, to = from + share;
     const bool any = ok && from < total;
     // where the share begins and ends, in the warp's halves
     Place p = {};
     if (any) {
       const long long x = lane < 16 ? from : min(to, total - 1);
-      int before_from = 0, before_to = 0;
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) {
-        const long long end = share_end[i * 32 + lane] * prm.kv_heads;
-        before_from += __popc(__ballot_sync(0xffffffffu, end <= from)), before_to += __popc(__ballot_sync(0xffffffffu, end <= min(to, total - 1)));
-      }
-      const int before = lane < 16 ? before_from : before_to;
+      const int before = first_above(share_end, kThreads, prm.kv_heads, x);
       long long rest = x - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads), all;
       p.b = before * run - 1;
       do {
@@ -251,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         rest -= all * prm.kv_heads;
       } while (p.b + 1 < prm.batch);
       const Costs costs(p.e, by_span, prm.causal);
-      p.kv_head = static_cast<int>(quotient(rest, all));
+      p.kv_head = small_quotient(rest, all);
       rest -= p.kv_head * all;
       int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
 #pragma unroll 1
@@ -266,12 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       __syncwarp();
     }
     auto of_half = [&](int from_lane) {
-      Place q;
-      int* words = reinterpret_cast<int*>(&q);
-      const int* mine = reinterpret_cast<const int*>(&p);
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(Place) / sizeof(int)); ++i) words[i] = __shfl_sync(0xffffffffu, mine[i], from_lane);
-      return q;
+      auto word = [&](int x) { return __shfl_sync(0xffffffffu, x, from_lane); };
+      return Place{word(p.b), word(p.kv_head), word(p.j), word(p.step), Extent{word(p.e.first), word(p.e.n), word(p.e.keys)}, __shfl_sync(0xffffffffu, p.into, from_lane)};
     };
     Place at = of_half(0), end = of_half(16);
     if (to >= total) end.b = prm.batch, end.kv_head = end.j = 0;  // nothing ends it
@@ -367,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         if (s.begun && !s.whole && lane == 0) {
           // workers behind this one whose share begins inside the item, before the middle of its last step
           const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(kTile) - kTile / 2);
-          prm.parts.heads[blockIdx.x] = Head{static_cast<int>(quotient(begins + limit - 1, share)) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
+          prm.parts.heads[blockIdx.x] = Head{small_quotient(begins + limit - 1, share) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
         }
       }
       // the next item
