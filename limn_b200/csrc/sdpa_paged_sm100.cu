@@ -40,7 +40,7 @@ constexpr int kMmaWarp = 9;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleSlack = 8.f;
 constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
-constexpr int kLeast = kItem;  // cost of the smallest share: about that of the smallest item
+constexpr int kLeast = 256;  // cost of the smallest share: about that of the smallest item
 
 // kPacked: how a tile of K or V lies in shared memory at head dim 128. Column block after column block (64 columns of all 128 rows each), a box
 // of TMA fetches 64 columns of a run of keys; packed, the two column blocks of 8 rows lie side by side, and a box fetches all columns of the
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       ok = next_segment(n_item, s);
       if (!ok || !s.valid) break;
       const bool both = s.both != 0;
-      const int n = s.count[t];
+      const int n = t ? s.count[1] : s.count[0];
       const int top_row = s.row0 + (both ? 0 : t) * tile_rows;       // the tile's first row
       const int row = top_row + row_in_tile;
       const bool there = row_in_tile < tile_rows && row < s.n * prm.group;
