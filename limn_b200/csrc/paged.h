@@ -103,6 +103,7 @@ struct Pass {
   // The kernel in front of this one in the stream is of the same call and concerns it not: what this pass reads was there before that one began. So it
   // need not be waited for until the end.
   int beside = 0;
+  int blocks = 0;  // that make the pass, one to a multiprocessor
 };
 
 // A sequence's extents: `first` token of `n`, `keys` in its pages. One that cannot be has n = 0 and is noted.

@@ -68,6 +68,7 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   unsigned char* memory = static_cast<unsigned char*>(workspace);
   const long long rows = static_cast<long long>(step->max_t_q) * prm.group;
+  if (int rc = sm_count(&prm.blocks)) return rc;
   if (prefix_len == 0) {
     if (int rc = launch_pass(prm, fp16, rows, memory, on)) return rc;
     return paged_join_launch(prm, fp16, rows > kPagedFewRows, on);

@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   __shared__ Shared shared[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float sl2 = prm.scale * kLog2e;
-  if (!prm.beside) ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
+  const bool known = prm.q_start == nullptr;  // one sequence of a known length: the shares need no memory
+  if (!prm.beside && !known) ptx::grid_dependency_wait();
 
   // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
   const int run = (prm.batch + kThreads - 1) / kThreads;
@@ -135,7 +135,6 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   const long long from = min(total, worker * share), to = min(total, from + share);
   const int span = static_cast<int>(to - from);
   if (lane == 0) shared[warp].enters = shared[warp].begins = 0;
-  if (threadIdx.x == 0) prm.parts.heads[blockIdx.x].followers = 0;
 
   Cursor at = {};
   if (span > 0) {
@@ -154,6 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     const int into = static_cast<int>(rest - static_cast<long long>(at.kv_head) * cost);
     at.unit = max(0, into - kBegin), at.cost = max(0, kBegin - into);
   }
+
+  if (!prm.beside && known) ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  if (threadIdx.x == 0) prm.parts.heads[blockIdx.x].followers = 0;
 
   // ---- copies: run ahead of the arithmetic with a cursor of their own ----
   Cursor ahead = at;
@@ -478,11 +481,9 @@ size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(s
 
 int paged_few_launch(Pass& pass, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream) {
   Parts by_warp;
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
-  pass.parts.place(workspace, sms, few_tile(rows), width);
-  by_warp.place(workspace + Parts::bytes(sms, few_tile(rows), width), sms * kWarps, few_tile(rows), width);
+  pass.parts.place(workspace, pass.blocks, few_tile(rows), width);
+  by_warp.place(workspace + Parts::bytes(pass.blocks, few_tile(rows), width), pass.blocks * kWarps, few_tile(rows), width);
   if (width == 64) return launch_few_d<64>(pass, by_warp, fp16, rows, stream);
   return launch_few_d<128>(pass, by_warp, fp16, rows, stream);
 }

@@ -169,13 +169,9 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     tma_prefetch_descriptor(&maps.k);
     tma_prefetch_descriptor(&maps.v);
   }
-  // up to here nothing has touched global memory
-  if (!prm.beside) grid_dependency_wait();
-  grid_launch_dependents();
-  if (threadIdx.x == 0) {
-    abort_flag = *reinterpret_cast<volatile unsigned*>(status) != kStatusOk;  // an earlier kernel gave up: this one stands down
-    prm.parts.heads[blockIdx.x].followers = 0;                                // (also then: nothing is joined)
-  }
+  // up to here nothing has touched global memory; and where all tokens are one sequence of a known length, the shares need none either
+  const bool known = prm.q_start == nullptr;
+  if (!prm.beside && !known) grid_dependency_wait();
   // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
   const int run = (prm.batch + kThreads - 1) / kThreads;
   {
@@ -197,19 +193,53 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     share_end[threadIdx.x] = mine;
   }
   __syncthreads();
-  bool ok = !abort_flag;
-  // tensor memory is allocated beside the producer's first loads
-  uint32_t tmem = 0;
-  if (warp != kProducerWarp) {
-    if (warp == kMmaWarp) {
-      tmem_alloc(smem_addr(&tmem_slot), kTmemCols);
-      tmem_relinquish();
+  // ---- where this CTA's share begins and ends: the producer's business ----
+  const long long total = share_end[kThreads - 1] * prm.kv_heads;
+  const long long share = max(static_cast<long long>(kLeast), prm.parts.share_of(total));
+  const long long from = blockIdx.x * share, to = from + share;
+  Place p = {};  // in the warp's halves
+  if (warp == kProducerWarp && from < total) {
+    const long long x = lane < 16 ? from : min(to, total - 1);
+    const int before = first_above(share_end, kThreads, prm.kv_heads, x);
+    long long rest = x - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads), all;
+    p.b = before * run - 1;
+    do {
+      ++p.b;
+      p.e = extent_of(prm, p.b);
+      all = Costs(p.e, by_span, prm.causal).all();
+      if (rest < all * prm.kv_heads) break;
+      rest -= all * prm.kv_heads;
+    } while (p.b + 1 < prm.batch);
+    const Costs costs(p.e, by_span, prm.causal);
+    p.kv_head = small_quotient(rest, all);
+    rest -= p.kv_head * all;
+    int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
+#pragma unroll 1
+    while (low < high) {
+      const int mid = (low + high + 1) / 2;
+      if (costs.before(mid) <= rest) low = mid;
+      else high = mid - 1;
     }
-    tc_fence_before_sync();
-    named_barrier_sync(kSetUp, kThreads - 32);
-    tc_fence_after_sync();
-    tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+    p.j = low;
+    p.into = rest - costs.before(low);
+    p.step = costs.step_at(low, p.into);
+    __syncwarp();
   }
+  if (!prm.beside && known) grid_dependency_wait();
+  grid_launch_dependents();
+  if (threadIdx.x == 0) {
+    abort_flag = *reinterpret_cast<volatile unsigned*>(status) != kStatusOk;  // an earlier kernel gave up: this one stands down
+    prm.parts.heads[blockIdx.x].followers = 0;                                // (also then: nothing is joined)
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_addr(&tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  bool ok = !abort_flag;
 
   auto wait = [&](int i, uint32_t parity, unsigned tag) { return __all_sync(0xffffffffu, mbar_wait(bar(i), parity, status, tag)); };
   auto next_segment = [&](unsigned n_item, Segment& s) {
@@ -226,39 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
 
   if (warp == kProducerWarp) {
     // ================= the share, and TMA =================
-    const long long total = share_end[kThreads - 1] * prm.kv_heads;
-    const long long share = max(static_cast<long long>(kLeast), prm.parts.share_of(total));
-    const long long from = blockIdx.x * share, to = from + share;
     const bool any = ok && from < total;
-    // where the share begins and ends, in the warp's halves
-    Place p = {};
-    if (any) {
-      const long long x = lane < 16 ? from : min(to, total - 1);
-      const int before = first_above(share_end, kThreads, prm.kv_heads, x);
-      long long rest = x - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads), all;
-      p.b = before * run - 1;
-      do {
-        ++p.b;
-        p.e = extent_of(prm, p.b);
-        all = Costs(p.e, by_span, prm.causal).all();
-        if (rest < all * prm.kv_heads) break;
-        rest -= all * prm.kv_heads;
-      } while (p.b + 1 < prm.batch);
-      const Costs costs(p.e, by_span, prm.causal);
-      p.kv_head = small_quotient(rest, all);
-      rest -= p.kv_head * all;
-      int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
-#pragma unroll 1
-      while (low < high) {
-        const int mid = (low + high + 1) / 2;
-        if (costs.before(mid) <= rest) low = mid;
-        else high = mid - 1;
-      }
-      p.j = low;
-      p.into = rest - costs.before(low);
-      p.step = costs.step_at(low, p.into);
-      __syncwarp();
-    }
     auto of_half = [&](int from_lane) {
       auto word = [&](int x) { return __shfl_sync(0xffffffffu, x, from_lane); };
       return Place{word(p.b), word(p.kv_head), word(p.j), word(p.step), Extent{word(p.e.first), word(p.e.n), word(p.e.keys)}, __shfl_sync(0xffffffffu, p.into, from_lane)};
@@ -805,12 +803,10 @@ int launch_many_d(const Pass& pass, bool fp16, unsigned* status, cudaStream_t st
 size_t paged_many_workspace(int width, int sms) { return Parts::bytes(sms, 2 * kTile, width); }
 
 int paged_many_launch(Pass& pass, bool fp16, unsigned char* workspace, cudaStream_t stream) {
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
   unsigned* status = nullptr;
   if (int rc = status_word(&status)) return rc;
   const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
-  pass.parts.place(workspace, sms, 2 * kTile, width);
+  pass.parts.place(workspace, pass.blocks, 2 * kTile, width);
   if (width == 64) return launch_many_d<64, false>(pass, fp16, status, stream);
   if (packs(pass, pass.k, pass.pieces) && packs(pass, pass.v, pass.pieces_v)) return launch_many_d<128, true>(pass, fp16, status, stream);
   return launch_many_d<128, false>(pass, fp16, status, stream);
