@@ -102,7 +102,9 @@ int check_paged(const char* name, const limn_b200_paged* s) {
     return fail(LIMN_B200_UNSUPPORTED, "%s: a paged cache is served for hd and hd_v multiples of 8 up to 128, got %d and %d", name, s->hd, s->hd_v);
   if (s->page_size % 8 != 0) return fail(LIMN_B200_UNSUPPORTED, "%s: the page size must be a multiple of 8, got %d", name, s->page_size);
   if (s->heads / s->kv_heads > 128) return fail(LIMN_B200_UNSUPPORTED, "%s: %d query heads to a key head, at most 128 are served", name, s->heads / s->kv_heads);
-  if (static_cast<long long>(s->max_pages) * s->page_size > 0x7fffffffLL - s->first_position)
+  constexpr long long kMost = 0x7fff0000LL;  // keys, positions and rows are counted in int, some key tiles past the last one included
+  if (static_cast<long long>(s->tokens) * s->heads > kMost) return fail(LIMN_B200_UNSUPPORTED, "%s: %d tokens of %d heads do not fit 31 bits", name, s->tokens, s->heads);
+  if (static_cast<long long>(s->max_pages) * s->page_size > kMost - s->first_position)
     return fail(LIMN_B200_UNSUPPORTED, "%s: positions of %d pages of %d from %d on do not fit 31 bits", name, s->max_pages, s->page_size, s->first_position);
   for (int i = 0; i < 3; ++i)
     if (s->k_strides[i] < 0 || (s->k_strides[i] & 7) || s->v_strides[i] < 0 || (s->v_strides[i] & 7))
@@ -140,7 +142,10 @@ int limn_b200_sdpa_paged(const limn_b200_paged* step, const void* q, void* out, 
 int limn_b200_sdpa_paged_prefix(const limn_b200_paged* step, const void* q, void* out, float* lse, const long long* strides, const int* prefix_table, int prefix_len,
                                 int causal, double scale, void* workspace, unsigned long long workspace_bytes, void* stream) {
   clear_error();
-  if (!prefix_table || prefix_len <= 0) return fail(LIMN_B200_BAD_ARGUMENT, "sdpa_paged_prefix: a prefix of %d keys, or no table of its pages", prefix_len);
+  reset_launches();
+  if (int rc = check_paged("sdpa_paged_prefix", step)) return rc;
+  if (!prefix_table || prefix_len <= 0 || prefix_len > 0x7fff0000)
+    return fail(LIMN_B200_BAD_ARGUMENT, "sdpa_paged_prefix: a prefix of %d keys, or no table of its pages", prefix_len);
   return paged_pass("sdpa_paged_prefix", step, q, out, lse, strides, prefix_table, prefix_len, causal, scale, workspace, workspace_bytes, stream);
 }
 

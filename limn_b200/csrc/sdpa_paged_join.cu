@@ -78,9 +78,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
   if (side == 0) store4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row), column, sums.acc, sums.m, sums.l);
 }
 
-// A (token, head) row to kSplit warps: what both passes left of it, of a sequence that is one. Rows of tokens that belong to none are left alone.
+// A (token, head) row to kSplit warps: what both passes left of it, of a sequence that is one. Rows of tokens that belong to none are left alone; all of
+// them where a kernel has given up, since a pass may then not have left what is read here.
 template <int D, bool kFp16, int kSplit>
-__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_finish_kernel(const Pass front, const Pass own) {
+__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_finish_kernel(const Pass front, const Pass own, const unsigned* status) {
   constexpr int kRows = kJoinWarps / kSplit, kLanes = D / 4, kAtOnce = 32 / kLanes;
   __shared__ float4 all_sums[kJoinWarps][32];
   __shared__ float2 all_stats[kJoinWarps];
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_finish_kernel(cons
   // (all asked for before whose token it is is known: the memory is there for every row)
   const float2 front_ml = front.leave.ml[row], own_ml = own.leave.ml[row];
   const float4 front_o = *reinterpret_cast<const float4*>(front.leave.o + row * D + column), own_o = *reinterpret_cast<const float4*>(own.leave.o + row * D + column);
+  if (__syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<const volatile unsigned*>(status) != ptx::kStatusOk)) return;
   const int b = sequence_of(own.q_start, own.batch, token, lane);
   if (b >= own.batch) return;  // (as is all of the block)
   const Extent e = extent_of(own, b);
@@ -134,9 +136,11 @@ int launch_join(const Pass& pass, cudaStream_t stream) {
 
 template <int D, bool kFp16, int kSplit>
 int launch_finish_s(const Pass& front, const Pass& own, cudaStream_t stream) {
+  unsigned* status = nullptr;
+  if (int rc = status_word(&status)) return rc;
   constexpr int kRows = kJoinWarps / kSplit;
   const dim3 grid(static_cast<unsigned>(own.tokens), static_cast<unsigned>((own.heads + kRows - 1) / kRows));
-  LIMN_CUDA(launch_overlapped(sdpa_paged_finish_kernel<D, kFp16, kSplit>, grid, dim3(kJoinWarps * 32), 0, stream, front, own), "launching the kernel that joins a prefix");
+  LIMN_CUDA(launch_overlapped(sdpa_paged_finish_kernel<D, kFp16, kSplit>, grid, dim3(kJoinWarps * 32), 0, stream, front, own, status), "launching the kernel that joins a prefix");
   note_launches(1);
   return LIMN_B200_OK;
 }

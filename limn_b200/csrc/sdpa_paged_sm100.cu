@@ -752,7 +752,11 @@ BoxShape pages_map(const Pass& p, const Pages& side, int pieces, int chunk) {
 }
 // Or all 128 columns, the two column blocks of 8 keys side by side. Five dimensions hold (column, key of 8, column block, 8 keys, page) and leave
 // none for the head, so it has to continue the column blocks (heads side by side in a token) or the pages (heads of a page one after the other).
-bool packs(const Pass& p, const Pages& side, int pieces) { return pieces == 16 && (p.kv_heads == 1 || side.head == 256 || side.page == p.kv_heads * side.head); }
+bool packs(const Pass& p, const Pages& side, int pieces) {
+  if (pieces != 16) return false;
+  if (p.kv_heads == 1 || side.head == 256) return true;
+  return side.page == p.kv_heads * side.head && static_cast<long long>(p.pages) * p.kv_heads <= 0x7fffffffLL;
+}
 BoxShape packed_map(const Pass& p, const Pages& side, int chunk, int* heads_side_by_side) {
   const bool beside = p.kv_heads == 1 || side.head == 256;
   *heads_side_by_side = beside;

@@ -35,7 +35,9 @@ def _address(operand: Any) -> int | None:
     kind = type(operand)
     read = _ADDRESS_OF.get(kind)
     if read is None:
-        read = _ADDRESS_OF[kind] = attrgetter("ptr") if hasattr(operand, "ptr") else methodcaller("data_ptr")
+        read = attrgetter("ptr") if hasattr(operand, "ptr") else methodcaller("data_ptr")
+        read(operand)  # raises before the type is remembered, where it has neither
+        _ADDRESS_OF[kind] = read
     return read(operand)
 
 

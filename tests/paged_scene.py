@@ -54,17 +54,21 @@ class Scene:
         self.row_room = row_room  # columns that lie between one row of q or out and the next
         self.q = (rng.standard_normal((self.tokens, heads, self.hd)) * mul).astype(np.float32).astype(dtype)
 
-    # ---- the cache as it lies in memory
+    # ---- the cache as it lies in memory: "token" (page, slot, head, column), "head" (page, head, slot, column), "roomy" as "token" with room
+    # behind every head's columns, "paired" as "token" with as much again between pages (where K and V share a buffer)
     def _in_memory(self, width):
         p, s, h = self.pages, self.page_size, self.kv_heads
-        return (p, s, h, width) if self.order == "token" else (p, h, s, width)
+        return {"token": (p, s, h, width), "head": (p, h, s, width), "roomy": (p, s, h, width + 8), "paired": (p, 2 * s, h, width)}[self.order]
 
     def strides(self, width):
         s, h = self.page_size, self.kv_heads
-        return (s * h * width, width, h * width) if self.order == "token" else (s * h * width, s * width, width)
+        return {"token": (s * h * width, width, h * width), "head": (s * h * width, s * width, width), "roomy": (s * h * (width + 8), width + 8, h * (width + 8)),
+                "paired": (2 * s * h * width, width, h * width)}[self.order]
 
     def by_slot(self, memory):
-        return memory if self.order == "token" else memory.transpose(0, 2, 1, 3)
+        if self.order == "head":
+            return memory.transpose(0, 2, 1, 3)
+        return memory[..., :-8] if self.order == "roomy" else memory
 
     def _fill(self, width, of_sequence, of_prefix, keep):
         memory = poison(self.dtype, self._in_memory(width))

@@ -123,6 +123,11 @@ SHAPES = [
     ("prompts gqa3 80", F16, 6, 2, 80, 80, 48, "token", PROMPTS),
     ("prompts 128 hd_v 48", F16, 4, 2, 128, 48, 128, "token", PROMPTS),
     ("prompts 100 to 1", BF16, 100, 1, 64, 64, 8, "head", [(5, 5), (20, 400), (1, 33)]),
+    ("generation, room between heads", BF16, 4, 2, 128, 128, 16, "roomy", GENERATION),
+    ("generation, K and V by page", F16, 4, 2, 64, 64, 16, "paired", GENERATION),
+    ("prompts, room between heads", BF16, 8, 2, 128, 128, 16, "roomy", PROMPTS),
+    ("prompts, K and V by page", BF16, 8, 2, 128, 128, 32, "paired", PROMPTS),
+    ("prompts, one key head, room", F16, 4, 1, 128, 128, 8, "roomy", PROMPTS),
     ("prompts 11 to 1, pages of 256", F16, 11, 1, 128, 128, 256, "token", [(50, 300), (100, 700)]),
 ]
 
@@ -263,7 +268,8 @@ def test_append_leaves_out_what_has_no_place():
     rng = np.random.default_rng(0)
     k, v = (rng.standard_normal((s.tokens, 1, 64)).astype(np.float32).astype(BF16) for _ in range(2))
     before = s.filled(with_new=False)
-    s.step.append(runtime.upload(k), runtime.upload(v))
+    k_dev, v_dev = runtime.upload(k), runtime.upload(v)
+    s.step.append(k_dev, v_dev)
     runtime.synchronize()
     assert s.error_bits() == 3
     for memory, was, new in ((s.k_dev, before[0], k), (s.v_dev, before[1], v)):
@@ -278,3 +284,261 @@ def test_nothing_to_do():
     s.check()
     empty = Scene([], spare_tokens=2).upload()
     empty.check()
+
+
+# ---------------------------------------------------------------- many sequences, long ones, far ones
+
+@pytest.mark.parametrize("heads", [2, 32])
+@pytest.mark.parametrize("prefix", [0, 20])
+def test_more_sequences_than_threads(heads, prefix):
+    """700 sequences, some without tokens or keys: every thread of a block adds up several."""
+    rng = np.random.default_rng(12)
+    seqs = [(int(n), int(n + c)) for n, c in zip(rng.integers(0, 3, 700), rng.integers(0, 40, 700))]
+    Scene(seqs, heads=heads, kv_heads=1, hd=64, page_size=8, seed=13, prefix=prefix).upload().check()
+
+
+@pytest.mark.parametrize("new", [1, 200])
+def test_a_long_sequence_among_short_ones(new):
+    """One problem is shared by nearly all workers, others share one."""
+    Scene([(1, 3), (new, 40000), (1, 17), (2, 2)], heads=2, kv_heads=1, hd=128, page_size=64, seed=14).upload().check()
+
+
+def test_a_prefix_far_longer_than_the_rest():
+    Scene([(1, 3), (2, 5)], heads=8, kv_heads=2, hd=64, page_size=16, seed=15, prefix=20000).upload().check()
+    Scene([(1, 3), (40, 50)], heads=8, kv_heads=2, hd=128, page_size=16, seed=15, prefix=9000).upload().check()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_offsets_past_31_bits(new):
+    """Pages 2^27 elements apart: the last one begins 2^31 elements, 2^32 bytes, in."""
+    from limn_b200 import runtime
+    from limn_b200._lib import check, lib
+    from limn_b200.paged import PagedBatch, PagedCache
+
+    s = Scene([(new, 100), (1, 30)], heads=4, kv_heads=1, hd=64, page_size=16, seed=16, spare_pages=10)
+    apart = 1 << 27
+    assert s.pages == 19 and int(s.table[s.table < s.pages].max()) * apart >= 2**31
+    k, v = s.filled(with_new=False)
+    far = [runtime.DeviceBuffer(2 * (apart * (s.pages - 1) + 16 * 64)) for _ in range(2)]
+    for host, memory in ((k, far[0]), (v, far[1])):
+        for page in range(s.pages):
+            check(lib().limn_b200_copy_h2d(memory.ptr + 2 * apart * page, np.ascontiguousarray(host[page]).ctypes.data, 16 * 64 * 2, None), "uploading a page")
+            runtime.synchronize()
+    s.upload()
+    cache = PagedCache(*far, dtype="bfloat16", pages=s.pages, page_size=16, kv_heads=1, hd=64, k_strides=(apart, 64, 64), v_strides=(apart, 64, 64))
+    s.step = PagedBatch(cache, heads=4, batch=2, tokens=s.tokens, max_t_q=s.max_t_q, page_table=s.table_dev, max_pages=s.max_pages, q_start=s.q_start_dev,
+                        kv_lens=s.kv_lens_dev, errors=s.errors)
+    new_k = np.concatenate([s.k[b][-n:] for b, n in enumerate(s.new)])
+    new_v = np.concatenate([s.v[b][-n:] for b, n in enumerate(s.new)])
+    new_k, new_v = runtime.upload(new_k), runtime.upload(new_v)
+    s.step.append(new_k, new_v)  # not turned: what the scene has
+    s.check()
+
+
+# ---------------------------------------------------------------- as they are used: together, captured, on streams
+
+def _frequencies(rotated):
+    return 10000.0 ** (-np.arange(rotated // 2) / (rotated // 2))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_prompt_and_then_token_by_token(hd):
+    """A model's layer over the life of two sequences: the prompt enters the cache in one step, then every step brings a token to
+    each (and none to the first in the third). In the end every row is what one causal pass of the library over all tokens gives, up
+    to the rounding of the weights on either side, which the definitions in float64 measure."""
+    from limn_b200 import runtime
+    from limn_b200._lib import check, lib
+    from limn_b200.paged import PagedBatch, PagedCache
+
+    rng = np.random.default_rng(17)
+    heads, kv_heads, page_size, max_pages, pages = 8, 2, 16, 12, 30
+    steps = [[100, 37], [1, 1], [1, 1], [0, 1], [1, 1], [1, 1], [3, 2]]
+    total = [sum(x) for x in zip(*steps)]
+    made = [{name: rng.standard_normal((t, h, hd)).astype(np.float32).astype(BF16) for name, h in (("q", heads), ("k", kv_heads), ("v", kv_heads))} for t in total]
+    table = rng.permutation(pages)[: 2 * max_pages].reshape(2, max_pages).astype(np.int32)
+    k_dev, v_dev = (runtime.upload(poison(BF16, (pages, page_size, kv_heads, hd))) for _ in range(2))
+    cache = PagedCache(k_dev, v_dev, dtype="bfloat16", pages=pages, page_size=page_size, kv_heads=kv_heads, hd=hd)
+    table_dev, errors, freqs = runtime.upload(table), runtime.upload(np.zeros(1, np.uint32)), runtime.upload(_frequencies(hd))
+    done, got, turned_q = [0, 0], [[], []], [[], []]
+    for new in steps:
+        start = np.array([0, new[0], sum(new)], np.int32)
+        step = PagedBatch(cache, heads=heads, batch=2, tokens=sum(new), max_t_q=max(new), page_table=table_dev, max_pages=max_pages, q_start=runtime.upload(start),
+                          kv_lens=runtime.upload(np.array([d + n for d, n in zip(done, new)], np.int32)), errors=errors)
+        now = {name: runtime.upload(np.concatenate([made[b][name][done[b] : done[b] + new[b]] for b in range(2)])) for name in "qkv"}
+        out, lse = runtime.empty(sum(new) * heads * hd * 2), runtime.empty(sum(new) * heads * 4)
+        step.append(now["k"], now["v"], q=now["q"], q_out=now["q"], frequencies=freqs, rotated=hd)
+        step.attention(now["q"], out, lse)
+        rows, turned = (runtime.download(x, np.uint16, (sum(new), heads, hd)).view(BF16) for x in (out, now["q"]))
+        for b in range(2):
+            got[b].append(rows[start[b] : start[b + 1]])
+            turned_q[b].append(turned[start[b] : start[b + 1]])
+            done[b] += new[b]
+    assert runtime.download(errors, np.uint32, (1,))[0] == 0
+    k_all, v_all = (runtime.download(x, np.uint16, (pages, page_size, kv_heads, hd)).view(BF16) for x in (k_dev, v_dev))
+    for b, t in enumerate(total):
+        slots = np.arange(t)
+        k, v = (x[table[b][slots // page_size], slots % page_size] for x in (k_all, v_all))
+        q, rows = np.concatenate(turned_q[b]), np.concatenate(got[b])
+        wide = np.repeat(k, heads // kv_heads, axis=1), np.repeat(v, heads // kv_heads, axis=1)
+        by_head = [runtime.upload(np.ascontiguousarray(x.transpose(1, 0, 2))) for x in (q, *wide)]
+        out, lse = runtime.empty(rows.nbytes), runtime.empty(heads * t * 4)
+        check(lib().limn_b200_sdpa_fwd(*(x.ptr for x in by_head), None, out.ptr, lse.ptr, 2, heads, t, t, hd, hd, 1, hd**-0.5, None), "sdpa")
+        dense = runtime.download(out, np.uint16, (heads, t, hd)).view(BF16).transpose(1, 0, 2).astype(np.float64)
+        s = np.einsum("thd,jhd->thj", q.astype(np.float64), wide[0].astype(np.float64)) * hd**-0.5
+        s[np.broadcast_to(np.arange(t)[:, None, None] < np.arange(t), s.shape)] = -np.inf
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        size = np.einsum("thj,jhd->thd", p, np.abs(wide[1].astype(np.float64)))
+        half = HALF_STEP[BF16]
+        # either side is off by half a step of its value and of the weights, and by 2^-13 of them (paged_scene.py)
+        assert (np.abs(rows.astype(np.float64) - dense) <= 2 * (half * np.abs(dense) * (1 + 2 * half) + (half + 2.0**-13) * size * (1 + half)) + 2.0**-23).all()
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_a_captured_step_follows_its_arrays(new):
+    """append and both attentions in one graph, replayed after offsets, lengths, tables, pages and operands have changed in place."""
+    torch = pytest.importorskip("torch")
+    from limn_b200 import runtime
+    from limn_b200.paged import PagedBatch, PagedCache
+
+    scenes = [Scene([(new, 300), (0, 40), (new, 90)], heads=4, kv_heads=2, hd=64, seed=20, prefix=50, max_pages=20, max_t_q=new),
+              Scene([(new, new), (new, 200), (0, 0)], heads=4, kv_heads=2, hd=64, seed=21, prefix=50, max_pages=20, max_t_q=new)]
+    pages = max(s.pages for s in scenes)
+    dev = torch.device("cuda")
+    k_dev, v_dev = (torch.zeros((pages, 16, 2, 64), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    q, out = (torch.zeros((2 * new, 4, 64), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    k_new, v_new = (torch.zeros((2 * new, 2, 64), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    out_prefix, lse, lse_prefix = torch.zeros_like(out), torch.zeros((2 * new, 4), device=dev), torch.zeros((2 * new, 4), device=dev)
+    ints = {name: torch.zeros(shape, dtype=torch.int32, device=dev) for name, shape in (("table", (3, 20)), ("q_start", (4,)), ("kv_lens", (3,)), ("prefix", (4,)), ("errors", (1,)))}
+    cache = PagedCache(k_dev, v_dev, dtype="bfloat16", pages=pages, page_size=16, kv_heads=2, hd=64)
+    step = PagedBatch(cache, heads=4, batch=3, tokens=2 * new, max_t_q=new, page_table=ints["table"], max_pages=20, q_start=ints["q_start"], kv_lens=ints["kv_lens"],
+                      errors=ints["errors"], first_position=50, max_prefix=50)
+
+    def bits(x):
+        return torch.from_numpy(x.view(np.int16).copy()).to(dev).view(torch.bfloat16)
+
+    def load(s):
+        k, v = s.filled(with_new=False)
+        k_dev[: s.pages].copy_(bits(k)), v_dev[: s.pages].copy_(bits(v))
+        q.copy_(bits(s.q))
+        for memory, rows in ((k_new, s.k), (v_new, s.v)):
+            memory.copy_(bits(np.concatenate([rows[b][len(rows[b]) - n :] for b, n in enumerate(s.new)])))
+        for name, x in (("table", s.table), ("q_start", s.start), ("kv_lens", s.keys), ("prefix", s.prefix_table)):
+            ints[name].copy_(torch.as_tensor(np.asarray(x, np.int32)))
+
+    def call(stream):
+        step.append(k_new, v_new, stream=stream)
+        step.attention(q, out, lse, stream=stream)
+        step.attention_with_prefix(q, out_prefix, lse_prefix, prefix_table=ints["prefix"], prefix_len=50, stream=stream)
+
+    load(scenes[0])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call(side.cuda_stream)  # once before the capture
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            call(torch.cuda.current_stream().cuda_stream)
+    for s in (scenes[1], scenes[0], scenes[1]):
+        load(s)
+        for x in (out, out_prefix):
+            x.view(torch.int16).fill_(0x7FFF)
+        lse.fill_(float("nan")), lse_prefix.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for prefix, o, l in ((50, out_prefix, lse_prefix), (0, out, lse)):
+            whole = s.prefix, s.prefix_k, s.prefix_v
+            if prefix == 0:
+                s.prefix, s.prefix_k, s.prefix_v = 0, s.prefix_k[:0], s.prefix_v[:0]
+            s.compare(o.view(torch.int16).cpu().numpy().view(BF16), l.cpu().numpy(), *s.expected())
+            s.prefix, s.prefix_k, s.prefix_v = whole
+    assert ints["errors"].item() == 0
+    del graph
+    assert runtime.device_status() == 0
+
+
+def test_two_batches_on_two_streams():
+    """Steps with workspaces of their own overlap without touching one another."""
+    from limn_b200 import runtime
+
+    scenes = [Scene([(1, 5000), (1, 70), (1, 900)], heads=8, kv_heads=2, hd=128, seed=22).upload(),
+              Scene([(60, 3000), (1, 70)], heads=8, kv_heads=2, hd=64, seed=23, prefix=400).upload()]
+    alone = [s.attend() for s in scenes]
+    streams = [runtime.Stream(), runtime.Stream()]
+    held = []
+    for _ in range(20):
+        for s, stream in zip(scenes, streams):
+            q = runtime.upload(s.q) if not hasattr(s, "q_dev") else s.q_dev
+            s.q_dev = q
+            out, lse = runtime.empty(s.tokens * s.heads * s.hd * 2, poison=None), runtime.empty(s.tokens * s.heads * 4, poison=None)
+            if s.prefix:
+                s.step.attention_with_prefix(q, out, lse, prefix_table=s.prefix_dev, prefix_len=s.prefix, stream=stream)
+            else:
+                s.step.attention(q, out, lse, stream=stream)
+            held.append((s, out, lse))
+    runtime.synchronize()
+    for s, out, lse in held:
+        want_o, want_l = alone[scenes.index(s)]
+        assert np.array_equal(runtime.download(out, np.uint16, want_o.shape), want_o.view(np.uint16))
+        assert np.array_equal(runtime.download(lse, np.float32, want_l.shape), want_l)
+
+
+def test_sequences_may_share_pages():
+    s = Scene([(1, 60), (1, 60), (1, 33)], heads=4, kv_heads=2, hd=64, seed=24)
+    s.table[1], s.k[1], s.v[1] = s.table[0], s.k[0], s.v[0]
+    s.upload().check()
+
+
+def test_no_word_for_errors():
+    from limn_b200.paged import PagedBatch
+
+    s = Scene([(1, 60), (30, 40)], heads=4, kv_heads=2, hd=64, seed=25)
+    table = s.table.copy()
+    table[0, 1] = -7
+    s.upload(table=table)
+    held = s.step._held
+    s.step = PagedBatch(held[0], heads=4, batch=2, tokens=s.tokens, max_t_q=30, page_table=s.table_dev, max_pages=s.max_pages, q_start=s.q_start_dev, kv_lens=s.kv_lens_dev)
+    have_o, _ = s.attend()
+    assert np.isnan(have_o[0].astype(np.float32)).all() and np.isfinite(have_o[1:].astype(np.float32)).all() and s.error_bits() == 0
+
+
+def test_launches_and_workspace():
+    import ctypes
+
+    from limn_b200._lib import last_error, lib
+
+    s = Scene([(1, 60), (2, 40)], heads=4, kv_heads=2, hd=64, seed=26, prefix=20).upload()
+    s.attend()
+    assert lib().limn_b200_last_launch_count() == 3
+    s.prefix = 0
+    s.attend()
+    assert lib().limn_b200_last_launch_count() == 2
+    need = ctypes.c_ulonglong()
+    assert lib().limn_b200_sdpa_paged_workspace(s.step._by_ref, 0, ctypes.byref(need)) == 0 and need.value > 0
+    with_prefix = ctypes.c_ulonglong()
+    assert lib().limn_b200_sdpa_paged_workspace(s.step._by_ref, 20, ctypes.byref(with_prefix)) == 0 and with_prefix.value > need.value
+    strides = (ctypes.c_longlong * 4)(256, 64, 256, 64)
+    q = 256
+    for workspace, size in ((None, need.value), (256, need.value - 1), (0, 0)):
+        assert lib().limn_b200_sdpa_paged(s.step._by_ref, q, q, q, strides, 1, 0.125, workspace, size, None) == 1 and "workspace" in last_error()
+    assert lib().limn_b200_last_launch_count() == 0
+
+
+def test_paged_kernels_stand_down_after_a_wait_that_ran_out():
+    """While the status word is set, the kernels that wait, and what joins their results, write nothing; the next call after it has been read is right."""
+    from limn_b200 import runtime
+    from limn_b200._lib import check, lib
+
+    s = Scene([(60, 500), (1, 70)], heads=4, kv_heads=2, hd=64, seed=27, prefix=0).upload()
+    behind = Scene([(60, 500), (1, 70)], heads=4, kv_heads=2, hd=64, seed=27, prefix=90).upload()
+    for scene in (s, behind):
+        scene.check()
+        flag = runtime.empty(4, poison=0)
+        check(lib().limn_b200_wait_probe(20000, flag.ptr, None), "wait probe")
+        have_o, have_l = scene.attend()
+        assert (have_o.view(np.uint16) == 0x7FFF).all() and np.isnan(have_l).all()
+        assert runtime.device_status() == 0x57417E57
+        scene.check()
+    assert runtime.device_status() == 0
