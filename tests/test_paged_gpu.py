@@ -123,6 +123,10 @@ SHAPES = [
     ("prompts gqa3 80", F16, 6, 2, 80, 80, 48, "token", PROMPTS),
     ("prompts 128 hd_v 48", F16, 4, 2, 128, 48, 128, "token", PROMPTS),
     ("prompts 100 to 1", BF16, 100, 1, 64, 64, 8, "head", [(5, 5), (20, 400), (1, 33)]),
+    ("generation gqa4 128, 4 key heads", BF16, 16, 4, 128, 128, 16, "token", GENERATION),
+    ("generation gqa3 64, 5 key heads", F16, 15, 5, 64, 64, 16, "head", GENERATION),
+    ("drafts mha 12, 80", F16, 12, 12, 80, 80, 48, "head", DRAFTS),
+    ("drafts gqa4 128, 8 key heads", BF16, 32, 8, 128, 128, 16, "token", DRAFTS),
     ("generation, room between heads", BF16, 4, 2, 128, 128, 16, "roomy", GENERATION),
     ("generation, K and V by page", F16, 4, 2, 64, 64, 16, "paired", GENERATION),
     ("prompts, room between heads", BF16, 8, 2, 128, 128, 16, "roomy", PROMPTS),
@@ -301,6 +305,26 @@ def test_more_sequences_than_threads(heads, prefix):
 def test_a_long_sequence_among_short_ones(new):
     """One problem is shared by nearly all workers, others share one."""
     Scene([(1, 3), (new, 40000), (1, 17), (2, 2)], heads=2, kv_heads=1, hd=128, page_size=64, seed=14).upload().check()
+
+
+@pytest.mark.parametrize("prefix", [0, 300])
+@pytest.mark.parametrize("new, heads", [(1, 4), (1, 32), (4, 16), (3, 20), (30, 8)])
+def test_what_the_workspace_held_is_of_no_concern(new, heads, prefix):
+    """The same call again gives the same bits, whatever the workspace held before it."""
+    from limn_b200 import runtime
+    from limn_b200.paged import PagedBatch
+
+    s = Scene([(new, 6000), (1, 3), (new, 900), (0, 10), (new, 40)], heads=heads, kv_heads=4, hd=128, page_size=16, seed=28, prefix=prefix).upload()
+    first = s.check()
+    held, size = s.step._held[0], s.step.workspace_bytes
+    rng = np.random.default_rng(3)
+    for bytes_ in (np.zeros(size, np.uint8), np.full(size, 0xFF, np.uint8), rng.integers(0, 256, size, dtype=np.uint8)):
+        memory = runtime.upload(bytes_)
+        s.step = PagedBatch(held, heads=heads, batch=5, tokens=s.tokens, max_t_q=s.max_t_q, page_table=s.table_dev, max_pages=s.max_pages, q_start=s.q_start_dev,
+                            kv_lens=s.kv_lens_dev, errors=s.errors, workspace=memory, max_prefix=300)
+        for _ in range(3):
+            again = s.attend()
+            assert np.array_equal(first[0].view(np.uint16), again[0].view(np.uint16)) and np.array_equal(first[1], again[1])
 
 
 def test_a_prefix_far_longer_than_the_rest():
