@@ -92,6 +92,10 @@ struct Pass {
   const int* kv_lens = nullptr;  // (batch); null with q_start: `keys` of them
   unsigned* errors = nullptr;
   int keys = 0;
+  // Keys that stand in front of every sequence's own: prefix_len of them in the pages that prefix_table names, counted as `front`, rounded up to whole units or
+  // key tiles: a sequence's key f + j is key j of its own pages. Those between do not exist.
+  const int* prefix_table = nullptr;
+  int prefix_len = 0, front = 0;
   int batch = 0, heads = 0, kv_heads = 0, group = 1;  // group: query heads to a key head
   Div by_group, by_page;                              // quotients by it and by page_size
   int pieces = 0, pieces_v = 0;                       // groups of 8 columns of a row of Q and K, of V and O
@@ -106,7 +110,7 @@ struct Pass {
   int blocks = 0;  // that make the pass, one to a multiprocessor
 };
 
-// A sequence's extents: `first` token of `n`, `keys` in its pages. One that cannot be has n = 0 and is noted.
+// A sequence's extents: `first` token of `n`, `keys` it has, those in front among them. One that cannot be has n = 0 and is noted.
 struct Extent {
   int first, n, keys;
 };
@@ -120,8 +124,16 @@ __device__ __forceinline__ Extent extent_of(const int* q_start, const int* kv_le
 }
 __device__ __forceinline__ Extent extent_of(const Pass& p, int b) {
   if (p.q_start == nullptr) return Extent{0, p.tokens, p.keys};
-  return extent_of(p.q_start, p.kv_lens, b, p.tokens, p.max_t_q, p.max_pages, p.page_size, p.errors);
+  Extent e = extent_of(p.q_start, p.kv_lens, b, p.tokens, p.max_t_q, p.max_pages, p.page_size, p.errors);
+  e.keys += p.front;
+  return e;
 }
+// Of the keys on key's side of the end of the front: up to where they exist, the table's entry for one of them, and its slot.
+__device__ __forceinline__ int side_end(const Pass& p, int key, int keys) { return key < p.front ? p.prefix_len : keys; }
+__device__ __forceinline__ int entry_for(const Pass& p, int b, int key) {
+  return key < p.front ? p.prefix_table[p.by_page.of(key)] : p.table[static_cast<long long>(b) * p.max_pages + p.by_page.of(key - p.front)];
+}
+__device__ __forceinline__ int slot_of(const Pass& p, int key) { return p.by_page.rest(key < p.front ? key : key - p.front); }
 
 // The sequence whose tokens `token` is among: how many sequences end at or before it (batch: none of them goes on past it). A warp's
 // 32-ary search over q_start[1..batch]; where the offsets do not rise the answer is some number up to batch.
@@ -196,6 +208,8 @@ __device__ __forceinline__ int first_above(const long long* ends, int n, int by,
 int check_paged(const char* name, const limn_b200_paged* step);
 int check_paged_pointers(const char* name, const limn_b200_paged* step);
 
+constexpr long long kMaxKeys = 0x7fff0000LL;  // keys, positions and rows are counted in int, some key tiles past the last one included
+constexpr int kPagedUnit = 16, kPagedTile = 128;  // keys that a prefix in front is rounded up to, by the kernel that makes the pass
 // The kernels that make a pass, for few rows to a key head and for any number. Each lays its parts out in `workspace` and says so in pass.parts.
 constexpr int kPagedFewRows = 16;  // max_t_q * group up to here
 size_t paged_few_workspace(int rows, int width, int sms);

@@ -2,6 +2,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "paged.h"
 #include "sm100_ptx.cuh"
 
@@ -9,6 +12,7 @@ namespace limn_b200 {
 namespace {
 
 using namespace paged;
+
 
 // Which kernel a pass of at most `rows` rows to a (sequence, key head) takes, and the workspace it has to itself.
 size_t pass_workspace(long long rows, int width, int sms) {
@@ -18,8 +22,30 @@ int launch_pass(Pass& pass, bool fp16, long long rows, unsigned char* workspace,
   return rows <= kPagedFewRows ? paged_few_launch(pass, fp16, static_cast<int>(rows), workspace, stream) : paged_many_launch(pass, fp16, workspace, stream);
 }
 
+// A call behind a prefix either reads it once for the whole batch, in a pass of its own over all rows, whose sums are joined with those of the pass over the
+// sequences' own keys; or it puts the prefix in front of every sequence's keys and makes one pass. The first reads and computes less. The second launches two
+// kernels instead of three and leaves no sums in memory. Which is faster goes by what either costs beyond the other, as far as the host knows it:
+//   apart: 4 us, and 16 bytes for each element of O, written and read at 3 TB/s;
+//   in front, few rows to a key head: the prefix is read once more for every sequence, mostly out of L2, at 12 TB/s;
+//   in front, more rows: a sequence's rows fill tiles of 128 less well than the batch's do; two such tiles by 128 keys of 128 columns take a multiprocessor 2.1 us.
+// Measured, 32 heads over 8 key heads of 128, 100 to 800 keys of their own, apart : in front, in us: one token of 8 sequences behind 1024 keys 20.8 : 16.7, of 32
+// 29.2 : 33.6, of 32 behind 8192 43.1 : 134.6, of 128 behind 128 72.1 : 53.5; 8 to 16 tokens of 32 sequences behind 1024 45.5 : 44.7, behind 8192 86.3 : 148.6;
+// 128 to 256 tokens of 32 sequences behind 1024 293.6 : 155.8, behind 8192 830.2 : 786.7.
+bool prefix_in_front(const limn_b200_paged* step, int prefix_len) {
+  if (static_cast<long long>(step->max_pages) * step->page_size + prefix_len > kMaxKeys) return false;  // (positions in front and behind count in one int)
+  const long long group = step->heads / step->kv_heads;
+  const double apart = 4 + 16.0 * step->hd_v * step->tokens * step->heads / 3e6;
+  if (step->max_t_q * group <= kPagedFewRows) {
+    const double bytes = 2.0 * prefix_len * step->kv_heads * (step->hd + step->hd_v);
+    return (step->batch - 1) * bytes / 12e6 <= apart;
+  }
+  const double rows = static_cast<double>(step->tokens) * group, width = std::max(step->hd, step->hd_v) > 64 ? 1 : 0.5;
+  const double more = step->batch * std::ceil(rows / step->batch / 128) - std::ceil(rows / 128);  // tiles
+  return more / 2 * step->kv_heads * std::ceil(prefix_len / 128.0) * width * 2.1 / 148 <= apart;
+}
+
 // The workspace of a call: the parts of the pass over the own keys; behind a prefix also those of the pass over it, and the rows' sums
-// over either.
+// over either, however long it is: a workspace that serves one prefix serves all.
 struct Workspace {
   size_t own, front, sums;  // sums: of one pass
   size_t bytes() const { return own + front + 2 * sums; }
@@ -69,7 +95,12 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   unsigned char* memory = static_cast<unsigned char*>(workspace);
   const long long rows = static_cast<long long>(step->max_t_q) * prm.group;
   if (int rc = sm_count(&prm.blocks)) return rc;
-  if (prefix_len == 0) {
+  const bool in_front = prefix_len > 0 && prefix_in_front(step, prefix_len);
+  if (in_front) {
+    const int whole = rows <= kPagedFewRows ? kPagedUnit : kPagedTile;
+    prm.prefix_table = prefix_table, prm.prefix_len = prefix_len, prm.front = (prefix_len + whole - 1) / whole * whole;
+  }
+  if (prefix_len == 0 || in_front) {
     if (int rc = launch_pass(prm, fp16, rows, memory, on)) return rc;
     return paged_join_launch(prm, fp16, rows > kPagedFewRows, on);
   }
@@ -102,9 +133,8 @@ int check_paged(const char* name, const limn_b200_paged* s) {
     return fail(LIMN_B200_UNSUPPORTED, "%s: a paged cache is served for hd and hd_v multiples of 8 up to 128, got %d and %d", name, s->hd, s->hd_v);
   if (s->page_size % 8 != 0) return fail(LIMN_B200_UNSUPPORTED, "%s: the page size must be a multiple of 8, got %d", name, s->page_size);
   if (s->heads / s->kv_heads > 128) return fail(LIMN_B200_UNSUPPORTED, "%s: %d query heads to a key head, at most 128 are served", name, s->heads / s->kv_heads);
-  constexpr long long kMost = 0x7fff0000LL;  // keys, positions and rows are counted in int, some key tiles past the last one included
-  if (static_cast<long long>(s->tokens) * s->heads > kMost) return fail(LIMN_B200_UNSUPPORTED, "%s: %d tokens of %d heads do not fit 31 bits", name, s->tokens, s->heads);
-  if (static_cast<long long>(s->max_pages) * s->page_size > kMost - s->first_position)
+  if (static_cast<long long>(s->tokens) * s->heads > kMaxKeys) return fail(LIMN_B200_UNSUPPORTED, "%s: %d tokens of %d heads do not fit 31 bits", name, s->tokens, s->heads);
+  if (static_cast<long long>(s->max_pages) * s->page_size > kMaxKeys - s->first_position)
     return fail(LIMN_B200_UNSUPPORTED, "%s: positions of %d pages of %d from %d on do not fit 31 bits", name, s->max_pages, s->page_size, s->first_position);
   for (int i = 0; i < 3; ++i)
     if (s->k_strides[i] < 0 || (s->k_strides[i] & 7) || s->v_strides[i] < 0 || (s->v_strides[i] & 7))
@@ -144,7 +174,7 @@ int limn_b200_sdpa_paged_prefix(const limn_b200_paged* step, const void* q, void
   clear_error();
   reset_launches();
   if (int rc = check_paged("sdpa_paged_prefix", step)) return rc;
-  if (!prefix_table || prefix_len <= 0 || prefix_len > 0x7fff0000)
+  if (!prefix_table || prefix_len <= 0 || prefix_len > kMaxKeys)
     return fail(LIMN_B200_BAD_ARGUMENT, "sdpa_paged_prefix: a prefix of %d keys, or no table of its pages", prefix_len);
   return paged_pass("sdpa_paged_prefix", step, q, out, lse, strides, prefix_table, prefix_len, causal, scale, workspace, workspace_bytes, stream);
 }

@@ -27,7 +27,8 @@ using namespace paged;
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kUnit = 16;  // keys
+constexpr int kUnit = kPagedUnit;  // keys
+static_assert(kUnit == 16);
 constexpr int kBegin = 4;  // units that a problem costs besides its keys: its queries, its page table, its way out
 constexpr float kSlack = 8.f;
 
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   unsigned none = 0;  // two bits for each place of the ring: which 8 of its unit's keys have a page that is none
   auto entry_of = [&](const Cursor& c, int blk) {
     const int key = (blk * 32 + lane) * 8;
-    return key < c.e.keys ? prm.table[static_cast<long long>(c.b) * prm.max_pages + prm.by_page.of(key)] : 0;
+    return key < side_end(prm, key, c.e.keys) ? entry_for(prm, c.b, key) : 0;
   };
   auto issue = [&]() {
     if (ahead.cost < span) {
@@ -195,7 +196,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
         const int raw = block >= 0 && blk == block + 1 ? entry_next : entry_of(ahead, blk);
         block = blk;
         entry_next = entry_of(ahead, blk + 1);
-        page = (blk * 32 + lane) * 8 < ahead.e.keys ? checked_page(raw, prm.pages, prm.errors) : -1;
+        const int key = (blk * 32 + lane) * 8;
+        page = key < side_end(prm, key, ahead.e.keys) ? checked_page(raw, prm.pages, prm.errors) : -1;
       }
       const int place_at = loaded % R::kStages;
       const uint32_t k_to = mine + place_at * 2 * R::kSide, v_to = k_to + R::kSide;
@@ -204,12 +206,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       for (int half = 0; half < 2; ++half) {
         const int key0 = ahead.unit * kUnit + half * 8;
         const int p = __shfl_sync(0xffffffffu, page, (key0 / 8) & 31);
-        const int slot = prm.by_page.rest(key0);
+        const int slot = slot_of(prm, key0), end = side_end(prm, key0, ahead.e.keys);
         const long long in_page = max(p, 0);
-        if (p < 0 && key0 < ahead.e.keys) none |= 1u << (2 * place_at + half);
+        if (p < 0 && key0 < end) none |= 1u << (2 * place_at + half);
         const unsigned char* k_from = prm.k.base + in_page * prm.k.page + ahead.kv_head * prm.k.head + slot * prm.k.slot;
         const unsigned char* v_from = prm.v.base + in_page * prm.v.page + ahead.kv_head * prm.v.head + slot * prm.v.slot;
-        const int rows_there = p >= 0 ? ahead.e.keys - key0 : 0;  // (the others are zeros, and what they would be is not read)
+        const int rows_there = p >= 0 ? end - key0 : 0;  // (the others are zeros, and what they would be is not read)
 #pragma unroll
         for (int j = 0; j < kCopies; ++j) {
           const bool there = row_of[j] < rows_there;
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int token = prm.by_group.of(nt * 8 + cq * 2 + c);
-        limit[nt][c] = prm.causal ? min(at.e.keys, at.e.keys - at.e.n + token + 1) : at.e.keys;
+        limit[nt][c] = prm.causal ? max(prm.front, min(at.e.keys, at.e.keys - at.e.n + token + 1)) : at.e.keys;
         m[nt][c] = -INFINITY, l[nt][c] = 0.f;
       }
 #pragma unroll
@@ -289,6 +291,13 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           if (key + (c >> 1) * 8 >= limit[nt][c & 1]) s[nt][c] = -INFINITY;
+    }
+    if (at.unit * kUnit < prm.front && at.unit * kUnit + kUnit > prm.prefix_len) {  // the last keys of the front do not exist
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (key + (c >> 1) * 8 >= prm.prefix_len) s[nt][c] = -INFINITY;
     }
     const unsigned none_here = (none >> (2 * place_at)) & 3u;
     if (none_here != 0u) {  // a row that sees a key of a page that is none: l is NaN from here on

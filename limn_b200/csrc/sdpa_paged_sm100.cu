@@ -33,7 +33,8 @@ namespace {
 using namespace ptx;
 using namespace paged;
 
-constexpr int kTile = 128;     // rows of a tile, keys of a key tile
+constexpr int kTile = kPagedTile;  // rows of a tile, keys of a key tile
+static_assert(kTile == 128);
 constexpr int kThreads = 320;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
@@ -98,19 +99,19 @@ __device__ __forceinline__ int tiles_of(int keys) { return (keys + kTile - 1) >>
 // ---- the cost of items, in keys (int holds an item's: 2^31 keys would be 2^35 bytes of a head). A sequence has `pairs` items per key head, pair j of tokens [j span, (j + 1) span) ----
 struct Costs {
   int pairs, span, half, seen_first;  // span: tokens of a pair; half: of a tile; seen_first: keys that are there before the first token
-  int keys, n, causal;
+  int keys, n, causal, least;  // least: keys that a token sees at the least, those in front; one, masked, where there are none
   Div by_span;
-  __device__ __forceinline__ Costs(const Extent& e, const Div& by_span_, int causal_)
-      : pairs(by_span_.of(e.n + static_cast<int>(by_span_.d) - 1)), span(by_span_.d), half(by_span_.d / 2), seen_first(e.keys - e.n), keys(e.keys), n(e.n), causal(causal_), by_span(by_span_) {}
-  // keys that the first `tokens` tokens see at most; one, masked, where that is none
-  __device__ __forceinline__ int seen(int tokens) const { return max(1, causal ? seen_first + min(tokens, n) : keys); }
+  __device__ __forceinline__ Costs(const Extent& e, const Div& by_span_, const Pass& p)
+      : pairs(by_span_.of(e.n + static_cast<int>(by_span_.d) - 1)), span(by_span_.d), half(by_span_.d / 2), seen_first(e.keys - e.n), keys(e.keys), n(e.n), causal(p.causal), least(max(1, p.front)), by_span(by_span_) {}
+  // keys that the first `tokens` tokens see at most
+  __device__ __forceinline__ int seen(int tokens) const { return max(least, causal ? seen_first + min(tokens, n) : keys); }
   __device__ __forceinline__ bool single(int j) const { return n - j * span <= half; }
   __device__ __forceinline__ int of(int j) const { return kItem + (single(j) ? (seen((j + 1) * span) + 1) / 2 : seen((j + 1) * span)); }
   // sum over the pairs in front of j (all of them two whole tiles)
   __device__ __forceinline__ long long before(long long j) const {
-    if (!causal) return j * (kItem + max(1, keys));
-    const long long none = seen_first >= 0 ? 0 : min(j, static_cast<long long>(by_span.of(-seen_first)));  // pairs whose last token sees nothing: 1 each
-    return j * kItem + none + (j - none) * seen_first + span * (j * (j + 1) / 2 - none * (none + 1) / 2);
+    if (!causal) return j * (kItem + max(least, keys));
+    const long long none = seen_first >= least ? 0 : min(j, static_cast<long long>(by_span.of(least - 1 - seen_first)));  // pairs whose last token sees the least
+    return j * kItem + none * least + (j - none) * seen_first + span * (j * (j + 1) / 2 - none * (none + 1) / 2);
   }
   __device__ __forceinline__ long long all() const { return pairs == 0 ? 0 : before(pairs - 1) + of(pairs - 1); }
   // steps of key tiles (pairs of key tiles for a single tile) of pair j
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
 #pragma unroll 1
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
-      if (b < prm.batch) mine += Costs(extent_of(prm, b), by_span, prm.causal).all();
+      if (b < prm.batch) mine += Costs(extent_of(prm, b), by_span, prm).all();
     }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -206,11 +207,11 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     do {
       ++p.b;
       p.e = extent_of(prm, p.b);
-      all = Costs(p.e, by_span, prm.causal).all();
+      all = Costs(p.e, by_span, prm).all();
       if (rest < all * prm.kv_heads) break;
       rest -= all * prm.kv_heads;
     } while (p.b + 1 < prm.batch);
-    const Costs costs(p.e, by_span, prm.causal);
+    const Costs costs(p.e, by_span, prm);
     p.kv_head = small_quotient(rest, all);
     rest -= p.kv_head * all;
     int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     const int my_chunk = lane & (chunks - 1), my_atom = (lane << chunk_log) / kTile;
     constexpr int kBoxAtoms = kPacked ? 1 : D / 64;  // boxes to a chunk
     while (more && ok) {
-      const Costs costs(at.e, by_span, prm.causal);
+      const Costs costs(at.e, by_span, prm);
       const bool last = at.b == end.b && at.kv_head == end.kv_head && at.j == end.j;
       const int steps = costs.steps(at.j), until = last ? end.step : steps;
       if (until > at.step) {
@@ -316,22 +317,22 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           __syncwarp();
         }
         if (!ok) break;
-        const int* table = prm.table + static_cast<long long>(s.b) * prm.max_pages;
         // the page of this lane's box of key tile `tile`; one that is none is a coordinate outside the cache, whose box TMA fills with zeros
         auto entry = [&](int tile) {
           const int key = tile * kTile + my_chunk * chunk;
-          return key < s.keys ? table[prm.by_page.of(key)] : 0;
+          return key < side_end(prm, key, s.keys) ? entry_for(prm, s.b, key) : 0;
         };
         int page_next[2] = {entry(s.first_tile), entry(s.first_tile + 1)};  // two tiles ahead
 #pragma unroll 1
         for (int j = 0; j < s.loads && ok; ++j, ++step) {
           const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
-          const bool fetch = key < s.keys && my_atom < kBoxAtoms;
+          const int end = side_end(prm, key, s.keys);  // (the same for the whole tile)
+          const bool fetch = key < end && my_atom < kBoxAtoms;
           const int page = fetch ? checked_page(page_next[0], prm.pages, prm.errors) : 0;
-          const int boxes = min(chunks, max(0, (s.keys - tile * kTile + chunk - 1) >> chunk_log));  // those that have keys
+          const int boxes = min(chunks, max(0, (end - tile * kTile + chunk - 1) >> chunk_log));  // those that have keys
           const uint32_t bytes = static_cast<uint32_t>(boxes * chunk) * (D * 2);
           page_next[0] = page_next[1], page_next[1] = entry(tile + 2);
-          const int in_page = prm.by_page.rest(key);
+          const int in_page = slot_of(prm, key);
           const int stage = step % B::kS;
           const uint32_t wrap = (step / B::kS) & 1;
           ok = wait(B::k_empty + stage, wrap ^ 1u, 0x0100u | stage);
@@ -455,7 +456,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           const int stage = here % B::kS, next = then % B::kS;
           ok = wait(B::v_full + stage, (here / B::kS) & 1, 0x0220u | stage);
           if (!ok) break;
-          const int left = s.keys - (s.first_tile + static_cast<int>(here - step)) * kTile;  // keys of the tile that there are
+          const int tile_at = (s.first_tile + static_cast<int>(here - step)) * kTile;
+          const int left = side_end(prm, tile_at, s.keys) - tile_at;  // keys of the tile that there are
           if (left < kTile && cleared != here + 1) {
             clear_rows(stage, max(0, left));
             cleared = here + 1;
@@ -537,14 +539,13 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         continue;
       }
       const int seen_first = s.keys - s.n;
-      const int sees = prm.causal ? min(s.keys, seen_first + prm.by_group.of(row) + 1) : s.keys;                // keys [0, sees)
-      const int sees_least = prm.causal ? min(s.keys, seen_first + prm.by_group.of(top_row) + 1) : s.keys;      // the tile's first token
-      const int* table = prm.table + static_cast<long long>(s.b) * prm.max_pages;
+      const int sees = prm.causal ? max(prm.front, min(s.keys, seen_first + prm.by_group.of(row) + 1)) : s.keys;            // keys [0, sees)
+      const int sees_least = prm.causal ? max(prm.front, min(s.keys, seen_first + prm.by_group.of(top_row) + 1)) : s.keys;  // the tile's first token
       auto key0 = [&](int j) { return (s.first_tile + (both ? 2 * j + t : j)) * kTile; };
       // pages are looked at once more here, a key tile ahead
       auto entry = [&](int j) {
         const int key = key0(j) + lane * chunk;
-        return lane < chunks && key < s.keys ? table[prm.by_page.of(key)] : 0;
+        return lane < chunks && key < side_end(prm, key, s.keys) ? entry_for(prm, s.b, key) : 0;
       };
       int entry_next = entry(0);
       float m = -INFINITY, l = 0.f;
@@ -561,9 +562,10 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         tmem_ld_wait();
         const int kv0 = key0(j);
         // a row that sees a key of a page that is none: l, and with it all of the row, is NaN from here on
-        if (none != 0u && (__ffs(none) - 1) * chunk < sees - kv0) l = NAN;
-        if (kv0 + kTile > sees_least) {
-          const int limit = sees - kv0;
+        const bool in_front = kv0 < prm.front;
+        const int limit = (in_front ? prm.prefix_len : sees) - kv0;
+        if (none != 0u && (__ffs(none) - 1) * chunk < limit) l = NAN;
+        if (kv0 + kTile > (in_front ? prm.prefix_len : sees_least)) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll

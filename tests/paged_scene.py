@@ -138,6 +138,8 @@ class Scene:
         out = np.full((self.tokens, self.heads, self.hd_v), np.nan)
         size, lse = out.copy(), np.full((self.tokens, self.heads), np.nan)
         for b, (n, length) in enumerate(self.seqs):
+            if n == 0:
+                continue
             rows = slice(self.start[b], self.start[b] + n)
             k = np.concatenate([self.prefix_k, self.k[b]]).astype(np.float64)
             v = np.concatenate([self.prefix_v, self.v[b]]).astype(np.float64)

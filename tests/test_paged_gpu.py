@@ -332,6 +332,119 @@ def test_a_prefix_far_longer_than_the_rest():
     Scene([(1, 3), (40, 50)], heads=8, kv_heads=2, hd=128, page_size=16, seed=15, prefix=9000).upload().check()
 
 
+# Behind a prefix that would cost much to read for every sequence, a call reads it once, for the whole batch. Sequences without tokens cost nothing, but how many
+# there are counts for that.
+IDLE = [(0, 0)] * 4000
+
+
+def launches() -> int:
+    from limn_b200._lib import lib
+
+    return lib().limn_b200_last_launch_count()
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("shape", SHAPES, ids=[s[0] for s in SHAPES])
+def test_a_prefix_read_once(shape, causal):
+    _, dtype, heads, kv_heads, hd, hd_v, page_size, order, seqs = shape
+    s = Scene(seqs + IDLE, dtype=dtype, heads=heads, kv_heads=kv_heads, hd=hd, hd_v=hd_v, page_size=page_size, order=order, prefix=300, spare_tokens=2,
+              seed=11, row_room=8).upload()
+    s.check(causal=causal)
+    assert launches() == 3
+
+
+@pytest.mark.parametrize("length", [8, 15, 16, 17, 120, 127, 128, 129, 255, 256, 257, 1024])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("once", [False, True], ids=["for each", "once"])
+def test_every_length_of_a_prefix(length, new, once):
+    """Where a prefix ends inside a unit or a tile of keys, beside sequences that have no keys, few, or see none of their own."""
+    s = Scene([(new, new), (1, 0), (new, new + 100), (2, 1)] + IDLE * (10 if once else 0), heads=8, kv_heads=2, hd=64, page_size=8, seed=length, prefix=length).upload()
+    s.check()
+    assert launches() == (3 if once else 2)
+    s.check(causal=False)
+
+
+@pytest.mark.parametrize("heads", [1, 2, 4])
+def test_more_tokens_than_keys_behind_a_prefix_read_once(heads):
+    s = Scene([(5, 3), (1, 0), (40, 2), (2, 200)] + IDLE, heads=heads, kv_heads=1, hd=64, seed=2, prefix=700).upload()
+    s.check()
+    assert launches() == 3
+
+
+@pytest.mark.parametrize("idle", [[], IDLE], ids=["for each", "once"])
+@pytest.mark.parametrize("new", [1, 60])
+def test_pages_that_are_none_behind_a_prefix(new, idle):
+    """One of a sequence's own: the rows that see it. One of the prefix: all rows."""
+    from limn_b200 import runtime
+
+    s = Scene([(new, 400), (new, 300), (1, 64)] + idle, heads=4, kv_heads=2, hd=64, page_size=16, seed=3, prefix=700)
+    table = s.table.copy()
+    table[1, 300 // 16 - 1] = -9  # slots 272 to 287
+    s.upload(table=table)
+    have_o, have_l = s.attend()
+    assert s.error_bits() == 1 and launches() == (3 if idle else 2)
+    want_o, want_l, size = s.expected()
+    sees = np.zeros(s.tokens, bool)
+    sees[s.start[1] : s.start[2]] = (300 - new + np.arange(new)) >= 272
+    assert np.isnan(have_o[sees].astype(np.float32)).all() and np.isnan(have_l[sees]).all()
+    half = HALF_STEP[BF16]
+    off = np.abs(have_o[~sees].astype(np.float64) - want_o[~sees])
+    assert (off <= half * np.abs(want_o[~sees]) * (1 + half) + (half + 2.0**-13) * size[~sees] + 2.0**-24).all()
+    assert (np.abs(have_l[~sees] - want_l[~sees]) <= 2.0**-13 + 2.0**-23 * np.abs(want_l[~sees])).all()
+    for which in (0, 20, 43):  # the last one holds 12 keys
+        bad = np.append(s.prefix_table, np.int32(NOWHERE))
+        bad[which] = s.pages
+        s.upload()
+        s.prefix_dev = runtime.upload(bad)
+        have_o, have_l = s.attend()
+        assert s.error_bits() == 1 and np.isnan(have_o.astype(np.float32)).all() and np.isnan(have_l).all()
+
+
+@pytest.mark.parametrize("new, heads", [(1, 4), (1, 32), (4, 16), (3, 20), (30, 8)])
+def test_what_the_workspace_held_is_of_no_concern_to_a_prefix_read_once(new, heads):
+    from limn_b200 import runtime
+    from limn_b200.paged import PagedBatch
+
+    s = Scene([(new, 600), (1, 3), (new, 900), (0, 10), (new, 40)] + IDLE, heads=heads, kv_heads=4, hd=128, page_size=16, seed=28, prefix=300).upload()
+    first = s.check()
+    assert launches() == 3
+    held, size = s.step._held[0], s.step.workspace_bytes
+    rng = np.random.default_rng(3)
+    for bytes_ in (np.full(size, 0xFF, np.uint8), rng.integers(0, 256, size, dtype=np.uint8)):
+        memory = runtime.upload(bytes_)
+        s.step = PagedBatch(held, heads=heads, batch=len(s.seqs), tokens=s.tokens, max_t_q=s.max_t_q, page_table=s.table_dev, max_pages=s.max_pages,
+                            q_start=s.q_start_dev, kv_lens=s.kv_lens_dev, errors=s.errors, workspace=memory)
+        for _ in range(3):
+            again = s.attend()
+            assert np.array_equal(first[0].view(np.uint16), again[0].view(np.uint16)) and np.array_equal(first[1], again[1])
+
+
+def test_a_workspace_serves_a_prefix_of_any_length():
+    """It is sized for one key: as much as any longer one needs."""
+    from limn_b200.paged import PagedBatch
+
+    s = Scene([(1, 60), (30, 40)] + IDLE, heads=4, kv_heads=2, hd=64, seed=29, prefix=900).upload()
+    s.step = PagedBatch(s.step._held[0], heads=4, batch=len(s.seqs), tokens=s.tokens, max_t_q=30, page_table=s.table_dev, max_pages=s.max_pages,
+                        q_start=s.q_start_dev, kv_lens=s.kv_lens_dev, errors=s.errors, first_position=900)
+    s.check()
+    assert launches() == 3
+
+
+def test_standing_down_behind_a_prefix_read_once():
+    from limn_b200 import runtime
+    from limn_b200._lib import check, lib
+
+    s = Scene([(60, 500), (1, 70)] + IDLE, heads=4, kv_heads=2, hd=64, seed=27, prefix=300).upload()
+    s.check()
+    assert launches() == 3
+    flag = runtime.empty(4, poison=0)
+    check(lib().limn_b200_wait_probe(20000, flag.ptr, None), "wait probe")
+    have_o, have_l = s.attend()
+    assert (have_o.view(np.uint16) == 0x7FFF).all() and np.isnan(have_l).all()
+    assert runtime.device_status() == 0x57417E57
+    s.check()
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_offsets_past_31_bits(new):
     """Pages 2^27 elements apart: the last one begins 2^31 elements, 2^32 bytes, in."""
@@ -534,11 +647,9 @@ def test_launches_and_workspace():
     from limn_b200._lib import last_error, lib
 
     s = Scene([(1, 60), (2, 40)], heads=4, kv_heads=2, hd=64, seed=26, prefix=20).upload()
-    s.attend()
-    assert lib().limn_b200_last_launch_count() == 3
-    s.prefix = 0
-    s.attend()
-    assert lib().limn_b200_last_launch_count() == 2
+    for s.prefix in (20, 0):
+        s.attend()
+        assert lib().limn_b200_last_launch_count() == 2
     need = ctypes.c_ulonglong()
     assert lib().limn_b200_sdpa_paged_workspace(s.step._by_ref, 0, ctypes.byref(need)) == 0 and need.value > 0
     with_prefix = ctypes.c_ulonglong()
