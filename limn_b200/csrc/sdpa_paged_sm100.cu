@@ -36,6 +36,10 @@ using namespace paged;
 constexpr int kTile = kPagedTile;  // rows of a tile, keys of a key tile
 static_assert(kTile == 128);
 constexpr int kThreads = 320;
+// What a step of an item with one tile costs, in keys. It computes as much as a step with two, a key tile of 128 each, but loads two key tiles to that one's one, which
+// no copy further ahead hides: by 176 prompt_pieces takes 219 us, by 128 (the arithmetic alone) 274, by 240 222. Pages of 8 make the producer issue twice
+// the boxes, and that bounds it: 224 takes 222 us where 176 takes 243.
+__device__ __forceinline__ int paged_single_step(int chunk_log) { return chunk_log == 3 ? 224 : 176; }
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr uint32_t kTmemCols = 512;
@@ -99,14 +103,14 @@ __device__ __forceinline__ int tiles_of(int keys) { return (keys + kTile - 1) >>
 // ---- the cost of items, in keys (int holds an item's: 2^31 keys would be 2^35 bytes of a head). A sequence has `pairs` items per key head, pair j of tokens [j span, (j + 1) span) ----
 struct Costs {
   int pairs, span, half, seen_first;  // span: tokens of a pair; half: of a tile; seen_first: keys that are there before the first token
-  int keys, n, causal, least;  // least: keys that a token sees at the least, those in front; one, masked, where there are none
+  int keys, n, causal, single_step, least;  // least: keys that a token sees at the least, those in front; one, masked, where there are none
   Div by_span;
-  __device__ __forceinline__ Costs(const Extent& e, const Div& by_span_, const Pass& p)
-      : pairs(by_span_.of(e.n + static_cast<int>(by_span_.d) - 1)), span(by_span_.d), half(by_span_.d / 2), seen_first(e.keys - e.n), keys(e.keys), n(e.n), causal(p.causal), least(max(1, p.front)), by_span(by_span_) {}
+  __device__ __forceinline__ Costs(const Extent& e, const Div& by_span_, const Pass& p, int chunk_log)
+      : pairs(by_span_.of(e.n + static_cast<int>(by_span_.d) - 1)), span(by_span_.d), half(by_span_.d / 2), seen_first(e.keys - e.n), keys(e.keys), n(e.n), causal(p.causal), single_step(paged_single_step(chunk_log)), least(max(1, p.front)), by_span(by_span_) {}
   // keys that the first `tokens` tokens see at most
   __device__ __forceinline__ int seen(int tokens) const { return max(least, causal ? seen_first + min(tokens, n) : keys); }
   __device__ __forceinline__ bool single(int j) const { return n - j * span <= half; }
-  __device__ __forceinline__ int of(int j) const { return kItem + (single(j) ? (seen((j + 1) * span) + 1) / 2 : seen((j + 1) * span)); }
+  __device__ __forceinline__ int of(int j) const { return kItem + (single(j) ? static_cast<int>((static_cast<long long>(seen((j + 1) * span)) * single_step) >> 8) + 1 : seen((j + 1) * span)); }
   // sum over the pairs in front of j (all of them two whole tiles)
   __device__ __forceinline__ long long before(long long j) const {
     if (!causal) return j * (kItem + max(least, keys));
@@ -119,9 +123,11 @@ struct Costs {
     const int tiles = tiles_of(seen((j + 1) * span));
     return single(j) ? (tiles + 1) >> 1 : tiles;
   }
+  __device__ __forceinline__ int step_cost(int j) const { return single(j) ? single_step : kTile; }
   // the step nearest to `cost` into pair j; what lies in front of the keys counts as the first one's beginning
   __device__ __forceinline__ int step_at(int j, long long cost) const {
-    return static_cast<int>(min(static_cast<long long>(steps(j)), max(0LL, cost - kItem + kTile / 2) >> 7));
+    const int into = max(0, static_cast<int>(cost) - kItem + step_cost(j) / 2);
+    return min(steps(j), single(j) ? into / single_step : into >> 7);
   }
 };
 
@@ -180,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
 #pragma unroll 1
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
-      if (b < prm.batch) mine += Costs(extent_of(prm, b), by_span, prm).all();
+      if (b < prm.batch) mine += Costs(extent_of(prm, b), by_span, prm, chunk_log).all();
     }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -207,11 +213,11 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     do {
       ++p.b;
       p.e = extent_of(prm, p.b);
-      all = Costs(p.e, by_span, prm).all();
+      all = Costs(p.e, by_span, prm, chunk_log).all();
       if (rest < all * prm.kv_heads) break;
       rest -= all * prm.kv_heads;
     } while (p.b + 1 < prm.batch);
-    const Costs costs(p.e, by_span, prm);
+    const Costs costs(p.e, by_span, prm, chunk_log);
     p.kv_head = small_quotient(rest, all);
     rest -= p.kv_head * all;
     int low = 0, high = costs.pairs - 1;  // the last pair that begins at or before `rest`
@@ -271,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     const int my_chunk = lane & (chunks - 1), my_atom = (lane << chunk_log) / kTile;
     constexpr int kBoxAtoms = kPacked ? 1 : D / 64;  // boxes to a chunk
     while (more && ok) {
-      const Costs costs(at.e, by_span, prm);
+      const Costs costs(at.e, by_span, prm, chunk_log);
       const bool last = at.b == end.b && at.kv_head == end.kv_head && at.j == end.j;
       const int steps = costs.steps(at.j), until = last ? end.step : steps;
       if (until > at.step) {
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         }
         if (s.begun && !s.whole && lane == 0) {
           // workers behind this one whose share begins inside the item, before the middle of its last step
-          const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(kTile) - kTile / 2);
+          const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(costs.step_cost(at.j)) - costs.step_cost(at.j) / 2);
           prm.parts.heads[blockIdx.x] = Head{small_quotient(begins + limit - 1, share) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
         }
       }
