@@ -187,10 +187,12 @@ int limn_b200_sdpa_bwd_kv_strided(const void* q, const void* k, const void* v, c
  * which has no cache (its decode shape is t_q < t_k of dense tensors, tests/test_attention.py:385-396).
  *   f16/bf16, hd and hd_v multiples of 8 up to 128, heads a multiple of kv_heads (query head h reads key head
  *   h / (heads / kv_heads)) and at most 128 to a key head, page_size a multiple of 8; strides in elements, multiples of 8, columns
- *   contiguous, bases 16-byte aligned. Anything else is refused and nothing is launched.
+ *   contiguous, bases 16-byte aligned, every other array as its type is. Positions, tokens * heads and max_pages * page_size fit 31 bits. Anything
+ *   else is refused and nothing is launched.
  * What only the device knows is checked there. A sequence whose offsets or length are impossible (q_start falling, beyond
  * `tokens` or more than max_t_q apart; kv_lens negative or beyond max_pages * page_size) is left out: nothing of it is appended
- * and no row of its result is written (where q_start falls, other sequences may be left out too). A page number outside [0, pages) is never followed: a new token that belongs there is
+ * and no row of its result is written (where q_start falls, other sequences may be left out too). One that brings more tokens than it has
+ * keys has no slots for the first of them: none of it is appended, and those tokens see no key. A page number outside [0, pages) is never followed: a new token that belongs there is
  * not appended, and a query row that sees a key there gets NaN (O and L). Either is noted in *errors (LIMN_B200_PAGED_BAD_*
  * bits are or-ed in; the caller clears the word). Tokens from q_start[batch] on, empty slots of pages, and pages that no table
  * names are neither read for a result nor written. */
@@ -221,7 +223,7 @@ enum limn_b200_pairing {
 
 /* Put the step's keys and values into their slots, turned to their positions, and turn the queries beside them.
  *   q (tokens, heads, hd) -> q_out, or both NULL; k (tokens, kv_heads, hd), v (tokens, kv_heads, hd_v) into the cache.
- *   strides: (token, head) pairs of q, q_out, k, v (4 pairs; those of absent operands are not read). q_out may be q.
+ *   strides: (token, head) pairs of q, q_out, k, v (4 pairs; those of absent operands are not read). q_out may be q, with its strides.
  *   The first `rotated` columns of a row (a multiple of 8, 0 to hd) turn: pair j of a token at position p = first_position + slot
  *   by the angle p * frequencies[j], (x, y) -> (x cos - y sin, x sin + y cos); frequencies is a device array of rotated / 2
  *   doubles (NULL where rotated is 0). The angle is reduced in float64, the turn is float32, rounded once.
@@ -240,15 +242,15 @@ int limn_b200_sdpa_paged(const limn_b200_paged* step, const void* q, void* out, 
                          int causal, double scale, void* workspace, unsigned long long workspace_bytes, void* stream);
 
 /* The same for a batch whose sequences all continue one prefix: every row sees the prefix_len keys of the pages prefix_table
- * names (device array, ceil(prefix_len / page_size) entries) and behind them its sequence's own as above. The prefix is
- * read once for the whole batch. Keys in a sequence's own pages are counted from the prefix's end: kv_lens, q_start and page_table do not
+ * names (device array, ceil(prefix_len / page_size) entries) and behind them its sequence's own as above. Where that costs less
+ * the prefix is read once for the whole batch, in a pass of its own, else in front of every sequence's keys; a result's bits depend on which. Keys in a sequence's own pages are counted from the prefix's end: kv_lens, q_start and page_table do not
  * include it, first_position does. */
 int limn_b200_sdpa_paged_prefix(const limn_b200_paged* step, const void* q, void* out, float* lse, const long long* strides,
                                 const int* prefix_table, int prefix_len, int causal, double scale,
                                 void* workspace, unsigned long long workspace_bytes, void* stream);
 
 /* Bytes of workspace a call for this step needs on the current device, whatever the device arrays hold; prefix_len 0 for
- * limn_b200_sdpa_paged. Pointers in *step are not looked at. */
+ * limn_b200_sdpa_paged, any other for a prefix of any length. Pointers in *step are not looked at. */
 int limn_b200_sdpa_paged_workspace(const limn_b200_paged* step, int prefix_len, unsigned long long* bytes);
 
 /* Which path the dispatcher picks for a problem (a limn_b200_path value), or -1 with an
@@ -269,7 +271,8 @@ int limn_b200_version(void);
 /* Kernels that wait (on TMA or tensor-core completion) give up after a bounded time and
  * record a code in a per-device status word instead of hanging; kernels of that kind launched on that
  * device afterwards return within some milliseconds, writing nothing, until the word has been read
- * (the float64, CUDA-core, decode and row-dot kernels wait for nothing and run). This synchronises the
+ * (the float64, CUDA-core, decode and row-dot kernels wait for nothing and run; so do limn_b200_kv_append and, for at most 16 query
+ * rows to a key head, limn_b200_sdpa_paged). This synchronises the
  * current device, reads its word into *status and clears it. Returns LIMN_B200_OK with *status == 0
  * when no kernel gave up, LIMN_B200_DEVICE_TIMEOUT with *status = 0x5741rrbb (role rr, barrier bb)
  * when one did. The reference reports a failed kernel from its batch barrier

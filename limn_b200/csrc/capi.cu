@@ -134,37 +134,14 @@ int find_encoder() {
 
 int make_box_map(const char* name, CUtensorMap* map, const void* base, bool fp16, const BoxShape& shape) {
   if (int rc = find_encoder()) return rc;
-  // kept for the same reason as in make_tile_map
-  struct Entry {
-    const void* base;
-    int fp16;
-    BoxShape shape;
-    CUtensorMap map;
-  };
-  constexpr int kEntries = 16;
-  thread_local Entry cache[kEntries];
-  thread_local int used = 0, next_slot = 0;
-  for (int i = 0; i < used; ++i) {
-    const Entry& e = cache[i];
-    bool same = e.base == base && e.fp16 == (fp16 ? 1 : 0);
-    for (int d = 0; d < 5; ++d) same = same && e.shape.dims[d] == shape.dims[d] && e.shape.box[d] == shape.box[d] && (d == 4 || e.shape.strides[d] == shape.strides[d]);
-    if (same) {
-      *map = e.map;
-      return LIMN_B200_OK;
-    }
-  }
   cuuint64_t dims[5], strides[4];
   cuuint32_t box[5];
   const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
   for (int d = 0; d < 5; ++d) dims[d] = shape.dims[d], box[d] = shape.box[d];
-  for (int d = 0; d < 4; ++d) strides[d] = static_cast<cuuint64_t>(shape.strides[d]);
+  for (int d = 0; d < 4; ++d) strides[d] = dims[d + 1] > 1 ? static_cast<cuuint64_t>(shape.strides[d]) : 16;  // (never stepped: whatever it says)
   const CUresult res = g_encode_tiled(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, elem,
                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (res != CUDA_SUCCESS) return fail(LIMN_B200_CUDA_ERROR, "cuda: %s: encoding a tensor map failed with CUresult %d", name, (int)res);
-  Entry& slot = cache[next_slot];
-  slot.base = base, slot.fp16 = fp16 ? 1 : 0, slot.shape = shape, slot.map = *map;
-  next_slot = (next_slot + 1) % kEntries;
-  if (used < kEntries) ++used;
   return LIMN_B200_OK;
 }
 

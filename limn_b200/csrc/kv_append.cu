@@ -200,6 +200,7 @@ extern "C" int limn_b200_kv_append(const limn_b200_paged* step, const void* q, c
   if (!k || !v || !strides || (q == nullptr) != (q_out == nullptr)) return fail(LIMN_B200_BAD_ARGUMENT, "kv_append: a required pointer is null");
   if (rotated < 0 || rotated > step->hd || rotated % 8 != 0) return fail(LIMN_B200_BAD_ARGUMENT, "kv_append: rotated columns must be a multiple of 8 from 0 to hd, got %d", rotated);
   if (rotated > 0 && !frequencies) return fail(LIMN_B200_BAD_ARGUMENT, "kv_append: rotated columns without frequencies");
+  if (reinterpret_cast<uintptr_t>(frequencies) & 7u) return fail(LIMN_B200_BAD_ARGUMENT, "kv_append: the frequencies are not 8-byte aligned");
   if (pairing != LIMN_B200_HALVES && pairing != LIMN_B200_NEIGHBOURS) return fail(LIMN_B200_BAD_ARGUMENT, "kv_append: unknown pairing code %d", pairing);
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u)
     return fail(LIMN_B200_BAD_ARGUMENT, "kv_append: an operand is not 16-byte aligned");

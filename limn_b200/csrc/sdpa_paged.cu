@@ -44,6 +44,12 @@ bool prefix_in_front(const limn_b200_paged* step, int prefix_len) {
   return more / 2 * step->kv_heads * std::ceil(prefix_len / 128.0) * width * 2.1 / 148 <= apart;
 }
 
+// Shares of the work are counted in 64 bits, a warp's in 32 of them, 16 keys at a time: 2^43 keys that (tile, key head) pairs see is far below either.
+bool countable(const limn_b200_paged* step, double keys) {
+  const double group = step->heads / step->kv_heads;
+  return step->kv_heads * (std::min(step->batch, step->tokens) + step->tokens * group / 64) * (keys + 256) <= 8.8e12;
+}
+
 // The workspace of a call: the parts of the pass over the own keys; behind a prefix also those of the pass over it, and the rows' sums
 // over either, however long it is: a workspace that serves one prefix serves all.
 struct Workspace {
@@ -71,6 +77,9 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   if (!q || !out || !lse || !strides) return fail(LIMN_B200_BAD_ARGUMENT, "%s: a required pointer is null", name);
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15u)
     return fail(LIMN_B200_BAD_ARGUMENT, "%s: an operand is not 16-byte aligned", name);
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(prefix_table)) & 3u)
+    return fail(LIMN_B200_BAD_ARGUMENT, "%s: lse or the prefix's table is not 4-byte aligned", name);
+  if (!countable(step, prefix_len)) return fail(LIMN_B200_UNSUPPORTED, "%s: %d sequences behind a prefix of %d keys are more work than a call counts", name, step->batch, prefix_len);
   for (int i = 0; i < 4; ++i)
     if (strides[i] < 0 || (strides[i] & 7)) return fail(LIMN_B200_BAD_ARGUMENT, "%s: strides must be non-negative multiples of 8 elements, got %lld", name, strides[i]);
   if (!(scale > 0.0) || scale > 1e30) return fail(LIMN_B200_UNSUPPORTED, "%s: the scale must be positive and finite", name);
@@ -136,6 +145,8 @@ int check_paged(const char* name, const limn_b200_paged* s) {
   if (static_cast<long long>(s->tokens) * s->heads > kMaxKeys) return fail(LIMN_B200_UNSUPPORTED, "%s: %d tokens of %d heads do not fit 31 bits", name, s->tokens, s->heads);
   if (static_cast<long long>(s->max_pages) * s->page_size > kMaxKeys - s->first_position)
     return fail(LIMN_B200_UNSUPPORTED, "%s: positions of %d pages of %d from %d on do not fit 31 bits", name, s->max_pages, s->page_size, s->first_position);
+  if (!countable(s, static_cast<double>(s->max_pages) * s->page_size))
+    return fail(LIMN_B200_UNSUPPORTED, "%s: %d sequences of up to %d pages of %d keys are more work than a call counts", name, s->batch, s->max_pages, s->page_size);
   for (int i = 0; i < 3; ++i)
     if (s->k_strides[i] < 0 || (s->k_strides[i] & 7) || s->v_strides[i] < 0 || (s->v_strides[i] & 7))
       return fail(LIMN_B200_BAD_ARGUMENT, "%s: cache strides must be non-negative multiples of 8 elements", name);
@@ -144,6 +155,8 @@ int check_paged(const char* name, const limn_b200_paged* s) {
 
 int check_paged_pointers(const char* name, const limn_b200_paged* s) {
   if (!s->k_cache || !s->v_cache || !s->page_table || !s->q_start || !s->kv_lens) return fail(LIMN_B200_BAD_ARGUMENT, "%s: a required pointer of the step is null", name);
+  if ((reinterpret_cast<uintptr_t>(s->page_table) | reinterpret_cast<uintptr_t>(s->q_start) | reinterpret_cast<uintptr_t>(s->kv_lens) | reinterpret_cast<uintptr_t>(s->errors)) & 3u)
+    return fail(LIMN_B200_BAD_ARGUMENT, "%s: the table, the offsets, the lengths or the word for errors is not 4-byte aligned", name);
   if ((reinterpret_cast<uintptr_t>(s->k_cache) | reinterpret_cast<uintptr_t>(s->v_cache)) & 15u) return fail(LIMN_B200_BAD_ARGUMENT, "%s: the cache is not 16-byte aligned", name);
   return LIMN_B200_OK;
 }

@@ -59,8 +59,9 @@ class PagedCache:
 
 class PagedBatch:
     """A batch of sequences over a cache. `errors` is a device word that collects LIMN_B200_PAGED_BAD_* bits (the caller zeroes
-    and reads it); `max_prefix` the longest shared prefix attention_with_prefix will be asked for. `workspace` is device
-    memory of `workspace_bytes`; without one the batch allocates its own."""
+    and reads it); `max_prefix` the longest shared prefix attention_with_prefix will be asked for, 0 for none (any other number takes the
+    same room). `workspace` is 16-byte aligned device memory of at least what a batch of these extents has as `workspace_bytes`, such as the `workspace` of
+    the batch over another layer of the same model, whose calls follow this one's on one stream; without one the batch allocates its own."""
 
     def __init__(self, cache: PagedCache, *, heads: int, batch: int, tokens: int, max_t_q: int, page_table: Any, max_pages: int,
                  q_start: Any, kv_lens: Any, first_position: int = 0, errors: Any = None, max_prefix: int = 1, workspace: Any = None):
@@ -82,7 +83,9 @@ class PagedBatch:
         self.workspace_bytes = need.value
         if workspace is None and need.value:
             workspace = DeviceBuffer(need.value)
-        self._workspace = workspace
+        if getattr(workspace, "nbytes", need.value) < need.value:
+            raise ValueError(f"limn_b200: the workspace has {workspace.nbytes} bytes, {need.value} are needed")
+        self.workspace = workspace
         self._workspace_at = _address(workspace)
 
     def append(self, k: Any, v: Any, *, q: Any = None, q_out: Any = None, k_strides=None, v_strides=None, q_strides=None, q_out_strides=None,

@@ -49,6 +49,7 @@ REFUSED = [
     (2, "31 bits", {"max_pages": 1 << 27, "page_size": 16}),
     (2, "31 bits", {"max_pages": 4, "first_position": 0x7FFFFFF0}),
     (2, "31 bits", {"tokens": 1 << 28, "heads": 16}),
+    (2, "counts", {"batch": 1 << 20, "tokens": 1 << 20, "heads": 128, "kv_heads": 128, "max_pages": 1 << 20}),
     (1, "strides", {"k_strides": triple(2048, 60, 128)}),
     (1, "strides", {"v_strides": triple(-2048, 64, 128)}),
 ]
@@ -60,6 +61,10 @@ POINTERS = [
     (1, "null", {"kv_lens": None}),
     (1, "aligned", {"k_cache": ONE + 8}),
     (1, "aligned", {"v_cache": ONE + 2}),
+    (1, "aligned", {"page_table": ONE + 2}),
+    (1, "aligned", {"q_start": ONE + 1}),
+    (1, "aligned", {"kv_lens": ONE + 2}),
+    (1, "aligned", {"errors": ONE + 3}),
 ]
 
 
@@ -96,7 +101,7 @@ def test_calls_that_cannot_be():
     append = lambda *, q=ONE, k=ONE, v=ONE, q_out=ONE, strides=pairs, freqs=ONE, rotated=64, pairing=0: L.limn_b200_kv_append(s, q, k, v, q_out, strides, freqs, rotated, pairing, None)  # noqa: E731
     for code, words, other in ((1, "null", {"k": None}), (1, "null", {"v": None}), (1, "null", {"q": None}), (1, "null", {"q_out": None}), (1, "null", {"strides": None}),
                                (1, "rotated", {"rotated": 72}), (1, "rotated", {"rotated": -8}), (1, "rotated", {"rotated": 12}), (1, "frequencies", {"freqs": None}),
-                               (1, "pairing", {"pairing": 2}), (1, "aligned", {"q": ONE + 4}), (1, "aligned", {"k": ONE + 8}),
+                               (1, "pairing", {"pairing": 2}), (1, "aligned", {"q": ONE + 4}), (1, "aligned", {"k": ONE + 8}), (1, "aligned", {"freqs": ONE + 4}),
                                (1, "strides", {"strides": (ctypes.c_longlong * 8)(256, 64, 256, 64, 128, 60, 128, 64)}),
                                (1, "strides", {"strides": (ctypes.c_longlong * 8)(-256, 64, 256, 64, 128, 64, 128, 64)})):
         assert append(**other) == code and words in last_error(), (other, last_error())
@@ -105,10 +110,13 @@ def test_calls_that_cannot_be():
 
     attend = lambda *, q=ONE, out=ONE, lse=ONE, strides=pairs, scale=0.125: L.limn_b200_sdpa_paged(s, q, out, lse, strides, 1, scale, ONE, 1 << 40, None)  # noqa: E731
     for code, words, other in ((1, "null", {"q": None}), (1, "null", {"out": None}), (1, "null", {"lse": None}), (1, "null", {"strides": None}), (1, "aligned", {"q": ONE + 8}),
-                               (1, "aligned", {"out": ONE + 2}), (2, "scale", {"scale": 0.0}), (2, "scale", {"scale": -0.1}), (2, "scale", {"scale": float("nan")}),
+                               (1, "aligned", {"out": ONE + 2}), (1, "aligned", {"lse": ONE + 2}), (2, "scale", {"scale": 0.0}), (2, "scale", {"scale": -0.1}), (2, "scale", {"scale": float("nan")}),
                                (2, "scale", {"scale": float("inf")}), (1, "strides", {"strides": (ctypes.c_longlong * 4)(256, 64, 256, 4)})):
         assert attend(**other) == code and words in last_error(), (other, last_error())
     prefix = lambda table, length: L.limn_b200_sdpa_paged_prefix(s, ONE, ONE, ONE, pairs, table, length, 1, 0.125, ONE, 1 << 40, None)  # noqa: E731
+    assert prefix(ONE + 2, 10) == 1 and "aligned" in last_error()
+    many = ctypes.byref(step(batch=1 << 20, tokens=1 << 20))
+    assert L.limn_b200_sdpa_paged_prefix(many, ONE, ONE, ONE, pairs, ONE, 0x7FFF0000, 1, 0.125, ONE, 1 << 40, None) == 2 and "counts" in last_error()
     assert prefix(None, 10) == 1 and prefix(ONE, 0) == 1 and prefix(ONE, -4) == 1 and "prefix" in last_error()
     assert L.limn_b200_sdpa_paged(None, ONE, ONE, ONE, pairs, 1, 0.125, ONE, 1 << 40, None) == 1 and "null step" in last_error()
     assert L.limn_b200_sdpa_paged_workspace(s, 0, None) == 1 and L.limn_b200_sdpa_paged_workspace(s, -1, ctypes.byref(ctypes.c_ulonglong())) == 1

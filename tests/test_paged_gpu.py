@@ -641,6 +641,50 @@ def test_no_word_for_errors():
     assert np.isnan(have_o[0].astype(np.float32)).all() and np.isfinite(have_o[1:].astype(np.float32)).all() and s.error_bits() == 0
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_strides_that_are_never_stepped(new):
+    """One page, one head: their strides may be anything, 0 too."""
+    from limn_b200 import runtime
+    from limn_b200.paged import PagedBatch, PagedCache
+
+    s = Scene([(new, 50)], heads=1, kv_heads=1, hd=128, page_size=64, seed=30, spare_pages=0).upload()
+    s.check()
+    cache = PagedCache(s.k_dev, s.v_dev, dtype="bfloat16", pages=1, page_size=64, kv_heads=1, hd=128, k_strides=(0, 0, 128), v_strides=(0, 0, 128))
+    step = PagedBatch(cache, heads=1, batch=1, tokens=new, max_t_q=new, page_table=s.table_dev, max_pages=1, q_start=s.q_start_dev, kv_lens=s.kv_lens_dev, max_prefix=0)
+    q = runtime.upload(s.q)
+    out, lse = runtime.upload(poison(BF16, (new, 1, 128))), runtime.upload(np.full((new, 1), np.nan, np.float32))
+    step.attention(q, out, lse, q_strides=(128, 0), out_strides=(128, 0))
+    runtime.synchronize()
+    s.compare(runtime.download(out, np.uint16, (new, 1, 128)).view(BF16), runtime.download(lse, np.float32, (new, 1)), *s.expected())
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_key_heads_that_are_the_same(new):
+    """A head stride of 0: all key heads read one."""
+    from limn_b200.paged import PagedBatch, PagedCache
+
+    s = Scene([(new, 300), (1, 40)], heads=4, kv_heads=1, hd=64, page_size=16, seed=31).upload()
+    want, _ = s.check()
+    cache = PagedCache(s.k_dev, s.v_dev, dtype="bfloat16", pages=s.pages, page_size=16, kv_heads=2, hd=64, k_strides=(1024, 0, 64), v_strides=(1024, 0, 64))
+    s.step = PagedBatch(cache, heads=4, batch=2, tokens=s.tokens, max_t_q=new, page_table=s.table_dev, max_pages=s.max_pages, q_start=s.q_start_dev, kv_lens=s.kv_lens_dev)
+    s.check()
+
+
+def test_layers_share_a_workspace():
+    """Calls that follow one another on a stream: batches over the caches of two layers, one workspace; and one that is too small."""
+    from limn_b200.paged import PagedBatch
+
+    first = Scene([(1, 900), (40, 300)], heads=8, kv_heads=2, hd=64, seed=32).upload()
+    second = Scene([(1, 900), (40, 300)], heads=8, kv_heads=2, hd=64, seed=33).upload()
+    more = dict(heads=8, batch=2, tokens=41, max_t_q=40, max_pages=second.max_pages, page_table=second.table_dev, q_start=second.q_start_dev, kv_lens=second.kv_lens_dev)
+    second.step = PagedBatch(second.step._held[0], workspace=first.step.workspace, **more)
+    for _ in range(2):
+        first.check()
+        second.check()
+    with pytest.raises(ValueError, match="workspace"):
+        PagedBatch(second.step._held[0], workspace=first.errors, **more)
+
+
 def test_launches_and_workspace():
     import ctypes
 
