@@ -8,6 +8,9 @@
 //
 // The angle p * f is taken as a number of turns in float64 and only its fraction goes to float32: at position 10^6 a float32
 // product would be off by 0.06 radians, this is off by 2 pi 2^-25. The turn is float32, rounded once to 16 bits.
+//
+// Measured: 24 600 tokens of 32 + 8 + 8 rows of 128 (605 MB) 95 us, 6.3 TB/s, 97 % of a plain copy's rate; 600 tokens of 36 rows of 80 5.2 us and one token 3.9 us,
+// of which some 3 us are the launch and the chain of dependent loads: offsets, length, table, rows.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -178,8 +181,11 @@ int launch_append(AppendParams& prm, int pairing, cudaStream_t stream) {
   auto kernel = neighbours ? kv_append_kernel<kFp16, 8, true> : (unit == 8 ? kv_append_kernel<kFp16, 8, false> : kv_append_kernel<kFp16, 4, false>);
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
+  // Eight warps to a token, fewer from where the grid has eight warps to a multiprocessor without. Few tokens wait for a token's rows one after the other, many gain
+  // nothing from more warps that each look up the token's place. One : up to eight : eight for all, in us, 32 heads over 8 key heads of 128: 64 tokens 6.3 : 4.7 :
+  // 4.7, 600 6.7 : 6.7 : 9.4, 5000 28.8 : 28.8 : 66; by up to 32 warps to a multiprocessor 1000 tokens took 9.9 where this takes 6.6.
   prm.warps_log = 3;
-  while (prm.warps_log > 0 && (static_cast<long long>(prm.tokens) << prm.warps_log) > 32LL * sms) --prm.warps_log;
+  while (prm.warps_log > 0 && (static_cast<long long>(prm.tokens) << prm.warps_log) > 8LL * sms) --prm.warps_log;
   const long long blocks = ((static_cast<long long>(prm.tokens) << prm.warps_log) + kWarps - 1) / kWarps;
   LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, prm), "launching the append kernel");
   note_launches(1);

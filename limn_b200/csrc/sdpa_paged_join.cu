@@ -1,6 +1,6 @@
 // What workers of a paged pass left of problems that they shared, put together; and the rows of two passes, over a prefix and over a
 // sequence's own keys. Sums of up to 148 parts, 512 bytes a row and part at most: bound by the latency of the loads, which are made four
-// at a time. The order is fixed, so two runs give the same bits.
+// at a time. The order is fixed, so two runs give the same bits. Joining 148 warps' parts of 256 rows takes 3 to 6 us, those of a long prompt's 148 x 256 rows 8.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -145,10 +145,11 @@ int launch_finish_s(const Pass& front, const Pass& own, cudaStream_t stream) {
   return LIMN_B200_OK;
 }
 
-// Few rows have many parts each, and wait for them; many rows have few.
+// Few rows have many parts each, and wait for them; many rows have few. Behind 8192 keys, four warps to a row : one, in us: 512 rows 33.5 : 39.5 (behind 20000), 2048
+// 52.5 : 53.5, 4096 77.7 : 72.3, 8192 125 : 112.
 template <int D, bool kFp16>
 int launch_finish(const Pass& front, const Pass& own, cudaStream_t stream) {
-  if (static_cast<long long>(own.tokens) * own.heads <= 4096) return launch_finish_s<D, kFp16, 4>(front, own, stream);
+  if (static_cast<long long>(own.tokens) * own.heads <= 2048) return launch_finish_s<D, kFp16, 4>(front, own, stream);
   return launch_finish_s<D, kFp16, 1>(front, own, stream);
 }
 

@@ -20,6 +20,10 @@
 // are zeroed before the product that reads them, since 0 * NaN would reach every row. (Boxes outside the cache, which TMA fills with zeros,
 // would do too: pages that are none are fetched so.)
 //
+// Measured, 32 heads over 8 of 128, bf16: a prompt of 8192 tokens 468 us, 1170 TFLOP/s, 71 % of the measured matrix rate and level with the dense forward: softmax and tensor
+// pipe in turn (the tensor pipe is active 55 % of the time). Eight pieces of 1 to 1000 tokens behind up to 7000 keys 219 us, 960 TFLOP/s: 13 us until the first
+// scores of a launch, items that their rows fill in part, parts. 16 questions of 20 to 150 tokens, 32 heads over 4, behind 4113 keys 117 us, 810 TFLOP/s.
+//
 // Warp roles (10 warps): 0-3 softmax and epilogue of tile 0, 4-7 of tile 1, 8 TMA producer, 9 MMA issuer and tensor-memory owner.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -37,7 +41,7 @@ constexpr int kTile = kPagedTile;  // rows of a tile, keys of a key tile
 static_assert(kTile == 128);
 constexpr int kThreads = 320;
 // What a step of an item with one tile costs, in keys. It computes as much as a step with two, a key tile of 128 each, but loads two key tiles to that one's one, which
-// no copy further ahead hides: by 176 prompt_pieces takes 219 us, by 128 (the arithmetic alone) 274, by 240 222. Pages of 8 make the producer issue twice
+// no copy further ahead hides: by 176 the eight pieces above take 219 us, by 128 (the arithmetic alone) 274, by 240 222. Pages of 8 make the producer issue twice
 // the boxes, and that bounds it: 224 takes 222 us where 176 takes 243.
 __device__ __forceinline__ int paged_single_step(int chunk_log) { return chunk_log == 3 ? 224 : 176; }
 constexpr int kProducerWarp = 8;
@@ -49,7 +53,8 @@ constexpr int kLeast = 256;  // cost of the smallest share: about that of the sm
 
 // kPacked: how a tile of K or V lies in shared memory at head dim 128. Column block after column block (64 columns of all 128 rows each), a box
 // of TMA fetches 64 columns of a run of keys; packed, the two column blocks of 8 rows lie side by side, and a box fetches all columns of the
-// run. A box costs the producer about 100 clocks to issue, whatever it holds, and a key tile of pages of 16 is 32 boxes or 16.
+// run. A box costs the producer about 100 clocks to issue, whatever it holds, and a key tile of pages of 16 is 32 boxes or 16: the eight pieces above 235 us and 220, with pages
+// of 8 286 and 219, with pages of 64 no difference.
 template <int D, bool kPacked>
 struct Layout {
   static constexpr int kTileBytes = kTile * D * 2;
