@@ -233,6 +233,7 @@ int limn_b200_kv_append(const limn_b200_paged* step, const void* q, const void* 
 
 /* Attention of the step's tokens over their sequences' pages (what limn_b200_kv_append has put there included).
  *   q (tokens, heads, hd), out (tokens, heads, hd_v), lse (tokens, heads) float32, dense; strides: (token, head) pairs of q, out.
+ *   out and lse overlap no operand. scale is from 1e-30 to 1e30. The same call gives the same bits; a row's last bits may depend on what else is in the batch.
  *   causal: token i sees the keys up to its own; otherwise all of its sequence's. A row that sees no key gets NaN and
  *   lse = -inf. Keys and values that a row does not see but another row of its sequence in this step does count as 0 * v in its sum, as
  *   everywhere in 16 bits here: an infinity among them gives NaN. Empty slots may hold anything.

@@ -83,7 +83,7 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   if (!countable(step, prefix_len)) return fail(LIMN_B200_UNSUPPORTED, "%s: %d sequences behind a prefix of %d keys are more work than a call counts", name, step->batch, prefix_len);
   for (int i = 0; i < 4; ++i)
     if (strides[i] < 0 || (strides[i] & 7)) return fail(LIMN_B200_BAD_ARGUMENT, "%s: strides must be non-negative multiples of 8 elements, got %lld", name, strides[i]);
-  if (!(scale > 0.0) || scale > 1e30) return fail(LIMN_B200_UNSUPPORTED, "%s: the scale must be positive and finite", name);
+  if (!(scale >= 1e-30 && scale <= 1e30)) return fail(LIMN_B200_UNSUPPORTED, "%s: the scale must be positive, from 1e-30 to 1e30", name);
   if (step->tokens == 0 || step->batch == 0) return LIMN_B200_OK;
   Workspace w;
   if (int rc = workspace_of(step, prefix_len, &w)) return rc;
@@ -144,6 +144,7 @@ int check_paged(const char* name, const limn_b200_paged* s) {
   if (s->page_size % 8 != 0) return fail(LIMN_B200_UNSUPPORTED, "%s: the page size must be a multiple of 8, got %d", name, s->page_size);
   if (s->heads / s->kv_heads > 128) return fail(LIMN_B200_UNSUPPORTED, "%s: %d query heads to a key head, at most 128 are served", name, s->heads / s->kv_heads);
   if (static_cast<long long>(s->tokens) * s->heads > kMaxKeys) return fail(LIMN_B200_UNSUPPORTED, "%s: %d tokens of %d heads do not fit 31 bits", name, s->tokens, s->heads);
+  if (s->batch > kMaxKeys) return fail(LIMN_B200_UNSUPPORTED, "%s: %d sequences do not fit 31 bits", name, s->batch);
   if (static_cast<long long>(s->max_pages) * s->page_size > kMaxKeys - s->first_position)
     return fail(LIMN_B200_UNSUPPORTED, "%s: positions of %d pages of %d from %d on do not fit 31 bits", name, s->max_pages, s->page_size, s->first_position);
   if (!countable(s, static_cast<double>(s->max_pages) * s->page_size))

@@ -49,6 +49,7 @@ REFUSED = [
     (2, "31 bits", {"max_pages": 1 << 27, "page_size": 16}),
     (2, "31 bits", {"max_pages": 4, "first_position": 0x7FFFFFF0}),
     (2, "31 bits", {"tokens": 1 << 28, "heads": 16}),
+    (2, "31 bits", {"batch": 0x7FFFFFFF}),
     (2, "counts", {"batch": 1 << 20, "tokens": 1 << 20, "heads": 128, "kv_heads": 128, "max_pages": 1 << 20}),
     (1, "strides", {"k_strides": triple(2048, 60, 128)}),
     (1, "strides", {"v_strides": triple(-2048, 64, 128)}),
@@ -111,7 +112,7 @@ def test_calls_that_cannot_be():
     attend = lambda *, q=ONE, out=ONE, lse=ONE, strides=pairs, scale=0.125: L.limn_b200_sdpa_paged(s, q, out, lse, strides, 1, scale, ONE, 1 << 40, None)  # noqa: E731
     for code, words, other in ((1, "null", {"q": None}), (1, "null", {"out": None}), (1, "null", {"lse": None}), (1, "null", {"strides": None}), (1, "aligned", {"q": ONE + 8}),
                                (1, "aligned", {"out": ONE + 2}), (1, "aligned", {"lse": ONE + 2}), (2, "scale", {"scale": 0.0}), (2, "scale", {"scale": -0.1}), (2, "scale", {"scale": float("nan")}),
-                               (2, "scale", {"scale": float("inf")}), (1, "strides", {"strides": (ctypes.c_longlong * 4)(256, 64, 256, 4)})):
+                               (2, "scale", {"scale": float("inf")}), (2, "scale", {"scale": 1e-46}), (1, "strides", {"strides": (ctypes.c_longlong * 4)(256, 64, 256, 4)})):
         assert attend(**other) == code and words in last_error(), (other, last_error())
     prefix = lambda table, length: L.limn_b200_sdpa_paged_prefix(s, ONE, ONE, ONE, pairs, table, length, 1, 0.125, ONE, 1 << 40, None)  # noqa: E731
     assert prefix(ONE + 2, 10) == 1 and "aligned" in last_error()

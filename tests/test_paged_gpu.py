@@ -670,6 +670,55 @@ def test_key_heads_that_are_the_same(new):
     s.check()
 
 
+@pytest.mark.parametrize("captured", [False, True], ids=["enqueued", "captured"])
+def test_calls_of_all_kinds_one_after_the_other_on_one_workspace(captured):
+    """Few rows and many, without a prefix, behind one that is read for each sequence and behind one that is read once, with nothing between them: each begins under the one in front
+    of it, and they have one workspace. Every result is, bit by bit, what the call gives alone."""
+    torch = pytest.importorskip("torch")
+    from limn_b200 import runtime
+    from limn_b200.paged import PagedBatch
+
+    new = {"few": [(1, 900), (2, 40), (1, 3000)], "many": [(90, 700), (1, 2000), (40, 60)]}
+    scenes = [Scene(new[kind] + idle, heads=8, kv_heads=2, hd=128, seed=40 + i, prefix=prefix).upload()
+              for i, (kind, prefix, idle) in enumerate([("few", 0, []), ("many", 0, []), ("few", 300, []), ("many", 300, IDLE), ("few", 300, IDLE), ("many", 300, [])])]
+    alone, calls = [], []
+    largest = max(scenes, key=lambda s: s.step.workspace_bytes).step.workspace
+    for s, kernels in zip(scenes, (2, 2, 2, 3, 3, 2), strict=True):
+        alone.append(s.check())
+        assert launches() == kernels
+        s.step = PagedBatch(s.step._held[0], heads=8, batch=len(s.seqs), tokens=s.tokens, max_t_q=s.max_t_q, page_table=s.table_dev, max_pages=s.max_pages,
+                            q_start=s.q_start_dev, kv_lens=s.kv_lens_dev, errors=s.errors, workspace=largest)
+        calls.append((runtime.upload(s.q), runtime.upload(poison(BF16, (2, s.tokens, 8, 128))), runtime.upload(np.full((2, s.tokens, 8), np.nan, np.float32))))
+
+    def all_of_them(stream):
+        for turn in range(2):
+            for s, (q, out, lse) in zip(scenes, calls, strict=True):
+                o, l = out.ptr + turn * s.tokens * 8 * 128 * 2, lse.ptr + turn * s.tokens * 8 * 4
+                if s.prefix:
+                    s.step.attention_with_prefix(q, o, l, prefix_table=s.prefix_dev, prefix_len=s.prefix, stream=stream)
+                else:
+                    s.step.attention(q, o, l, stream=stream)
+
+    runtime.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        if captured:
+            with torch.cuda.graph(graph, stream=side):
+                all_of_them(torch.cuda.current_stream().cuda_stream)
+            graph.replay()
+            graph.replay()
+        else:
+            all_of_them(side.cuda_stream)
+    side.synchronize()
+    for s, (_, out, lse), (want_o, want_l) in zip(scenes, calls, alone, strict=True):
+        have_o, have_l = runtime.download(out, np.uint16, (2, s.tokens, 8, 128)), runtime.download(lse, np.float32, (2, s.tokens, 8))
+        for turn in range(2):
+            assert np.array_equal(have_o[turn], want_o.view(np.uint16)) and np.array_equal(have_l[turn], want_l)
+    del graph
+    assert runtime.device_status() == 0
+
+
 def test_layers_share_a_workspace():
     """Calls that follow one another on a stream: batches over the caches of two layers, one workspace; and one that is too small."""
     from limn_b200.paged import PagedBatch
