@@ -1,6 +1,7 @@
 // What workers of a paged pass left of problems that they shared, put together; and the rows of two passes, over a prefix and over a
 // sequence's own keys. Sums of up to 148 parts, 512 bytes a row and part at most: bound by the latency of the loads, which are made four
-// at a time. The order is fixed, so two runs give the same bits. Joining 148 warps' parts of 256 rows takes 3 to 6 us, those of a long prompt's 148 x 256 rows 8.
+// at a time. The order is fixed, so two runs give the same bits. What a join adds to a call, the launch and what the
+// pass in front of it leaves in memory for it included: 2.4 us of a batch of few rows, 9 us of 148 x 256 rows of 128 columns (38 MB of parts).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -11,8 +12,9 @@ namespace {
 
 using namespace paged;
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 4;  // (small blocks find room beside a pass that is ending: 0.5 to 1 % of a call against 8)
 constexpr int kUnroll = 4;
+constexpr int kEach = 2;       // (one row 1 % slower, and four, which take 100 registers, 2 %)
 
 // The parts of a problem that begins with worker `w`, `by` of them at a time beginning with part `from`: part 0 is the head's, part i the i-th follower's.
 template <int D>
@@ -46,10 +48,9 @@ __device__ __forceinline__ void add_sides(Sums& sums, float sl2) {
   }
 }
 
-// A row of one problem: kSplit warps share its parts.
-template <int D, bool kFp16, int kSplit>
+// A row of one problem: the warps of a block share its parts.
+template <int D, bool kFp16>
 __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const Pass prm) {
-  constexpr int kRows = kJoinWarps / kSplit;
   constexpr int kLanes = D / 4;          // lanes to a row
   constexpr int kAtOnce = 32 / kLanes;   // parts a warp takes side by side
   __shared__ float4 all_sums[kJoinWarps][32];
@@ -59,23 +60,62 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
   const Head head = prm.parts.heads[blockIdx.x];
   if (head.followers == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.y * kRows + warp / kSplit, split = warp % kSplit;
-  const int column = (lane % kLanes) * 4, side = lane / kLanes;
+  const int r = blockIdx.y, column = (lane % kLanes) * 4, side = lane / kLanes;
   const float sl2 = prm.scale * kLog2e;
-  const int row = head.row0 + r / 128 * head.tile_rows + r % 128;
-  if (r % 128 >= head.tile_rows || row >= head.n * prm.group) return;  // (in the whole block, or without a barrier behind it)
+  const int row = head.row0 + r;  // (few rows: one tile)
+  if (r >= head.tile_rows || row >= head.n * prm.group) return;  // (the whole block)
   Sums sums;
-  add_parts<D>(sums, prm.parts, blockIdx.x, head.followers, r, column, split * kAtOnce + side, kSplit * kAtOnce, sl2);
+  add_parts<D>(sums, prm.parts, blockIdx.x, head.followers, r, column, warp * kAtOnce + side, kJoinWarps * kAtOnce, sl2);
   add_sides<D>(sums, sl2);
-  if (kSplit > 1) {
-    all_sums[warp][lane] = sums.acc;
-    if (lane == 0) all_stats[warp] = make_float2(sums.m, sums.l);
-    __syncthreads();
-    if (split > 0) return;
+  all_sums[warp][lane] = sums.acc;
+  if (lane == 0) all_stats[warp] = make_float2(sums.m, sums.l);
+  __syncthreads();
+  if (warp > 0) return;
 #pragma unroll 1
-    for (int i = 1; i < kSplit; ++i) sums.add(all_stats[warp + i].x, all_stats[warp + i].y, all_sums[warp + i][lane], sl2);
-  }
+  for (int i = 1; i < kJoinWarps; ++i) sums.add(all_stats[i].x, all_stats[i].y, all_sums[i][lane], sl2);
   if (side == 0) store4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row), column, sums.acc, sums.m, sums.l);
+}
+
+// Many rows of one problem, which few workers share: D / 4 lanes to a row, kEach rows one behind the other whose parts are asked for together.
+template <int D, bool kFp16>
+__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_rows_kernel(const Pass prm) {
+  constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kParts = 2;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const Head head = prm.parts.heads[blockIdx.x];
+  if (head.followers == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int column = (lane % kLanes) * 4, r0 = (blockIdx.y * kJoinWarps + warp) * kEach * kAtOnce + lane / kLanes;
+  const float sl2 = prm.scale * kLog2e;
+  auto row_at = [&](int r) { return head.row0 + r / 128 * head.tile_rows + r % 128; };
+  Sums sums[kEach];
+  bool there[kEach];
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int r = r0 + u * kAtOnce;
+    there[u] = r % 128 < head.tile_rows && row_at(r) < head.n * prm.group;
+  }
+#pragma unroll 1
+  for (int i0 = 0; i0 <= head.followers; i0 += kParts) {
+    float2 ml[kEach][kParts];
+    float4 o[kEach][kParts];
+#pragma unroll
+    for (int u = 0; u < kEach; ++u)
+#pragma unroll
+      for (int v = 0; v < kParts; ++v) {
+        const int i = i0 + v;
+        const long long part = (i == 0 ? 2LL * blockIdx.x + 1 : 2LL * (blockIdx.x + i)) * prm.parts.rows + r0 + u * kAtOnce;
+        ml[u][v] = make_float2(-INFINITY, 0.f), o[u][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (there[u] && i <= head.followers) ml[u][v] = prm.parts.ml[part], o[u][v] = *reinterpret_cast<const float4*>(prm.parts.o + part * D + column);
+      }
+#pragma unroll
+    for (int u = 0; u < kEach; ++u)
+#pragma unroll
+      for (int v = 0; v < kParts; ++v) sums[u].add(ml[u][v].x, ml[u][v].y, o[u][v], sl2);
+  }
+#pragma unroll
+  for (int u = 0; u < kEach; ++u)
+    if (there[u]) store4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row_at(r0 + u * kAtOnce)), column, sums[u].acc, sums[u].m, sums[u].l);
 }
 
 // A (token, head) row to kSplit warps: what both passes left of it, of a sequence that is one. Rows of tokens that belong to none are left alone; all of
@@ -125,11 +165,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_finish_kernel(cons
   if (side == 0) store4<D, kFp16>(own, RowPlace{row, own.out + token * own.o_token + head * own.o_head}, column, sums.acc, sums.m, sums.l);
 }
 
-template <int D, bool kFp16, int kSplit>
-int launch_join(const Pass& pass, cudaStream_t stream) {
-  const unsigned rows = static_cast<unsigned>((pass.parts.rows * kSplit + kJoinWarps - 1) / kJoinWarps);
-  LIMN_CUDA(launch_overlapped(sdpa_paged_join_kernel<D, kFp16, kSplit>, dim3(static_cast<unsigned>(pass.parts.workers), rows), dim3(kJoinWarps * 32), 0, stream, pass),
-            "launching the kernel that joins parts");
+template <int D, bool kFp16>
+int launch_join(const Pass& pass, bool many_rows, cudaStream_t stream) {
+  constexpr int kRows = kJoinWarps * kEach * (128 / D);  // rows to a block of the kernel for many
+  const unsigned blocks = static_cast<unsigned>(many_rows ? pass.parts.rows / kRows : pass.parts.rows);
+  auto kernel = many_rows ? sdpa_paged_join_rows_kernel<D, kFp16> : sdpa_paged_join_kernel<D, kFp16>;
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers), blocks), dim3(kJoinWarps * 32), 0, stream, pass), "launching the kernel that joins parts");
   note_launches(1);
   return LIMN_B200_OK;
 }
@@ -155,13 +196,9 @@ int launch_finish(const Pass& front, const Pass& own, cudaStream_t stream) {
 
 }  // namespace
 
-int paged_join_launch(const Pass& pass, bool fp16, bool warp_a_row, cudaStream_t stream) {
-  if (warp_a_row) {
-    if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 1>(pass, stream) : launch_join<64, false, 1>(pass, stream);
-    return fp16 ? launch_join<128, true, 1>(pass, stream) : launch_join<128, false, 1>(pass, stream);
-  }
-  if (pass.parts.width == 64) return fp16 ? launch_join<64, true, 8>(pass, stream) : launch_join<64, false, 8>(pass, stream);
-  return fp16 ? launch_join<128, true, 8>(pass, stream) : launch_join<128, false, 8>(pass, stream);
+int paged_join_launch(const Pass& pass, bool fp16, bool many_rows, cudaStream_t stream) {
+  if (pass.parts.width == 64) return fp16 ? launch_join<64, true>(pass, many_rows, stream) : launch_join<64, false>(pass, many_rows, stream);
+  return fp16 ? launch_join<128, true>(pass, many_rows, stream) : launch_join<128, false>(pass, many_rows, stream);
 }
 
 int paged_finish_launch(const Pass& front, const Pass& own, bool fp16, cudaStream_t stream) {
