@@ -107,16 +107,48 @@ template <int D, bool kFp16, int NT>
 __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass prm, const Parts by_warp) {
   using R = Ring<D>;
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ long long share_end[kThreads];  // cost of the sequences up to and with a thread's, per key head
   __shared__ Shared shared[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float sl2 = prm.scale * kLog2e;
   const bool known = prm.q_start == nullptr;  // one sequence of a known length: the shares need no memory
   if (!prm.beside && !known) ptx::grid_dependency_wait();
 
-  // ---- the shares: every thread adds up its run of sequences, the block adds up the threads ----
-  const int run = (prm.batch + kThreads - 1) / kThreads;
-  {
+  // ---- the shares ----
+  const int worker = blockIdx.x * kWarps + warp;
+  if (lane == 0) shared[warp].enters = shared[warp].begins = 0;
+  Cursor at = {};
+  long long share, from, to;
+  int span;
+  auto share_out = [&](long long total) {
+    share = by_warp.share_of(total);
+    from = min(total, worker * share), to = min(total, from + share);
+    span = static_cast<int>(to - from);
+  };
+  auto begin_at = [&](long long rest, int cost) {
+    at.kv_head = small_quotient(rest, cost);
+    const int into = static_cast<int>(rest - static_cast<long long>(at.kv_head) * cost);
+    at.unit = max(0, into - kBegin), at.cost = max(0, kBegin - into);
+  };
+  if (prm.batch <= 32) {
+    // a lane has a sequence, and every warp adds them up for itself
+    const Extent e = lane < prm.batch ? extent_of(prm, lane) : Extent{0, 0, 0};
+    long long upto = cost_of(e);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += other;
+    }
+    share_out(__shfl_sync(0xffffffffu, upto, 31) * prm.kv_heads);
+    if (span > 0) {
+      at.b = __popc(__ballot_sync(0xffffffffu, upto * prm.kv_heads <= from));  // (below 32: `from` is below the total)
+      at.e = Extent{__shfl_sync(0xffffffffu, e.first, at.b), __shfl_sync(0xffffffffu, e.n, at.b), __shfl_sync(0xffffffffu, e.keys, at.b)};
+      at.units = units_of(at.e);
+      const int cost = cost_of(at.e);
+      begin_at(from - (__shfl_sync(0xffffffffu, upto, at.b) - cost) * prm.kv_heads, cost);
+    }
+  } else {
+    // every thread adds up its run of sequences, the block adds up the threads
+    const int run = (prm.batch + kThreads - 1) / kThreads;
     long long mine = 0;
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
@@ -128,36 +160,28 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       const long long other = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += other;
     }
+    __shared__ long long share_end[kThreads];  // cost of the sequences up to and with a thread's, per key head
     __shared__ long long warp_sum[kWarps];
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
     for (int w = 0; w < warp; ++w) upto += warp_sum[w];
     share_end[threadIdx.x] = upto;
     __syncthreads();
-  }
-  const int worker = blockIdx.x * kWarps + warp;
-  const long long total = share_end[kThreads - 1] * prm.kv_heads;
-  const long long share = by_warp.share_of(total);
-  const long long from = min(total, worker * share), to = min(total, from + share);
-  const int span = static_cast<int>(to - from);
-  if (lane == 0) shared[warp].enters = shared[warp].begins = 0;
-
-  Cursor at = {};
-  if (span > 0) {
-    const int before = first_above(share_end, kThreads, prm.kv_heads, from);  // the run of sequences that `from` falls into
-    long long rest = from - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
-    at.b = before * run - 1;
-    int cost;
-    do {
-      ++at.b;
-      at.e = extent_of(prm, at.b);
-      at.units = units_of(at.e), cost = cost_of(at.e);
-      if (rest < static_cast<long long>(cost) * prm.kv_heads) break;
-      rest -= static_cast<long long>(cost) * prm.kv_heads;
-    } while (at.b + 1 < prm.batch);
-    at.kv_head = small_quotient(rest, cost);
-    const int into = static_cast<int>(rest - static_cast<long long>(at.kv_head) * cost);
-    at.unit = max(0, into - kBegin), at.cost = max(0, kBegin - into);
+    share_out(share_end[kThreads - 1] * prm.kv_heads);
+    if (span > 0) {
+      const int before = first_above(share_end, kThreads, prm.kv_heads, from);  // the run of sequences that `from` falls into
+      long long rest = from - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
+      at.b = before * run - 1;
+      int cost;
+      do {
+        ++at.b;
+        at.e = extent_of(prm, at.b);
+        at.units = units_of(at.e), cost = cost_of(at.e);
+        if (rest < static_cast<long long>(cost) * prm.kv_heads) break;
+        rest -= static_cast<long long>(cost) * prm.kv_heads;
+      } while (at.b + 1 < prm.batch);
+      begin_at(rest, cost);
+    }
   }
 
   if (!prm.beside && known) ptx::grid_dependency_wait();
