@@ -130,7 +130,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
     at.unit = max(0, into - kBegin), at.cost = max(0, kBegin - into);
   };
   if (prm.batch <= 32) {
-    // a lane has a sequence, and every warp adds them up for itself
+    // a lane has a sequence, and every warp adds them up for itself, without barriers or reading an extent again: eight sequences of 2000 keys 13.6 us, by the block 14.6. (Up to 128,
+    // four to a lane: 0 to 0.4 us slower than this up to 32, and no faster than the block beyond)
     const Extent e = lane < prm.batch ? extent_of(prm, lane) : Extent{0, 0, 0};
     long long upto = cost_of(e);
 #pragma unroll
