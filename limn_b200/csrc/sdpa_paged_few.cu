@@ -17,7 +17,7 @@
 //
 // Measured: 64 sequences of 500 to 8191 keys, 32 heads over 8 of 128 (1.12 GB) 180 us, 6.2 TB/s, 95 % of a plain copy's rate; two of 131 000 keys (0.95 GB) 155 us, 6.1
 // TB/s; 24 of 3000 keys and 1 to 5 tokens, 12 heads of 80 (139 MB) 37 us, 3.7 TB/s: the copies' 16-byte pieces fill 10 lanes of 16 and the beginning
-// weighs; one of 2000 keys, 8 heads of 64 (4 MB) 10 us with the join, nearly all of it beginnings: code fetched for the first time, some 50 clocks a line, and
+// weighs; one of 2000 keys, 8 heads of 64 (4 MB) 9 us with the join, nearly all of it beginnings: code fetched for the first time, some 50 clocks a line, and
 // four loads that hang on one another before the first key arrives.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -297,7 +297,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
       __syncwarp();
     }
     issue();
-    if (step < 0) continue;
+    if (step < 0) {
+      if (ahead.cost >= span) {  // no more to copy: the places left stay empty (the turns that would say so one by one are 0.4 us of a call of few keys)
+        for (; step < -1; ++step) copies_commit();
+      }
+      continue;
+    }
     const int place_at = step % R::kStages;
     const uint32_t k_at = mine + place_at * 2 * R::kSide, v_at = k_at + R::kSide;
     float s[NT][4];
