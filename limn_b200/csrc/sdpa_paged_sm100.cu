@@ -696,14 +696,20 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         const float m_1 = *const_cast<volatile float*>(&merge_m[row_in_tile]), l_1 = *const_cast<volatile float*>(&merge_l[row_in_tile]);
         merge_stats(m, l, m_1, l_1, sl2, keep, from_1);
       }
-      auto take = [&](int col, uint32_t (&o)[32]) {
-        tmem_ld32(t_o + col, o);
+      // kTogether times 32 columns of the row. (All 64 of a head: 191 us where 32 at a time take 194; 64 of 128, with more code than 32: no gain)
+      constexpr int kTogether = D == 64 ? 2 : 1;
+      auto take = [&](int col, uint32_t (&o)[kTogether][32]) {
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) tmem_ld32(t_o + col + 32 * k, o[k]);
         if (both) {
-          uint32_t o_1[32];
-          tmem_ld32(t_o + D + col, o_1);
+          uint32_t o_1[kTogether][32];
+#pragma unroll
+          for (int k = 0; k < kTogether; ++k) tmem_ld32(t_o + D + col + 32 * k, o_1[k]);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep + __uint_as_float(o_1[i]) * from_1);
+          for (int k = 0; k < kTogether; ++k)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[k][i] = __float_as_uint(__uint_as_float(o[k][i]) * keep + __uint_as_float(o_1[k][i]) * from_1);
         } else {
           tmem_ld_wait();
         }
@@ -720,19 +726,23 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           to_row[i] = at == 0ull ? nullptr : reinterpret_cast<unsigned char*>(at) + 16 * (lane & 3);
         }
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          take(32 * c, o);
-          uint32_t w[4][4];
+        for (int c0 = 0; c0 < D / 32; c0 += kTogether) {
+          uint32_t o[kTogether][32];
+          take(32 * c0, o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
-            w[i / 4][i % 4] = kFp16 ? pack_f16(a, b) : pack_bf16(a, b);
+          for (int k = 0; k < kTogether; ++k) {
+            const int c = c0 + k;
+            uint32_t w[4][4];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float a = __uint_as_float(o[k][2 * i]) * inv, b = __uint_as_float(o[k][2 * i + 1]) * inv;
+              w[i / 4][i % 4] = kFp16 ? pack_f16(a, b) : pack_bf16(a, b);
+            }
+            swap_rows_for_pieces<4>(w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (to_row[i] != nullptr && 4 * c + (lane & 3) < prm.pieces_v) *reinterpret_cast<uint4*>(to_row[i] + 64 * c) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
           }
-          swap_rows_for_pieces<4>(w);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (to_row[i] != nullptr && 4 * c + (lane & 3) < prm.pieces_v) *reinterpret_cast<uint4*>(to_row[i] + 64 * c) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
         }
         if (there) prm.lse[place.row] = m * prm.scale + logf(l);
       } else {
@@ -740,23 +750,23 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         // bytes of each row it touches; rows that there are not go along. To the rows' sums every thread writes its own row
         float* to = s.whole ? prm.leave.o + place.row * D : prm.parts.o + (part - lane + (lane & ~3)) * D + 4 * (lane & 3);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          take(32 * c, o);
+        for (int c0 = 0; c0 < D / 32; c0 += kTogether) {
+          uint32_t o[kTogether][32];
+          take(32 * c0, o);
           if (s.whole) {
             if (there) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 32 * kTogether; i += 4) *reinterpret_cast<uint4*>(to + 32 * c0 + i) = make_uint4(o[i / 32][i % 32], o[i / 32][i % 32 + 1], o[i / 32][i % 32 + 2], o[i / 32][i % 32 + 3]);
             }
           } else {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < 2 * kTogether; ++half) {
               uint32_t w[4][4];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i / 4][i % 4] = o[16 * half + i];
+              for (int i = 0; i < 16; ++i) w[i / 4][i % 4] = o[half / 2][16 * (half % 2) + i];
               swap_rows_for_pieces<4>(w);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(to + i * D + 32 * c + 16 * half) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(to + i * D + 32 * c0 + 16 * half) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
             }
           }
         }
