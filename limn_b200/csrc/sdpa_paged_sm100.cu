@@ -24,7 +24,7 @@
 // pipe in turn (the tensor pipe is active 55 % of the time). Eight pieces of 1 to 1000 tokens behind up to 7000 keys 219 us, 960 TFLOP/s: 13 us until the first
 // scores of a launch, items that their rows fill in part, parts. 16 questions of 20 to 150 tokens, 32 heads over 4, behind 4113 keys 117 us, 810 TFLOP/s.
 //
-// Warp roles (10 warps): 0-3 softmax and epilogue of tile 0, 4-7 of tile 1, 8 TMA producer, 9 MMA issuer and tensor-memory owner.
+// Warp roles (12 warps): 0-3 softmax and epilogue of tile 0, 4-7 of tile 1, 8 TMA producer, 9 MMA issuer and tensor-memory owner; 10 and 11 have gone home.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -39,7 +39,12 @@ using namespace paged;
 
 constexpr int kTile = kPagedTile;  // rows of a tile, keys of a key tile
 static_assert(kTile == 128);
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+// A launch gets 168 registers a thread, here three groups of four warps; the softmax threads hold a row of 128 scores and take 40 more each from the third group, whose
+// last two warps have nothing to do. Without that (10 warps, 148 bytes of them spilled) an 8192-token prompt takes 467 us, with it 448, with 184 for the softmax 465; at head
+// dim 64 pieces of prompts 190, 175 and 184.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * 128 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168);
 // What a step of an item with one tile costs, in keys. It computes as much as a step with two, a key tile of 128 each, but loads two key tiles to that one's one, which
 // no copy further ahead hides: by 176 the eight pieces above take 219 us, by 128 (the arithmetic alone) 274, by 240 222. Pages of 8 make the producer issue twice
 // the boxes, and that bounds it: 224 takes 222 us where 176 takes 243.
@@ -293,261 +298,265 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     return true;
   };
 
-  if (warp == kProducerWarp) {
-    // ================= the share, and TMA =================
-    const bool any = ok && from < total;
-    auto of_half = [&](int from_lane) {
-      auto word = [&](int x) { return __shfl_sync(0xffffffffu, x, from_lane); };
-      return Place{word(p.b), word(p.kv_head), word(p.j), word(p.step), Extent{word(p.e.first), word(p.e.n), word(p.e.keys)}, __shfl_sync(0xffffffffu, p.into, from_lane)};
-    };
-    Place at = of_half(0), end = of_half(16);
-    if (to >= total) end.b = prm.batch, end.kv_head = end.j = 0;  // nothing ends it
-    unsigned n_item = 0, q_uses[2] = {0u, 0u}, step = 0;
-    bool more = any;
-    // a lane fetches one box of a key tile: `chunk` keys of one page, 64 columns
-    const int chunks = kTile >> chunk_log;
-    const int my_chunk = lane & (chunks - 1), my_atom = (lane << chunk_log) / kTile;
-    constexpr int kBoxAtoms = kPacked ? 1 : D / 64;  // boxes to a chunk
-    while (more && ok) {
-      const Costs costs(at.e, by_span, prm, chunk_log);
-      const bool last = at.b == end.b && at.kv_head == end.kv_head && at.j == end.j;
-      const int steps = costs.steps(at.j), until = last ? end.step : steps;
-      if (until > at.step) {
-        Segment s;
-        const bool single = costs.single(at.j);
-        const int tiles = tiles_of(costs.seen((at.j + 1) * costs.span));  // key tiles of the item
-        s.valid = 1, s.b = at.b, s.first = at.e.first, s.n = at.e.n, s.keys = at.e.keys, s.kv_head = at.kv_head;
-        s.row0 = at.j * 2 * tile_rows;
-        s.begun = at.step == 0, s.whole = at.step == 0 && until == steps;
-        if (single) {
-          s.first_tile = 2 * at.step;
-          s.loads = min(2 * until, tiles) - s.first_tile;
-          s.both = s.loads > 1;
-          s.count[1] = s.loads / 2, s.count[0] = s.loads - s.count[1];
-        } else {
-          s.first_tile = at.step;
-          const int tiles_0 = tiles_of(costs.seen(at.j * costs.span + costs.half));
-          s.count[0] = max(0, min(until, tiles_0) - at.step);
-          s.count[1] = until - at.step;
-          s.loads = s.count[1], s.both = 0;
-        }
-        const unsigned slot = n_item & 1u;
-        ok = wait(B::work_empty + slot, ((n_item >> 1) & 1u) ^ 1u, 0x0120u | slot);
-        if (!ok) break;
-        if (lane == 0) {
-          ring[slot] = s;
-          mbar_arrive(bar(B::work_full + slot));
-        }
-        __syncwarp();
-        ++n_item;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (s.count[t] == 0) continue;
-          ok = wait(B::q_empty + t, (q_uses[t] & 1u) ^ 1u, 0x0130u | t);
+  if (warp >= kProducerWarp) {
+    registers_down<kOtherRegs>();
+    if (warp == kProducerWarp) {
+      // ================= the share, and TMA =================
+      const bool any = ok && from < total;
+      auto of_half = [&](int from_lane) {
+        auto word = [&](int x) { return __shfl_sync(0xffffffffu, x, from_lane); };
+        return Place{word(p.b), word(p.kv_head), word(p.j), word(p.step), Extent{word(p.e.first), word(p.e.n), word(p.e.keys)}, __shfl_sync(0xffffffffu, p.into, from_lane)};
+      };
+      Place at = of_half(0), end = of_half(16);
+      if (to >= total) end.b = prm.batch, end.kv_head = end.j = 0;  // nothing ends it
+      unsigned n_item = 0, q_uses[2] = {0u, 0u}, step = 0;
+      bool more = any;
+      // a lane fetches one box of a key tile: `chunk` keys of one page, 64 columns
+      const int chunks = kTile >> chunk_log;
+      const int my_chunk = lane & (chunks - 1), my_atom = (lane << chunk_log) / kTile;
+      constexpr int kBoxAtoms = kPacked ? 1 : D / 64;  // boxes to a chunk
+      while (more && ok) {
+        const Costs costs(at.e, by_span, prm, chunk_log);
+        const bool last = at.b == end.b && at.kv_head == end.kv_head && at.j == end.j;
+        const int steps = costs.steps(at.j), until = last ? end.step : steps;
+        if (until > at.step) {
+          Segment s;
+          const bool single = costs.single(at.j);
+          const int tiles = tiles_of(costs.seen((at.j + 1) * costs.span));  // key tiles of the item
+          s.valid = 1, s.b = at.b, s.first = at.e.first, s.n = at.e.n, s.keys = at.e.keys, s.kv_head = at.kv_head;
+          s.row0 = at.j * 2 * tile_rows;
+          s.begun = at.step == 0, s.whole = at.step == 0 && until == steps;
+          if (single) {
+            s.first_tile = 2 * at.step;
+            s.loads = min(2 * until, tiles) - s.first_tile;
+            s.both = s.loads > 1;
+            s.count[1] = s.loads / 2, s.count[0] = s.loads - s.count[1];
+          } else {
+            s.first_tile = at.step;
+            const int tiles_0 = tiles_of(costs.seen(at.j * costs.span + costs.half));
+            s.count[0] = max(0, min(until, tiles_0) - at.step);
+            s.count[1] = until - at.step;
+            s.loads = s.count[1], s.both = 0;
+          }
+          const unsigned slot = n_item & 1u;
+          ok = wait(B::work_empty + slot, ((n_item >> 1) & 1u) ^ 1u, 0x0120u | slot);
           if (!ok) break;
-          ++q_uses[t];
           if (lane == 0) {
-            mbar_expect_tx(bar(B::q_full + t), static_cast<uint32_t>(tile_rows) * D * 2);
-            const int token = s.first + (2 * at.j + (s.both ? 0 : t)) * tile_tokens;
-#pragma unroll
-            for (int a = 0; a < D / 64; ++a) tma_load_5d(base + L::kQOff + t * L::kTileBytes + a * L::kAtomBytes, &maps.q, bar(B::q_full + t), a * 64, s.kv_head * prm.group, token, 0, 0);
+            ring[slot] = s;
+            mbar_arrive(bar(B::work_full + slot));
           }
           __syncwarp();
-        }
-        if (!ok) break;
-        // the page of this lane's box of key tile `tile`; one that is none is a coordinate outside the cache, whose box TMA fills with zeros
-        auto entry = [&](int tile) {
-          const int key = tile * kTile + my_chunk * chunk;
-          return key < side_end(prm, key, s.keys) ? entry_for(prm, s.b, key) : 0;
-        };
-        int page_next[2] = {entry(s.first_tile), entry(s.first_tile + 1)};  // two tiles ahead
-#pragma unroll 1
-        for (int j = 0; j < s.loads && ok; ++j, ++step) {
-          const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
-          const int end = side_end(prm, key, s.keys);  // (the same for the whole tile)
-          const bool fetch = key < end && my_atom < kBoxAtoms;
-          const int page = fetch ? checked_page(page_next[0], prm.pages, prm.errors) : 0;
-          const int boxes = min(chunks, max(0, (end - tile * kTile + chunk - 1) >> chunk_log));  // those that have keys
-          const uint32_t bytes = static_cast<uint32_t>(boxes * chunk) * (D * 2);
-          page_next[0] = page_next[1], page_next[1] = entry(tile + 2);
-          const int in_page = slot_of(prm, key);
-          const int stage = step % B::kS;
-          const uint32_t wrap = (step / B::kS) & 1;
-          ok = wait(B::k_empty + stage, wrap ^ 1u, 0x0100u | stage);
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(bar(B::k_full + stage), bytes);
-          __syncwarp();
-          const uint32_t box = stage * L::kTileBytes + my_atom * L::kAtomBytes + my_chunk * (chunk / 8) * L::kKVGroup;
-          auto load = [&](uint32_t to, const CUtensorMap& map, int side, uint32_t full) {
-            if constexpr (kPacked) tma_load_5d(to, &map, full, 0, 0, side ? s.kv_head * (D / 64) : 0, in_page >> 3, side ? page : page * prm.kv_heads + s.kv_head);
-            else tma_load_5d(to, &map, full, my_atom * 64, in_page, s.kv_head, page, 0);
-          };
-          if (fetch) load(base + L::kKOff + box, maps.k, maps.k_side, bar(B::k_full + stage));
-          __syncwarp();
-          ok = wait(B::v_empty + stage, wrap ^ 1u, 0x0110u | stage);
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(bar(B::v_full + stage), bytes);
-          __syncwarp();
-          if (fetch) load(base + L::kVOff + box, maps.v, maps.v_side, bar(B::v_full + stage));
-          __syncwarp();
-        }
-        if (s.begun && !s.whole && lane == 0) {
-          // workers behind this one whose share begins inside the item, before the middle of its last step
-          const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(costs.step_cost(at.j)) - costs.step_cost(at.j) / 2);
-          prm.parts.heads[blockIdx.x] = Head{small_quotient(begins + limit - 1, share) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
-        }
-      }
-      // the next item
-      if (last) break;
-      at.step = 0;
-      if (++at.j < costs.pairs) continue;
-      at.j = 0;
-      if (++at.kv_head < prm.kv_heads) continue;
-      at.kv_head = 0;
-      do {
-        if (++at.b >= prm.batch) {
-          more = false;
-          break;
-        }
-        at.e = extent_of(prm, at.b);
-      } while (at.e.n == 0);
-    }
-    const unsigned slot = n_item & 1u;
-    if (ok) ok = wait(B::work_empty + slot, ((n_item >> 1) & 1u) ^ 1u, 0x0121u | slot);
-    if (ok && lane == 0) {
-      ring[slot].valid = 0;
-      mbar_arrive(bar(B::work_full + slot));
-    }
-  } else if (warp == kMmaWarp) {
-    // ================= MMA issuer =================
-    constexpr uint32_t idesc_s = mma_idesc(kTile, kTile, kFp16, false, false);
-    constexpr uint32_t idesc_pv = mma_idesc(kTile, D, kFp16, false, true);
-    auto issue_s = [&](int t, int stage) {
-      const uint32_t q_lo = desc_lo(base + L::kQOff + t * L::kTileBytes, 0);
-      const uint32_t k_lo = desc_lo(base + L::kKOff + stage * L::kTileBytes, 0);
-      const uint32_t c = tmem + L::kSCol + t * 128;
-      mma_ss_lo<false, desc_hi(L::kKVGroup)>(c, q_lo, k_lo, idesc_s);
+          ++n_item;
 #pragma unroll
-      for (int kk = 1; kk < D / 16; ++kk) {  // (offsets in 16-byte units)
-        mma_ss_lo<true, desc_hi(L::kKVGroup)>(c, q_lo + (kk / 4) * (L::kAtomBytes >> 4) + (kk % 4) * 2, k_lo + (kk / 4) * (L::kKVAtom >> 4) + (kk % 4) * 2, idesc_s);
-      }
-    };
-    auto issue_pv = [&](int t, int stage, int part, bool first) {
-      const uint32_t v_lo = desc_lo(base + L::kVOff + stage * L::kTileBytes, L::kKVAtom);
-      const uint32_t c = tmem + L::kOCol + t * D;
-      const uint32_t a = tmem + L::kSCol + t * 128;
-#pragma unroll
-      for (int kk = 4 * part; kk < 4 * part + 4; ++kk) mma_ts_lo<desc_hi(L::kKVGroup)>(c, a + kk * 8, v_lo + kk * (2 * L::kKVGroup >> 4), idesc_pv, (kk > 0 || !first) ? 1u : 0u);
-    };
-    // rows from `from` on of the V tile in `stage` become zeros: slots of a sequence's last page that it has not filled, and what was there before
-    auto clear_rows = [&](int stage, int from) {
-#pragma unroll 1
-      for (int i = from * (D / 8) + lane; i < kTile * (D / 8); i += 32) {
-        const int row = i / (D / 8), piece = i % (D / 8);
-        st_shared_v4(base + L::kVOff + stage * L::kTileBytes + (row / 8) * L::kKVGroup + (piece / 8) * L::kKVAtom + (row % 8) * 128 + (piece % 8) * 16, 0u, 0u, 0u, 0u);
-      }
-      fence_async_shared();
-      __syncwarp();
-    };
-    unsigned q_uses[2] = {0u, 0u};  // segments finished in which the tile in place t had key tiles
-    unsigned tiles[2] = {0u, 0u};   // key tiles it has been through, over all segments
-    unsigned step = 0;
-    for (unsigned n_item = 0; ok; ++n_item) {
-      Segment s;
-      ok = next_segment(n_item, s);
-      if (!ok || !s.valid) break;
-      const bool both = s.both != 0;
-      auto at = [&](int t, int j) { return step + (both ? 2 * j + t : j); };
-      unsigned cleared = 0;  // + 1 of the load whose rows past the sequence's end have been cleared
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (s.count[t] > 0 && ok) ok = wait(B::q_full + t, q_uses[t] & 1u, 0x0200u | t);
-      if (!ok) break;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (s.count[t] > 0 && ok) {
-          const unsigned first = at(t, 0);
-          const int stage = first % B::kS;
-          ok = wait(B::k_full + stage, (first / B::kS) & 1, 0x0210u);
-          if (!ok) break;
-          tc_fence_after_sync();
-          // (the S_t region is free: MMAs run in issue order, and the last one issued for this tile consumed the P_t there)
-          if (elect_one()) {
-            issue_s(t, stage);
-            mma_commit(bar(B::s_full + t));
-            if (s.count[t] == 1) mma_commit(bar(B::q_empty + t));
-            if (both) mma_commit(bar(B::k_empty + stage));
-          }
-          __syncwarp();
-        }
-      if (!ok) break;
-      if (!both && elect_one()) mma_commit(bar(B::k_empty + step % B::kS));
-      __syncwarp();
-      const int rounds = max(s.count[0], s.count[1]);
-#pragma unroll 1
-      for (int j = 0; j < rounds && ok; ++j) {
-        bool issued_next = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!ok || j >= s.count[t]) continue;
-          const unsigned here = at(t, j), then = at(t, j + 1);
-          const int stage = here % B::kS, next = then % B::kS;
-          ok = wait(B::v_full + stage, (here / B::kS) & 1, 0x0220u | stage);
-          if (!ok) break;
-          const int tile_at = (s.first_tile + static_cast<int>(here - step)) * kTile;
-          const int left = side_end(prm, tile_at, s.keys) - tile_at;  // keys of the tile that there are
-          if (left < kTile && cleared != here + 1) {
-            clear_rows(stage, max(0, left));
-            cleared = here + 1;
-          }
-          const uint32_t phase = tiles[t] & 1u;
-          ok = wait(B::p_half + t, phase, 0x0260u | t);
-          if (!ok) break;
-          // the segment's first product overwrites O_t: the epilogue before must have read it
-          if (j == 0) ok = wait(B::o_free + t, (q_uses[t] & 1u) ^ 1u, 0x0270u | t);
-          if (!ok) break;
-          tc_fence_after_sync();
-          if (elect_one()) issue_pv(t, stage, 0, j == 0);
-          __syncwarp();
-          ok = wait(B::p_full + t, phase, 0x0230u | t);
-          if (!ok) break;
-          tc_fence_after_sync();
-          const bool last = j + 1 >= s.count[t];
-          if (elect_one()) {
-            issue_pv(t, stage, 1, j == 0);
-            if (last) mma_commit(bar(B::o_full + t));
-            if (both) mma_commit(bar(B::v_empty + stage));
-          }
-          __syncwarp();
-          ++tiles[t];
-          if (!last) {
-            // the scores can only follow the product that consumed the P_t lying over them
-            ok = wait(B::k_full + next, (then / B::kS) & 1, 0x0240u | next);
+          for (int t = 0; t < 2; ++t) {
+            if (s.count[t] == 0) continue;
+            ok = wait(B::q_empty + t, (q_uses[t] & 1u) ^ 1u, 0x0130u | t);
             if (!ok) break;
-            tc_fence_after_sync();
-            if (elect_one()) {
-              issue_s(t, next);
-              mma_commit(bar(B::s_full + t));
-              if (j + 2 == s.count[t]) mma_commit(bar(B::q_empty + t));
-              if (both) mma_commit(bar(B::k_empty + next));
+            ++q_uses[t];
+            if (lane == 0) {
+              mbar_expect_tx(bar(B::q_full + t), static_cast<uint32_t>(tile_rows) * D * 2);
+              const int token = s.first + (2 * at.j + (s.both ? 0 : t)) * tile_tokens;
+#pragma unroll
+              for (int a = 0; a < D / 64; ++a) tma_load_5d(base + L::kQOff + t * L::kTileBytes + a * L::kAtomBytes, &maps.q, bar(B::q_full + t), a * 64, s.kv_head * prm.group, token, 0, 0);
             }
             __syncwarp();
-            issued_next = true;
+          }
+          if (!ok) break;
+          // the page of this lane's box of key tile `tile`; one that is none is a coordinate outside the cache, whose box TMA fills with zeros
+          auto entry = [&](int tile) {
+            const int key = tile * kTile + my_chunk * chunk;
+            return key < side_end(prm, key, s.keys) ? entry_for(prm, s.b, key) : 0;
+          };
+          int page_next[2] = {entry(s.first_tile), entry(s.first_tile + 1)};  // two tiles ahead
+#pragma unroll 1
+          for (int j = 0; j < s.loads && ok; ++j, ++step) {
+            const int tile = s.first_tile + j, key = tile * kTile + my_chunk * chunk;
+            const int end = side_end(prm, key, s.keys);  // (the same for the whole tile)
+            const bool fetch = key < end && my_atom < kBoxAtoms;
+            const int page = fetch ? checked_page(page_next[0], prm.pages, prm.errors) : 0;
+            const int boxes = min(chunks, max(0, (end - tile * kTile + chunk - 1) >> chunk_log));  // those that have keys
+            const uint32_t bytes = static_cast<uint32_t>(boxes * chunk) * (D * 2);
+            page_next[0] = page_next[1], page_next[1] = entry(tile + 2);
+            const int in_page = slot_of(prm, key);
+            const int stage = step % B::kS;
+            const uint32_t wrap = (step / B::kS) & 1;
+            ok = wait(B::k_empty + stage, wrap ^ 1u, 0x0100u | stage);
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(bar(B::k_full + stage), bytes);
+            __syncwarp();
+            const uint32_t box = stage * L::kTileBytes + my_atom * L::kAtomBytes + my_chunk * (chunk / 8) * L::kKVGroup;
+            auto load = [&](uint32_t to, const CUtensorMap& map, int side, uint32_t full) {
+              if constexpr (kPacked) tma_load_5d(to, &map, full, 0, 0, side ? s.kv_head * (D / 64) : 0, in_page >> 3, side ? page : page * prm.kv_heads + s.kv_head);
+              else tma_load_5d(to, &map, full, my_atom * 64, in_page, s.kv_head, page, 0);
+            };
+            if (fetch) load(base + L::kKOff + box, maps.k, maps.k_side, bar(B::k_full + stage));
+            __syncwarp();
+            ok = wait(B::v_empty + stage, wrap ^ 1u, 0x0110u | stage);
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(bar(B::v_full + stage), bytes);
+            __syncwarp();
+            if (fetch) load(base + L::kVOff + box, maps.v, maps.v_side, bar(B::v_full + stage));
+            __syncwarp();
+          }
+          if (s.begun && !s.whole && lane == 0) {
+            // workers behind this one whose share begins inside the item, before the middle of its last step
+            const long long begins = to - end.into, limit = min(static_cast<long long>(costs.of(at.j)), kItem + steps * static_cast<long long>(costs.step_cost(at.j)) - costs.step_cost(at.j) / 2);
+            prm.parts.heads[blockIdx.x] = Head{small_quotient(begins + limit - 1, share) - static_cast<int>(blockIdx.x), s.first, s.n, s.kv_head, s.row0, tile_rows};
           }
         }
-        if (!ok) break;
-        if (!both && elect_one()) {
-          mma_commit(bar(B::v_empty + (step + j) % B::kS));
-          if (issued_next) mma_commit(bar(B::k_empty + (step + j + 1) % B::kS));
-        }
-        __syncwarp();
+        // the next item
+        if (last) break;
+        at.step = 0;
+        if (++at.j < costs.pairs) continue;
+        at.j = 0;
+        if (++at.kv_head < prm.kv_heads) continue;
+        at.kv_head = 0;
+        do {
+          if (++at.b >= prm.batch) {
+            more = false;
+            break;
+          }
+          at.e = extent_of(prm, at.b);
+        } while (at.e.n == 0);
       }
-      step += s.loads;
+      const unsigned slot = n_item & 1u;
+      if (ok) ok = wait(B::work_empty + slot, ((n_item >> 1) & 1u) ^ 1u, 0x0121u | slot);
+      if (ok && lane == 0) {
+        ring[slot].valid = 0;
+        mbar_arrive(bar(B::work_full + slot));
+      }
+    } else if (warp == kMmaWarp) {
+      // ================= MMA issuer =================
+      constexpr uint32_t idesc_s = mma_idesc(kTile, kTile, kFp16, false, false);
+      constexpr uint32_t idesc_pv = mma_idesc(kTile, D, kFp16, false, true);
+      auto issue_s = [&](int t, int stage) {
+        const uint32_t q_lo = desc_lo(base + L::kQOff + t * L::kTileBytes, 0);
+        const uint32_t k_lo = desc_lo(base + L::kKOff + stage * L::kTileBytes, 0);
+        const uint32_t c = tmem + L::kSCol + t * 128;
+        mma_ss_lo<false, desc_hi(L::kKVGroup)>(c, q_lo, k_lo, idesc_s);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (s.count[t] > 0) ++q_uses[t];
+        for (int kk = 1; kk < D / 16; ++kk) {  // (offsets in 16-byte units)
+          mma_ss_lo<true, desc_hi(L::kKVGroup)>(c, q_lo + (kk / 4) * (L::kAtomBytes >> 4) + (kk % 4) * 2, k_lo + (kk / 4) * (L::kKVAtom >> 4) + (kk % 4) * 2, idesc_s);
+        }
+      };
+      auto issue_pv = [&](int t, int stage, int part, bool first) {
+        const uint32_t v_lo = desc_lo(base + L::kVOff + stage * L::kTileBytes, L::kKVAtom);
+        const uint32_t c = tmem + L::kOCol + t * D;
+        const uint32_t a = tmem + L::kSCol + t * 128;
+#pragma unroll
+        for (int kk = 4 * part; kk < 4 * part + 4; ++kk) mma_ts_lo<desc_hi(L::kKVGroup)>(c, a + kk * 8, v_lo + kk * (2 * L::kKVGroup >> 4), idesc_pv, (kk > 0 || !first) ? 1u : 0u);
+      };
+      // rows from `from` on of the V tile in `stage` become zeros: slots of a sequence's last page that it has not filled, and what was there before
+      auto clear_rows = [&](int stage, int from) {
+#pragma unroll 1
+        for (int i = from * (D / 8) + lane; i < kTile * (D / 8); i += 32) {
+          const int row = i / (D / 8), piece = i % (D / 8);
+          st_shared_v4(base + L::kVOff + stage * L::kTileBytes + (row / 8) * L::kKVGroup + (piece / 8) * L::kKVAtom + (row % 8) * 128 + (piece % 8) * 16, 0u, 0u, 0u, 0u);
+        }
+        fence_async_shared();
+        __syncwarp();
+      };
+      unsigned q_uses[2] = {0u, 0u};  // segments finished in which the tile in place t had key tiles
+      unsigned tiles[2] = {0u, 0u};   // key tiles it has been through, over all segments
+      unsigned step = 0;
+      for (unsigned n_item = 0; ok; ++n_item) {
+        Segment s;
+        ok = next_segment(n_item, s);
+        if (!ok || !s.valid) break;
+        const bool both = s.both != 0;
+        auto at = [&](int t, int j) { return step + (both ? 2 * j + t : j); };
+        unsigned cleared = 0;  // + 1 of the load whose rows past the sequence's end have been cleared
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (s.count[t] > 0 && ok) ok = wait(B::q_full + t, q_uses[t] & 1u, 0x0200u | t);
+        if (!ok) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (s.count[t] > 0 && ok) {
+            const unsigned first = at(t, 0);
+            const int stage = first % B::kS;
+            ok = wait(B::k_full + stage, (first / B::kS) & 1, 0x0210u);
+            if (!ok) break;
+            tc_fence_after_sync();
+            // (the S_t region is free: MMAs run in issue order, and the last one issued for this tile consumed the P_t there)
+            if (elect_one()) {
+              issue_s(t, stage);
+              mma_commit(bar(B::s_full + t));
+              if (s.count[t] == 1) mma_commit(bar(B::q_empty + t));
+              if (both) mma_commit(bar(B::k_empty + stage));
+            }
+            __syncwarp();
+          }
+        if (!ok) break;
+        if (!both && elect_one()) mma_commit(bar(B::k_empty + step % B::kS));
+        __syncwarp();
+        const int rounds = max(s.count[0], s.count[1]);
+#pragma unroll 1
+        for (int j = 0; j < rounds && ok; ++j) {
+          bool issued_next = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || j >= s.count[t]) continue;
+            const unsigned here = at(t, j), then = at(t, j + 1);
+            const int stage = here % B::kS, next = then % B::kS;
+            ok = wait(B::v_full + stage, (here / B::kS) & 1, 0x0220u | stage);
+            if (!ok) break;
+            const int tile_at = (s.first_tile + static_cast<int>(here - step)) * kTile;
+            const int left = side_end(prm, tile_at, s.keys) - tile_at;  // keys of the tile that there are
+            if (left < kTile && cleared != here + 1) {
+              clear_rows(stage, max(0, left));
+              cleared = here + 1;
+            }
+            const uint32_t phase = tiles[t] & 1u;
+            ok = wait(B::p_half + t, phase, 0x0260u | t);
+            if (!ok) break;
+            // the segment's first product overwrites O_t: the epilogue before must have read it
+            if (j == 0) ok = wait(B::o_free + t, (q_uses[t] & 1u) ^ 1u, 0x0270u | t);
+            if (!ok) break;
+            tc_fence_after_sync();
+            if (elect_one()) issue_pv(t, stage, 0, j == 0);
+            __syncwarp();
+            ok = wait(B::p_full + t, phase, 0x0230u | t);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const bool last = j + 1 >= s.count[t];
+            if (elect_one()) {
+              issue_pv(t, stage, 1, j == 0);
+              if (last) mma_commit(bar(B::o_full + t));
+              if (both) mma_commit(bar(B::v_empty + stage));
+            }
+            __syncwarp();
+            ++tiles[t];
+            if (!last) {
+              // the scores can only follow the product that consumed the P_t lying over them
+              ok = wait(B::k_full + next, (then / B::kS) & 1, 0x0240u | next);
+              if (!ok) break;
+              tc_fence_after_sync();
+              if (elect_one()) {
+                issue_s(t, next);
+                mma_commit(bar(B::s_full + t));
+                if (j + 2 == s.count[t]) mma_commit(bar(B::q_empty + t));
+                if (both) mma_commit(bar(B::k_empty + next));
+              }
+              __syncwarp();
+              issued_next = true;
+            }
+          }
+          if (!ok) break;
+          if (!both && elect_one()) {
+            mma_commit(bar(B::v_empty + (step + j) % B::kS));
+            if (issued_next) mma_commit(bar(B::k_empty + (step + j + 1) % B::kS));
+          }
+          __syncwarp();
+        }
+        step += s.loads;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (s.count[t] > 0) ++q_uses[t];
+      }
     }
   } else {
+    registers_up<kSoftmaxRegs>();
     // ================= softmax + epilogue, one thread per row =================
     const int t = warp >> 2;
     const int row_in_tile = threadIdx.x & 127;
