@@ -20,9 +20,9 @@
 // are zeroed before the product that reads them, since 0 * NaN would reach every row. (Boxes outside the cache, which TMA fills with zeros,
 // would do too: pages that are none are fetched so.)
 //
-// Measured, 32 heads over 8 of 128, bf16: a prompt of 8192 tokens 468 us, 1170 TFLOP/s, 71 % of the measured matrix rate and level with the dense forward: softmax and tensor
-// pipe in turn (the tensor pipe is active 55 % of the time). Eight pieces of 1 to 1000 tokens behind up to 7000 keys 219 us, 960 TFLOP/s: 13 us until the first
-// scores of a launch, items that their rows fill in part, parts. 16 questions of 20 to 150 tokens, 32 heads over 4, behind 4113 keys 117 us, 810 TFLOP/s.
+// Measured, 32 heads over 8 of 128, bf16: a prompt of 8192 tokens 449 us, 1225 TFLOP/s, 75 % of the measured matrix rate: softmax and tensor pipe in turn (the tensor pipe is active
+// 59 % of the time). Eight pieces of 1 to 1000 tokens behind up to 7000 keys 216 us, 970 TFLOP/s: 12 us until the first scores of a launch, items that
+// their rows fill in part, parts. 16 questions of 20 to 150 tokens, 32 heads over 4, behind 4113 keys 108 us, 880 TFLOP/s.
 //
 // Warp roles (12 warps): 0-3 softmax and epilogue of tile 0, 4-7 of tile 1, 8 TMA producer, 9 MMA issuer and tensor-memory owner; 10 and 11 have gone home.
 #include <cuda_bf16.h>
@@ -46,7 +46,7 @@ constexpr int kThreads = 384;
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(2 * 128 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168);
 // What a step of an item with one tile costs, in keys. It computes as much as a step with two, a key tile of 128 each, but loads two key tiles to that one's one, which
-// no copy further ahead hides: by 176 the eight pieces above take 219 us, by 128 (the arithmetic alone) 274, by 240 222. Pages of 8 make the producer issue twice
+// no copy further ahead hides: by 176 the eight pieces above took 219 us, by 128 (the arithmetic alone) 274, by 240 222 (with the registers below 3 us less). Pages of 8 make the producer issue twice
 // the boxes, and that bounds it: 224 takes 222 us where 176 takes 243.
 __device__ __forceinline__ int paged_single_step(int chunk_log) { return chunk_log == 3 ? 224 : 176; }
 constexpr int kProducerWarp = 8;
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
             for (int i = 0; i < 32; i += 2) {
               const uint64_t x2 = f2_fma(f2_pack_bits(x[c][i], x[c][i + 1]), sl2_2, shift2);
               float p0, p1;
-              if (D == 64 && ((i >> 1) & 7) < 2) {  // (as in the dense forward: some of the exponentials on the FMA pipe)
+              if (D == 64 && ((i >> 1) & 7) < 2) {  // (as in the dense forward: some of the exponentials on the FMA pipe; at head dim 128 an eighth of them costs 2.5 %)
                 exp2_poly2<5>(x2, p0, p1);
               } else {
                 f2_unpack(x2, p0, p1);
