@@ -54,7 +54,7 @@ constexpr int kMmaWarp = 9;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleSlack = 8.f;
 constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
-constexpr int kLeast = 256;  // cost of the smallest share: about that of the smallest item
+constexpr int kLeast = 256;    // cost of the smallest share: about that of the smallest item, and of no step more, so that a share inside an item has one at least
 
 // kPacked: how a tile of K or V lies in shared memory at head dim 128. Column block after column block (64 columns of all 128 rows each), a box
 // of TMA fetches 64 columns of a run of keys; packed, the two column blocks of 8 rows lie side by side, and a box fetches all columns of the
