@@ -289,11 +289,16 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   };
   bool fresh = true;  //  a problem, or the share, begins
   // (the first turns only issue copies; one loop for all, since code that a launch runs once is fetched once, at some 50 clocks a line)
+  // Long shares of rows that lie one behind the other (pages head by head) come faster with one unit on the way than with two: two sequences of 131 000 keys 148 us : 154, 64 of up to
+  // 8191 177 : 182. Token by token it is the other way round (150 : 145 and 180 : 177), so it is for short shares (64 of 500 keys, 25 units a warp, 26.8 : 26.1) and narrower
+  // rows, whose copies are not all that a unit takes (96 columns 152 : 138).
+  const bool one_ahead = D == 128 && span >= 64 && prm.k.slot == 2 * D && prm.v.slot == 2 * D && prm.pieces == D / 8 && prm.pieces_v == D / 8;
 #pragma unroll 1
-  for (int step = 1 - R::kStages; at.cost < span; ++step) {
+  for (int step = (one_ahead ? 2 : 1) - R::kStages; at.cost < span; ++step) {
     if (fresh) begin(), fresh = false;
     if (step >= 0) {
-      copies_wait<R::kStages - 2>();
+      if (one_ahead) copies_wait<R::kStages - 3>();
+      else copies_wait<R::kStages - 2>();
       __syncwarp();
     }
     issue();

@@ -307,6 +307,18 @@ def test_a_long_sequence_among_short_ones(new):
     Scene([(1, 3), (new, 40000), (1, 17), (2, 2)], heads=2, kv_heads=1, hd=128, page_size=64, seed=14).upload().check()
 
 
+@pytest.mark.parametrize("new, heads", [(1, 4), (4, 4)])
+@pytest.mark.parametrize("order", ["head", "token"])
+def test_long_shares(order, new, heads):
+    """64 sequences of 20 000 keys: 67 units of 16 keys and more to every warp of 148 blocks, in pages that they all name."""
+    s = Scene([(new, 20000)], heads=heads, kv_heads=1, hd=128, page_size=64, order=order, seed=35, max_t_q=new)
+    many = 64
+    s.seqs, s.new, s.keys, s.k, s.v = s.seqs * many, s.new * many, s.keys * many, s.k * many, s.v * many
+    s.table, s.start, s.tokens = np.repeat(s.table, many, axis=0), np.arange(many + 1) * new, many * new
+    s.q = np.random.default_rng(36).standard_normal((s.tokens, heads, 128)).astype(np.float32).astype(BF16)
+    s.upload().check()
+
+
 @pytest.mark.parametrize("prefix", [0, 300])
 @pytest.mark.parametrize("new, heads", [(1, 4), (1, 32), (4, 16), (3, 20), (30, 8)])
 def test_what_the_workspace_held_is_of_no_concern(new, heads, prefix):
