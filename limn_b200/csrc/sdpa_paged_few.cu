@@ -15,12 +15,14 @@
 // m moves only when a row's maximum has outgrown it by 8 in log2 units (weights then reach 2^8, which 16 bits hold), as in
 // the tensor-core forward; l is summed from the weights before they are rounded.
 //
-// Measured: 64 sequences of 500 to 8191 keys, 32 heads over 8 of 128 (1.12 GB) 180 us, 6.2 TB/s, 95 % of a plain copy's rate; two of 131 000 keys (0.95 GB) 155 us, 6.1
+// Measured: 64 sequences of 500 to 8191 keys, 32 heads over 8 of 128 (1.12 GB) 180 us, 6.2 TB/s, 95 % of a plain copy's rate; two of 131 000 keys (0.95 GB) 148 us, 6.4
 // TB/s; 24 of 3000 keys and 1 to 5 tokens, 12 heads of 80 (139 MB) 37 us, 3.7 TB/s: the copies' 16-byte pieces fill 10 lanes of 16 and the beginning
 // weighs; one of 2000 keys, 8 heads of 64 (4 MB) 9 us with the join, nearly all of it beginnings: code fetched for the first time, some 50 clocks a line, and
 // four loads that hang on one another before the first key arrives.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "paged_rows.cuh"
 #include "sm100_ptx.cuh"
@@ -30,8 +32,16 @@ namespace {
 
 using namespace paged;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+// Warps of a block, which have its registers and its shared memory to themselves: 8, or 12 for narrow rows. A unit of those is fewer bytes and no less work, which more warps hide;
+// but they make smaller shares, more of them to a problem, and of rows that lie token by token they read less in order. 8 : 12, in us, keys of 64 columns: two sequences of
+// 131 000 keys, head by head, 91 : 81; 24 of 30 000 200 : 177; 64 of up to 8191, token by token, 110 : 114, of 32 columns 111 : 90; eight of 2000 12.0 : 12.8; one 8.9 : 10.
+constexpr int kMostWarps = 12;
+int most_warps(int width, int rows) { return width == 64 && rows <= 8 ? kMostWarps : 8; }
+int warps_for(const Pass& p, int width, int rows) {
+  const double keys = static_cast<double>(std::min(p.batch, p.tokens)) * p.kv_heads * (p.kv_lens != nullptr ? static_cast<double>(p.max_pages) * p.page_size + p.front : p.keys);
+  const bool in_order = p.k.slot == 16 * p.pieces && p.v.slot == 16 * p.pieces_v;
+  return keys >= 1 << 18 && (in_order || p.pieces + p.pieces_v <= 8) ? most_warps(width, rows) : 8;
+}
 constexpr int kUnit = kPagedUnit;  // keys
 static_assert(kUnit == 16);
 constexpr int kBegin = 4;  // units that a problem costs besides its keys: its queries, its page table, its way out
@@ -71,12 +81,12 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 // columns instead, for rows that have no more: 8 % slower at 80, the lanes' copies and rows of memory no longer matching). The 16-byte
 // pieces of a row are exchanged so that the eight rows of a matrix that ldmatrix reads fall on distinct banks and a copied row fills whole lines (rows
 // 16 bytes further apart than they are long instead: 10 % slower).
-template <int D>
+template <int D, int W>
 struct Ring {
   static constexpr int kSide = kUnit * D * 2;  // K or V of a unit
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kStages = D == 128 ? 3 : 48 / W;
   static constexpr int kWarpBytes = kStages * 2 * kSide;
-  static constexpr int kBytes = kWarps * kWarpBytes;  // 192 KB
+  static constexpr int kBytes = W * kWarpBytes;  // 192 KB
   __device__ static __forceinline__ uint32_t place(int row, int piece) { return row * (D * 2) + ((piece ^ (row & 7)) << 4); }
 };
 
@@ -103,9 +113,10 @@ struct Shared {
   long long end;            // the unit behind the beginning problem's last
 };
 
-template <int D, bool kFp16, int NT>
-__global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass prm, const Parts by_warp) {
-  using R = Ring<D>;
+template <int D, bool kFp16, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pass prm, const Parts by_warp) {
+  using R = Ring<D, kWarps>;
+  constexpr int kThreads = kWarps * 32;
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ Shared shared[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -501,40 +512,43 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_few_kernel(const Pass 
   }
 }
 
-template <int D, bool kFp16, int NT>
+template <int D, bool kFp16, int NT, int kWarps>
 int launch_few(const Pass& pass, const Parts& by_warp, cudaStream_t stream) {
-  auto kernel = sdpa_paged_few_kernel<D, kFp16, NT>;
+  auto kernel = sdpa_paged_few_kernel<D, kFp16, NT, kWarps>;
   static bool sized[64] = {};
   int device = 0;
   LIMN_CUDA(cudaGetDevice(&device), "asking for the current device");
   if (device >= 0 && device < 64 && !sized[device]) {
-    LIMN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<D>::kBytes), "sizing shared memory for the paged sdpa kernel");
+    LIMN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<D, kWarps>::kBytes), "sizing shared memory for the paged sdpa kernel");
     sized[device] = true;
   }
-  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers)), dim3(kThreads), Ring<D>::kBytes, stream, pass, by_warp), "launching the paged sdpa kernel");
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers)), dim3(kWarps * 32), Ring<D, kWarps>::kBytes, stream, pass, by_warp), "launching the paged sdpa kernel");
   note_launches(1);
   return LIMN_B200_OK;
 }
 
 template <int D>
-int launch_few_d(const Pass& pass, const Parts& by_warp, bool fp16, int rows, cudaStream_t stream) {
-  if (rows <= 8) return fp16 ? launch_few<D, true, 1>(pass, by_warp, stream) : launch_few<D, false, 1>(pass, by_warp, stream);
-  return fp16 ? launch_few<D, true, 2>(pass, by_warp, stream) : launch_few<D, false, 2>(pass, by_warp, stream);
+int launch_few_d(const Pass& pass, const Parts& by_warp, bool fp16, int rows, int warps, cudaStream_t stream) {
+  if constexpr (D == 64) {
+    if (warps == kMostWarps) return fp16 ? launch_few<D, true, 1, kMostWarps>(pass, by_warp, stream) : launch_few<D, false, 1, kMostWarps>(pass, by_warp, stream);
+  }
+  if (rows <= 8) return fp16 ? launch_few<D, true, 1, 8>(pass, by_warp, stream) : launch_few<D, false, 1, 8>(pass, by_warp, stream);
+  return fp16 ? launch_few<D, true, 2, 8>(pass, by_warp, stream) : launch_few<D, false, 2, 8>(pass, by_warp, stream);
 }
 
 int few_tile(int rows) { return rows <= 8 ? 8 : kPagedFewRows; }
 
 }  // namespace
 
-size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(sms, few_tile(rows), width) + Parts::bytes(sms * kWarps, few_tile(rows), width); }
+size_t paged_few_workspace(int rows, int width, int sms) { return Parts::bytes(sms, few_tile(rows), width) + Parts::bytes(sms * most_warps(width, rows), few_tile(rows), width); }
 
 int paged_few_launch(Pass& pass, bool fp16, int rows, unsigned char* workspace, cudaStream_t stream) {
   Parts by_warp;
-  const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128;
+  const int width = pass.pieces <= 8 && pass.pieces_v <= 8 ? 64 : 128, warps = warps_for(pass, width, rows);
   pass.parts.place(workspace, pass.blocks, few_tile(rows), width);
-  by_warp.place(workspace + Parts::bytes(pass.blocks, few_tile(rows), width), pass.blocks * kWarps, few_tile(rows), width);
-  if (width == 64) return launch_few_d<64>(pass, by_warp, fp16, rows, stream);
-  return launch_few_d<128>(pass, by_warp, fp16, rows, stream);
+  by_warp.place(workspace + Parts::bytes(pass.blocks, few_tile(rows), width), pass.blocks * warps, few_tile(rows), width);
+  if (width == 64) return launch_few_d<64>(pass, by_warp, fp16, rows, warps, stream);
+  return launch_few_d<128>(pass, by_warp, fp16, rows, warps, stream);
 }
 
 }  // namespace limn_b200

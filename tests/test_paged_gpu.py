@@ -307,15 +307,28 @@ def test_a_long_sequence_among_short_ones(new):
     Scene([(1, 3), (new, 40000), (1, 17), (2, 2)], heads=2, kv_heads=1, hd=128, page_size=64, seed=14).upload().check()
 
 
-@pytest.mark.parametrize("new, heads", [(1, 4), (4, 4)])
+NARROW = [s for s in SHAPES if max(s[4], s[5]) <= 64 and s[2] // s[3] <= 8 and s[0].startswith("generation")]
+
+
+@pytest.mark.parametrize("prefix", [0, 300])
+@pytest.mark.parametrize("shape", NARROW, ids=[s[0] for s in NARROW])
+def test_tables_with_room_for_many_keys(shape, prefix):
+    """How many keys there can be decides how many warps a block of narrow rows has: here 2^18 to a sequence, and few that there are."""
+    _, dtype, heads, kv_heads, hd, hd_v, page_size, order, seqs = shape
+    for order in {order, "head"}:
+        Scene(seqs, dtype=dtype, heads=heads, kv_heads=kv_heads, hd=hd, hd_v=hd_v, page_size=page_size, order=order, prefix=prefix, spare_tokens=2, seed=37,
+              max_pages=(1 << 18) // page_size).upload().check()
+
+
+@pytest.mark.parametrize("new, heads, hd", [(1, 4, 128), (4, 4, 128), (1, 4, 64), (2, 4, 24)])
 @pytest.mark.parametrize("order", ["head", "token"])
-def test_long_shares(order, new, heads):
-    """64 sequences of 20 000 keys: 67 units of 16 keys and more to every warp of 148 blocks, in pages that they all name."""
-    s = Scene([(new, 20000)], heads=heads, kv_heads=1, hd=128, page_size=64, order=order, seed=35, max_t_q=new)
+def test_long_shares(order, new, heads, hd):
+    """64 sequences of 20 000 keys: 44 units of 16 keys and more to every warp of 148 blocks, in pages that they all name."""
+    s = Scene([(new, 20000)], heads=heads, kv_heads=1, hd=hd, page_size=64, order=order, seed=35, max_t_q=new)
     many = 64
     s.seqs, s.new, s.keys, s.k, s.v = s.seqs * many, s.new * many, s.keys * many, s.k * many, s.v * many
     s.table, s.start, s.tokens = np.repeat(s.table, many, axis=0), np.arange(many + 1) * new, many * new
-    s.q = np.random.default_rng(36).standard_normal((s.tokens, heads, 128)).astype(np.float32).astype(BF16)
+    s.q = np.random.default_rng(36).standard_normal((s.tokens, heads, hd)).astype(np.float32).astype(BF16)
     s.upload().check()
 
 
