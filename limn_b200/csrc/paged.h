@@ -116,10 +116,12 @@ struct Extent {
 };
 __device__ __forceinline__ Extent extent_of(const int* q_start, const int* kv_lens, int b, int tokens, int max_t_q, int max_pages, int page_size, unsigned* errors) {
   const long long first = q_start[b], end = q_start[b + 1], keys = kv_lens[b];
-  if (first < 0 || end < first || end > tokens || end - first > max_t_q || keys < 0 || keys > static_cast<long long>(max_pages) * page_size) {
+  const bool idle = first == end;  // it brings no token: its length, which may be of an earlier step, is of no concern
+  if (first < 0 || end < first || end > tokens || end - first > max_t_q || (!idle && (keys < 0 || keys > static_cast<long long>(max_pages) * page_size))) {
     if (errors != nullptr) atomicOr(errors, LIMN_B200_PAGED_BAD_SEQUENCE);
     return Extent{0, 0, 0};
   }
+  if (idle) return Extent{static_cast<int>(first), 0, 0};
   return Extent{static_cast<int>(first), static_cast<int>(end - first), static_cast<int>(keys)};
 }
 __device__ __forceinline__ Extent extent_of(const Pass& p, int b) {
