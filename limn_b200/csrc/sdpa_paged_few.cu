@@ -374,9 +374,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
           alpha[nt][c] = ptx::exp2_approx((m[nt][c] - top) * sl2);
           m[nt][c] = top, moved = true;
         }
-        const float shift = m[nt][c] == -INFINITY ? 0.f : -m[nt][c] * sl2;
-        s[nt][c] = ptx::exp2_approx(fmaf(s[nt][c], sl2, shift));
-        s[nt][c + 2] = ptx::exp2_approx(fmaf(s[nt][c + 2], sl2, shift));
+        // (the difference first: a rounded m * sl2 would be in every weight, 2^-24 of it in log2 units, whatever the scores' size)
+        const float against = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+        s[nt][c] = ptx::exp2_approx((s[nt][c] - against) * sl2);
+        s[nt][c + 2] = ptx::exp2_approx((s[nt][c + 2] - against) * sl2);
         l[nt][c] = fmaf(l[nt][c], alpha[nt][c], s[nt][c] + s[nt][c + 2]);
       }
       p[nt][0] = transposed(kFp16 ? ptx::pack_f16(s[nt][0], s[nt][1]) : ptx::pack_bf16(s[nt][0], s[nt][1]));

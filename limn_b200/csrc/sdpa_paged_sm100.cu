@@ -53,6 +53,10 @@ constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleSlack = 8.f;
+// A weight's exponent is s * scale - m * scale in log2 units, one multiply-add a score, and m * scale is rounded: by 2^-15 at 2^10, which is no more than the score's
+// own float32 error there. Beyond, m is taken off the scores first (a weight against a maximum of 2^31 would not be a number otherwise). The
+// vote for it is 1 % of the 8192-token prompt, taken for each tile or only where a maximum has moved.
+constexpr float kFar = 1024.f;
 constexpr int kItem = 256;     // what an item costs besides its keys, in keys: Q, the first scores, the way out
 constexpr int kLeast = 256;    // cost of the smallest share: about that of the smallest item, and of no step more, so that a share inside an item has one at least
 
@@ -631,7 +635,16 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
           alpha = exp2_approx((m - mx) * sl2);
           m = mx;
         }
-        const float shift = m == -INFINITY ? 0.f : -m * sl2;
+        float shift = m == -INFINITY ? 0.f : -m * sl2;
+        const bool far = fabsf(shift) > kFar;
+        if (__any_sync(0xffffffffu, far)) {
+          const float against = far ? m : 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[c][i] = __float_as_uint(__uint_as_float(x[c][i]) - against);
+          shift = far ? 0.f : shift;
+        }
         const uint64_t shift2 = f2_pack(shift, shift);
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll

@@ -38,3 +38,32 @@ def test_a_place_that_brings_no_token_may_have_any_length(new, prefix, idle):
     s.check()
     s.check(causal=False)
     assert launches() == (3 if prefix and idle else 2)
+
+
+# ---------------------------------------------------------------- scores of any size
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("scale", [2.0**-99, 2.0**-6, 1.0, 2.0**10, 2.0**27, 2.0**99], ids=lambda x: f"2^{int(np.log2(x))}")
+def test_the_smallest_and_the_largest_scale(scale, new, hd):
+    """Queries and keys of whole numbers, whose products are exact in float32, up to 16 * hd, and scales that are powers of two: what is left of the score's error is the
+    rounding of log2(e) * scale, 2^-23 of the distance to the row's largest score. A weight that counts is at most 2^-30 of the largest, 21 away: 2^-18, inside the
+    comparison's 2^-13. L's 2^-23 of itself is the rounding of the largest score's product with the scale, and of the sum. Tied scores share their row."""
+    rng = np.random.default_rng(43)
+    s = Scene([(new, 700), (1, 90), (min(new, 5), 2000)], heads=4, kv_heads=2, hd=hd, seed=42)
+    s.q = rng.integers(-4, 5, s.q.shape).astype(np.float32).astype(s.dtype)
+    s.k = [rng.integers(-4, 5, k.shape).astype(np.float32).astype(s.dtype) for k in s.k]
+    s.upload().check(scale=scale)
+
+
+@pytest.mark.parametrize("idle", [[], IDLE], ids=["for each", "read once"])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("scale", [2.0**20, 2.0**99], ids=lambda x: f"2^{int(np.log2(x))}")
+def test_the_largest_scale_behind_a_prefix(scale, new, idle):
+    rng = np.random.default_rng(45)
+    s = Scene([(new, 700), (1, 90)] + idle, heads=4, kv_heads=2, hd=64, seed=44, prefix=500)
+    s.q = rng.integers(-4, 5, s.q.shape).astype(np.float32).astype(s.dtype)
+    s.k = [rng.integers(-4, 5, k.shape).astype(np.float32).astype(s.dtype) for k in s.k]
+    s.prefix_k = rng.integers(-4, 5, s.prefix_k.shape).astype(np.float32).astype(s.dtype)
+    s.upload().check(scale=scale)
+    assert launches() == (3 if idle else 2)
