@@ -50,7 +50,7 @@ __device__ __forceinline__ void add_sides(Sums& sums, float sl2) {
 
 // A row of one problem: the warps of a block share its parts.
 template <int D, bool kFp16>
-__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const Pass prm) {
+__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const Pass prm, const unsigned*) {
   constexpr int kLanes = D / 4;          // lanes to a row
   constexpr int kAtOnce = 32 / kLanes;   // parts a warp takes side by side
   __shared__ float4 all_sums[kJoinWarps][32];
@@ -76,14 +76,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
   if (side == 0) store4<D, kFp16>(prm, row_place(prm, head.first, head.kv_head, row), column, sums.acc, sums.m, sums.l);
 }
 
-// Many rows of one problem, which few workers share: D / 4 lanes to a row, kEach rows one behind the other whose parts are asked for together.
+// Many rows of one problem, which few workers share: D / 4 lanes to a row, kEach rows one behind the other whose parts are asked for together. None where a
+// kernel has given up: a worker of the pass may then not have left the parts that another has announced. (The pass of few rows waits for nothing.)
 template <int D, bool kFp16>
-__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_rows_kernel(const Pass prm) {
+__global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_rows_kernel(const Pass prm, const unsigned* status) {
   constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kParts = 2;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const Head head = prm.parts.heads[blockIdx.x];
-  if (head.followers == 0) return;
+  if (head.followers == 0 || *reinterpret_cast<const volatile unsigned*>(status) != ptx::kStatusOk) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int column = (lane % kLanes) * 4, r0 = (blockIdx.y * kJoinWarps + warp) * kEach * kAtOnce + lane / kLanes;
   const float sl2 = prm.scale * kLog2e;
@@ -169,8 +170,10 @@ template <int D, bool kFp16>
 int launch_join(const Pass& pass, bool many_rows, cudaStream_t stream) {
   constexpr int kRows = kJoinWarps * kEach * (128 / D);  // rows to a block of the kernel for many
   const unsigned blocks = static_cast<unsigned>(many_rows ? pass.parts.rows / kRows : pass.parts.rows);
+  unsigned* status = nullptr;
+  if (int rc = status_word(&status)) return rc;
   auto kernel = many_rows ? sdpa_paged_join_rows_kernel<D, kFp16> : sdpa_paged_join_kernel<D, kFp16>;
-  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers), blocks), dim3(kJoinWarps * 32), 0, stream, pass), "launching the kernel that joins parts");
+  LIMN_CUDA(launch_overlapped(kernel, dim3(static_cast<unsigned>(pass.parts.workers), blocks), dim3(kJoinWarps * 32), 0, stream, pass, status), "launching the kernel that joins parts");
   note_launches(1);
   return LIMN_B200_OK;
 }

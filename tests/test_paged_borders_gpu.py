@@ -67,3 +67,34 @@ def test_the_largest_scale_behind_a_prefix(scale, new, idle):
     s.prefix_k = rng.integers(-4, 5, s.prefix_k.shape).astype(np.float32).astype(s.dtype)
     s.upload().check(scale=scale)
     assert launches() == (3 if idle else 2)
+
+
+# ---------------------------------------------------------------- giving up in the middle of a call
+
+def test_what_a_kernel_that_gave_up_left_undone_is_not_joined():
+    """A wait runs out on another stream while a prompt is being computed: its blocks leave their waits, some of them before they have left the parts that others count
+    on. Every row is right or as it was; the workspace holds numbers that would show. The word says who gave up, and the next call is right."""
+    from limn_b200 import runtime
+    from limn_b200._lib import check, lib
+
+    s = Scene([(20000, 20000)], heads=16, kv_heads=2, hd=128, page_size=64, seed=46).upload()
+    good_o, good_l = s.attend()
+    q, room = runtime.upload(s.q), s.step.workspace
+    main, side, flag = runtime.Stream(), runtime.Stream(), runtime.empty(4, poison=0)
+    caught = 0
+    for budget in (400_000, 800_000, 1_600_000):  # clock ticks: parts of the prompt's 2 ms
+        out, lse = runtime.empty(good_o.nbytes, poison=0x7F), runtime.empty(good_l.nbytes, poison=0x7F)
+        check(lib().limn_b200_mem_set(room.ptr, 0x3F, room.nbytes, None), "filling the workspace")
+        runtime.synchronize()
+        check(lib().limn_b200_wait_probe(budget, flag.ptr, side.handle), "wait probe")
+        s.step.attention(q, out, lse, stream=main)
+        have_o, have_l = runtime.download(out, np.uint16, good_o.shape), runtime.download(lse, np.uint32, good_l.shape)
+        assert runtime.device_status() == 0x57417E57
+        as_it_was = (have_o == 0x7F7F).all(-1) & (have_l == 0x7F7F7F7F)
+        right = (have_o == good_o.view(np.uint16)).all(-1) & (have_l == good_l.view(np.uint32))
+        assert (as_it_was | right).all(), f"{np.count_nonzero(~(as_it_was | right))} rows are neither right nor as they were"
+        caught += bool(as_it_was.any() and right.any())
+    assert caught, "no attempt met the call in its middle"
+    again_o, again_l = s.attend()
+    assert np.array_equal(again_o.view(np.uint16), good_o.view(np.uint16)) and np.array_equal(again_l, good_l)
+    assert runtime.device_status() == 0
