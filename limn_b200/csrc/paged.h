@@ -104,9 +104,6 @@ struct Pass {
   float scale = 0.f;
   Parts parts;
   RowSums leave;  // where rows go instead of `out`, or null
-  // The kernel in front of this one in the stream is of the same call and concerns it not: what this pass reads was there before that one began. So it
-  // need not be waited for until the end.
-  int beside = 0;
   int blocks = 0;  // that make the pass, one to a multiprocessor
 };
 

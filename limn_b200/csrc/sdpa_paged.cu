@@ -115,13 +115,13 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
     return paged_join_launch(prm, fp16, rows > kPagedFewRows, on);
   }
   // every row over the prefix, as one sequence of all tokens that sees all of it (tokens that belong to no sequence too: nothing asks for those); every row
-  // over its own keys, on the multiprocessors as they become free; and the two together
+  // over its own keys; and the two together. Each kernel waits for the one in front of it before it reads memory: only that makes what was
+  // written before the call, the step's new keys among it, visible to it.
   const int width = prm.pieces <= 8 && prm.pieces_v <= 8 ? 64 : 128;
   const size_t all_rows = static_cast<size_t>(step->tokens) * step->heads;
   Pass front = prm;
   front.table = prefix_table, front.q_start = nullptr, front.kv_lens = nullptr, front.keys = prefix_len, front.batch = 1, front.causal = 0;
   front.leave.place(memory + w.own + w.front, all_rows, width), prm.leave.place(memory + w.own + w.front + w.sums, all_rows, width);
-  prm.beside = 1;
   if (int rc = launch_pass(front, fp16, static_cast<long long>(step->tokens) * prm.group, memory + w.own, on)) return rc;
   if (int rc = launch_pass(prm, fp16, rows, memory, on)) return rc;
   return paged_finish_launch(front, prm, fp16, on);

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float sl2 = prm.scale * kLog2e;
   const bool known = prm.q_start == nullptr;  // one sequence of a known length: the shares need no memory
-  if (!prm.beside && !known) ptx::grid_dependency_wait();
+  if (!known) ptx::grid_dependency_wait();
 
   // ---- the shares ----
   const int worker = blockIdx.x * kWarps + warp;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
     }
   }
 
-  if (!prm.beside && known) ptx::grid_dependency_wait();
+  if (known) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   if (threadIdx.x == 0) prm.parts.heads[blockIdx.x].followers = 0;
 
@@ -458,7 +458,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
     next_problem(prm, at);
     begun = fresh = true;
   }
-  if (prm.beside) ptx::grid_dependency_wait();  // (whoever waits for this kernel has waited for the one before it)
 
   // ---- the block's parts: chain 0 enters from the block before, chain 1 + w begins with warp w ----
   __syncthreads();

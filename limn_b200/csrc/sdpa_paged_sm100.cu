@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   }
   // up to here nothing has touched global memory; and where all tokens are one sequence of a known length, the shares need none either
   const bool known = prm.q_start == nullptr;
-  if (!prm.beside && !known) grid_dependency_wait();
+  if (!known) grid_dependency_wait();
   // ---- where this CTA's share begins and ends: the producer's business ----
   long long total = 0, share = 0, from = 0, to = 0;
   Place p = {};  // in the warp's halves
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
       place_in(rest, all);
     }
   }
-  if (!prm.beside && known) grid_dependency_wait();
+  if (known) grid_dependency_wait();
   grid_launch_dependents();
   if (threadIdx.x == 0) {
     abort_flag = *reinterpret_cast<volatile unsigned*>(status) != kStatusOk;  // an earlier kernel gave up: this one stands down
@@ -805,7 +805,6 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
   }
 
   // ---- teardown ----
-  if (prm.beside) grid_dependency_wait();  // (whoever waits for this kernel has waited for the one before it)
   tc_fence_before_sync();
   __syncthreads();
   if (warp == kMmaWarp) {

@@ -98,3 +98,62 @@ def test_what_a_kernel_that_gave_up_left_undone_is_not_joined():
     again_o, again_l = s.attend()
     assert np.array_equal(again_o.view(np.uint16), good_o.view(np.uint16)) and np.array_equal(again_l, good_l)
     assert runtime.device_status() == 0
+
+
+# ---------------------------------------------------------------- one operator after the other
+
+@pytest.mark.parametrize("captured", [False, True], ids=["enqueued", "captured"])
+@pytest.mark.parametrize("new, heads", [(1, 8), (3, 8), (60, 8)])
+def test_what_append_has_just_written_is_seen_behind_a_prefix_read_once(new, heads, captured):
+    """Append, and right behind it the passes over the prefix and over the sequences' own keys, again and again with other tokens in the same arrays and nothing
+    between them: every result is, bit by bit, what the call gives when the device is waited for before each."""
+    torch = pytest.importorskip("torch")
+    from limn_b200 import runtime
+
+    s = Scene([(new, 500), (new, new), (1, 40)] + IDLE, heads=heads, kv_heads=2, hd=128, page_size=16, seed=47, prefix=700).upload(with_new=False)
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(48)
+    made = [{name: torch.randn((s.tokens, h, 128), generator=gen, device=dev).to(torch.bfloat16) for name, h in (("q", heads), ("k", 2), ("v", 2))} for _ in range(3)]
+    now = {name: torch.zeros_like(x) for name, x in made[0].items()}
+    turned, out, lse = torch.zeros_like(now["q"]), torch.zeros_like(now["q"]), torch.zeros((s.tokens, heads), device=dev)
+    freqs = 10000.0 ** (-torch.arange(64, dtype=torch.float64, device=dev) / 64)
+
+    def call(stream, between=lambda: None):
+        s.step.append(now["k"], now["v"], q=now["q"], q_out=turned, frequencies=freqs, rotated=128, stream=stream)
+        between()
+        s.step.attention_with_prefix(turned, out, lse, prefix_table=s.prefix_dev, prefix_len=700, stream=stream)
+
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        alone = []
+        for x in made:
+            for name in now:
+                now[name].copy_(x[name])
+            side.synchronize()
+            call(side.cuda_stream, side.synchronize)
+            assert launches() == 3
+            side.synchronize()
+            alone.append((out.clone(), lse.clone()))
+        assert not torch.equal(alone[0][0], alone[1][0])
+        side.synchronize()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                call(torch.cuda.current_stream().cuda_stream)
+        got = []
+        for turn in range(30):
+            for name in now:
+                now[name].copy_(made[turn % 3][name])
+            if captured:
+                graph.replay()
+            else:
+                call(side.cuda_stream)
+            got.append((out.clone(), lse.clone()))
+        side.synchronize()
+    for turn, (o, l) in enumerate(got):
+        assert torch.equal(o.view(torch.int16), alone[turn % 3][0].view(torch.int16)) and torch.equal(l, alone[turn % 3][1]), f"turn {turn}"
+    assert s.error_bits() == 0
+    if captured:
+        del graph
+    assert runtime.device_status() == 0
