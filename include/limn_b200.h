@@ -191,7 +191,7 @@ int limn_b200_sdpa_bwd_kv_strided(const void* q, const void* k, const void* v, c
  *   else is refused and nothing is launched.
  * What only the device knows is checked there. A sequence whose offsets or length are impossible (q_start falling, beyond
  * `tokens` or more than max_t_q apart; kv_lens negative or beyond max_pages * page_size, unless the sequence brings no token) is left out: nothing of it is appended
- * and no row of its result is written (where q_start falls, other sequences may be left out too). One that brings more tokens than it has
+ * and no row of its result is written. Where q_start falls anywhere, no row of any sequence's result is written, and other sequences' tokens may not be appended. One that brings more tokens than it has
  * keys has no slots for the first of them: none of it is appended, and those tokens see no key. A page number outside [0, pages) is never followed: a new token that belongs there is
  * not appended, and a query row that sees a key there gets NaN (O and L). Either is noted in *errors (LIMN_B200_PAGED_BAD_*
  * bits are or-ed in; the caller clears the word). Tokens from q_start[batch] on, empty slots of pages, and pages that no table

@@ -21,7 +21,9 @@ struct Pages {
 // One worker's share of the work may begin and end inside a problem. What it has of a problem that others share is a part: the sums
 // O (unnormalised) and the statistics m (the score the weights are measured against, raw units) and l of its rows. A worker has
 // room for two parts, 2 w: of a problem that began with a worker before, 2 w + 1: of one that begins here and goes on. The worker where
-// a problem begins says in heads[w] which rows the parts are of and how many workers follow; 0 followers: nothing to join.
+// a problem begins says in heads[w] which rows the parts are of and how many workers follow; 0 followers: nothing to join; kServesNone:
+// nor has the pass anything for any row.
+constexpr int kServesNone = -1;
 struct Head {
   int followers;
   int first, n;   // the sequence's first token, and tokens
@@ -107,7 +109,10 @@ struct Pass {
   int blocks = 0;  // that make the pass, one to a multiprocessor
 };
 
-// A sequence's extents: `first` token of `n`, `keys` it has, those in front among them. One that cannot be has n = 0 and is noted.
+// A sequence's extents: `first` token of `n`, `keys` it has, those in front among them. One that cannot be has n = 0 and is noted; one whose offsets fall
+// has first = kFalls besides: where any do, sequences that are possible each by itself could have tokens in common, so the pass serves none of them (every
+// worker looks at all of them to find its share, and so at this).
+constexpr int kFalls = -1;
 struct Extent {
   int first, n, keys;
 };
@@ -116,7 +121,7 @@ __device__ __forceinline__ Extent extent_of(const int* q_start, const int* kv_le
   const bool idle = first == end;  // it brings no token: its length, which may be of an earlier step, is of no concern
   if (first < 0 || end < first || end > tokens || end - first > max_t_q || (!idle && (keys < 0 || keys > static_cast<long long>(max_pages) * page_size))) {
     if (errors != nullptr) atomicOr(errors, LIMN_B200_PAGED_BAD_SEQUENCE);
-    return Extent{0, 0, 0};
+    return Extent{end < first ? kFalls : 0, 0, 0};
   }
   if (idle) return Extent{static_cast<int>(first), 0, 0};
   return Extent{static_cast<int>(first), static_cast<int>(end - first), static_cast<int>(keys)};

@@ -140,17 +140,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
     const int into = static_cast<int>(rest - static_cast<long long>(at.kv_head) * cost);
     at.unit = max(0, into - kBegin), at.cost = max(0, kBegin - into);
   };
+  bool falls;  // q_start does, somewhere: nothing is served
   if (prm.batch <= 32) {
     // a lane has a sequence, and every warp adds them up for itself, without barriers or reading an extent again: eight sequences of 2000 keys 13.6 us, by the block 14.6. (Up to 128,
     // four to a lane: 0 to 0.4 us slower than this up to 32, and no faster than the block beyond)
     const Extent e = lane < prm.batch ? extent_of(prm, lane) : Extent{0, 0, 0};
+    falls = __any_sync(0xffffffffu, e.first == kFalls);
     long long upto = cost_of(e);
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const long long other = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += other;
     }
-    share_out(__shfl_sync(0xffffffffu, upto, 31) * prm.kv_heads);
+    share_out(falls ? 0 : __shfl_sync(0xffffffffu, upto, 31) * prm.kv_heads);
     if (span > 0) {
       at.b = __popc(__ballot_sync(0xffffffffu, upto * prm.kv_heads <= from));  // (below 32: `from` is below the total)
       at.e = Extent{__shfl_sync(0xffffffffu, e.first, at.b), __shfl_sync(0xffffffffu, e.n, at.b), __shfl_sync(0xffffffffu, e.keys, at.b)};
@@ -162,9 +164,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
     // every thread adds up its run of sequences, the block adds up the threads
     const int run = (prm.batch + kThreads - 1) / kThreads;
     long long mine = 0;
+    bool mine_falls = false;
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
-      if (b < prm.batch) mine += cost_of(extent_of(prm, b));
+      if (b >= prm.batch) break;
+      const Extent e = extent_of(prm, b);
+      mine += cost_of(e), mine_falls |= e.first == kFalls;
     }
     long long upto = mine;
 #pragma unroll
@@ -175,11 +180,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
     __shared__ long long share_end[kThreads];  // cost of the sequences up to and with a thread's, per key head
     __shared__ long long warp_sum[kWarps];
     if (lane == 31) warp_sum[warp] = upto;
-    __syncthreads();
+    falls = __syncthreads_or(mine_falls);
     for (int w = 0; w < warp; ++w) upto += warp_sum[w];
     share_end[threadIdx.x] = upto;
     __syncthreads();
-    share_out(share_end[kThreads - 1] * prm.kv_heads);
+    share_out(falls ? 0 : share_end[kThreads - 1] * prm.kv_heads);
     if (span > 0) {
       const int before = first_above(share_end, kThreads, prm.kv_heads, from);  // the run of sequences that `from` falls into
       long long rest = from - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads);
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) sdpa_paged_few_kernel(const Pa
 
   if (known) ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  if (threadIdx.x == 0) prm.parts.heads[blockIdx.x].followers = 0;
+  if (threadIdx.x == 0) prm.parts.heads[blockIdx.x].followers = falls ? kServesNone : 0;
 
   // ---- copies: run ahead of the arithmetic with a cursor of their own ----
   Cursor ahead = at;

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_kernel(const 
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const Head head = prm.parts.heads[blockIdx.x];
-  if (head.followers == 0) return;
+  if (head.followers <= 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.y, column = (lane % kLanes) * 4, side = lane / kLanes;
   const float sl2 = prm.scale * kLog2e;
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_join_rows_kernel(c
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const Head head = prm.parts.heads[blockIdx.x];
-  if (head.followers == 0 || *reinterpret_cast<const volatile unsigned*>(status) != ptx::kStatusOk) return;
+  if (head.followers <= 0 || *reinterpret_cast<const volatile unsigned*>(status) != ptx::kStatusOk) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int column = (lane % kLanes) * 4, r0 = (blockIdx.y * kJoinWarps + warp) * kEach * kAtOnce + lane / kLanes;
   const float sl2 = prm.scale * kLog2e;
@@ -134,13 +134,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) sdpa_paged_finish_kernel(cons
   const float sl2 = own.scale * kLog2e;
   const long long row = static_cast<long long>(token) * own.heads + head;
   // (all asked for before whose token it is is known: the memory is there for every row)
+  const bool served = own.parts.heads[0].followers != kServesNone;
   const float2 front_ml = front.leave.ml[row], own_ml = own.leave.ml[row];
   const float4 front_o = *reinterpret_cast<const float4*>(front.leave.o + row * D + column), own_o = *reinterpret_cast<const float4*>(own.leave.o + row * D + column);
   if (__syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<const volatile unsigned*>(status) != ptx::kStatusOk)) return;
   const int b = sequence_of(own.q_start, own.batch, token, lane);
-  if (b >= own.batch) return;  // (as is all of the block)
+  if (!served || b >= own.batch) return;  // (as is all of the block)
   const Extent e = extent_of(own, b);
-  if (token < e.first || token - e.first >= e.n) return;  // (so where the offsets are out of order)
+  if (token < e.first || token - e.first >= e.n) return;
   Sums sums;
   auto add = [&](const Pass& pass, const float2& ml, const float4& o) {
     if (ml.y == kInParts) {

@@ -216,10 +216,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     p.step = costs.step_at(low, p.into);
     __syncwarp();
   };
+  bool falls = false;  // q_start does, somewhere: nothing is served (the producer knows)
   if (prm.batch <= 32) {
     // a lane has a sequence, and the producer adds them up for itself: without barriers or reading an extent again (two prompts of 542 tokens at most 20.3 us, by the block 21.2)
     if (warp == kProducerWarp) {
       const Extent e = lane < prm.batch ? extent_of(prm, lane) : Extent{0, 0, 0};
+      falls = __any_sync(0xffffffffu, e.first == kFalls);
       const long long all = Costs(e, by_span, prm, chunk_log).all();
       long long upto = all;
 #pragma unroll
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
         const long long other = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += other;
       }
-      const long long x = share_out(__shfl_sync(0xffffffffu, upto, 31));
+      const long long x = share_out(falls ? 0 : __shfl_sync(0xffffffffu, upto, 31));
       if (from < total) {
         const int begins = __popc(__ballot_sync(0xffffffffu, upto * prm.kv_heads <= from)), ends = __popc(__ballot_sync(0xffffffffu, upto * prm.kv_heads <= min(to, total - 1)));
         p.b = lane < 16 ? begins : ends;
@@ -240,10 +242,13 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     // every thread adds up its run of sequences, the block adds up the threads
     const int run = (prm.batch + kThreads - 1) / kThreads;
     long long mine = 0;
+    bool mine_falls = false;
 #pragma unroll 1
     for (int i = 0; i < run; ++i) {
       const int b = threadIdx.x * run + i;
-      if (b < prm.batch) mine += Costs(extent_of(prm, b), by_span, prm, chunk_log).all();
+      if (b >= prm.batch) break;
+      const Extent e = extent_of(prm, b);
+      mine += Costs(e, by_span, prm, chunk_log).all(), mine_falls |= e.first == kFalls;
     }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -253,12 +258,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     __shared__ long long share_end[kThreads];
     __shared__ long long warp_sum[kThreads / 32];
     if (lane == 31) warp_sum[warp] = mine;
-    __syncthreads();
+    falls = __syncthreads_or(mine_falls);
 #pragma unroll 1
     for (int w = 0; w < warp; ++w) mine += warp_sum[w];
     share_end[threadIdx.x] = mine;
     __syncthreads();
-    const long long x = share_out(share_end[kThreads - 1]);
+    const long long x = share_out(falls ? 0 : share_end[kThreads - 1]);
     if (warp == kProducerWarp && from < total) {
       const int before = first_above(share_end, kThreads, prm.kv_heads, x);
       long long rest = x - (before == 0 ? 0 : share_end[before - 1] * prm.kv_heads), all;
@@ -306,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdpa_paged_many_kernel(const __gr
     registers_down<kOtherRegs>();
     if (warp == kProducerWarp) {
       // ================= the share, and TMA =================
+      if (falls && lane == 0) prm.parts.heads[blockIdx.x].followers = kServesNone;
       const bool any = ok && from < total;
       auto of_half = [&](int from_lane) {
         auto word = [&](int x) { return __shfl_sync(0xffffffffu, x, from_lane); };

@@ -157,3 +157,24 @@ def test_what_append_has_just_written_is_seen_behind_a_prefix_read_once(new, hea
     if captured:
         del graph
     assert runtime.device_status() == 0
+
+
+# ---------------------------------------------------------------- offsets that fall
+
+@pytest.mark.parametrize("most", [8, 60], ids=["few rows", "many rows"])
+@pytest.mark.parametrize("prefix, idle", [(0, 0), (0, 500), (300, 0), (300, 4000)], ids=["alone", "alone, many places", "behind", "behind, read once"])
+@pytest.mark.parametrize("start", [[0, 5, 3, 8], [0, 6, 0, 6], [2, 8, 1, 1], [0, 3, 8, 7]], ids=str)
+def test_where_offsets_fall_no_row_is_written(start, prefix, idle, most):
+    """Sequences that are possible each by itself have tokens in common then: whichever came last would stay. The word says so, run after run, and the next call
+    with offsets that rise is right."""
+    from limn_b200 import runtime
+
+    s = Scene([(5, 40), (1, 30), (2, 50)] + [(0, 0)] * idle, heads=2, kv_heads=1, hd=64, page_size=16, seed=49, prefix=prefix, max_t_q=most)
+    for _ in range(2):
+        s.upload(q_start=[*start, *[start[-1]] * idle])
+        have_o, have_l = s.attend()
+        assert (have_o.view(np.uint16) == 0x7FFF).all() and np.isnan(have_l).all()
+        assert s.error_bits() == 2
+        assert launches() == (3 if prefix and idle else 2)
+        s.upload().check()
+    assert runtime.device_status() == 0
