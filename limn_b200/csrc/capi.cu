@@ -265,6 +265,16 @@ int dispatch_op(Op op, const char* name, const Problem& p) {
 
 using namespace limn_b200;
 
+namespace {
+// Memory is freed when its last owner is collected, which a host language may do at any time, in the middle of a capture too. Calls that
+// are not captured would spoil a capture in the (default) global mode; freeing what no captured call uses harms none.
+struct DuringCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  DuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~DuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
 extern "C" {
 
 int limn_b200_sdpa_fwd(const void* q, const void* k, const void* v, const void* key_mask, void* out, void* lse,
@@ -497,6 +507,7 @@ int limn_b200_mem_alloc(void** device_ptr, unsigned long long nbytes) {
 }
 int limn_b200_mem_free(void* device_ptr) {
   clear_error();
+  const DuringCapture allowed;
   LIMN_CUDA(cudaFree(device_ptr), "freeing device memory");
   return LIMN_B200_OK;
 }
@@ -512,6 +523,7 @@ int limn_b200_host_alloc(void** pinned_ptr, unsigned long long nbytes) {
 }
 int limn_b200_host_free(void* pinned_ptr) {
   clear_error();
+  const DuringCapture allowed;
   LIMN_CUDA(cudaFreeHost(pinned_ptr), "freeing pinned host memory");
   return LIMN_B200_OK;
 }

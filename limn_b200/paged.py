@@ -12,7 +12,8 @@ that carries one as `.ptr` (limn's buffers, limn_b200.runtime.DeviceBuffer) or `
 int32 and are read on the device by each call, so one PagedBatch serves step after step, and its captured calls follow what
 the arrays hold when they are replayed. Calls launch on `stream` (None: the legacy default stream), do not synchronise and
 allocate nothing; a PagedBatch allocates its workspace when it is made, unless it is given one. Calls of one PagedBatch
-that can overlap on the GPU would share that workspace: give each stream a PagedBatch of its own.
+that can overlap on the GPU would share that workspace: give each stream a PagedBatch of its own. Captured calls keep using it:
+keep the PagedBatch as long as the graph.
 """
 
 from __future__ import annotations

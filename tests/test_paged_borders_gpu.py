@@ -178,3 +178,27 @@ def test_where_offsets_fall_no_row_is_written(start, prefix, idle, most):
         assert launches() == (3 if prefix and idle else 2)
         s.upload().check()
     assert runtime.device_status() == 0
+
+
+# ---------------------------------------------------------------- what is collected while a step is captured
+
+def test_a_batch_may_be_collected_during_a_capture():
+    """Its workspace, and pinned memory, are freed in the middle of the capture of another batch's calls, which goes on."""
+    torch = pytest.importorskip("torch")
+    from limn_b200 import runtime
+
+    s = Scene([(1, 300), (2, 40)], heads=4, kv_heads=2, hd=64, seed=50).upload()
+    good_o, good_l = s.attend()
+    going = [Scene([(1, 30)], heads=4, kv_heads=2, hd=64, seed=51).upload(), runtime.PinnedArray((100,), np.float32)]
+    q, out, lse = runtime.upload(s.q), runtime.empty(good_o.nbytes), runtime.empty(good_l.nbytes)
+    runtime.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        going.pop()
+        s.step.attention(q, out, lse, stream=torch.cuda.current_stream().cuda_stream)
+        going.pop()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert np.array_equal(runtime.download(out, np.uint16, good_o.shape), good_o.view(np.uint16)) and np.array_equal(runtime.download(lse, np.float32, good_l.shape), good_l)
+    del graph
+    assert runtime.device_status() == 0
