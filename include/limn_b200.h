@@ -245,7 +245,7 @@ int limn_b200_sdpa_paged(const limn_b200_paged* step, const void* q, void* out, 
 /* The same for a batch whose sequences all continue one prefix: every row sees the prefix_len keys of the pages prefix_table
  * names (device array, ceil(prefix_len / page_size) entries) and behind them its sequence's own as above. Where that costs less
  * the prefix is read once for the whole batch, in a pass of its own, else in front of every sequence's keys; a result's bits depend on which. Keys in a sequence's own pages are counted from the prefix's end: kv_lens, q_start and page_table do not
- * include it, first_position does. */
+ * include it, first_position does. At most 262140 heads. */
 int limn_b200_sdpa_paged_prefix(const limn_b200_paged* step, const void* q, void* out, float* lse, const long long* strides,
                                 const int* prefix_table, int prefix_len, int causal, double scale,
                                 void* workspace, unsigned long long workspace_bytes, void* stream);

@@ -222,7 +222,8 @@ size_t paged_many_workspace(int width, int sms);
 int paged_many_launch(paged::Pass& pass, bool fp16, unsigned char* workspace, cudaStream_t stream);
 // Behind a pass: rows whose problems were shared, out of their parts (of the kernel for few rows, whose problems have few rows and many parts, or of the other one).
 int paged_join_launch(const paged::Pass& pass, bool fp16, bool many_rows, cudaStream_t stream);
-// Behind two passes that leave their rows' sums: the rows of both together.
+// Behind two passes that leave their rows' sums: the rows of both together, of up to so many heads (a block has four of one token, or one where rows are few).
+constexpr int kPagedFinishHeads = 4 * 65535;
 int paged_finish_launch(const paged::Pass& front, const paged::Pass& own, bool fp16, cudaStream_t stream);
 
 }  // namespace limn_b200

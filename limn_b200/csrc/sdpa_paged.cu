@@ -191,6 +191,7 @@ int limn_b200_sdpa_paged_prefix(const limn_b200_paged* step, const void* q, void
   if (int rc = check_paged("sdpa_paged_prefix", step)) return rc;
   if (!prefix_table || prefix_len <= 0 || prefix_len > kMaxKeys)
     return fail(LIMN_B200_BAD_ARGUMENT, "sdpa_paged_prefix: a prefix of %d keys, or no table of its pages", prefix_len);
+  if (step->heads > kPagedFinishHeads) return fail(LIMN_B200_UNSUPPORTED, "sdpa_paged_prefix: %d heads, at most %d are served behind a prefix", step->heads, kPagedFinishHeads);
   return paged_pass("sdpa_paged_prefix", step, q, out, lse, strides, prefix_table, prefix_len, causal, scale, workspace, workspace_bytes, stream);
 }
 

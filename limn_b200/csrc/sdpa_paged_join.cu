@@ -184,6 +184,7 @@ int launch_finish_s(const Pass& front, const Pass& own, cudaStream_t stream) {
   unsigned* status = nullptr;
   if (int rc = status_word(&status)) return rc;
   constexpr int kRows = kJoinWarps / kSplit;
+  static_assert(kSplit > 1 || kRows * 65535 >= kPagedFinishHeads);
   const dim3 grid(static_cast<unsigned>(own.tokens), static_cast<unsigned>((own.heads + kRows - 1) / kRows));
   LIMN_CUDA(launch_overlapped(sdpa_paged_finish_kernel<D, kFp16, kSplit>, grid, dim3(kJoinWarps * 32), 0, stream, front, own, status), "launching the kernel that joins a prefix");
   note_launches(1);
