@@ -8,7 +8,8 @@
 
 The binding of limn_b200_kv_append, limn_b200_sdpa_paged and limn_b200_sdpa_paged_prefix (include/limn_b200.h, which says
 what each does with which extents). Every operand is device memory of the current device: an address, or an object
-that carries one as `.ptr` (limn's buffers, limn_b200.runtime.DeviceBuffer) or `data_ptr()`. Offsets, lengths and tables are
+that carries one as `.ptr` (limn's buffers, limn_b200.runtime.DeviceBuffer) or `data_ptr()`. A tensor also says what it holds and where: one of another type or
+device, one that is too small, or one that is not dense and comes without strides is refused with a ValueError. Offsets, lengths and tables are
 int32 and are read on the device by each call, so one PagedBatch serves step after step, and its captured calls follow what
 the arrays hold when they are replayed. Calls launch on `stream` (None: the legacy default stream), do not synchronise and
 allocate nothing; a PagedBatch allocates its workspace when it is made, unless it is given one. Calls of one PagedBatch
@@ -28,8 +29,11 @@ from limn_b200.registry import _note_launch
 from limn_b200.runtime import DeviceBuffer, Stream
 
 
-# How an operand's address is read, by its type (asking an object for an attribute it lacks takes longer than all the rest of a call).
+# How an operand's address is read, by its type (asking an object for an attribute it lacks takes longer than all the rest of a call), and the types that
+# say more of what they hold.
 _ADDRESS_OF: dict[type, Callable[[Any], int | None]] = {type(None): lambda x: None, int: lambda x: x}
+_TENSORS: set[type] = set()
+_DTYPE_NAMES: dict[Any, str] = {}  # a tensor library's dtype objects
 
 
 def _address(operand: Any) -> int | None:
@@ -38,8 +42,28 @@ def _address(operand: Any) -> int | None:
     if read is None:
         read = attrgetter("ptr") if hasattr(operand, "ptr") else methodcaller("data_ptr")
         read(operand)  # raises before the type is remembered, where it has neither
+        if not hasattr(operand, "ptr") and all(hasattr(operand, name) for name in ("dtype", "nbytes", "get_device", "is_contiguous")):
+            _TENSORS.add(kind)
         _ADDRESS_OF[kind] = read
     return read(operand)
+
+
+def _dtype_name(dtype: Any) -> str:
+    name = _DTYPE_NAMES.get(dtype)
+    if name is None:
+        name = _DTYPE_NAMES[dtype] = str(dtype).rpartition(".")[2]
+    return name
+
+
+def _array(operand: Any, name: str, dtypes: tuple[str, ...], nbytes: int) -> tuple[int | None, int | None]:
+    """Address and device of an array that a batch keeps, as far as it says: a dense tensor of one of `dtypes`, or anything, of at least `nbytes`."""
+    at = _address(operand)
+    is_tensor = type(operand) in _TENSORS
+    if is_tensor and (_dtype_name(operand.dtype) not in dtypes or not operand.is_contiguous() or operand.get_device() < 0):
+        raise ValueError(f"limn_b200: {name} must be a dense {' or '.join(dtypes)} tensor on a GPU, got {operand.dtype} on {operand.device}, strides {operand.stride()}")
+    if getattr(operand, "nbytes", nbytes) < nbytes:
+        raise ValueError(f"limn_b200: {name} has {operand.nbytes} bytes, {nbytes} are read")
+    return at, operand.get_device() if is_tensor else None
 
 
 class PagedCache:
@@ -56,6 +80,24 @@ class PagedCache:
         self.hd, self.hd_v = hd, hd if hd_v is None else hd_v
         self.k_strides = tuple(k_strides or (page_size * kv_heads * self.hd, self.hd, kv_heads * self.hd))
         self.v_strides = tuple(v_strides or (page_size * kv_heads * self.hd_v, self.hd_v, kv_heads * self.hd_v))
+        self._check("k", k, dtype, self.hd, self.k_strides)
+        self._check("v", v, dtype, self.hd_v, self.v_strides)
+
+    def _check(self, name: str, side: Any, dtype: str, width: int, strides: tuple[int, ...]) -> None:
+        if len(strides) != 3:
+            raise ValueError(f"limn_b200: the strides of {name} are (page, head, slot), got {strides}")
+        _address(side)
+        if type(side) in _TENSORS:
+            if _dtype_name(side.dtype) != dtype or side.get_device() < 0:
+                raise ValueError(f"limn_b200: the pages of {name} are {dtype} on a GPU, got {side.dtype} on {side.device}")
+            room = side.untyped_storage().nbytes() // 2 - side.storage_offset()  # a view's pages may lie beyond what it shows of them
+        elif hasattr(side, "nbytes"):
+            room = side.nbytes // 2
+        else:
+            return
+        reach = sum((n - 1) * stride for n, stride in zip((self.pages, self.kv_heads, self.page_size), strides, strict=True)) + width
+        if reach > room and dtype in ("float16", "bfloat16"):  # (of other types the library serves none)
+            raise ValueError(f"limn_b200: the pages of {name} reach over {reach} elements, there are {room}")
 
 
 class PagedBatch:
@@ -68,15 +110,28 @@ class PagedBatch:
                  q_start: Any, kv_lens: Any, first_position: int = 0, errors: Any = None, max_prefix: int = 1, workspace: Any = None):
         # the objects stay referenced as long as the step may read their memory
         self._held = (cache, page_table, q_start, kv_lens, errors)
-        self._step = Paged(_address(cache.k), _address(cache.v), _address(page_table), _address(q_start), _address(kv_lens), _address(errors),
+        arrays = (_array(page_table, "page_table", ("int32",), 4 * batch * max_pages), _array(q_start, "q_start", ("int32",), 4 * (batch + 1)),
+                  _array(kv_lens, "kv_lens", ("int32",), 4 * batch), _array(errors, "errors", ("int32", "uint32"), 4))
+        _address(workspace)
+        devices = {device for _, device in arrays} | {x.get_device() for x in (cache.k, cache.v, workspace) if type(x) in _TENSORS}
+        devices.discard(None)
+        if len(devices) > 1:
+            raise ValueError(f"limn_b200: the arrays of a batch are on one device, got {sorted(devices)}")
+        self._device = devices.pop() if devices else None
+        self._step = Paged(_address(cache.k), _address(cache.v), *(at for at, _ in arrays),
                            (ctypes.c_longlong * 3)(*cache.k_strides), (ctypes.c_longlong * 3)(*cache.v_strides), cache.dtype, batch, heads,
                            cache.kv_heads, cache.hd, cache.hd_v, cache.page_size, cache.pages, max_pages, tokens, max_t_q, first_position)
         self._by_ref = ctypes.byref(self._step)
+        self._step_at = ctypes.addressof(self._step)
         self._head_dim = cache.hd
         # (token, head) strides of dense operands: q, q_out, k, v and out
         self._dense = {"q": (heads * cache.hd, cache.hd), "k": (cache.kv_heads * cache.hd, cache.hd),
                        "v": (cache.kv_heads * cache.hd_v, cache.hd_v), "out": (heads * cache.hd_v, cache.hd_v)}
-        self._packed: dict[tuple, Any] = {}
+        self._packed: dict[tuple, tuple[Any, int]] = {}
+        # what a tensor has to hold, if it is dense: type, bytes
+        rows, kind = 2 * tokens, next(name for name, code in DTYPE_CODES.items() if code == cache.dtype)
+        self._wants = {"q": (kind, rows * heads * cache.hd), "q_out": (kind, rows * heads * cache.hd), "k": (kind, rows * cache.kv_heads * cache.hd),
+                       "v": (kind, rows * cache.kv_heads * cache.hd_v), "out": (kind, rows * heads * cache.hd_v), "lse": ("float32", 4 * tokens * heads)}
         loaded = lib()
         self._append, self._attend, self._attend_prefix = loaded.limn_b200_kv_append, loaded.limn_b200_sdpa_paged, loaded.limn_b200_sdpa_paged_prefix
         need = ctypes.c_ulonglong()
@@ -99,8 +154,10 @@ class PagedBatch:
         strides = self._packed.get((q_strides, q_out_strides, k_strides, v_strides))
         if strides is None:
             strides = self._pack((q_strides, q_out_strides, k_strides, v_strides), ("q", "q", "k", "v"))
-        code = self._append(self._by_ref, _address(q), _address(k), _address(v), _address(q_out), strides, _address(frequencies), rotated,
-                            PAIRING_CODES[pairing], stream.handle if isinstance(stream, Stream) else stream)
+        at = self._at
+        code = self._append(self._step_at, at(q, "q", q_strides), at(k, "k", k_strides), at(v, "v", v_strides), at(q_out, "q_out", q_out_strides), strides[1],
+                            at(frequencies, "frequencies", None, ("float64", 4 * rotated)), rotated, PAIRING_CODES[pairing],
+                            stream.handle if isinstance(stream, Stream) else stream)
         if code:
             check(code, "launching kv_append")
 
@@ -111,8 +168,9 @@ class PagedBatch:
         strides = self._packed.get((q_strides, out_strides))
         if strides is None:
             strides = self._pack((q_strides, out_strides), ("q", "out"))
-        code = self._attend(self._by_ref, _address(q), _address(out), _address(lse), strides, causal, self._head_dim**-0.5 if scale is None else scale,
-                            self._workspace_at, self.workspace_bytes, stream.handle if isinstance(stream, Stream) else stream)
+        at = self._at
+        code = self._attend(self._step_at, at(q, "q", q_strides), at(out, "out", out_strides), at(lse, "lse"), strides[1], causal,
+                            self._head_dim**-0.5 if scale is None else scale, self._workspace_at, self.workspace_bytes, stream.handle if isinstance(stream, Stream) else stream)
         if code:
             check(code, "launching sdpa_paged")
         _note_launch()
@@ -123,19 +181,41 @@ class PagedBatch:
         strides = self._packed.get((q_strides, out_strides))
         if strides is None:
             strides = self._pack((q_strides, out_strides), ("q", "out"))
-        code = self._attend_prefix(self._by_ref, _address(q), _address(out), _address(lse), strides, _address(prefix_table), prefix_len, causal,
+        at, pages = self._at, -(-prefix_len // self._step.page_size)
+        code = self._attend_prefix(self._step_at, at(q, "q", q_strides), at(out, "out", out_strides), at(lse, "lse"), strides[1],
+                                   at(prefix_table, "prefix_table", None, ("int32", 4 * pages)), prefix_len, causal,
                                    self._head_dim**-0.5 if scale is None else scale, self._workspace_at, self.workspace_bytes,
                                    stream.handle if isinstance(stream, Stream) else stream)
         if code:
             check(code, "launching sdpa_paged_prefix")
         _note_launch()
 
+    def _at(self, operand: Any, name: str, strides: tuple | None = None, wants: tuple[str, int] | None = None) -> int | None:
+        """Where a call's operand begins; a tensor has the type and, without strides, the extent that the call goes by, and is on the batch's device."""
+        if type(operand) not in _TENSORS:
+            at = _address(operand)
+            if type(operand) not in _TENSORS:  # (else seen for the first time)
+                return at
+        dtype, nbytes = wants or self._wants[name]
+        # (one test of what nearly always holds, a tenth of a microsecond for each thing asked; why it does not is found out below)
+        if (_DTYPE_NAMES.get(operand.dtype) == dtype and operand.get_device() == self._device
+                and (strides is not None or (operand.nbytes >= nbytes and operand.is_contiguous()))):
+            return operand.data_ptr()
+        device = operand.get_device()
+        if _dtype_name(operand.dtype) != dtype or device < 0 or (device != self._device and self._device is not None):
+            where = "a GPU" if self._device is None else f"device {self._device}"
+            raise ValueError(f"limn_b200: {name} must be {dtype} on {where}, got {operand.dtype} on {operand.device}")
+        if strides is None and not (operand.is_contiguous() and operand.nbytes >= nbytes):
+            raise ValueError(f"limn_b200: {name} without strides must be dense, of {nbytes} bytes, got shape {tuple(operand.shape)}, strides {operand.stride()}")
+        return operand.data_ptr()
+
     def _pack(self, given: tuple, names: tuple[str, ...]):
         """The strides of a call as the library takes them; kept, since a batch's calls are alike step after step."""
-        flat = [int(x) for strides, name in zip(given, names, strict=True) for x in (self._dense[name] if strides is None else strides)]
-        if len(flat) != 2 * len(names):
+        if any(strides is not None and len(strides) != 2 for strides in given):
             raise ValueError(f"limn_b200: strides are (token, head) pairs, got {given}")
+        flat = [int(x) for strides, name in zip(given, names, strict=True) for x in (self._dense[name] if strides is None else strides)]
         if len(self._packed) >= 64:
             self._packed.clear()
-        packed = self._packed[given] = (ctypes.c_longlong * len(flat))(*flat)
-        return packed
+        packed = (ctypes.c_longlong * len(flat))(*flat)
+        self._packed[given] = packed, ctypes.addressof(packed)
+        return self._packed[given]
