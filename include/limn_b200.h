@@ -188,7 +188,7 @@ int limn_b200_sdpa_bwd_kv_strided(const void* q, const void* k, const void* v, c
  *   f16/bf16, hd and hd_v multiples of 8 up to 128, heads a multiple of kv_heads (query head h reads key head
  *   h / (heads / kv_heads)) and at most 128 to a key head, page_size a multiple of 8; strides in elements, multiples of 8, columns
  *   contiguous, bases 16-byte aligned, every other array as its type is. Positions, tokens * heads and max_pages * page_size fit 31 bits. Anything
- *   else is refused and nothing is launched.
+ *   else is refused and nothing is launched, a cache in host memory or on another device than the current one too.
  * What only the device knows is checked there. A sequence whose offsets or length are impossible (q_start falling, beyond
  * `tokens` or more than max_t_q apart; kv_lens negative or beyond max_pages * page_size, unless the sequence brings no token) is left out: nothing of it is appended
  * and no row of its result is written. Where q_start falls anywhere, no row of any sequence's result is written, and other sequences' tokens may not be appended. One that brings more tokens than it has

@@ -213,6 +213,7 @@ extern "C" int limn_b200_kv_append(const limn_b200_paged* step, const void* q, c
   for (int i = q ? 0 : 4; i < 8; ++i)
     if (strides[i] < 0 || (strides[i] & 7)) return fail(LIMN_B200_BAD_ARGUMENT, "kv_append: strides must be non-negative multiples of 8 elements, got %lld", strides[i]);
   if (step->tokens == 0 || step->batch == 0) return LIMN_B200_OK;
+  if (int rc = check_paged_device("kv_append", step)) return rc;
   AppendParams prm = {};
   prm.k = static_cast<const unsigned char*>(k), prm.v = static_cast<const unsigned char*>(v);
   if (q) {

@@ -211,6 +211,8 @@ __device__ __forceinline__ int first_above(const long long* ends, int n, int by,
 // Checks of a step that every entry point makes, of its extents and strides and of its pointers; `name` is the op's.
 int check_paged(const char* name, const limn_b200_paged* step);
 int check_paged_pointers(const char* name, const limn_b200_paged* step);
+// Whether the cache is memory that the current device's kernels can read, asked last of all.
+int check_paged_device(const char* name, const limn_b200_paged* step);
 
 constexpr long long kMaxKeys = 0x7fff0000LL;  // keys, positions and rows are counted in int, some key tiles past the last one included
 constexpr int kPagedUnit = 16, kPagedTile = 128;  // keys that a prefix in front is rounded up to, by the kernel that makes the pass

@@ -89,6 +89,7 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   if (int rc = workspace_of(step, prefix_len, &w)) return rc;
   if (w.bytes() > 0 && (!workspace || workspace_bytes < w.bytes()))
     return fail(LIMN_B200_BAD_ARGUMENT, "%s: the workspace has %llu bytes, %llu are needed", name, workspace_bytes, static_cast<unsigned long long>(w.bytes()));
+  if (int rc = check_paged_device(name, step)) return rc;
   Pass prm;
   prm.q = static_cast<const unsigned char*>(q), prm.out = static_cast<unsigned char*>(out), prm.lse = lse;
   prm.q_token = 2 * strides[0], prm.q_head = 2 * strides[1], prm.o_token = 2 * strides[2], prm.o_head = 2 * strides[3];
@@ -160,6 +161,17 @@ int check_paged_pointers(const char* name, const limn_b200_paged* s) {
   if ((reinterpret_cast<uintptr_t>(s->page_table) | reinterpret_cast<uintptr_t>(s->q_start) | reinterpret_cast<uintptr_t>(s->kv_lens) | reinterpret_cast<uintptr_t>(s->errors)) & 3u)
     return fail(LIMN_B200_BAD_ARGUMENT, "%s: the table, the offsets, the lengths or the word for errors is not 4-byte aligned", name);
   if ((reinterpret_cast<uintptr_t>(s->k_cache) | reinterpret_cast<uintptr_t>(s->v_cache)) & 15u) return fail(LIMN_B200_BAD_ARGUMENT, "%s: the cache is not 16-byte aligned", name);
+  return LIMN_B200_OK;
+}
+
+int check_paged_device(const char* name, const limn_b200_paged* s) {
+  int device = 0;
+  cudaPointerAttributes of = {};
+  LIMN_CUDA(cudaGetDevice(&device), "asking for the current device");
+  LIMN_CUDA(cudaPointerGetAttributes(&of, s->k_cache), "asking where the cache is");  // (70 ns)
+  if (of.type == cudaMemoryTypeUnregistered) return fail(LIMN_B200_BAD_ARGUMENT, "%s: the cache is not device memory", name);
+  if (of.type == cudaMemoryTypeDevice && of.device != device)
+    return fail(LIMN_B200_BAD_ARGUMENT, "%s: the cache is on device %d, the current one is %d", name, of.device, device);
   return LIMN_B200_OK;
 }
 }  // namespace limn_b200

@@ -202,3 +202,27 @@ def test_a_batch_may_be_collected_during_a_capture():
     assert np.array_equal(runtime.download(out, np.uint16, good_o.shape), good_o.view(np.uint16)) and np.array_equal(runtime.download(lse, np.float32, good_l.shape), good_l)
     del graph
     assert runtime.device_status() == 0
+
+
+# ---------------------------------------------------------------- where the cache is
+
+def test_a_cache_that_is_not_device_memory():
+    """Host memory that no kernel could read is refused before anything is launched."""
+    import ctypes
+
+    from limn_b200 import runtime
+    from limn_b200._lib import last_error, lib
+
+    s = Scene([(1, 30), (2, 40)], heads=4, kv_heads=2, hd=64, seed=52).upload()
+    s.check()
+    host = np.zeros(s.pages * 16 * 2 * 64 + 8, np.uint16)
+    at, pairs = -(-host.ctypes.data // 16) * 16, (ctypes.c_longlong * 8)(256, 64, 256, 64, 128, 64, 128, 64)
+    q, out, lse, new = runtime.upload(s.q), runtime.empty(s.q.nbytes), runtime.empty(s.tokens * 4 * 4), runtime.empty(s.tokens * 2 * 64 * 2)
+    step, room = s.step._step, s.step.workspace
+    on_device, step.k_cache = step.k_cache, at
+    for got in (lib().limn_b200_sdpa_paged(s.step._by_ref, q.ptr, out.ptr, lse.ptr, pairs, 1, 0.125, room.ptr, room.nbytes, None),
+                lib().limn_b200_sdpa_paged_prefix(s.step._by_ref, q.ptr, out.ptr, lse.ptr, pairs, s.table_dev.ptr, 5, 1, 0.125, room.ptr, room.nbytes, None),
+                lib().limn_b200_kv_append(s.step._by_ref, None, new.ptr, new.ptr, None, pairs, None, 0, 0, None)):
+        assert got == 1 and "device memory" in last_error() and launches() == 0
+    step.k_cache = on_device
+    s.check()
