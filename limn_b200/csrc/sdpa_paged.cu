@@ -26,23 +26,24 @@ int launch_pass(Pass& pass, bool fp16, long long rows, unsigned char* workspace,
 // A call behind a prefix either reads it once for the whole batch, in a pass of its own over all rows, whose sums are joined with those of the pass over the
 // sequences' own keys; or it puts the prefix in front of every sequence's keys and makes one pass. The first reads and computes less. The second launches two
 // kernels instead of three and leaves no sums in memory. Which is faster goes by what either costs beyond the other, as far as the host knows it:
-//   apart: 4 us, and 16 bytes for each element of O, written and read at 3 TB/s;
+//   apart: 6 us, and 16 bytes for each element of O, written and read at 3 TB/s;
 //   in front, few rows to a key head: the prefix is read once more for every sequence, mostly out of L2, at 12 TB/s;
 //   in front, more rows: a sequence's rows fill tiles of 128 less well than the batch's do; two such tiles by 128 keys of 128 columns take a multiprocessor 2.1 us.
-// Measured, 32 heads over 8 key heads of 128, 100 to 800 keys of their own, apart : in front, in us: one token of 8 sequences behind 1024 keys 20.8 : 16.7, of 32
-// 29.2 : 33.6, of 32 behind 8192 43.1 : 134.6, of 128 behind 128 72.1 : 53.5; 8 to 16 tokens of 32 sequences behind 1024 45.5 : 44.7, behind 8192 86.3 : 148.6;
-// 128 to 256 tokens of 32 sequences behind 1024 293.6 : 155.8, behind 8192 830.2 : 786.7.
-bool prefix_in_front(const limn_b200_paged* step, int prefix_len) {
+// Measured, 32 heads over 8 key heads of 128, 100 to 800 keys of their own, apart : in front, in us: one token of 8 sequences behind 2048 keys 26.3 : 18.8, of 32
+// behind 1024 33.7 : 31.7 and 2048 34.4 : 46.2, of 32 behind 8192 43.0 : 132, of 128 behind 128 73 : 54; up to 200 own keys, 8 to 16 tokens of 32 sequences behind 1024 43.4 : 45.7,
+// behind 8192 82 : 145; 128 to 256 tokens of 32 sequences behind 1024 293 : 151, behind 8192 816 : 726. Over these and other heads (8 over 1, 28 over 4, 16 over 2 of 64), 106
+// calls, the rule is never wrong by more than 3 us.
+bool prefix_in_front(const limn_b200_paged* step, int prefix_len, int sms) {
   if (static_cast<long long>(step->max_pages) * step->page_size + prefix_len > kMaxKeys) return false;  // (positions in front and behind count in one int)
   const long long group = step->heads / step->kv_heads;
-  const double apart = 4 + 16.0 * step->hd_v * step->tokens * step->heads / 3e6;
+  const double apart = 6 + 16.0 * step->hd_v * step->tokens * step->heads / 3e6;
   if (step->max_t_q * group <= kPagedFewRows) {
     const double bytes = 2.0 * prefix_len * step->kv_heads * (step->hd + step->hd_v);
     return (step->batch - 1) * bytes / 12e6 <= apart;
   }
   const double rows = static_cast<double>(step->tokens) * group, width = std::max(step->hd, step->hd_v) > 64 ? 1 : 0.5;
   const double more = step->batch * std::ceil(rows / step->batch / 128) - std::ceil(rows / 128);  // tiles
-  return more / 2 * step->kv_heads * std::ceil(prefix_len / 128.0) * width * 2.1 / 148 <= apart;
+  return more / 2 * step->kv_heads * std::ceil(prefix_len / 128.0) * width * 2.1 / sms <= apart;
 }
 
 // Shares of the work are counted in 64 bits, a warp's in 32 of them, 16 keys at a time: 2^43 keys that (tile, key head) pairs see is far below either.
@@ -106,7 +107,7 @@ int paged_pass(const char* name, const limn_b200_paged* step, const void* q, voi
   unsigned char* memory = static_cast<unsigned char*>(workspace);
   const long long rows = static_cast<long long>(step->max_t_q) * prm.group;
   if (int rc = sm_count(&prm.blocks)) return rc;
-  const bool in_front = prefix_len > 0 && prefix_in_front(step, prefix_len);
+  const bool in_front = prefix_len > 0 && prefix_in_front(step, prefix_len, prm.blocks);
   if (in_front) {
     const int whole = rows <= kPagedFewRows ? kPagedUnit : kPagedTile;
     prm.prefix_table = prefix_table, prm.prefix_len = prefix_len, prm.front = (prefix_len + whole - 1) / whole * whole;
