@@ -9,7 +9,7 @@
 // The angle p * f is taken as a number of turns in float64 and only its fraction goes to float32: at position 10^6 a float32
 // product would be off by 0.06 radians, this is off by 2 pi 2^-25. The turn is float32, rounded once to 16 bits.
 //
-// Measured: 24 600 tokens of 32 + 8 + 8 rows of 128 (605 MB) 95 us, 6.3 TB/s, 97 % of a plain copy's rate; 600 tokens of 36 rows of 80 5.2 us and one token 3.9 us,
+// Measured: 24 600 tokens of 32 + 8 + 8 rows of 128 (605 MB) 95 us, 6.3 TB/s, 97 % of a plain copy's rate; without the host 600 tokens of 36 rows of 80 5.0 us and one token 4.1 us,
 // of which some 3 us are the launch and the chain of dependent loads: offsets, length, table, rows.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -13,12 +13,14 @@
 //   O^T (columns x rows) += V^T P^T         A = V by ldmatrix.trans
 // Tensor-memory MMAs have nothing to add here: their 128 rows would hold 1 to 16, and the tensor pipe is idle most of the time.
 // m moves only when a row's maximum has outgrown it by 8 in log2 units (weights then reach 2^8, which 16 bits hold), as in
-// the tensor-core forward; l is summed from the weights before they are rounded.
+// the tensor-core forward. The weights are rounded to the operands' type because the matrix instructions take both operands in one; it is half a step of each, while their sum
+// l is taken before and is free of it.
 //
-// Measured: 64 sequences of 500 to 8191 keys, 32 heads over 8 of 128 (1.12 GB) 180 us, 6.2 TB/s, 95 % of a plain copy's rate; two of 131 000 keys (0.95 GB) 148 us, 6.4
-// TB/s; 24 of 3000 keys and 1 to 5 tokens, 12 heads of 80 (139 MB) 37 us, 3.7 TB/s: the copies' 16-byte pieces fill 10 lanes of 16 and the beginning
-// weighs; one of 2000 keys, 8 heads of 64 (4 MB) 9 us with the join, nearly all of it beginnings: code fetched for the first time, some 50 clocks a line, and
-// four loads that hang on one another before the first key arrives.
+// Measured, a call with its join among others: 64 sequences of 500 to 8191 keys, 32 heads over 8 of 128 (1.12 GB) 184 us, 6.1 TB/s, 93 % of a plain copy's rate (sustained, at the
+// 1762 MHz that the power cap leaves); two of 131 000 keys (0.95 GB) 153 us, 6.2 TB/s; 24 of 3000 keys and 1 to 5 tokens, 12 heads of 80 (139 MB) 37 us, 3.8 TB/s: the copies'
+// 16-byte pieces fill 10 lanes of 16 and the beginning weighs; one of 2000 keys, 8 heads of 64 (4 MB) 8.7 us on the device, nearly all of it beginnings: code fetched
+// for the first time, some 50 clocks a line, and four loads that hang on one another before the first key arrives.
+// What is compared further down was timed as calls in a graph, without the host, on a GPU that had rested (1965 MHz).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

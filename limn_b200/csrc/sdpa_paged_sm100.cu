@@ -20,9 +20,13 @@
 // are zeroed before the product that reads them, since 0 * NaN would reach every row. (Boxes outside the cache, which TMA fills with zeros,
 // would do too: pages that are none are fetched so.)
 //
-// Measured, 32 heads over 8 of 128, bf16: a prompt of 8192 tokens 449 us, 1225 TFLOP/s, 75 % of the measured matrix rate: softmax and tensor pipe in turn (the tensor pipe is active
-// 59 % of the time). Eight pieces of 1 to 1000 tokens behind up to 7000 keys 216 us, 970 TFLOP/s: 12 us until the first scores of a launch, items that
-// their rows fill in part, parts. 16 questions of 20 to 150 tokens, 32 heads over 4, behind 4113 keys 108 us, 880 TFLOP/s.
+// P is rounded to the operands' type, which the product that reads it from tensor memory asks for: half a step of each weight; their sum l is taken before.
+//
+// Measured, calls with their join one after the other, 32 heads over 8 of 128, bf16: a prompt of 8192 tokens 524 us, 1050 TFLOP/s, 75 % of the measured sustained matrix rate
+// (1612 MHz under the power cap; 450 us on a GPU that has rested): softmax and tensor pipe in turn (the tensor pipe is active 59 % of the time). Eight pieces of 1 to 1000 tokens
+// behind up to 7000 keys 257 us, 818 TFLOP/s (1552 MHz; 220 rested): 12 us until the first scores of a launch, items that their rows fill in part, parts. 16 questions
+// of 20 to 150 tokens, 32 heads over 4, behind 4113 keys 122 us, 778 TFLOP/s.
+// What is compared further down was timed as calls in a graph, without the host, on a GPU that had rested (1965 MHz).
 //
 // Warp roles (12 warps): 0-3 softmax and epilogue of tile 0, 4-7 of tile 1, 8 TMA producer, 9 MMA issuer and tensor-memory owner; 10 and 11 have gone home.
 #include <cuda_bf16.h>
