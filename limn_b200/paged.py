@@ -56,13 +56,13 @@ def _dtype_name(dtype: Any) -> str:
 
 
 def _array(operand: Any, name: str, dtypes: tuple[str, ...], nbytes: int) -> tuple[int | None, int | None]:
-    """Address and device of an array that a batch keeps, as far as it says: a dense tensor of one of `dtypes`, or anything, of at least `nbytes`."""
+    """Address and device of an array that a batch keeps, as far as it says: a dense tensor of one of `dtypes` (none: of any), or anything, of at least `nbytes`."""
     at = _address(operand)
     is_tensor = type(operand) in _TENSORS
-    if is_tensor and (_dtype_name(operand.dtype) not in dtypes or not operand.is_contiguous() or operand.get_device() < 0):
+    if is_tensor and ((dtypes and _dtype_name(operand.dtype) not in dtypes) or not operand.is_contiguous() or operand.get_device() < 0):
         raise ValueError(f"limn_b200: {name} must be a dense {' or '.join(dtypes)} tensor on a GPU, got {operand.dtype} on {operand.device}, strides {operand.stride()}")
     if getattr(operand, "nbytes", nbytes) < nbytes:
-        raise ValueError(f"limn_b200: {name} has {operand.nbytes} bytes, {nbytes} are read")
+        raise ValueError(f"limn_b200: the {name} has {operand.nbytes} bytes, {nbytes} are needed")
     return at, operand.get_device() if is_tensor else None
 
 
@@ -112,12 +112,6 @@ class PagedBatch:
         self._held = (cache, page_table, q_start, kv_lens, errors)
         arrays = (_array(page_table, "page_table", ("int32",), 4 * batch * max_pages), _array(q_start, "q_start", ("int32",), 4 * (batch + 1)),
                   _array(kv_lens, "kv_lens", ("int32",), 4 * batch), _array(errors, "errors", ("int32", "uint32"), 4))
-        _address(workspace)
-        devices = {device for _, device in arrays} | {x.get_device() for x in (cache.k, cache.v, workspace) if type(x) in _TENSORS}
-        devices.discard(None)
-        if len(devices) > 1:
-            raise ValueError(f"limn_b200: the arrays of a batch are on one device, got {sorted(devices)}")
-        self._device = devices.pop() if devices else None
         self._step = Paged(_address(cache.k), _address(cache.v), *(at for at, _ in arrays),
                            (ctypes.c_longlong * 3)(*cache.k_strides), (ctypes.c_longlong * 3)(*cache.v_strides), cache.dtype, batch, heads,
                            cache.kv_heads, cache.hd, cache.hd_v, cache.page_size, cache.pages, max_pages, tokens, max_t_q, first_position)
@@ -139,10 +133,12 @@ class PagedBatch:
         self.workspace_bytes = need.value
         if workspace is None and need.value:
             workspace = DeviceBuffer(need.value)
-        if getattr(workspace, "nbytes", need.value) < need.value:
-            raise ValueError(f"limn_b200: the workspace has {workspace.nbytes} bytes, {need.value} are needed")
         self.workspace = workspace
-        self._workspace_at = _address(workspace)
+        self._workspace_at, device = _array(workspace, "workspace", (), need.value)
+        devices = {device, *(device for _, device in arrays), *(x.get_device() for x in (cache.k, cache.v) if type(x) in _TENSORS)} - {None}
+        if len(devices) > 1:
+            raise ValueError(f"limn_b200: the arrays of a batch are on one device, got {sorted(devices)}")
+        self._device = devices.pop() if devices else None
 
     def append(self, k: Any, v: Any, *, q: Any = None, q_out: Any = None, k_strides=None, v_strides=None, q_strides=None, q_out_strides=None,
                frequencies: Any = None, rotated: int = 0, pairing: str = "halves", stream: Any = None) -> None:

@@ -127,12 +127,21 @@ def test_pages_of_a_shared_buffer():
     ("one device", {"errors": Tensor("int32", 1, device=1)}),
     ("one device", {"workspace": Tensor("uint8", 4096, device=1)}),
     ("workspace", {"workspace": Tensor("uint8", 4095)}),
+    ("workspace", {"workspace": Tensor("uint8", 4096, dense=False)}),
 ])
 def test_arrays_that_a_batch_cannot_read(calls, what, other):
     batch()
     batch(page_table=Buffer(48), q_start=512, kv_lens=Buffer(12), errors=Tensor("uint32", 1), workspace=1 << 20)
     with pytest.raises(ValueError, match=what):
         batch(**other)
+
+
+def test_a_workspace_that_only_says_it_is_on_the_cpu(calls):
+    """Everything else is buffers, of which no device is known."""
+    from limn_b200.paged import PagedCache
+
+    with pytest.raises(ValueError, match="workspace"):
+        batch(PagedCache(512, 512, **EXTENTS), page_table=512, q_start=512, kv_lens=512, workspace=Tensor("uint8", 4096, device=-1))
 
 
 GOOD = {"q": Tensor(numel=5 * 4 * 64, ptr=16), "k": Tensor(numel=5 * 2 * 64, ptr=32), "v": Tensor(numel=5 * 2 * 64, ptr=48), "q_out": Tensor(numel=5 * 4 * 64, ptr=64),
