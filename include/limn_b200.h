@@ -226,7 +226,8 @@ enum limn_b200_pairing {
  *   strides: (token, head) pairs of q, q_out, k, v (4 pairs; those of absent operands are not read). q_out may be q, with its strides.
  *   The first `rotated` columns of a row (a multiple of 8, 0 to hd) turn: pair j of a token at position p = first_position + slot
  *   by the angle p * frequencies[j], (x, y) -> (x cos - y sin, x sin + y cos); frequencies is a device array of rotated / 2
- *   doubles (NULL where rotated is 0). The angle is reduced in float64, the turn is float32, rounded once.
+ *   doubles (NULL where rotated is 0). The angle is reduced in float64, the turn is float32, rounded once. Of a token that is not appended
+ *   the row of q_out is not written either.
  *   Two new tokens of the batch must not share a slot. */
 int limn_b200_kv_append(const limn_b200_paged* step, const void* q, const void* k, const void* v, void* q_out,
                         const long long* strides, const double* frequencies, int rotated, int pairing, void* stream);

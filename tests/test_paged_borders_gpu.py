@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import numpy as np
 import pytest
-from paged_scene import Scene
+from paged_scene import Scene, poison
 
 pytestmark = pytest.mark.gpu
 
@@ -226,3 +226,32 @@ def test_a_cache_that_is_not_device_memory():
         assert got == 1 and "device memory" in last_error() and launches() == 0
     step.k_cache = on_device
     s.check()
+
+
+# ---------------------------------------------------------------- orders of memory
+
+@pytest.mark.parametrize("hd, hd_v", [(64, 64), (128, 128), (80, 40)])
+@pytest.mark.parametrize("new", [1, 3, 70])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_heads_outermost_in_queries_results_and_cache(prefix, new, hd, hd_v):
+    """(head, token, column) operands and (head, page, slot, column) pages: the largest stride belongs to the head."""
+    from limn_b200 import runtime
+    from limn_b200.paged import PagedBatch, PagedCache
+
+    s = Scene([(new, 300), (1, 40), (new, new)], heads=8, kv_heads=4, hd=hd, hd_v=hd_v, page_size=16, seed=53, prefix=prefix, spare_tokens=1)
+    k, v = (np.ascontiguousarray(x.transpose(2, 0, 1, 3)) for x in s.filled())
+    s.upload()
+    sides = runtime.upload(k), runtime.upload(v)
+    cache = PagedCache(*sides, dtype="bfloat16", pages=s.pages, page_size=16, kv_heads=4, hd=hd, hd_v=hd_v, k_strides=(16 * hd, s.pages * 16 * hd, hd),
+                       v_strides=(16 * hd_v, s.pages * 16 * hd_v, hd_v))
+    step = PagedBatch(cache, heads=8, batch=3, tokens=s.tokens, max_t_q=new, page_table=s.table_dev, max_pages=s.max_pages, q_start=s.q_start_dev, kv_lens=s.kv_lens_dev, errors=s.errors)
+    q = runtime.upload(np.ascontiguousarray(s.q.transpose(1, 0, 2)))
+    out, lse = runtime.upload(poison(s.dtype, (8, s.tokens, hd_v))), runtime.upload(np.full((s.tokens, 8), np.nan, np.float32))
+    more = {"q_strides": (hd, s.tokens * hd), "out_strides": (hd_v, s.tokens * hd_v)}
+    if prefix:
+        step.attention_with_prefix(q, out, lse, prefix_table=s.prefix_dev, prefix_len=prefix, **more)
+    else:
+        step.attention(q, out, lse, **more)
+    have = runtime.download(out, np.uint16, (8, s.tokens, hd_v)).view(s.dtype).transpose(1, 0, 2)
+    s.compare(np.ascontiguousarray(have), runtime.download(lse, np.float32, (s.tokens, 8)), *s.expected())
+    assert s.error_bits() == 0
