@@ -238,9 +238,9 @@ int limn_b200_kv_append(const limn_b200_paged* step, const void* q, const void* 
  *   causal: token i sees the keys up to its own; otherwise all of its sequence's. A row that sees no key gets NaN and
  *   lse = -inf. Keys and values that a row does not see but another row of its sequence in this step does count as 0 * v in its sum, as
  *   everywhere in 16 bits here: an infinity among them gives NaN. Empty slots may hold anything.
- *   A row's weights (at most 2^8 times the largest that is left in the end) are rounded to the operands' type before they multiply v, half a step each; scores, their
- *   sum and the products' sums are float32, the weights' sum is of the unrounded ones. Against 64 bits out is off by 1.2 to 1.4 times what 32 bits throughout would be off by,
- *   which is out's own rounding.
+ *   A row's weights are rounded to the operands' type before they multiply v, half a step each (float16 holds none below 2^-25 of the largest); scores and sums are float32, as the
+ *   matrix instructions make them, and the weights' sum is of the unrounded ones. Against 64 bits out is off by 1.2 to 1.4 times what 32 bits throughout would be off by, which is
+ *   out's own rounding. Keys that each weigh less than 2^-23 of what the row has gathered count in lse and may be lost from out: a hundred thousand of them 0.2 % of it.
  *   workspace: device memory of limn_b200_sdpa_paged_workspace bytes, 16-byte aligned, contents of no concern before
  *   and after the call; calls that can overlap on the GPU need one each. */
 int limn_b200_sdpa_paged(const limn_b200_paged* step, const void* q, void* out, float* lse, const long long* strides,
